@@ -13,6 +13,7 @@
 
 #include "ffn_device.h"
 #include "ffn_kernels.h"
+#include "ffn_ray_kernels.h"
 
 namespace {
 
@@ -597,6 +598,11 @@ void destroy_events(Handle* h) {
 }
 
 }  // namespace
+
+int ffn::set_error(int code, const char* msg) {
+  g_err = msg;
+  return code;
+}
 
 extern "C" {
 

@@ -1,0 +1,470 @@
+// ffn_experts.hip -- layers of experts on ragged groups of rows: the grouping, the product, its gradients.
+#include "ffn_ray_common.h"
+#include "ffn_ray_kernels.h"
+
+namespace ffn {
+
+// ---------------------------------------------------------------------------
+// The grouping: a stable counting sort of row indices by expert.  Counts per block of 4096 rows, a scan per expert over
+// the blocks, and a move in which a row's place comes from ballots over the lanes that hold equal ids, so the order
+// depends on the ids alone.
+
+constexpr int PL_NT = 256, PL_ITEMS = 16, PL_BLOCK = PL_NT * PL_ITEMS, PL_BINS = FFN_MAX_EXPERTS + 1;
+constexpr int EX_ROWS = 128;  // slots of a product tile
+
+// where the parts of a plan are, in words
+struct PlanView {
+  int bins;  // experts + 1: the last bin is that of the rows of no expert
+  uint32_t n, chunk;
+  uint64_t counts, offsets, rows, tiles, n_tiles, chunks, n_chunks, chunk_first, words;
+};
+__host__ __device__ inline PlanView plan_view(uint32_t n, int experts) {
+  PlanView v;
+  v.bins = experts + 1;
+  v.n = n;
+  // slots of a weight-gradient partial: about 512 of them, of 256 to 8192 slots
+  uint64_t c = ((uint64_t)n / 512 + 63) / 64 * 64;
+  v.chunk = (uint32_t)(c < 256 ? 256 : c > 8192 ? 8192 : c);
+  v.counts = 0;
+  v.offsets = v.bins;
+  v.chunk_first = 2 * (uint64_t)v.bins;
+  v.tiles = (3 * (uint64_t)v.bins + 2) / 2 * 2;
+  v.n_tiles = ((uint64_t)n + EX_ROWS - 1) / EX_ROWS + v.bins;
+  v.chunks = v.tiles + 2 * v.n_tiles;
+  v.n_chunks = ((uint64_t)n + v.chunk - 1) / v.chunk + v.bins;
+  v.rows = v.chunks + 2 * v.n_chunks;
+  v.words = v.rows + n;
+  return v;
+}
+
+__device__ __forceinline__ uint32_t bin_of(const int32_t* ids, int64_t i, int bins) {
+  return min((uint32_t)ids[i], (uint32_t)(bins - 1));
+}
+
+__global__ __launch_bounds__(PL_NT) void k_plan_count(const int32_t* __restrict__ ids, PlanView v,
+                                                      uint32_t* __restrict__ block_counts) {
+  __shared__ uint32_t cnt[PL_BINS];
+  for (int b = threadIdx.x; b < v.bins; b += PL_NT) cnt[b] = 0u;
+  __syncthreads();
+  const int64_t b0 = (int64_t)blockIdx.x * PL_BLOCK;
+#pragma unroll
+  for (int q = 0; q < PL_ITEMS; ++q) {
+    const int64_t i = b0 + q * PL_NT + threadIdx.x;
+    if (i < v.n) atomicAdd(&cnt[bin_of(ids, i, v.bins)], 1u);
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < v.bins; b += PL_NT) block_counts[(int64_t)b * gridDim.x + blockIdx.x] = cnt[b];
+}
+
+// inclusive sum over a wavefront
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint32_t y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+
+// one wavefront a bin: exclusive sums over the blocks in place, the total to the plan's counts
+__global__ __launch_bounds__(64) void k_plan_scan(uint32_t* __restrict__ block_counts, int blocks,
+                                                  uint32_t* __restrict__ plan, PlanView v) {
+  const int lane = threadIdx.x;
+  uint32_t* c = block_counts + (int64_t)blockIdx.x * blocks;
+  uint32_t sum = 0u;
+  for (int b0 = 0; b0 < blocks; b0 += 64) {
+    const uint32_t x = b0 + lane < blocks ? c[b0 + lane] : 0u;
+    const uint32_t s = wave_scan(x, lane);
+    if (b0 + lane < blocks) c[b0 + lane] = sum + s - x;
+    sum += __shfl(s, 63);
+  }
+  if (lane == 0) plan[v.counts + blockIdx.x] = sum;
+}
+
+// out[b] = sum of f(in[a]) over a < b, for all bins and (out[bins]) the total; in may be global, out is in LDS
+template <typename F>
+__device__ __forceinline__ void bin_scan(const uint32_t* in, int bins, uint32_t* out, uint32_t* part, F f) {
+  constexpr int PER = (PL_BINS + PL_NT - 1) / PL_NT;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint32_t x[PER], sum = 0u;
+#pragma unroll
+  for (int q = 0; q < PER; ++q) {
+    const int b = tid * PER + q;
+    x[q] = b < bins ? f(in[b]) : 0u;
+    sum += x[q];
+  }
+  const uint32_t s = wave_scan(sum, lane);
+  if (lane == 63) part[wave] = s;
+  __syncthreads();
+  uint32_t at = s - sum;
+  for (int w = 0; w < wave; ++w) at += part[w];
+#pragma unroll
+  for (int q = 0; q < PER; ++q) {
+    const int b = tid * PER + q;
+    if (b < bins) out[b] = at;
+    at += x[q];
+    if (b == bins - 1) out[bins] = at;
+  }
+  __syncthreads();
+}
+
+// entries {bin, index of the piece among its bin's} of a table of pieces of `size` slots
+__device__ __forceinline__ void fill_table(uint2* table, uint64_t n, uint64_t from, const uint32_t* first, int bins) {
+  for (uint64_t t = from + threadIdx.x; t < from + PL_BLOCK && t < n; t += PL_NT) {
+    uint2 e = make_uint2(0xFFFFFFFFu, 0u);
+    if (t < first[bins]) {
+      int lo = 0, hi = bins - 1;  // the last bin whose first piece is not past t
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (first[mid] <= t) lo = mid;
+        else hi = mid - 1;
+      }
+      e = make_uint2((uint32_t)lo, (uint32_t)(t - first[lo]));
+    }
+    table[t] = e;
+  }
+}
+
+__global__ __launch_bounds__(PL_NT) void k_plan_move(const int32_t* __restrict__ ids, PlanView v, int bits, int blocks,
+                                                     int tile_blocks, const uint32_t* __restrict__ block_counts,
+                                                     uint32_t* __restrict__ plan) {
+  constexpr int NW = PL_NT / 64;
+  __shared__ uint32_t first[PL_BINS + 1], part[NW], cnt[NW][PL_BINS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t* counts = plan + v.counts;
+  if ((int)blockIdx.x >= blocks) {
+    const int t = blockIdx.x - blocks;
+    if (t < tile_blocks) {
+      bin_scan(counts, v.bins, first, part, [](uint32_t c) { return (c + EX_ROWS - 1) / EX_ROWS; });
+      fill_table((uint2*)(plan + v.tiles), v.n_tiles, (uint64_t)t * PL_BLOCK, first, v.bins);
+    } else {
+      const uint32_t size = v.chunk;
+      bin_scan(counts, v.bins, first, part, [size](uint32_t c) { return (c + size - 1) / size; });
+      fill_table((uint2*)(plan + v.chunks), v.n_chunks, (uint64_t)(t - tile_blocks) * PL_BLOCK, first, v.bins);
+      if (t == tile_blocks)
+        for (int b = tid; b < v.bins; b += PL_NT) plan[v.chunk_first + b] = first[b];
+    }
+    return;
+  }
+  bin_scan(counts, v.bins, first, part, [](uint32_t c) { return c; });
+  if (blockIdx.x == 0)
+    for (int b = tid; b < v.bins; b += PL_NT) plan[v.offsets + b] = first[b];
+  if (v.n == 0) return;
+  for (int b = tid; b < NW * PL_BINS; b += PL_NT) (&cnt[0][0])[b] = 0u;
+  __syncthreads();
+  // wavefront w holds rows [w PL_BLOCK / NW, ...) of the block, 64 consecutive ones per trip
+  const int64_t w0 = (int64_t)blockIdx.x * PL_BLOCK + (int64_t)wave * (PL_BLOCK / NW);
+  const uint64_t below = (1ull << lane) - 1ull;
+  uint32_t bin[PL_ITEMS], rank[PL_ITEMS];
+#pragma unroll
+  for (int q = 0; q < PL_ITEMS; ++q) {
+    const int64_t i = w0 + q * 64 + lane;
+    const bool there = i < v.n;
+    bin[q] = there ? bin_of(ids, i, v.bins) : 0u;
+    uint64_t same = __ballot(there);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t m = __ballot((bin[q] >> b) & 1u);
+      same &= ((bin[q] >> b) & 1u) ? m : ~m;
+    }
+    const uint32_t before = cnt[wave][bin[q]];
+    rank[q] = before + (uint32_t)__popcll(same & below);
+    __builtin_amdgcn_wave_barrier();
+    if (there && (same & below) == 0ull) cnt[wave][bin[q]] = before + (uint32_t)__popcll(same);
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  for (int b = tid; b < v.bins; b += PL_NT) {
+    uint32_t at = first[b] + block_counts[(int64_t)b * blocks + blockIdx.x];
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const uint32_t c = cnt[w][b];
+      cnt[w][b] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < PL_ITEMS; ++q) {
+    const int64_t i = w0 + q * 64 + lane;
+    if (i < v.n) plan[v.rows + cnt[wave][bin[q]] + rank[q]] = (uint32_t)i;
+  }
+}
+
+static int plan_blocks(uint32_t n) { return (int)(((uint64_t)n + PL_BLOCK - 1) / PL_BLOCK); }
+
+uint64_t expert_plan_words(uint32_t n, int experts) { return plan_view(n, experts).words; }
+uint64_t expert_plan_workspace(uint32_t n, int experts) {
+  return (uint64_t)plan_blocks(n) * (experts + 1) * sizeof(uint32_t);
+}
+
+hipError_t launch_expert_plan(const int32_t* ids, uint32_t n, int experts, uint32_t* plan, uint32_t* workspace,
+                              hipStream_t st) {
+  const PlanView v = plan_view(n, experts);
+  const int blocks = plan_blocks(n);
+  int bits = 1;
+  while ((1 << bits) < v.bins) ++bits;
+  if (blocks) k_plan_count<<<blocks, PL_NT, 0, st>>>(ids, v, workspace);
+  k_plan_scan<<<v.bins, 64, 0, st>>>(workspace, blocks, plan, v);
+  const int tb = (int)((v.n_tiles + PL_BLOCK - 1) / PL_BLOCK), cb = (int)((v.n_chunks + PL_BLOCK - 1) / PL_BLOCK);
+  // without rows the offsets are written by no mover
+  k_plan_move<<<(blocks ? blocks : 1) + tb + cb, PL_NT, 0, st>>>(ids, v, bits, blocks ? blocks : 1, tb, workspace, plan);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// The products.
+
+constexpr int EX_NT = 256, EX_W = 64;  // W_e goes through LDS in tiles of 64 x 64
+
+// W[r0 .. r0 + 63][c0 .. c0 + 63] to LDS, 0 past the matrix.  PERM: row m = 8 g + j of each 32 goes where col_frag reads
+// slot j of lane group g, so that the K order is that of the other operand's 16-byte loads.
+template <typename T, bool PERM>
+__device__ __forceinline__ void stage_w(T* tile, const T* __restrict__ W, int rows, int cols, int r0, int c0) {
+  constexpr int EL = 16 / (int)sizeof(T), CPR = EX_W / EL;
+#pragma unroll
+  for (int i = 0; i < EX_W * CPR / EX_NT; ++i) {
+    const int c = threadIdx.x + i * EX_NT, row = c / CPR, col = (c % CPR) * EL;
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (r0 + row < rows && c0 + col < cols) v = *reinterpret_cast<const uint4*>(W + (int64_t)(r0 + row) * cols + c0 + col);
+    int to = row;
+    if (PERM) {
+      const int g = (row & 31) >> 3, j = row & 7;
+      to = (row & 32) + (j < 4 ? 4 * g + j : 16 + 4 * g + j - 4);
+    }
+    *reinterpret_cast<uint4*>(tile + to * lds_row<T, EX_W> + col) = v;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ typename Mat<T>::frag zero_frag() {
+  typename Mat<T>::frag f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = (T)0.f;
+  return f;
+}
+
+// BACK = false: y = act(x W_e^T + b_e);  true: dx = (dy where y > 0) W_e.  128 slots by 64 columns a block, 32 slots a
+// wavefront: the product is formed transposed (slots along the lanes), so a lane's rows of x come by 16-byte loads
+// straight into the operand and its four values of a result row go out by one store.
+template <typename T, bool BACK>
+__global__ __launch_bounds__(EX_NT) void k_expert(ffn_experts a, PlanView v, int64_t total, int col_tiles) {
+  __shared__ T ws[EX_W * lds_row<T, EX_W>];
+  const int64_t per = (total + 7) / 8, work = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (work >= total) return;
+  const uint2 tile = reinterpret_cast<const uint2*>(a.plan + v.tiles)[work / col_tiles];
+  if (tile.x >= (uint32_t)v.bins) return;
+  const int col0 = (int)(work % col_tiles) * EX_W;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
+  const uint32_t first = a.plan[v.offsets + tile.x] + tile.y * EX_ROWS, end = a.plan[v.offsets + tile.x] + a.plan[v.counts + tile.x];
+  const bool none = tile.x == (uint32_t)v.bins - 1;
+  const int depth = BACK ? a.out : a.in, width = BACK ? a.in : a.out;
+  int64_t xr[2], yr[2];
+  bool there[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const uint32_t slot = first + wave * 32 + s * 16 + c;
+    there[s] = slot < end;
+    const int64_t row = there[s] ? a.plan[v.rows + slot] : 0;
+    xr[s] = a.flags & FFN_EXPERTS_X_SLOTS ? (int64_t)slot : row;
+    yr[s] = a.flags & FFN_EXPERTS_Y_SLOTS ? (int64_t)slot : row;
+  }
+  f32x4 acc[4][2];
+#pragma unroll
+  for (int b = 0; b < 4; ++b) acc[b][0] = acc[b][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (!none) {
+    const T* W = (const T*)a.W + (int64_t)tile.x * a.out * a.in;
+    for (int k0 = 0; k0 < depth; k0 += EX_W) {
+      if (BACK) stage_w<T, true>(ws, W, a.out, a.in, k0, col0);
+      else stage_w<T, false>(ws, W, a.out, a.in, col0, k0);
+      typename Mat<T>::frag f[2][2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          const int col = k0 + 32 * ks + 8 * g;
+          f[s][ks] = zero_frag<T>();
+          if (there[s] && col < depth) {
+            if constexpr (BACK) {
+              f[s][ks] = *reinterpret_cast<const typename Mat<T>::frag*>((const T*)a.dy + yr[s] * a.dy_row + col);
+              if (a.relu) {
+                const typename Mat<T>::frag y = *reinterpret_cast<const typename Mat<T>::frag*>((const T*)a.y + yr[s] * a.out + col);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  if (!((float)y[j] > 0.f)) f[s][ks][j] = (T)0.f;
+              }
+            } else {
+              f[s][ks] = *reinterpret_cast<const typename Mat<T>::frag*>((const T*)a.x + xr[s] * a.x_row + col);
+            }
+          }
+        }
+      __syncthreads();
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          typename Mat<T>::frag w;
+          if constexpr (BACK) w = col_frag<T, EX_W>(ws, 32 * ks, 16 * b, lane);
+          else w = row_frag<T, EX_W>(ws, 16 * b + c, ks, lane);
+#pragma unroll
+          for (int s = 0; s < 2; ++s) acc[b][s] = Mat<T>::mma(w, f[s][ks], acc[b][s]);
+        }
+      __syncthreads();
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const int col = col0 + 16 * b + 4 * g;
+    if (col >= width) continue;
+    f32x4 bias = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (!BACK && a.b && !none)
+      bias = __builtin_convertvector(*reinterpret_cast<const typename Mat<T>::quad*>((const T*)a.b + (int64_t)tile.x * a.out + col), f32x4);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (!there[s]) continue;
+      typename Mat<T>::quad q;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float val = acc[b][s][r] + bias[r];
+        if (!BACK && a.relu) val = val < 0.f ? 0.f : val;  // a NaN stays one
+        q[r] = (T)val;
+      }
+      T* to = BACK ? (T*)a.dx + xr[s] * a.in : (T*)a.y + yr[s] * a.out;
+      *reinterpret_cast<typename Mat<T>::quad*>(to + col) = q;
+    }
+  }
+}
+
+// Sum over a chunk of an expert's slots of g^T x: 64 x 64 values a block, 32 x 32 a wavefront.  The slots are the K of
+// the product, so both operands are columns of their LDS tiles.  g against ones gives db's share.
+template <typename T>
+__global__ __launch_bounds__(EX_NT) void k_expert_dw(ffn_experts a, PlanView v, int64_t total, int m_tiles, int k_tiles) {
+  constexpr int EL = 16 / (int)sizeof(T), CPR = EX_W / EL, N = EX_W * CPR / EX_NT;
+  __shared__ T gs[EX_W * lds_row<T, EX_W>], xs[EX_W * lds_row<T, EX_W>];
+  const int64_t per = (total + 7) / 8, work = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (work >= total) return;
+  const int64_t piece = work / (m_tiles * k_tiles);
+  const uint2 chunk = reinterpret_cast<const uint2*>(a.plan + v.chunks)[piece];
+  if (chunk.x >= (uint32_t)v.bins - 1) return;
+  const int k0 = (int)(work % k_tiles) * EX_W, m0 = (int)(work / k_tiles % m_tiles) * EX_W;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
+  const int mw = (wave >> 1) * 32, kw = (wave & 1) * 32;
+  const uint32_t off = a.plan[v.offsets + chunk.x], group = a.plan[v.counts + chunk.x];
+  const uint32_t from = chunk.y * v.chunk, to = min(group, from + v.chunk);
+  f32x4 acc[2][2], sum[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) acc[i][0] = acc[i][1] = sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  typename Mat<T>::frag ones;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ones[j] = (T)1.f;
+  for (uint32_t s0 = from; s0 < to; s0 += EX_W) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int ch = tid + i * EX_NT, row = ch / CPR, col = (ch % CPR) * EL;
+      uint4 gv = make_uint4(0u, 0u, 0u, 0u), xv = gv;
+      if (s0 + row < to) {
+        const uint32_t slot = off + s0 + row;
+        const int64_t r = a.plan[v.rows + slot];
+        const int64_t xr = a.flags & FFN_EXPERTS_X_SLOTS ? (int64_t)slot : r, yr = a.flags & FFN_EXPERTS_Y_SLOTS ? (int64_t)slot : r;
+        if (k0 + col < a.in) xv = *reinterpret_cast<const uint4*>((const T*)a.x + xr * a.x_row + k0 + col);
+        if (m0 + col < a.out) {
+          gv = *reinterpret_cast<const uint4*>((const T*)a.dy + yr * a.dy_row + m0 + col);
+          if (a.relu) {
+            const uint4 yv = *reinterpret_cast<const uint4*>((const T*)a.y + yr * a.out + m0 + col);
+            typedef T vec __attribute__((ext_vector_type(EL)));
+            vec gg = __builtin_bit_cast(vec, gv);
+            const vec yy = __builtin_bit_cast(vec, yv);
+#pragma unroll
+            for (int j = 0; j < EL; ++j)
+              if (!((float)yy[j] > 0.f)) gg[j] = (T)0.f;
+            gv = __builtin_bit_cast(uint4, gg);
+          }
+        }
+      }
+      *reinterpret_cast<uint4*>(gs + row * lds_row<T, EX_W> + col) = gv;
+      *reinterpret_cast<uint4*>(xs + row * lds_row<T, EX_W> + col) = xv;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      typename Mat<T>::frag gf[2], xf[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        gf[i] = col_frag<T, EX_W>(gs, 32 * h, mw + 16 * i, lane);
+        xf[i] = col_frag<T, EX_W>(xs, 32 * h, kw + 16 * i, lane);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = Mat<T>::mma(gf[i], xf[j], acc[i][j]);
+        sum[i] = Mat<T>::mma(gf[i], ones, sum[i]);
+      }
+    }
+    __syncthreads();
+  }
+  const int64_t size = (int64_t)a.out * a.in + a.out;
+  float* part = (float*)a.workspace + piece * size;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int m = m0 + mw + 16 * i + 4 * g + r;
+      if (m >= a.out) continue;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int k = k0 + kw + 16 * j + c;
+        if (k < a.in) part[(int64_t)m * a.in + k] = acc[i][j][r];
+      }
+      if (k0 == 0 && kw == 0 && c == 0) part[(int64_t)a.out * a.in + m] = sum[i][r];
+    }
+}
+
+// dW and db: the partials of an expert's chunks, in order
+__global__ __launch_bounds__(EX_NT) void k_expert_join(ffn_experts a, PlanView v) {
+  const int64_t mk = (int64_t)a.out * a.in, size = mk + a.out;
+  const int64_t at = (int64_t)blockIdx.x * EX_NT + threadIdx.x;
+  if (at >= size) return;
+  const int e = blockIdx.y;
+  const uint32_t first = a.plan[v.chunk_first + e], last = a.plan[v.chunk_first + e + 1];
+  const float* part = (const float*)a.workspace;
+  float s = 0.f;
+  for (uint32_t p = first; p < last; ++p) s += part[p * size + at];
+  if (at < mk) {
+    if (a.dW) a.dW[e * mk + at] = s;
+  } else if (a.db) {
+    a.db[(int64_t)e * a.out + at - mk] = s;
+  }
+}
+
+uint64_t expert_workspace(const ffn_experts& a) {
+  if (!a.dW && !a.db) return 0;
+  return plan_view(a.n, a.n_experts).n_chunks * ((uint64_t)a.out * a.in + a.out) * sizeof(float);
+}
+
+template <typename T>
+static hipError_t run(const ffn_experts& a, bool backward, hipStream_t st) {
+  const PlanView v = plan_view(a.n, a.n_experts);
+  const int width = backward ? a.in : a.out, cols = (width + EX_W - 1) / EX_W;
+  const int64_t total = (int64_t)v.n_tiles * cols;
+  const unsigned grid = (unsigned)((total + 7) / 8 * 8);
+  if (!backward) {
+    k_expert<T, false><<<grid, EX_NT, 0, st>>>(a, v, total, cols);
+    return hipGetLastError();
+  }
+  if (a.dx) k_expert<T, true><<<grid, EX_NT, 0, st>>>(a, v, total, cols);
+  if (a.dW || a.db) {
+    const int mt = (a.out + EX_W - 1) / EX_W, kt = (a.in + EX_W - 1) / EX_W;
+    const int64_t pieces = (int64_t)v.n_chunks * mt * kt;
+    k_expert_dw<T><<<(unsigned)((pieces + 7) / 8 * 8), EX_NT, 0, st>>>(a, v, pieces, mt, kt);
+    const int64_t size = (int64_t)a.out * a.in + a.out;
+    k_expert_join<<<dim3((unsigned)((size + EX_NT - 1) / EX_NT), a.n_experts), EX_NT, 0, st>>>(a, v);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_experts(const ffn_experts& a, bool backward, hipStream_t st) {
+  if (a.dtype == FFN_BF16) return run<__bf16>(a, backward, st);
+  if (a.dtype == FFN_F16) return run<_Float16>(a, backward, st);
+  return run<float>(a, backward, st);
+}
+
+}  // namespace ffn

@@ -27,6 +27,9 @@ EXPORTS = [
     "ffn_occ_decay", "ffn_sample", "ffn_hash_encode_fwd", "ffn_hash_encode_bwd", "ffn_adam",
     "ffn_set_profiling", "ffn_stage_times", "ffn_occ_bitfield", "ffn_march", "ffn_render", "ffn_make_batch",
     "ffn_march_noalloc", "ffn_train_step_marched", "ffn_make_batch_weighted",
+    "ffn_ray_attention_workspace", "ffn_ray_attention_fwd", "ffn_ray_attention_bwd", "ffn_ray_scan_marks",
+    "ffn_ray_scan_workspace", "ffn_ray_scan_fwd", "ffn_ray_scan_bwd", "ffn_expert_plan_size", "ffn_expert_plan",
+    "ffn_expert_linear_fwd", "ffn_expert_linear_workspace", "ffn_expert_linear_bwd",
 ]
 ABI_VERSION = 3  # FFN_ABI_VERSION of the header these structures and signatures follow
 MARCH_NOALLOC_MAX_RAYS = 1 << 20
@@ -86,6 +89,46 @@ class FfnMarchParams(C.Structure):
 
 
 RENDER_NO_WAIT = 1  # FFN_RENDER_NO_WAIT
+
+
+class FfnRaySet(C.Structure):
+    _fields_ = [("counts", _vp), ("offsets", _vp), ("ray_ids", _vp), ("num_rays", C.c_uint32), ("n", C.c_uint32)]
+
+
+class FfnRayAttn(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("dim", C.c_int32),
+        ("scale", C.c_float), ("cap", C.c_float), ("causal", C.c_int32), ("reserved", C.c_int32),
+        ("q_rays", FfnRaySet), ("k_rays", FfnRaySet), ("q", _vp), ("k", _vp), ("v", _vp),
+        ("q_row", C.c_int64), ("q_head", C.c_int64), ("k_row", C.c_int64), ("k_head", C.c_int64),
+        ("v_row", C.c_int64), ("v_head", C.c_int64), ("slopes", _vp), ("t_q", _vp), ("t_k", _vp),
+        ("t_q_row", C.c_int64), ("t_k_row", C.c_int64), ("prefix", _vp), ("o", _vp), ("lse", _vp),
+        ("dout", _vp), ("do_row", C.c_int64), ("do_head", C.c_int64), ("dq", _vp), ("dk", _vp), ("dv", _vp),
+        ("workspace", _vp), ("workspace_bytes", C.c_uint64),
+    ]
+
+
+class FfnRayScan(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("channels", C.c_int32), ("reverse", C.c_int32), ("reserved", C.c_int32),
+        ("rays", FfnRaySet), ("gate", _vp), ("x", _vp), ("gate_row", C.c_int64), ("x_row", C.c_int64),
+        ("h0", _vp), ("h", _vp), ("last", _vp), ("marks", _vp), ("dh", _vp), ("dh_row", C.c_int64),
+        ("dlast", _vp), ("dgate", _vp), ("dx", _vp), ("dh0", _vp), ("workspace", _vp),
+        ("workspace_bytes", C.c_uint64),
+    ]
+
+
+MAX_EXPERTS = 1024  # FFN_MAX_EXPERTS
+EXPERTS_X_SLOTS, EXPERTS_Y_SLOTS = 1, 2
+
+
+class FfnExperts(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("n_experts", C.c_int32), ("d_in", C.c_int32), ("d_out", C.c_int32),
+        ("relu", C.c_int32), ("flags", C.c_int32), ("n", C.c_uint32), ("reserved", C.c_uint32), ("plan", _vp),
+        ("x", _vp), ("x_row", C.c_int64), ("W", _vp), ("b", _vp), ("y", _vp), ("dy", _vp), ("dy_row", C.c_int64),
+        ("dx", _vp), ("dW", _vp), ("db", _vp), ("workspace", _vp), ("workspace_bytes", C.c_uint64),
+    ]
 
 
 def march_params(res, dt, max_steps, T_stop=1e-4, chunk=32, sh_multiplier=1.0, sample_capacity=0,
@@ -149,11 +192,20 @@ def load(path: Path | str | None = None) -> C.CDLL:
                                             C.c_uint32, C.c_uint32, C.c_uint32, _vp, _vp, _vp, _vp]
     lib.ffn_set_profiling.argtypes = [_vp, C.c_int32]
     lib.ffn_stage_times.argtypes = [_vp, _fp, C.POINTER(C.c_int32), C.c_int32]
-    for name in ("ffn_create", "ffn_destroy", "ffn_bind_params", "ffn_train_step", "ffn_occ_decay", "ffn_sample",
-                 "ffn_hash_encode_fwd", "ffn_hash_encode_bwd", "ffn_adam", "ffn_set_profiling", "ffn_stage_times",
-                 "ffn_occ_bitfield", "ffn_march", "ffn_render", "ffn_make_batch", "ffn_march_noalloc",
-                 "ffn_train_step_marched", "ffn_make_batch_weighted"):
-        getattr(lib, name).restype = C.c_int
+    u64p = C.POINTER(C.c_uint64)
+    for op, args in (("attention", FfnRayAttn), ("scan", FfnRayScan)):
+        getattr(lib, f"ffn_ray_{op}_workspace").argtypes = [C.POINTER(args), C.c_int32, u64p]
+        getattr(lib, f"ffn_ray_{op}_fwd").argtypes = [C.POINTER(args), _vp]
+        getattr(lib, f"ffn_ray_{op}_bwd").argtypes = [C.POINTER(args), _vp]
+    lib.ffn_ray_scan_marks.argtypes = [C.POINTER(FfnRayScan), u64p]
+    lib.ffn_expert_plan_size.argtypes = [C.c_uint32, C.c_int32, u64p, u64p]
+    lib.ffn_expert_plan.argtypes = [_vp, C.c_uint32, C.c_int32, _vp, C.c_uint64, _vp, C.c_uint64, _vp]
+    lib.ffn_expert_linear_workspace.argtypes = [C.POINTER(FfnExperts), u64p]
+    lib.ffn_expert_linear_fwd.argtypes = [C.POINTER(FfnExperts), _vp]
+    lib.ffn_expert_linear_bwd.argtypes = [C.POINTER(FfnExperts), _vp]
+    for name in EXPORTS:
+        if name != "ffn_last_error":
+            getattr(lib, name).restype = C.c_int
     if path is None:
         _LIB = lib
     return lib

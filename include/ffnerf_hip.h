@@ -332,6 +332,160 @@ int ffn_make_batch_weighted(const float* images, uint32_t n_images, uint32_t wid
 int ffn_set_profiling(void* handle, int32_t enable);
 int ffn_stage_times(void* handle, float* total_ms, int32_t* launches, int32_t reset);
 
+/* ---- operators along rays, and expert layers -----------------------------
+ * No counterpart in the reference, whose networks see one sample at a time.
+ * For models that mix the samples of a ray before they are composited, and for
+ * scenes whose regions have layers of their own.  They work on the packed
+ * samples that ffn_march leaves, need no handle, allocate nothing and never
+ * wait: every call can be captured into a graph.  Buffers are the caller's;
+ * where a call needs scratch, its *_workspace function says how much, and two
+ * calls that may overlap need two workspaces. */
+
+enum { FFN_F32 = 0, FFN_F16 = 1, FFN_BF16 = 2 };                    /* element types of the operators */
+
+/* Rows of rays, packed: ray r has rows offsets[r] .. offsets[r] + counts[r] - 1
+ * of n (< 2^31 - 256), and ray_ids[i] is the ray of row i (ffn_march's counts,
+ * offsets and ray_ids).  Rays must not overlap.  A row that is in no ray (its
+ * id is no ray, or its place is outside that ray's rows) sees nothing, and
+ * what a call writes for it is 0. */
+typedef struct ffn_ray_set {
+  const uint32_t* counts;               /* [num_rays] */
+  const uint32_t* offsets;              /* [num_rays] */
+  const uint32_t* ray_ids;              /* [n] */
+  uint32_t num_rays;
+  uint32_t n;
+} ffn_ray_set;
+
+/* Attention among the rows of a ray.  With a the place of query i among its
+ * ray's nq queries, b the place of key j among the same ray's nk keys, and
+ * head h reading key head h / (heads / kv_heads):
+ *   s = scale q_i . k_j;  c = cap tanh(s / cap) (cap > 0), s (cap = 0)
+ *   l_ij = c - slopes[h] |t_q[i] - t_k[j]|           (slopes may be NULL: 0)
+ *   seen: same ray and, if causal, b <= a + nk - nq or b < prefix[ray]
+ *   o_i = sum_j softmax_j(l_ij) v_j,   lse_i = log sum_j exp(l_ij)
+ * A query that sees nothing has o = 0 and lse = -infinity; what a key that is
+ * not seen holds (infinities and NaN too) changes nothing.  The queries may be
+ * the keys' own set (all samples attend) or another set of the same rays (one
+ * query a ray; a ray's new samples against all of them).
+ * q [n_q][heads][dim], k and v [n_k][kv_heads][dim] of dtype with unit stride
+ * along dim; other strides in elements.  dim a multiple of 8, at most 128;
+ * rows 16-byte aligned.  o [n_q][heads][dim] of dtype, lse [n_q][heads] float,
+ * both contiguous.  Sums are held in float. */
+typedef struct ffn_ray_attn {
+  int32_t dtype;
+  int32_t heads, kv_heads, dim;
+  float scale, cap;
+  int32_t causal;
+  int32_t reserved;
+  ffn_ray_set q_rays, k_rays;           /* same num_rays */
+  const void *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;  /* strides, elements */
+  const float* slopes;                  /* [heads] or NULL */
+  const float *t_q, *t_k;               /* with slopes: depths, strides in elements */
+  int64_t t_q_row, t_k_row;
+  const uint32_t* prefix;               /* [num_rays] or NULL; used if causal */
+  void* o;
+  float* lse;
+  /* backward only: dout as q (strides do_row, do_head), dq, dk, dv contiguous */
+  const void* dout;
+  int64_t do_row, do_head;
+  void *dq, *dk, *dv;
+  void* workspace;
+  uint64_t workspace_bytes;
+} ffn_ray_attn;
+
+/* Scratch of a forward (backward = 0) or backward call with these sizes. */
+int ffn_ray_attention_workspace(const ffn_ray_attn* a, int32_t backward, uint64_t* bytes);
+int ffn_ray_attention_fwd(const ffn_ray_attn* a, void* stream);
+/* Gradients of sum(o dout): dq [n_q][heads][dim], dk and dv
+ * [n_k][kv_heads][dim] (summed over the query heads that share a key head) of
+ * dtype.  Reads the forward's o and lse.  slopes, t, scale and cap get none.
+ * No atomics: two calls give the same bits. */
+int ffn_ray_attention_bwd(const ffn_ray_attn* a, void* stream);
+
+/* The gated recurrence along rays, per channel and in float:
+ *   h_t = (1 - z_t) h_{t-1} + z_t x_t,  z = sigmoid(gate)
+ * over a ray's rows in order (reverse = 0) or from its last row to its first
+ * (1), from h0[ray] (NULL: 0).  It is the compositing recurrence for any number
+ * of feature channels: back to front, with opacity 1 - exp(-softplus(gate)) =
+ * sigmoid(gate).  gate and x [n][channels] of dtype with unit stride along the
+ * channels; h [n][channels] of dtype, contiguous; h0, last, dlast, dh0
+ * [num_rays][channels] float: last is the state after a ray's last step (h0 for
+ * a ray without rows).  marks (NULL without a backward pass): states the
+ * forward keeps for the backward, of ffn_ray_scan_marks bytes. */
+typedef struct ffn_ray_scan {
+  int32_t dtype, channels, reverse, reserved;
+  ffn_ray_set rays;
+  const void *gate, *x;
+  int64_t gate_row, x_row;              /* row strides, elements */
+  const float* h0;                      /* or NULL */
+  void* h;
+  float* last;                          /* or NULL */
+  float* marks;
+  /* backward only; dh as x (stride dh_row), dgate and dx contiguous */
+  const void* dh;
+  int64_t dh_row;
+  const float* dlast;                   /* or NULL */
+  void *dgate, *dx;
+  float* dh0;                           /* or NULL */
+  void* workspace;
+  uint64_t workspace_bytes;
+} ffn_ray_scan;
+
+int ffn_ray_scan_marks(const ffn_ray_scan* a, uint64_t* bytes);
+int ffn_ray_scan_workspace(const ffn_ray_scan* a, int32_t backward, uint64_t* bytes);
+int ffn_ray_scan_fwd(const ffn_ray_scan* a, void* stream);
+/* Gradients of sum(h dh) + sum(last dlast), from gate, x, h0 and the forward's
+ * marks of the same sizes. */
+int ffn_ray_scan_bwd(const ffn_ray_scan* a, void* stream);
+
+#define FFN_MAX_EXPERTS 1024
+/* Rows grouped by expert.  ids [n]: the expert of each row; an id outside
+ * [0, n_experts) gives the row to none.  plan (ffn_expert_plan_size words of 4
+ * bytes) receives counts [n_experts + 1] and then offsets
+ * [n_experts + 1] of the groups (the last: the rows of no expert), tables of the
+ * product kernels, and as its last n words rows: the row of each slot, grouped
+ * by expert, in their own order within a group.  n < 2^31 - 256, n_experts <=
+ * FFN_MAX_EXPERTS. */
+int ffn_expert_plan_size(uint32_t n, int32_t n_experts, uint64_t* plan_words, uint64_t* workspace_bytes);
+int ffn_expert_plan(const int32_t* ids, uint32_t n, int32_t n_experts, uint32_t* plan, uint64_t plan_words,
+                    void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* A layer of every expert on its own rows: y = x W_e^T + b_e, with relu
+ * max(y, 0).  x [n][in] of dtype with row stride x_row, y [n][out] contiguous,
+ * W [n_experts][out][in], b [n_experts][out] (NULL: 0) of dtype.  in and out
+ * multiples of 8 up to 4096, rows 16-byte aligned.  Rows of x and y are the
+ * caller's rows, or the plan's slots where the flags say so (so that the layers
+ * of a network stay in slot order between its first and its last).  Rows of no
+ * expert give 0. */
+#define FFN_EXPERTS_X_SLOTS 1
+#define FFN_EXPERTS_Y_SLOTS 2
+typedef struct ffn_experts {
+  int32_t dtype, n_experts, in, out;
+  int32_t relu, flags;
+  uint32_t n;
+  uint32_t reserved;
+  const uint32_t* plan;
+  const void* x;
+  int64_t x_row;
+  const void *W, *b;
+  void* y;                              /* backward: the forward's output, read with relu only */
+  /* backward only: dy as y with row stride dy_row; dx [n][in] contiguous of dtype, in x's rows; dW, db float;
+     any of dx, dW, db may be NULL */
+  const void* dy;
+  int64_t dy_row;
+  void* dx;
+  float *dW, *db;
+  void* workspace;
+  uint64_t workspace_bytes;
+} ffn_experts;
+
+int ffn_expert_linear_fwd(const ffn_experts* a, void* stream);
+int ffn_expert_linear_workspace(const ffn_experts* a, uint64_t* bytes);  /* of the backward */
+/* dx = g W_e, dW_e = sum g^T x, db_e = sum g, with g = dy (relu: where y > 0).
+ * Experts without rows get 0.  No atomics: two calls give the same bits. */
+int ffn_expert_linear_bwd(const ffn_experts* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
