@@ -23,6 +23,8 @@ int launched(hipError_t e, const char* what) {
 // row numbers are 32-bit with room for a tile past the end
 constexpr uint32_t MAX_ROWS = 0x7FFFFF00u;
 
+constexpr int MAX_SCAN_STRIDE = 1 << 27;
+
 int elem(int32_t dtype) { return dtype == FFN_F32 ? 4 : dtype == FFN_F16 || dtype == FFN_BF16 ? 2 : 0; }
 
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -91,6 +93,11 @@ int check_scan(const ffn_ray_scan* a, bool backward) {
   if (((uintptr_t)a->gate | (uintptr_t)a->x | (uintptr_t)a->h) & odd) return fail(-1, "misaligned buffer");
   if (backward && ((uintptr_t)a->dh | (uintptr_t)a->dgate | (uintptr_t)a->dx) & odd)
     return fail(-1, "misaligned gradient buffer");
+  // the kernels step through a few rows with 32-bit offsets
+  const int64_t far = (int64_t)MAX_SCAN_STRIDE / elem(a->dtype);
+  if (a->gate_row > far || a->gate_row < -far || a->x_row > far || a->x_row < -far ||
+      (backward && (a->dh_row > far || a->dh_row < -far)))
+    return fail(-1, "rows more than %d bytes apart", MAX_SCAN_STRIDE);
   const uint64_t need = ffn::scan_workspace(*a, backward);
   if (need && (!a->workspace || !aligned(a->workspace) || a->workspace_bytes < need))
     return fail(-1, "workspace of %llu bytes, %llu wanted", (unsigned long long)(a->workspace ? a->workspace_bytes : 0),

@@ -5,7 +5,8 @@
 //   * by rays: one whole ray.  One launch, every value read once.
 //   * by parts: a part of the packed rows of a fixed length, whatever rays it holds, so that few long rays fill the GPU
 //     too.  A part that begins inside a ray needs the state there: k_scan_ends composes, per part, the steps of the ray
-//     that leaves it (h -> A h + B), k_scan_chain the parts of a ray, in a fixed order.  That reads gate and x a second
+//     that leaves it (h -> A h + B), k_scan_groups those of neighbouring
+//     parts, in a fixed order.  That reads gate and x a second
 //     time, but only of rays that cross a part's end.
 // The backward pass walks the other way with D_t = dh_t + (1 - z_{t+1}) D_{t+1}.
 #include "ffn_ray_common.h"
@@ -14,7 +15,7 @@
 namespace ffn {
 
 constexpr int SC_NT = 256;
-constexpr int SC_MARK = 16;  // a state is kept every so many rows of a walk for the backward pass
+constexpr int SC_MARK = 8;  // a state is kept every so many rows of a walk for the backward pass
 
 // Places are counted in the direction of the walk: place p is row p, or row n - 1 - p.
 struct Walk {
@@ -45,33 +46,50 @@ __device__ __forceinline__ int64_t ray_at(const ffn_ray_scan& a, const Walk& w, 
   return -1;
 }
 
-// V neighbouring channels
+// V neighbouring channels as they lie in memory: kept as words until they are used (as vectors of 16-bit elements the
+// compiler spreads them over a register each)
+template <int BYTES> struct Words;
+template <> struct Words<2> { typedef uint16_t type; };
+template <> struct Words<4> { typedef uint32_t type; };
+template <> struct Words<8> { typedef uint2 type; };
 template <typename T, int V> struct Chan {
-  typedef T vec __attribute__((ext_vector_type(V)));
+  typedef typename Words<V * (int)sizeof(T)>::type vec;
 };
-template <typename T> struct Chan<T, 1> {
-  typedef T vec;
-};
-template <int V, typename X> __device__ __forceinline__ float get(const X& x, int i) {
-  if constexpr (V == 1) return (float)x;
-  else return (float)x[i];
+template <typename T, int V> __device__ __forceinline__ float get(const typename Chan<T, V>::vec& x, int i) {
+  uint32_t w;
+  if constexpr (V * sizeof(T) == 8) w = sizeof(T) == 4 ? (i ? x.y : x.x) : (i >> 1 ? x.y : x.x);
+  else w = x;
+  if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+  else if constexpr (__is_same(T, __bf16)) return __uint_as_float(i & 1 ? w & 0xFFFF0000u : w << 16);
+  else return (float)__builtin_bit_cast(_Float16, (uint16_t)(i & 1 ? w >> 16 : w & 0xFFFFu));
 }
-template <typename T, int V> __device__ __forceinline__ void put(typename Chan<T, V>::vec& x, int i, float v) {
-  if constexpr (V == 1) x = (T)v;
-  else x[i] = (T)v;
+template <typename T, int V> __device__ __forceinline__ typename Chan<T, V>::vec pack(const float (&f)[V]) {
+  typedef T tvec __attribute__((ext_vector_type(V)));
+  if constexpr (V == 1) {
+    const T t = (T)f[0];
+    return __builtin_bit_cast(typename Chan<T, V>::vec, t);
+  } else {
+    tvec t;
+#pragma unroll
+    for (int v = 0; v < V; ++v) t[v] = (T)f[v];
+    return __builtin_bit_cast(typename Chan<T, V>::vec, t);
+  }
 }
 
 __device__ __forceinline__ float sigmoid_f(float g) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
 }
 
-// N rows from p on, of which `left` are there: the last one again for the others, so that no lane branches
+// N rows from p on, `step` bytes apart, of which `left` are there: the last one again for the others, so that no lane
+// branches
 template <typename T, int V, int N>
-__device__ __forceinline__ void load_rows(typename Chan<T, V>::vec (&to)[N], const T* p, int64_t stride, int left) {
+__device__ __forceinline__ void load_rows(typename Chan<T, V>::vec (&to)[N], const T* p, int step, int left) {
+  int off = 0;
 #pragma unroll
   for (int u = 0; u < N; ++u) {
-    to[u] = *reinterpret_cast<const typename Chan<T, V>::vec*>(p);
-    p += u + 1 < left ? stride : 0;
+    to[u] = *reinterpret_cast<const typename Chan<T, V>::vec*>(reinterpret_cast<const char*>(p) + off);
+    off += u + 1 < left ? step : 0;
+    asm volatile("" : "+v"(off));  // opaque: else all N addresses are formed, and held, before the first load
   }
 }
 
@@ -82,9 +100,11 @@ struct Cols {
   int ch;
   Walk w;
   const T *gate, *x;
-  int64_t gs, xs;
+  int64_t gs, xs;  // from a place to the next, in elements
+  int gb, xb;      // in bytes
   __device__ __forceinline__ Cols(const ffn_ray_scan& a, int c)
-      : ch(c), w(a), gate((const T*)a.gate + c), x((const T*)a.x + c), gs(w.step * a.gate_row), xs(w.step * a.x_row) {}
+      : ch(c), w(a), gate((const T*)a.gate + c), x((const T*)a.x + c), gs(w.step * a.gate_row), xs(w.step * a.x_row),
+        gb((int)(gs * (int)sizeof(T))), xb((int)(xs * (int)sizeof(T))) {}
 };
 
 // h over `len` > 0 places from `from` on; marks are kept at multiples of SC_MARK of the walk, and at its start if `mark0`
@@ -92,15 +112,15 @@ template <typename T, int V>
 __device__ __forceinline__ void walk_fwd(const ffn_ray_scan& a, const Cols<T, V>& c, int64_t from, int len, bool mark0,
                                          float (&h)[V]) {
   typedef typename Cols<T, V>::vec vec;
-  constexpr int U = 8;
+  constexpr int U = SC_MARK;
   const int64_t row = c.w.row(from);
   const T* gp = c.gate + row * a.gate_row;
   const T* xp = c.x + row * a.x_row;
   T* hp = (T*)a.h + row * a.channels + c.ch;
   const int64_t hs = (int64_t)c.w.step * a.channels;
   vec g[U], x[U];
-  load_rows<T, V, U>(g, gp, c.gs, len);
-  load_rows<T, V, U>(x, xp, c.xs, len);
+  load_rows<T, V, U>(g, gp, c.gb, len);
+  load_rows<T, V, U>(x, xp, c.xb, len);
   for (int k = 0; k < len; k += U) {
     vec gc[U], xc[U];
 #pragma unroll
@@ -108,10 +128,10 @@ __device__ __forceinline__ void walk_fwd(const ffn_ray_scan& a, const Cols<T, V>
     if (k + U < len) {
       gp += U * c.gs;
       xp += U * c.xs;
-      load_rows<T, V, U>(g, gp, c.gs, len - k - U);
-      load_rows<T, V, U>(x, xp, c.xs, len - k - U);
+      load_rows<T, V, U>(g, gp, c.gb, len - k - U);
+      load_rows<T, V, U>(x, xp, c.xb, len - k - U);
     }
-    if (a.marks && k % SC_MARK == 0 && (k || mark0)) {
+    if (a.marks && (k || mark0)) {
       float* m = a.marks + (from + k) / SC_MARK * a.channels + c.ch;
 #pragma unroll
       for (int v = 0; v < V; ++v) m[v] = h[v];
@@ -119,14 +139,12 @@ __device__ __forceinline__ void walk_fwd(const ffn_ray_scan& a, const Cols<T, V>
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (k + u < len) {
-        vec out;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float z = sigmoid_f(get<V>(gc[u], v));
-          h[v] = __builtin_fmaf(1.f - z, h[v], z * get<V>(xc[u], v));
-          put<T, V>(out, v, h[v]);
+          const float z = sigmoid_f(get<T, V>(gc[u], v));
+          h[v] = __builtin_fmaf(1.f - z, h[v], z * get<T, V>(xc[u], v));
         }
-        *reinterpret_cast<vec*>(hp) = out;
+        *reinterpret_cast<vec*>(hp) = pack<T, V>(h);
       }
       hp += hs;
     }
@@ -150,9 +168,9 @@ __device__ __forceinline__ void walk_bwd(const ffn_ray_scan& a, const Cols<T, V>
   T* og = (T*)a.dgate + row * a.channels + c.ch;
   T* ox = (T*)a.dx + row * a.channels + c.ch;
   vec g[L], x[L], dh[L];
-  load_rows<T, V, L>(g, gp, c.gs, len - k);
-  load_rows<T, V, L>(x, xp, c.xs, len - k);
-  load_rows<T, V, L>(dh, dp, ds, len - k);
+  load_rows<T, V, L>(g, gp, c.gb, len - k);
+  load_rows<T, V, L>(x, xp, c.xb, len - k);
+  load_rows<T, V, L>(dh, dp, (int)(ds * sizeof(T)), len - k);
   for (; k >= 0; k -= L) {
     const float* m = k || mark0 ? a.marks + (from + k) / L * a.channels + c.ch : start;
     float h[V], z[L][V], q[L][V];
@@ -164,10 +182,13 @@ __device__ __forceinline__ void walk_bwd(const ffn_ray_scan& a, const Cols<T, V>
       dc[u] = dh[u];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float zz = sigmoid_f(get<V>(g[u], v)), keep = 1.f - zz, xx = get<V>(x[u], v);
+        const float zz = sigmoid_f(get<T, V>(g[u], v)), keep = 1.f - zz, xx = get<T, V>(x[u], v);
         z[u][v] = zz;
         q[u][v] = (xx - h[v]) * (zz * keep);
         h[v] = __builtin_fmaf(keep, h[v], zz * xx);
+        // opaque: formed here, before the next piece's rows are asked for (else both pieces' rows are held), and 1 - z
+        // formed again below instead of kept
+        asm volatile("" : "+v"(z[u][v]), "+v"(q[u][v]));
       }
     }
     const int left = len - k;
@@ -175,23 +196,23 @@ __device__ __forceinline__ void walk_bwd(const ffn_ray_scan& a, const Cols<T, V>
     if (k > 0) {
       gp -= L * c.gs, xp -= L * c.xs, dp -= L * ds;
       og -= L * os, ox -= L * os;
-      load_rows<T, V, L>(g, gp, c.gs, L);
-      load_rows<T, V, L>(x, xp, c.xs, L);
-      load_rows<T, V, L>(dh, dp, ds, L);
+      load_rows<T, V, L>(g, gp, c.gb, L);
+      load_rows<T, V, L>(x, xp, c.xb, L);
+      load_rows<T, V, L>(dh, dp, (int)(ds * sizeof(T)), L);
     }
 #pragma unroll
     for (int u = L - 1; u >= 0; --u) {
       if (u < left) {
-        vec vg, vx;
+        float vg[V], vx[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float D = get<V>(dc[u], v) + d[v];
-          put<T, V>(vx, v, z[u][v] * D);
-          put<T, V>(vg, v, q[u][v] * D);
+          const float D = get<T, V>(dc[u], v) + d[v];
+          vx[v] = z[u][v] * D;
+          vg[v] = q[u][v] * D;
           d[v] = (1.f - z[u][v]) * D;
         }
-        *reinterpret_cast<vec*>(wx) = vx;
-        *reinterpret_cast<vec*>(wg) = vg;
+        *reinterpret_cast<vec*>(wx) = pack<T, V>(vx);
+        *reinterpret_cast<vec*>(wg) = pack<T, V>(vg);
       }
       wx -= os, wg -= os;
     }
@@ -253,62 +274,11 @@ __global__ __launch_bounds__(SC_NT) void k_scan_rays(ffn_ray_scan a, int64_t ray
   }
 }
 
-// By parts of `size` places (a multiple of SC_MARK): carry[part][channel] is the state at the part's start (BACK: D at
-// its end).  The blocks past part_blocks give the rays without rows their last state.  Large inputs: parts in falling
-// order, since k_scan_ends has just read the last ones (they are still in the last-level cache).
-template <typename T, int V, bool BACK>
-__global__ __launch_bounds__(SC_NT) void k_scan_parts(ffn_ray_scan a, int size, int64_t parts, int64_t part_blocks,
-                                                      const float* __restrict__ carry) {
-  const int lanes = a.channels / V;
-  if (blockIdx.x >= part_blocks) {
-    const int64_t id = (blockIdx.x - part_blocks) * SC_NT + threadIdx.x, ray = id / lanes;
-    if (ray >= a.rays.num_rays) return;
-    const Span64 s = places_of(a, (uint32_t)ray);
-    if (s.to > s.from) return;
-    const int ch = (int)(id % lanes) * V;
-    float h[V];
-    load_state<V>(h, BACK ? a.dlast : a.h0, ray, a.channels, ch);
-    store_state<V>(BACK ? a.dh0 : a.last, ray, a.channels, ch, h);
-    return;
-  }
-  const int64_t id = (part_blocks - 1 - blockIdx.x) * SC_NT + threadIdx.x;
-  const int64_t part = id / lanes;
-  if (part >= parts) return;
-  const Cols<T, V> c(a, (int)(id % lanes) * V);
-  const int64_t p0 = part * size, p1 = min(p0 + size, (int64_t)a.rays.n);
-  float h[V];
-  int64_t p = BACK ? p1 - 1 : p0;
-  while (BACK ? p >= p0 : p < p1) {
-    Span64 s;
-    const int64_t ray = ray_at(a, c.w, p, s);
-    if (ray < 0) {
-      typename Cols<T, V>::vec zero;
-#pragma unroll
-      for (int v = 0; v < V; ++v) put<T, V>(zero, v, 0.f);
-      const int64_t at = c.w.row(p) * a.channels + c.ch;
-      *reinterpret_cast<typename Cols<T, V>::vec*>((BACK ? (T*)a.dx : (T*)a.h) + at) = zero;
-      if (BACK) *reinterpret_cast<typename Cols<T, V>::vec*>((T*)a.dgate + at) = zero;
-      p += BACK ? -1 : 1;
-      continue;
-    }
-    const int64_t from = max(s.from, p0), to = min(s.to, p1);
-    const int len = (int)(to - from);
-    const bool inside = from > s.from;  // the walk begins inside the ray
-    if constexpr (BACK) {
-      if (to < s.to) load_state<V>(h, carry, part, a.channels, c.ch);
-      else load_state<V>(h, a.dlast, ray, a.channels, c.ch);
-      walk_bwd<T, V>(a, c, from, len, inside, a.h0 ? a.h0 + ray * a.channels + c.ch : nullptr, h);
-      if (!inside) store_state<V>(a.dh0, ray, a.channels, c.ch, h);
-      p = from - 1;
-    } else {
-      if (inside) load_state<V>(h, carry, part, a.channels, c.ch);
-      else load_state<V>(h, a.h0, ray, a.channels, c.ch);
-      walk_fwd<T, V>(a, c, from, len, inside, h);
-      if (to == s.to) store_state<V>(a.last, ray, a.channels, c.ch, h);
-      p = to;
-    }
-  }
-}
+constexpr int GROUP = 64, GR_C = 16;
+// k_scan_ends' and k_scan_groups' results: [parts][channels], [runs][channels]
+struct Ends {
+  float *A, *B, *run_A, *run_B;
+};
 
 // The ray that leaves each part in the direction of the walk: the part's steps of it as h -> A h + B, with A = 0 where
 // the ray begins (BACK: ends) in the part, so that B is the state.  A = B = 0 where none leaves.
@@ -342,8 +312,8 @@ __global__ __launch_bounds__(SC_NT) void k_scan_ends(ffn_ray_scan a, int size, i
     const T* xp = BACK ? (const T*)a.dh + row * a.dh_row + c.ch : c.x + row * a.x_row;
     const int64_t gs = dir * c.gs, xs = BACK ? -c.w.step * a.dh_row : c.xs;
     vec g[U], x[U];
-    load_rows<T, V, U>(g, gp, gs, len);
-    load_rows<T, V, U>(x, xp, xs, len);
+    load_rows<T, V, U>(g, gp, (int)(gs * sizeof(T)), len);
+    load_rows<T, V, U>(x, xp, (int)(xs * sizeof(T)), len);
     for (int k = 0; k < len; k += U) {
       vec gc[U], xc[U];
 #pragma unroll
@@ -351,18 +321,18 @@ __global__ __launch_bounds__(SC_NT) void k_scan_ends(ffn_ray_scan a, int size, i
       if (k + U < len) {
         gp += U * gs;
         xp += U * xs;
-        load_rows<T, V, U>(g, gp, gs, len - k - U);
-        load_rows<T, V, U>(x, xp, xs, len - k - U);
+        load_rows<T, V, U>(g, gp, (int)(gs * sizeof(T)), len - k - U);
+        load_rows<T, V, U>(x, xp, (int)(xs * sizeof(T)), len - k - U);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (k + u < len) {
 #pragma unroll
           for (int v = 0; v < V; ++v) {
-            const float z = sigmoid_f(get<V>(gc[u], v)), keep = 1.f - z;
+            const float z = sigmoid_f(get<T, V>(gc[u], v)), keep = 1.f - z;
             A[v] *= keep;
             // BACK: the D that leaves a step is (1 - z) (dh + D)
-            B[v] = BACK ? keep * (B[v] + get<V>(xc[u], v)) : __builtin_fmaf(keep, B[v], z * get<V>(xc[u], v));
+            B[v] = BACK ? keep * (B[v] + get<T, V>(xc[u], v)) : __builtin_fmaf(keep, B[v], z * get<T, V>(xc[u], v));
           }
         }
     }
@@ -374,39 +344,106 @@ __global__ __launch_bounds__(SC_NT) void k_scan_ends(ffn_ray_scan a, int size, i
   }
 }
 
-// carry[j]: what enters part j (BACK: from the part after it).  A block a channel: a thread composes its run of parts, the
-// runs are scanned in LDS, and the thread walks its run again.
-constexpr int CH_NT = 1024;
+// Runs of GROUP parts, in the order of the walk: what the parts before each one in its run make of a state, in place, and
+// what the whole run makes of it.  A block takes a run and 16 channels (a cache line of the parts' rows).
 template <bool BACK>
-__global__ __launch_bounds__(CH_NT) void k_scan_chain(int channels, int64_t parts, const float* __restrict__ A_of,
-                                                      const float* __restrict__ B_of, float* __restrict__ carry) {
-  __shared__ float sa[CH_NT], sb[CH_NT];
-  const int ch = blockIdx.x, tid = threadIdx.x;
-  const int64_t run = (parts + CH_NT - 1) / CH_NT, j0 = min(tid * run, parts), j1 = min(j0 + run, parts);
-  auto at = [&](int64_t j) { return (BACK ? parts - 1 - j : j) * channels + ch; };
-  float A = 1.f, B = 0.f;
-  for (int64_t j = j0; j < j1; ++j) {
-    const float a = A_of[at(j)], b = B_of[at(j)];
-    A *= a;
-    B = __builtin_fmaf(a, B, b);
-  }
-  sa[tid] = A;
-  sb[tid] = B;
+__global__ __launch_bounds__(GR_C * GROUP) void k_scan_groups(int channels, int64_t parts, float* __restrict__ A_of,
+                                                              float* __restrict__ B_of, float* __restrict__ run_A,
+                                                              float* __restrict__ run_B) {
+  __shared__ float sa[GROUP][GR_C], sb[GROUP][GR_C];
+  const int c = threadIdx.x % GR_C, t = threadIdx.x / GR_C, ch = blockIdx.y * GR_C + c;
+  const int64_t j = (int64_t)blockIdx.x * GROUP + t, at = (BACK ? parts - 1 - j : j) * channels + ch;
+  const bool there = j < parts && ch < channels;
+  float A = there ? A_of[at] : 1.f, B = there ? B_of[at] : 0.f;
+  sa[t][c] = A;
+  sb[t][c] = B;
   __syncthreads();
-  for (int d = 1; d < CH_NT; d *= 2) {
+  for (int d = 1; d < GROUP; d *= 2) {
     float a = 1.f, b = 0.f;
-    if (tid >= d) a = sa[tid - d], b = sb[tid - d];
+    if (t >= d) a = sa[t - d][c], b = sb[t - d][c];
     __syncthreads();
     B = __builtin_fmaf(A, b, B);
     A *= a;
-    sa[tid] = A;
-    sb[tid] = B;
+    sa[t][c] = A;
+    sb[t][c] = B;
     __syncthreads();
   }
-  float h = tid ? sb[tid - 1] : 0.f;
-  for (int64_t j = j0; j < j1; ++j) {
-    carry[at(j)] = h;
-    h = __builtin_fmaf(A_of[at(j)], h, B_of[at(j)]);
+  if (!there) return;
+  A_of[at] = t ? sa[t - 1][c] : 1.f;
+  B_of[at] = t ? sb[t - 1][c] : 0.f;
+  if (t == GROUP - 1 || j == parts - 1) {
+    run_A[(int64_t)blockIdx.x * channels + ch] = A;
+    run_B[(int64_t)blockIdx.x * channels + ch] = B;
+  }
+}
+
+// What enters part j inside a ray whose walk began in part j0: the runs since then, then the parts of j's own run.
+template <int V, bool BACK>
+__device__ __forceinline__ void enter(float (&h)[V], const Ends& e, int64_t parts, int64_t j, int64_t j0, int channels,
+                                      int ch) {
+  const int64_t r0 = (BACK ? parts - 1 - j0 : j0) / GROUP, r1 = (BACK ? parts - 1 - j : j) / GROUP;
+#pragma unroll
+  for (int v = 0; v < V; ++v) h[v] = 0.f;  // the run in which the walk began forgets it
+#pragma unroll 4
+  for (int64_t r = r0; r < r1; ++r)
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      h[v] = __builtin_fmaf(e.run_A[r * channels + ch + v], h[v], e.run_B[r * channels + ch + v]);
+#pragma unroll
+  for (int v = 0; v < V; ++v) h[v] = __builtin_fmaf(e.A[j * channels + ch + v], h[v], e.B[j * channels + ch + v]);
+}
+
+// By parts of `size` places (a multiple of SC_MARK).  The blocks past part_blocks give the rays without rows their last state.  Large inputs: parts in falling
+// order, since k_scan_ends has just read the last ones (they are still in the last-level cache).
+template <typename T, int V, bool BACK>
+__global__ __launch_bounds__(SC_NT) void k_scan_parts(ffn_ray_scan a, int size, int64_t parts, int64_t part_blocks,
+                                                      Ends e) {
+  const int lanes = a.channels / V;
+  if (blockIdx.x >= part_blocks) {
+    const int64_t id = (blockIdx.x - part_blocks) * SC_NT + threadIdx.x, ray = id / lanes;
+    if (ray >= a.rays.num_rays) return;
+    const Span64 s = places_of(a, (uint32_t)ray);
+    if (s.to > s.from) return;
+    const int ch = (int)(id % lanes) * V;
+    float h[V];
+    load_state<V>(h, BACK ? a.dlast : a.h0, ray, a.channels, ch);
+    store_state<V>(BACK ? a.dh0 : a.last, ray, a.channels, ch, h);
+    return;
+  }
+  const int64_t id = (part_blocks - 1 - blockIdx.x) * SC_NT + threadIdx.x;
+  const int64_t part = id / lanes;
+  if (part >= parts) return;
+  const Cols<T, V> c(a, (int)(id % lanes) * V);
+  const int64_t p0 = part * size, p1 = min(p0 + size, (int64_t)a.rays.n);
+  float h[V];
+  int64_t p = BACK ? p1 - 1 : p0;
+  while (BACK ? p >= p0 : p < p1) {
+    Span64 s;
+    const int64_t ray = ray_at(a, c.w, p, s);
+    if (ray < 0) {
+      const typename Cols<T, V>::vec zero{};
+      const int64_t at = c.w.row(p) * a.channels + c.ch;
+      *reinterpret_cast<typename Cols<T, V>::vec*>((BACK ? (T*)a.dx : (T*)a.h) + at) = zero;
+      if (BACK) *reinterpret_cast<typename Cols<T, V>::vec*>((T*)a.dgate + at) = zero;
+      p += BACK ? -1 : 1;
+      continue;
+    }
+    const int64_t from = max(s.from, p0), to = min(s.to, p1);
+    const int len = (int)(to - from);
+    const bool inside = from > s.from;  // the walk begins inside the ray
+    if constexpr (BACK) {
+      if (to < s.to) enter<V, true>(h, e, parts, part, (s.to - 1) / size, a.channels, c.ch);
+      else load_state<V>(h, a.dlast, ray, a.channels, c.ch);
+      walk_bwd<T, V>(a, c, from, len, inside, a.h0 ? a.h0 + ray * a.channels + c.ch : nullptr, h);
+      if (!inside) store_state<V>(a.dh0, ray, a.channels, c.ch, h);
+      p = from - 1;
+    } else {
+      if (inside) enter<V, false>(h, e, parts, part, s.from / size, a.channels, c.ch);
+      else load_state<V>(h, a.h0, ray, a.channels, c.ch);
+      walk_fwd<T, V>(a, c, from, len, inside, h);
+      if (to == s.to) store_state<V>(a.last, ray, a.channels, c.ch, h);
+      p = to;
+    }
   }
 }
 
@@ -414,18 +451,22 @@ static bool aligned(const void* p, int64_t row, int bytes, int size) {
   return ((uintptr_t)p | (uintptr_t)(row * size)) % bytes == 0;
 }
 
-// Which walk: by rays where they are many and short.  PLAN_THREADS: threads (of channels / 2 lanes a ray or part) that
-// fill the GPU.
-constexpr int64_t SC_THREADS = 262144;
+// Which walk.  By rays, the longest one is the least that a call takes (about 0.1 us a row); that is hidden where there
+// are rays for several rounds of threads, and short where there are few rows.  By parts it takes two more launches and a
+// second read of what crosses parts.  196,000 samples of 5003 rays, 37 channels: 97 us by rays, 45 by parts; 4.6 million
+// samples of 2^18 rays, 64 channels: 418 and 590; 1000 samples of 64 rays: 8 and 33.
+constexpr int64_t SC_THREADS = 262144;  // threads at work at once
+static int64_t words_a_row(const ffn_ray_scan& a) {  // of 4 bytes: threads a ray or part
+  return a.dtype == FFN_F32 ? a.channels : (a.channels + 1) / 2;
+}
 static bool by_rays(const ffn_ray_scan& a) {
-  const int64_t lanes = (a.channels + 1) / 2, avg = a.rays.num_rays ? (int64_t)a.rays.n / a.rays.num_rays : 0;
-  return avg <= 64 || (avg <= 512 && a.rays.num_rays * lanes >= SC_THREADS / 2);
+  if (a.rays.n <= 4096) return (int64_t)a.rays.n <= 64 * (int64_t)a.rays.num_rays;
+  return a.rays.num_rays * words_a_row(a) >= 4 * SC_THREADS && a.rays.n <= 256 * (int64_t)a.rays.num_rays;
 }
 static int part_size(const ffn_ray_scan& a) {
-  const int64_t lanes = (a.channels + 1) / 2;
-  int64_t s = (int64_t)a.rays.n * lanes / SC_THREADS;
+  int64_t s = (int64_t)a.rays.n * words_a_row(a) / SC_THREADS;
   s = (s + SC_MARK - 1) / SC_MARK * SC_MARK;
-  return (int)(s < 64 ? 64 : s > 4096 ? 4096 : s);
+  return (int)(s < 32 ? 32 : s > 4096 ? 4096 : s);
 }
 
 template <typename T, int V, bool BACK>
@@ -437,12 +478,16 @@ static hipError_t run(const ffn_ray_scan& a, hipStream_t st) {
     return hipGetLastError();
   }
   const int size = part_size(a);
-  const int64_t parts = ((int64_t)a.rays.n + size - 1) / size, states = parts * a.channels;
-  float *A = (float*)a.workspace, *B = A + states, *carry = B + states;
+  const int64_t parts = ((int64_t)a.rays.n + size - 1) / size, runs = (parts + GROUP - 1) / GROUP;
+  float* w = (float*)a.workspace;
+  const Ends e{w, w + parts * a.channels, w + 2 * parts * a.channels, w + (2 * parts + runs) * a.channels};
   const int64_t pb = (parts * lanes + SC_NT - 1) / SC_NT, rb = (a.rays.num_rays * lanes + SC_NT - 1) / SC_NT;
-  k_scan_ends<T, V, BACK><<<(unsigned)pb, SC_NT, 0, st>>>(a, size, parts, A, B);
-  k_scan_chain<BACK><<<a.channels, CH_NT, 0, st>>>(a.channels, parts, A, B, carry);
-  k_scan_parts<T, V, BACK><<<(unsigned)(pb + rb), SC_NT, 0, st>>>(a, size, parts, pb, carry);
+  if (parts) {
+    k_scan_ends<T, V, BACK><<<(unsigned)pb, SC_NT, 0, st>>>(a, size, parts, e.A, e.B);
+    k_scan_groups<BACK><<<dim3((unsigned)runs, (a.channels + GR_C - 1) / GR_C), GR_C * GROUP, 0, st>>>(
+        a.channels, parts, e.A, e.B, e.run_A, e.run_B);
+  }
+  if (pb + rb) k_scan_parts<T, V, BACK><<<(unsigned)(pb + rb), SC_NT, 0, st>>>(a, size, parts, pb, e);
   return hipGetLastError();
 }
 
@@ -465,12 +510,14 @@ uint64_t scan_marks(const ffn_ray_scan& a) {
 uint64_t scan_workspace(const ffn_ray_scan& a, bool) {
   if (by_rays(a)) return 0;
   const int size = part_size(a);
-  return ((uint64_t)a.rays.n + size - 1) / size * a.channels * 3 * sizeof(float);
+  const uint64_t parts = ((uint64_t)a.rays.n + size - 1) / size, runs = (parts + GROUP - 1) / GROUP;
+  return 2 * (parts + runs) * a.channels * sizeof(float);
 }
 
 template <typename T>
 static hipError_t by_direction(const ffn_ray_scan& a, bool backward, hipStream_t st) {
-  return backward ? by_width<T, 2, true>(a, st) : by_width<T, sizeof(T) == 4 ? 2 : 4, false>(a, st);
+  constexpr int V = 4 / (int)sizeof(T);  // 4 bytes a lane: with 8 the forward of 2^18 rays takes 524 us instead of 418
+  return backward ? by_width<T, V, true>(a, st) : by_width<T, V, false>(a, st);
 }
 
 hipError_t launch_scan(const ffn_ray_scan& a, bool backward, hipStream_t st) {

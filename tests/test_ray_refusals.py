@@ -66,7 +66,7 @@ def _scan(**kw):
 
 @pytest.mark.parametrize("kw,match", [
     (dict(dtype=-1), "dtype=-1"), (dict(channels=0), "channels=0"), (dict(channels=65537), "channels=65537"),
-    (dict(reverse=2), "reverse=2"), (dict(x=None), "NULL buffer"), (dict(gate=P + 1), "misaligned"),
+    (dict(reverse=2), "reverse=2"), (dict(x_row=(1 << 25) + 1), "bytes apart"), (dict(x=None), "NULL buffer"), (dict(gate=P + 1), "misaligned"),
     (dict(rays=fl.FfnRaySet(num_rays=4, n=64, ray_ids=P)), "NULL counts"),
     (dict(rays=fl.FfnRaySet(counts=P, offsets=P, num_rays=4, n=64)), "NULL ray_ids"),
 ])
