@@ -168,9 +168,9 @@ __global__ __launch_bounds__(PL_NT) void k_plan_move(const int32_t* __restrict__
     }
     const uint32_t before = cnt[wave][bin[q]];
     rank[q] = before + (uint32_t)__popcll(same & below);
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     if (there && (same & below) == 0ull) cnt[wave][bin[q]] = before + (uint32_t)__popcll(same);
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
   }
   __syncthreads();
   for (int b = tid; b < v.bins; b += PL_NT) {
@@ -214,113 +214,139 @@ hipError_t launch_expert_plan(const int32_t* ids, uint32_t n, int experts, uint3
 // ---------------------------------------------------------------------------
 // The products.
 
-constexpr int EX_NT = 256, EX_W = 64;  // W_e goes through LDS in tiles of 64 x 64
+constexpr int EX_NT = 256, EX_K = 64;  // the products' sums go in steps of 64
 
-// W[r0 .. r0 + 63][c0 .. c0 + 63] to LDS, 0 past the matrix.  PERM: row m = 8 g + j of each 32 goes where col_frag reads
-// slot j of lane group g, so that the K order is that of the other operand's 16-byte loads.
-template <typename T, bool PERM>
-__device__ __forceinline__ void stage_w(T* tile, const T* __restrict__ W, int rows, int cols, int r0, int c0) {
-  constexpr int EL = 16 / (int)sizeof(T), CPR = EX_W / EL;
+// One step's part of W_e on its way to LDS: R x C values from [r0][c0], 0 past the matrix.  PERM: row m = 8 g + j of each
+// 32 goes where col_frag reads slot j of lane group g, so that the K order is that of the other operand's 16-byte loads.
+template <typename T, int R, int C, bool PERM>
+struct StageW {
+  static constexpr int EL = 16 / (int)sizeof(T), CPR = C / EL, N = R * CPR / EX_NT;
+  uint4 v[N];
+  __device__ __forceinline__ void load(const T* __restrict__ W, int rows, int cols, int r0, int c0) {
 #pragma unroll
-  for (int i = 0; i < EX_W * CPR / EX_NT; ++i) {
-    const int c = threadIdx.x + i * EX_NT, row = c / CPR, col = (c % CPR) * EL;
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (r0 + row < rows && c0 + col < cols) v = *reinterpret_cast<const uint4*>(W + (int64_t)(r0 + row) * cols + c0 + col);
-    int to = row;
-    if (PERM) {
-      const int g = (row & 31) >> 3, j = row & 7;
-      to = (row & 32) + (j < 4 ? 4 * g + j : 16 + 4 * g + j - 4);
+    for (int i = 0; i < N; ++i) {
+      const int c = threadIdx.x + i * EX_NT, row = r0 + c / CPR, col = c0 + (c % CPR) * EL;
+      v[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < rows && col < cols) v[i] = *reinterpret_cast<const uint4*>(W + (int64_t)row * cols + col);
     }
-    *reinterpret_cast<uint4*>(tile + to * lds_row<T, EX_W> + col) = v;
   }
-}
-
-template <typename T>
-__device__ __forceinline__ typename Mat<T>::frag zero_frag() {
-  typename Mat<T>::frag f;
+  __device__ __forceinline__ void store(T* tile) const {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = (T)0.f;
-  return f;
+    for (int i = 0; i < N; ++i) {
+      const int c = threadIdx.x + i * EX_NT, row = c / CPR;
+      int to = row;
+      if (PERM) {
+        const int g = (row & 31) >> 3, j = row & 7;
+        to = (row & ~31) + (j < 4 ? 4 * g + j : 16 + 4 * g + j - 4);
+      }
+      *reinterpret_cast<uint4*>(tile + to * lds_row<T, C> + (c % CPR) * EL) = v[i];
+    }
+  }
+};
+
+// keeps the values whose y is positive
+template <typename V>
+__device__ __forceinline__ V where_positive(V g, const V& y) {
+  constexpr int N = sizeof(V) / sizeof(g[0]);
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (!((float)y[j] > 0.f)) g[j] = 0;
+  return g;
 }
 
-// BACK = false: y = act(x W_e^T + b_e);  true: dx = (dy where y > 0) W_e.  128 slots by 64 columns a block, 32 slots a
-// wavefront: the product is formed transposed (slots along the lanes), so a lane's rows of x come by 16-byte loads
-// straight into the operand and its four values of a result row go out by one store.
-template <typename T, bool BACK>
-__global__ __launch_bounds__(EX_NT) void k_expert(ffn_experts a, PlanView v, int64_t total, int col_tiles) {
-  __shared__ T ws[EX_W * lds_row<T, EX_W>];
+// BACK = false: y = act(x W_e^T + b_e);  true: dx = (dy where y > 0) W_e.  128 slots by 16 NB columns a block, 32 slots a
+// wavefront.  The product is formed transposed (slots along the lanes), so that a lane's rows come by 16-byte loads
+// straight into the operand; W_e goes through LDS.  Results turn in LDS, so that rows go out whole: stored from the
+// product's own layout (8 bytes a lane, 32 in a row) a write-bound layer takes nearly twice as long.
+template <typename T, bool BACK, int NB>
+__global__ __launch_bounds__(EX_NT, 2) void k_expert(ffn_experts a, PlanView v, int64_t total, int col_tiles) {
+  typedef typename Mat<T>::frag frag;
+  constexpr int C = 16 * NB, EL = 16 / (int)sizeof(T);
+  constexpr int W_SIZE = BACK ? EX_K * lds_row<T, C> : C * lds_row<T, EX_K>, OUT_SIZE = 4 * 16 * lds_row<T, C>;
+  __shared__ __align__(16) T lds[W_SIZE > OUT_SIZE ? W_SIZE : OUT_SIZE];
   const int64_t per = (total + 7) / 8, work = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if (work >= total) return;
   const uint2 tile = reinterpret_cast<const uint2*>(a.plan + v.tiles)[work / col_tiles];
   if (tile.x >= (uint32_t)v.bins) return;
-  const int col0 = (int)(work % col_tiles) * EX_W;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
-  const uint32_t first = a.plan[v.offsets + tile.x] + tile.y * EX_ROWS, end = a.plan[v.offsets + tile.x] + a.plan[v.counts + tile.x];
+  const int col0 = (int)(work % col_tiles) * C;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+  const uint32_t off = a.plan[v.offsets + tile.x], first = off + tile.y * EX_ROWS, end = off + a.plan[v.counts + tile.x];
   const bool none = tile.x == (uint32_t)v.bins - 1;
   const int depth = BACK ? a.out : a.in, width = BACK ? a.in : a.out;
-  int64_t xr[2], yr[2];
+  const bool in_slots = a.flags & (BACK ? FFN_EXPERTS_Y_SLOTS : FFN_EXPERTS_X_SLOTS);
+  const bool out_slots = a.flags & (BACK ? FFN_EXPERTS_X_SLOTS : FFN_EXPERTS_Y_SLOTS);
+  uint32_t slot[2], row[2];
   bool there[2];
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
-    const uint32_t slot = first + wave * 32 + s * 16 + c;
-    there[s] = slot < end;
-    const int64_t row = there[s] ? a.plan[v.rows + slot] : 0;
-    xr[s] = a.flags & FFN_EXPERTS_X_SLOTS ? (int64_t)slot : row;
-    yr[s] = a.flags & FFN_EXPERTS_Y_SLOTS ? (int64_t)slot : row;
+    slot[s] = first + wave * 32 + s * 16 + c;
+    there[s] = slot[s] < end;
+    row[s] = there[s] ? a.plan[v.rows + slot[s]] : 0u;
   }
-  f32x4 acc[4][2];
+  f32x4 acc[NB][2];
 #pragma unroll
-  for (int b = 0; b < 4; ++b) acc[b][0] = acc[b][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int b = 0; b < NB; ++b) acc[b][0] = acc[b][1] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (!none) {
     const T* W = (const T*)a.W + (int64_t)tile.x * a.out * a.in;
-    for (int k0 = 0; k0 < depth; k0 += EX_W) {
-      if (BACK) stage_w<T, true>(ws, W, a.out, a.in, k0, col0);
-      else stage_w<T, false>(ws, W, a.out, a.in, col0, k0);
-      typename Mat<T>::frag f[2][2];
+    StageW<T, BACK ? EX_K : C, BACK ? C : EX_K, BACK> w;
+    const T* in[2];
+    const T* gate[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int64_t r = in_slots ? slot[s] : row[s];
+      in[s] = (BACK ? (const T*)a.dy + r * a.dy_row : (const T*)a.x + r * a.x_row) + 8 * g;
+      gate[s] = BACK ? (const T*)a.y + r * a.out + 8 * g : nullptr;
+    }
+    frag f[2][2];
+    auto fetch = [&](int k0) {
+      if (BACK) w.load(W, a.out, a.in, k0, col0);
+      else w.load(W, a.out, a.in, col0, k0);
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-          const int col = k0 + 32 * ks + 8 * g;
-          f[s][ks] = zero_frag<T>();
-          if (there[s] && col < depth) {
-            if constexpr (BACK) {
-              f[s][ks] = *reinterpret_cast<const typename Mat<T>::frag*>((const T*)a.dy + yr[s] * a.dy_row + col);
-              if (a.relu) {
-                const typename Mat<T>::frag y = *reinterpret_cast<const typename Mat<T>::frag*>((const T*)a.y + yr[s] * a.out + col);
+          const int k = k0 + 32 * ks;
+          frag x;
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  if (!((float)y[j] > 0.f)) f[s][ks][j] = (T)0.f;
-              }
-            } else {
-              f[s][ks] = *reinterpret_cast<const typename Mat<T>::frag*>((const T*)a.x + xr[s] * a.x_row + col);
-            }
+          for (int j = 0; j < 8; ++j) x[j] = (T)0.f;
+          if (there[s] && k + 8 * g < depth) {
+            x = *reinterpret_cast<const frag*>(in[s] + k);
+            if (BACK && a.relu) x = where_positive(x, *reinterpret_cast<const frag*>(gate[s] + k));
           }
+          f[s][ks] = x;
         }
+    };
+    fetch(0);
+    for (int k0 = 0; k0 < depth; k0 += EX_K) {
+      w.store(lds);
+      frag x[2][2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) x[s][0] = f[s][0], x[s][1] = f[s][1];
       __syncthreads();
+      if (k0 + EX_K < depth) fetch(k0 + EX_K);
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
+      for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          typename Mat<T>::frag w;
-          if constexpr (BACK) w = col_frag<T, EX_W>(ws, 32 * ks, 16 * b, lane);
-          else w = row_frag<T, EX_W>(ws, 16 * b + c, ks, lane);
+        for (int b = 0; b < NB; ++b) {
+          const frag m = BACK ? col_frag<T, C>(lds, 32 * ks, 16 * b, lane) : row_frag<T, EX_K>(lds, 16 * b + c, ks, lane);
 #pragma unroll
-          for (int s = 0; s < 2; ++s) acc[b][s] = Mat<T>::mma(w, f[s][ks], acc[b][s]);
+          for (int s = 0; s < 2; ++s) acc[b][s] = Mat<T>::mma(m, x[s][ks], acc[b][s]);
         }
       __syncthreads();
     }
   }
+  // 16 rows of the wavefront at a time; no other wavefront touches its part of the LDS
+  T* turn = lds + wave * 16 * lds_row<T, C>;
+  const int cols = min(width - col0, C);
+  T* out = (BACK ? (T*)a.dx : (T*)a.y) + col0;
 #pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    const int col = col0 + 16 * b + 4 * g;
-    if (col >= width) continue;
-    f32x4 bias = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (!BACK && a.b && !none)
-      bias = __builtin_convertvector(*reinterpret_cast<const typename Mat<T>::quad*>((const T*)a.b + (int64_t)tile.x * a.out + col), f32x4);
+  for (int s = 0; s < 2; ++s) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      if (!there[s]) continue;
+    for (int b = 0; b < NB; ++b) {
+      const int col = 16 * b + 4 * g;
+      f32x4 bias = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (!BACK && a.b && !none && col < cols)
+        bias = __builtin_convertvector(*reinterpret_cast<const typename Mat<T>::quad*>((const T*)a.b + (int64_t)tile.x * a.out + col0 + col), f32x4);
       typename Mat<T>::quad q;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -328,75 +354,123 @@ __global__ __launch_bounds__(EX_NT) void k_expert(ffn_experts a, PlanView v, int
         if (!BACK && a.relu) val = val < 0.f ? 0.f : val;  // a NaN stays one
         q[r] = (T)val;
       }
-      T* to = BACK ? (T*)a.dx + xr[s] * a.in : (T*)a.y + yr[s] * a.out;
-      *reinterpret_cast<typename Mat<T>::quad*>(to + col) = q;
+      *reinterpret_cast<typename Mat<T>::quad*>(turn + c * lds_row<T, C> + col) = q;
     }
+    wave_sync();
+    const uint32_t to = out_slots ? slot[s] : row[s];
+#pragma unroll
+    for (int i = 0; i < 16 * C / EL / 64; ++i) {
+      const int at = i * 64 + lane, r = at / (C / EL), col = at % (C / EL) * EL;
+      const uint32_t dest = __shfl(to, r);  // of lane r: row r of the 16
+      const bool live = first + wave * 32 + s * 16 + r < end;
+      if (live && col < cols)
+        *reinterpret_cast<uint4*>(out + (int64_t)dest * width + col) = *reinterpret_cast<const uint4*>(turn + r * lds_row<T, C> + col);
+    }
+    wave_sync();
   }
 }
 
-// Sum over a chunk of an expert's slots of g^T x: 64 x 64 values a block, 32 x 32 a wavefront.  The slots are the K of
-// the product, so both operands are columns of their LDS tiles.  g against ones gives db's share.
-template <typename T>
-__global__ __launch_bounds__(EX_NT) void k_expert_dw(ffn_experts a, PlanView v, int64_t total, int m_tiles, int k_tiles) {
-  constexpr int EL = 16 / (int)sizeof(T), CPR = EX_W / EL, N = EX_W * CPR / EX_NT;
-  __shared__ T gs[EX_W * lds_row<T, EX_W>], xs[EX_W * lds_row<T, EX_W>];
+// Sum over `merge` chunks of an expert's slots of g^T x, g = dy where y > 0: TM x TK values a block in four
+// wavefronts.  The slots are the K of the product, so both operands are columns of their LDS tiles.  g against ones gives
+// db's share.
+template <typename T, int TM, int TK>
+__global__ __launch_bounds__(EX_NT) void k_expert_dw(ffn_experts a, PlanView v, int64_t total, int m_tiles, int k_tiles,
+                                                     int merge) {
+  typedef typename Mat<T>::frag frag;
+  constexpr int EL = 16 / (int)sizeof(T), S = 64;  // slots of a step
+  constexpr int GC = TM / EL, XC = TK / EL, NG = S * GC / EX_NT, NX = S * XC / EX_NT, NM = TM / 32, NK = TK / 32;
+  __shared__ __align__(16) T gs[S * lds_row<T, TM>];
+  __shared__ __align__(16) T xs[S * lds_row<T, TK>];
   const int64_t per = (total + 7) / 8, work = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if (work >= total) return;
   const int64_t piece = work / (m_tiles * k_tiles);
   const uint2 chunk = reinterpret_cast<const uint2*>(a.plan + v.chunks)[piece];
-  if (chunk.x >= (uint32_t)v.bins - 1) return;
-  const int k0 = (int)(work % k_tiles) * EX_W, m0 = (int)(work / k_tiles % m_tiles) * EX_W;
+  if (chunk.x >= (uint32_t)v.bins - 1 || chunk.y % merge) return;
+  const int k0 = (int)(work % k_tiles) * TK, m0 = (int)(work / k_tiles % m_tiles) * TM;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
-  const int mw = (wave >> 1) * 32, kw = (wave & 1) * 32;
+  const int mw = (wave >> 1) * (TM / 2), kw = (wave & 1) * (TK / 2);
   const uint32_t off = a.plan[v.offsets + chunk.x], group = a.plan[v.counts + chunk.x];
-  const uint32_t from = chunk.y * v.chunk, to = min(group, from + v.chunk);
-  f32x4 acc[2][2], sum[2];
+  const uint32_t from = off + chunk.y * v.chunk, to = off + min(group, (chunk.y + merge) * v.chunk);
+  typedef T vec __attribute__((ext_vector_type(EL)));
+  vec gv[NG], yv[NG], xv[NX];
+  const bool x_slots = a.flags & FFN_EXPERTS_X_SLOTS, y_slots = a.flags & FFN_EXPERTS_Y_SLOTS;
+  uint32_t gr[NG], xr[NX];  // the rows of the next step
+  auto rows = [&](uint32_t s0) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) acc[i][0] = acc[i][1] = sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  typename Mat<T>::frag ones;
+    for (int i = 0; i < NG; ++i) {
+      const uint32_t slot = s0 + (tid + i * EX_NT) / GC;
+      gr[i] = slot < to ? (y_slots ? slot : a.plan[v.rows + slot]) : 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < NX; ++i) {
+      const uint32_t slot = s0 + (tid + i * EX_NT) / XC;
+      xr[i] = slot < to ? (x_slots ? slot : a.plan[v.rows + slot]) : 0u;
+    }
+  };
+  auto fetch = [&](uint32_t s0) {
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const int ch = tid + i * EX_NT, col = m0 + ch % GC * EL;
+#pragma unroll
+      for (int j = 0; j < EL; ++j) gv[i][j] = (T)0.f;
+      if (s0 + ch / GC < to && col < a.out) {
+        gv[i] = *reinterpret_cast<const vec*>((const T*)a.dy + gr[i] * a.dy_row + col);
+        if (a.relu) yv[i] = *reinterpret_cast<const vec*>((const T*)a.y + (int64_t)gr[i] * a.out + col);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NX; ++i) {
+      const int ch = tid + i * EX_NT, col = k0 + ch % XC * EL;
+#pragma unroll
+      for (int j = 0; j < EL; ++j) xv[i][j] = (T)0.f;
+      if (s0 + ch / XC < to && col < a.in) xv[i] = *reinterpret_cast<const vec*>((const T*)a.x + xr[i] * a.x_row + col);
+    }
+  };
+  f32x4 acc[NM][NK], sum[NM];
+#pragma unroll
+  for (int i = 0; i < NM; ++i) {
+    sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NK; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const bool sums = k0 == 0 && kw == 0;
+  frag ones;
 #pragma unroll
   for (int j = 0; j < 8; ++j) ones[j] = (T)1.f;
-  for (uint32_t s0 = from; s0 < to; s0 += EX_W) {
+  rows(from);
+  fetch(from);
+  rows(from + S);
+  for (uint32_t s0 = from; s0 < to; s0 += S) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int ch = tid + i * EX_NT, row = ch / CPR, col = (ch % CPR) * EL;
-      uint4 gv = make_uint4(0u, 0u, 0u, 0u), xv = gv;
-      if (s0 + row < to) {
-        const uint32_t slot = off + s0 + row;
-        const int64_t r = a.plan[v.rows + slot];
-        const int64_t xr = a.flags & FFN_EXPERTS_X_SLOTS ? (int64_t)slot : r, yr = a.flags & FFN_EXPERTS_Y_SLOTS ? (int64_t)slot : r;
-        if (k0 + col < a.in) xv = *reinterpret_cast<const uint4*>((const T*)a.x + xr * a.x_row + k0 + col);
-        if (m0 + col < a.out) {
-          gv = *reinterpret_cast<const uint4*>((const T*)a.dy + yr * a.dy_row + m0 + col);
-          if (a.relu) {
-            const uint4 yv = *reinterpret_cast<const uint4*>((const T*)a.y + yr * a.out + m0 + col);
-            typedef T vec __attribute__((ext_vector_type(EL)));
-            vec gg = __builtin_bit_cast(vec, gv);
-            const vec yy = __builtin_bit_cast(vec, yv);
+    for (int i = 0; i < NG; ++i) {
+      const int ch = tid + i * EX_NT;
+      if (a.relu) gv[i] = where_positive(gv[i], yv[i]);
+      *reinterpret_cast<vec*>(gs + ch / GC * lds_row<T, TM> + ch % GC * EL) = gv[i];
+    }
 #pragma unroll
-            for (int j = 0; j < EL; ++j)
-              if (!((float)yy[j] > 0.f)) gg[j] = (T)0.f;
-            gv = __builtin_bit_cast(uint4, gg);
-          }
-        }
-      }
-      *reinterpret_cast<uint4*>(gs + row * lds_row<T, EX_W> + col) = gv;
-      *reinterpret_cast<uint4*>(xs + row * lds_row<T, EX_W> + col) = xv;
+    for (int i = 0; i < NX; ++i) {
+      const int ch = tid + i * EX_NT;
+      *reinterpret_cast<vec*>(xs + ch / XC * lds_row<T, TK> + ch % XC * EL) = xv[i];
     }
     __syncthreads();
+    if (to - s0 > S) {
+      fetch(s0 + S);
+      rows(s0 + 2 * S);
+    }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      typename Mat<T>::frag gf[2], xf[2];
+    for (int h = 0; h < S / 32; ++h) {
+      frag gf[NM];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        gf[i] = col_frag<T, EX_W>(gs, 32 * h, mw + 16 * i, lane);
-        xf[i] = col_frag<T, EX_W>(xs, 32 * h, kw + 16 * i, lane);
+      for (int i = 0; i < NM; ++i) gf[i] = col_frag<T, TM>(gs, 32 * h, mw + 16 * i, lane);
+#pragma unroll
+      for (int j = 0; j < NK; ++j) {
+        const frag xf = col_frag<T, TK>(xs, 32 * h, kw + 16 * j, lane);
+#pragma unroll
+        for (int i = 0; i < NM; ++i) acc[i][j] = Mat<T>::mma(gf[i], xf, acc[i][j]);
       }
+      if (sums) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = Mat<T>::mma(gf[i], xf[j], acc[i][j]);
-        sum[i] = Mat<T>::mma(gf[i], ones, sum[i]);
+        for (int i = 0; i < NM; ++i) sum[i] = Mat<T>::mma(gf[i], ones, sum[i]);
       }
     }
     __syncthreads();
@@ -404,22 +478,22 @@ __global__ __launch_bounds__(EX_NT) void k_expert_dw(ffn_experts a, PlanView v, 
   const int64_t size = (int64_t)a.out * a.in + a.out;
   float* part = (float*)a.workspace + piece * size;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < NM; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int m = m0 + mw + 16 * i + 4 * g + r;
       if (m >= a.out) continue;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < NK; ++j) {
         const int k = k0 + kw + 16 * j + c;
         if (k < a.in) part[(int64_t)m * a.in + k] = acc[i][j][r];
       }
-      if (k0 == 0 && kw == 0 && c == 0) part[(int64_t)a.out * a.in + m] = sum[i][r];
+      if (sums && c == 0) part[(int64_t)a.out * a.in + m] = sum[i][r];
     }
 }
 
 // dW and db: the partials of an expert's chunks, in order
-__global__ __launch_bounds__(EX_NT) void k_expert_join(ffn_experts a, PlanView v) {
+__global__ __launch_bounds__(EX_NT) void k_expert_join(ffn_experts a, PlanView v, int merge) {
   const int64_t mk = (int64_t)a.out * a.in, size = mk + a.out;
   const int64_t at = (int64_t)blockIdx.x * EX_NT + threadIdx.x;
   if (at >= size) return;
@@ -427,7 +501,7 @@ __global__ __launch_bounds__(EX_NT) void k_expert_join(ffn_experts a, PlanView v
   const uint32_t first = a.plan[v.chunk_first + e], last = a.plan[v.chunk_first + e + 1];
   const float* part = (const float*)a.workspace;
   float s = 0.f;
-  for (uint32_t p = first; p < last; ++p) s += part[p * size + at];
+  for (uint32_t p = first; p < last; p += merge) s += part[p * size + at];
   if (at < mk) {
     if (a.dW) a.dW[e * mk + at] = s;
   } else if (a.db) {
@@ -440,23 +514,45 @@ uint64_t expert_workspace(const ffn_experts& a) {
   return plan_view(a.n, a.n_experts).n_chunks * ((uint64_t)a.out * a.in + a.out) * sizeof(float);
 }
 
+template <typename T, bool BACK, int NB>
+static void product(const ffn_experts& a, const PlanView& v, hipStream_t st) {
+  const int width = BACK ? a.in : a.out, cols = (width + 16 * NB - 1) / (16 * NB);
+  const int64_t total = (int64_t)v.n_tiles * cols;
+  k_expert<T, BACK, NB><<<(unsigned)((total + 7) / 8 * 8), EX_NT, 0, st>>>(a, v, total, cols);
+}
+template <typename T, bool BACK>
+static void product(const ffn_experts& a, const PlanView& v, hipStream_t st) {
+  const int width = BACK ? a.in : a.out;
+  if (width <= 64) product<T, BACK, 4>(a, v, st);
+  else if (width <= 128 || sizeof(T) == 4) product<T, BACK, 8>(a, v, st);  // float: 16 would not fit the registers
+  else if constexpr (sizeof(T) == 2) product<T, BACK, 16>(a, v, st);
+}
+
+template <typename T, int TM, int TK>
+static void weight_gradient(const ffn_experts& a, const PlanView& v, hipStream_t st) {
+  const int mt = (a.out + TM - 1) / TM, kt = (a.in + TK - 1) / TK;
+  // as many chunks a block as there are blocks a chunk: about 512 of them share the slots, and the partials stay few
+  const int merge = mt * kt < 8 ? mt * kt : 8;
+  const int64_t pieces = (int64_t)v.n_chunks * mt * kt, size = (int64_t)a.out * a.in + a.out;
+  k_expert_dw<T, TM, TK><<<(unsigned)((pieces + 7) / 8 * 8), EX_NT, 0, st>>>(a, v, pieces, mt, kt, merge);
+  k_expert_join<<<dim3((unsigned)((size + EX_NT - 1) / EX_NT), a.n_experts), EX_NT, 0, st>>>(a, v, merge);
+}
+
 template <typename T>
 static hipError_t run(const ffn_experts& a, bool backward, hipStream_t st) {
   const PlanView v = plan_view(a.n, a.n_experts);
-  const int width = backward ? a.in : a.out, cols = (width + EX_W - 1) / EX_W;
-  const int64_t total = (int64_t)v.n_tiles * cols;
-  const unsigned grid = (unsigned)((total + 7) / 8 * 8);
   if (!backward) {
-    k_expert<T, false><<<grid, EX_NT, 0, st>>>(a, v, total, cols);
+    product<T, false>(a, v, st);
     return hipGetLastError();
   }
-  if (a.dx) k_expert<T, true><<<grid, EX_NT, 0, st>>>(a, v, total, cols);
+  if (a.dx && a.n) product<T, true>(a, v, st);
   if (a.dW || a.db) {
-    const int mt = (a.out + EX_W - 1) / EX_W, kt = (a.in + EX_W - 1) / EX_W;
-    const int64_t pieces = (int64_t)v.n_chunks * mt * kt;
-    k_expert_dw<T><<<(unsigned)((pieces + 7) / 8 * 8), EX_NT, 0, st>>>(a, v, pieces, mt, kt);
-    const int64_t size = (int64_t)a.out * a.in + a.out;
-    k_expert_join<<<dim3((unsigned)((size + EX_NT - 1) / EX_NT), a.n_experts), EX_NT, 0, st>>>(a, v);
+    const bool m = a.out > 64, k = a.in > 64;
+    if constexpr (sizeof(T) == 4) weight_gradient<T, 64, 64>(a, v, st);  // bound by its products, not by reads
+    else if (m && k) weight_gradient<T, 128, 128>(a, v, st);
+    else if (m) weight_gradient<T, 128, 64>(a, v, st);
+    else if (k) weight_gradient<T, 64, 128>(a, v, st);
+    else weight_gradient<T, 64, 64>(a, v, st);
   }
   return hipGetLastError();
 }

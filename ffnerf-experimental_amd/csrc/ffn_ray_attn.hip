@@ -629,7 +629,7 @@ __global__ __launch_bounds__(AT_NT) void k_attn_row(ffn_ray_attn a, int splits, 
       vst.store(vs, lane);
       ts[lane] = tst;
       if (seen.hi - row0 > AT_TILE) fetch(row0 + AT_TILE);
-      __builtin_amdgcn_wave_barrier();
+      wave_sync();
       logits(s, th, t, ts, g);
       if (seen.hi - row0 < AT_TILE) {
 #pragma unroll
@@ -640,7 +640,7 @@ __global__ __launch_bounds__(AT_NT) void k_attn_row(ffn_ray_attn a, int splits, 
       }
       sm.step(s, acc);
       add_weighted<T, DP>(acc, s, vs, false, row0, seen, lane);
-      __builtin_amdgcn_wave_barrier();
+      wave_sync();
     }
     if (splits == 1) {
       float lse;

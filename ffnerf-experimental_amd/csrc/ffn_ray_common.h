@@ -16,6 +16,14 @@ typedef __bf16 b16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
+// Between LDS writes of a wavefront and its own lanes' reads of them: the LDS takes a wavefront's accesses in order, so
+// only the compiler has to be kept from moving them.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
 // one lane's eight K values of a 16x16x32 matrix operand, and its four values of the product
 template <typename T> struct Mat;
 template <> struct Mat<__bf16> {
