@@ -11,7 +11,7 @@
 
 namespace ffn {
 
-constexpr int AT_NT = 256, AT_TILE = 64;  // four wavefronts of 16 kept rows; rows of a streamed tile
+constexpr int AT_NT = 256, AT_TILE = 64;  // four wavefronts; rows of a streamed tile
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct Range {
@@ -48,6 +48,7 @@ __device__ __forceinline__ Range queries_of(const ffn_ray_attn& a, int64_t j) {
   return {(int)min(qo + from, n), (int)min(qo + nq, n)};
 }
 
+// sums and maxima over the four lane groups
 __device__ __forceinline__ float swap_add(float v) {
   v += __shfl_xor(v, 16);
   return v + __shfl_xor(v, 32);
@@ -57,8 +58,8 @@ __device__ __forceinline__ float swap_max(float v) {
   return fmaxf(v, __shfl_xor(v, 32));
 }
 
-// What the wavefront's 16 rows see: lane c holds row c's range.  [lo, hi) covers all of them; a tile inside
-// [all_lo, all_hi) is seen by every row.
+// What 16 kept rows see: lane c holds row c's range.  [lo, hi) covers all of them; a piece inside [all_lo, all_hi) is
+// seen by every row.
 struct Span {
   int lo, hi, all_lo, all_hi;
 };
@@ -78,6 +79,9 @@ __device__ __forceinline__ Span span_of(const Range& r) {
   s.all_hi = __builtin_amdgcn_readfirstlane(s.all_hi);
   return s;
 }
+__device__ __forceinline__ bool sees(int row, const Range& r) {
+  return (unsigned)(row - r.lo) < (unsigned)(r.hi - r.lo);
+}
 
 // AT_TILE rows of one head on their way to LDS (rows outside [row0, end) and columns past dim as 0)
 template <typename T, int DP, int NT = AT_NT>
@@ -92,15 +96,18 @@ struct Staged {
       if (row < end && col < dim) v[i] = *reinterpret_cast<const uint4*>(base + row * stride + col);
     }
   }
-  // returns whether any of this thread's values is infinite or NaN
-  __device__ __forceinline__ bool store(T* tile, int tid) const {
-    bool bad = false;
+  __device__ __forceinline__ void store(T* tile, int tid) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int c = tid + i * NT;
       *reinterpret_cast<uint4*>(tile + (c / CPR) * lds_row<T, DP> + (c % CPR) * EL) = v[i];
-      bad |= any_nonfinite<T>(v[i]);
     }
+  }
+  // whether any of this thread's values is infinite or NaN
+  __device__ __forceinline__ bool nonfinite() const {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) bad |= any_nonfinite<T>(v[i]);
     return bad;
   }
 };
@@ -118,8 +125,14 @@ __device__ __forceinline__ void load_frags(typename Mat<T>::frag (&f)[KS], const
   }
 }
 
-// tanh to single precision: the odd series where 1 - 2 / (1 + e^2x) would cancel
-__device__ __forceinline__ float tanh_f(float x) {
+// tanh to single precision.  Pieces whose arguments all lie in [-1, 1], the usual ones, take the quotient of Lambert's
+// continued fraction (error 4e-8 at 1); others 1 - 2 / (1 + e^2x), and the odd series where that would cancel.
+__device__ __forceinline__ float tanh_near(float x) {
+  const float x2 = x * x;
+  const float n = __builtin_fmaf(x2, x2 + 105.f, 945.f), d = __builtin_fmaf(x2, __builtin_fmaf(x2, 15.f, 420.f), 945.f);
+  return x * n * __builtin_amdgcn_rcpf(d);
+}
+__device__ __forceinline__ float tanh_any(float x) {
   const float x2 = x * x;
   float p = __builtin_fmaf(x2, 62.f / 2835.f, -17.f / 315.f);
   p = __builtin_fmaf(x2, p, 2.f / 15.f);
@@ -130,91 +143,131 @@ __device__ __forceinline__ float tanh_f(float x) {
   return fabsf(x) < 0.25f ? small : big;
 }
 
-// Products of 16 x 64 rows -> logits in units of log 2; th: tanh of the capped scores (only with a cap).  x: the streamed
-// rows' depths in LDS.  The unit lets every exponential be one v_exp_f32.
+// A piece of 32 streamed rows is what is scored, masked and skipped at once: two product tiles.
+constexpr int PIECE = 32;
+typedef f32x4 Piece[2];
+template <typename F> __device__ __forceinline__ void each(F f) {
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) f(b, r);
+}
+
+// Products -> logits: the exponential is 2^(mul s - ...), so that without a cap the scale and the unit cost nothing.
+// x: the streamed rows' depths in LDS.
+template <bool CAP>
 struct Logits {
-  float scale2, cap, inv_cap, cap2, slope2;
+  float mul, pre, inv_cap, cap2, slope;
   bool bias;
-  __device__ __forceinline__ Logits(const ffn_ray_attn& a, int head)
-      : scale2(a.scale * LOG2E), cap(a.cap), inv_cap(a.cap > 0.f ? a.scale / a.cap : 0.f), cap2(a.cap * LOG2E),
-        slope2(a.slopes ? a.slopes[head] * LOG2E : 0.f), bias(a.slopes != nullptr) {}
-  __device__ __forceinline__ void operator()(f32x4 (&s)[4], f32x4 (&th)[4], float t, const float* x, int g) const {
-    if (cap > 0.f) {
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          th[b][r] = tanh_f(s[b][r] * inv_cap);
-          s[b][r] = cap2 * th[b][r];
-        }
-    } else {
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[b][r] *= scale2;
+  __device__ __forceinline__ Logits(const ffn_ray_attn& a, int head) {
+    const float scale2 = a.scale * LOG2E;
+    inv_cap = CAP ? a.scale / a.cap : 0.f;
+    cap2 = a.cap * LOG2E;
+    bias = a.slopes != nullptr;
+    // s stays the bare product while mul is positive (maxima are taken of s)
+    const bool bare = !CAP && scale2 > 1e-30f;
+    mul = bare ? scale2 : 1.f;
+    pre = bare ? 1.f : scale2;
+    slope = bias ? a.slopes[head] * LOG2E / mul : 0.f;
+  }
+  __device__ __forceinline__ void operator()(Piece& s, Piece& th, float t, const float* x, int g) const {
+    if constexpr (CAP) {
+      float top = 0.f;
+      each([&](int b, int r) {
+        th[b][r] = s[b][r] * inv_cap;
+        top = fmaxf(top, fabsf(th[b][r]));
+      });
+      if (__any(!(top <= 1.f))) each([&](int b, int r) { th[b][r] = tanh_any(th[b][r]); });
+      else each([&](int b, int r) { th[b][r] = tanh_near(th[b][r]); });
+      each([&](int b, int r) { s[b][r] = cap2 * th[b][r]; });
+    } else if (pre != 1.f) {
+      each([&](int b, int r) { s[b][r] *= pre; });
     }
     if (bias) {
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
+      for (int b = 0; b < 2; ++b) {
         const f32x4 tx = *reinterpret_cast<const f32x4*>(x + 16 * b + 4 * g);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[b][r] = __builtin_fmaf(-slope2, fabsf(t - tx[r]), s[b][r]);
+        for (int r = 0; r < 4; ++r) s[b][r] = __builtin_fmaf(-slope, fabsf(t - tx[r]), s[b][r]);
       }
     }
   }
 };
 
-__device__ __forceinline__ bool sees(int row, const Range& r) {
-  return (unsigned)(row - r.lo) < (unsigned)(r.hi - r.lo);
-}
-
-// acc += tile^T w over the tile's 64 rows, where a row of the tile holds an infinity or a NaN: pair by pair, so that a
-// weight of 0 that only a mask made does not meet it
-template <typename T, int DP>
-__device__ __noinline__ void add_careful(f32x4* acc, const f32x4* w, const T* tile, int row0, Range seen, int lane) {
-  const int g = lane >> 4, c = lane & 15;
-  for (int row = 0; row < AT_TILE; ++row) {
-    const float mine = w[row >> 4][row & 3];
-    const float ww = __shfl(mine, 16 * ((row >> 2) & 3) + c);
-    if (!sees(row0 + row, seen)) continue;
-    for (int db = 0; db < DP / 16; ++db)
-      for (int r = 0; r < 4; ++r)
-        acc[db][r] = __builtin_fmaf(ww, (float)tile[row * lds_row<T, DP> + 16 * db + 4 * g + r], acc[db][r]);
-  }
-}
-
-// acc += tile^T w: the tile's 64 rows are the K of the product
-template <typename T, int DP>
-__device__ __forceinline__ void add_weighted(f32x4 (&acc)[DP / 16], const f32x4 (&w)[4], const T* tile, bool careful,
-                                             int row0, const Range& seen, int lane) {
-  if (careful) {
-    f32x4 a2[DP / 16], w2[4];
-    for (int i = 0; i < DP / 16; ++i) a2[i] = acc[i];
-    for (int i = 0; i < 4; ++i) w2[i] = w[i];
-    add_careful<T, DP>(a2, w2, tile, row0, seen, lane);
-    for (int i = 0; i < DP / 16; ++i) acc[i] = a2[i];
-    return;
-  }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const typename Mat<T>::frag f = product_frag<T>(w[2 * h], w[2 * h + 1]);
-#pragma unroll
-    for (int db = 0; db < DP / 16; ++db)
-      acc[db] = Mat<T>::mma(col_frag<T, DP>(tile, 32 * h, 16 * db, lane), f, acc[db]);
-  }
-}
-
-// s = tile rows . kept rows
-template <typename T, int DP>
-__device__ __forceinline__ void products(f32x4 (&s)[4], const T* tile, const typename Mat<T>::frag (&kept)[DP / 32],
+// s[q] = 32 tile rows . kept rows of set q
+template <typename T, int DP, int NQ>
+__device__ __forceinline__ void products(Piece (&s)[NQ], const T* tile, const typename Mat<T>::frag (&kept)[NQ][DP / 32],
                                          int lane) {
 #pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int b = 0; b < 2; ++b) {
 #pragma unroll
-    for (int ks = 0; ks < DP / 32; ++ks)
-      s[b] = Mat<T>::mma(row_frag<T, DP>(tile, 16 * b + (lane & 15), ks, lane), kept[ks], s[b]);
+    for (int q = 0; q < NQ; ++q) s[q][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < DP / 32; ++ks) {
+      const typename Mat<T>::frag f = row_frag<T, DP>(tile, 16 * b + (lane & 15), ks, lane);
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) s[q][b] = Mat<T>::mma(f, kept[q][ks], s[q][b]);
+    }
   }
+}
+
+// a fragment with its infinities and NaN as 0
+template <typename T>
+__device__ __forceinline__ typename Mat<T>::frag finite_frag(typename Mat<T>::frag f) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (!(fabsf((float)f[j]) < INFINITY)) f[j] = (T)0.f;
+  return f;
+}
+
+// acc[q] += tile^T w[q]: the 32 tile rows are the K of the product.  Where the tile holds infinities or NaN (bad), pairs
+// that do not see each other must not meet, since a weight of 0 times them is not 0: the product takes them as 0, and the
+// pairs that do see each other are added one by one.
+template <typename T, int DP, int NQ>
+__device__ __forceinline__ void add_weighted(f32x4 (&acc)[NQ][DP / 16], const Piece (&w)[NQ], const T* tile, bool bad,
+                                             int row0, const Range (&seen)[NQ], int lane) {
+  typename Mat<T>::frag f[NQ], m[DP / 16];
+#pragma unroll
+  for (int db = 0; db < DP / 16; ++db) m[db] = col_frag<T, DP>(tile, 0, 16 * db, lane);
+  if (bad) {
+#pragma unroll
+    for (int db = 0; db < DP / 16; ++db) m[db] = finite_frag<T>(m[db]);
+  }
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) f[q] = product_frag<T>(w[q][0], w[q][1]);
+#pragma unroll
+  for (int db = 0; db < DP / 16; ++db)
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) acc[q][db] = Mat<T>::mma(m[db], f[q], acc[q][db]);
+  if (bad) {
+    const int g = lane >> 4, c = lane & 15;
+#pragma unroll 1
+    for (int row = 0; row < PIECE; ++row) {
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        float mine = 0.f;
+        each([&](int b, int r) { mine = row >> 4 == b && (row & 3) == r ? w[q][b][r] : mine; });
+        const float ww = __shfl(mine, 16 * ((row >> 2) & 3) + c);
+        const bool see = sees(row0 + row, seen[q]);
+#pragma unroll
+        for (int db = 0; db < DP / 16; ++db) {
+          const f32x4 x = __builtin_convertvector(
+              *reinterpret_cast<const typename Mat<T>::quad*>(tile + row * lds_row<T, DP> + 16 * db + 4 * g), f32x4);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (see && !(fabsf(x[k]) < INFINITY)) acc[q][db][k] = __builtin_fmaf(ww, x[k], acc[q][db][k]);
+        }
+      }
+    }
+  }
+}
+
+// what is not seen gets `v`
+__device__ __forceinline__ void mask(Piece& s, int row0, const Span& w, const Range& seen, int g, float v) {
+  if (row0 < w.all_lo || row0 + PIECE > w.all_hi)
+    each([&](int b, int r) {
+      if (!sees(row0 + 16 * b + 4 * g + r, seen)) s[b][r] = v;
+    });
 }
 
 template <typename T, int DP>
@@ -235,21 +288,22 @@ __device__ __forceinline__ void store_row(T* __restrict__ row, const f32x4 (&acc
 // numbers end at 2^-14, and the exponential's at 2^-126 (it gives 0 below).
 constexpr float W_SHIFT = 14.f, W_UNSHIFT = 1.f / 16384.f;
 
-// Running softmax of one row, its sum still apart by lane group
+// Running softmax of one row, its sum still apart by lane group.  m is a maximum that lags: it is raised, and the sums are
+// rescaled, only when a logit passes it by more than SLACK (which fp16's weights, 2^14 and more, have room for), so that
+// most pieces need no exchange between lanes.
+template <typename T>
 struct Softmax {
+  static constexpr float SLACK = __is_same(T, _Float16) ? 1.f : 8.f;
   float m = -INFINITY, l = 0.f;
   // weights in place of the logits
   template <int NACC>
-  __device__ __forceinline__ void step(f32x4 (&s)[4], f32x4 (&acc)[NACC]) {
+  __device__ __forceinline__ void step(Piece& s, float mul, f32x4 (&acc)[NACC]) {
     float mx = s[0][0];
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[b][r]);
-    mx = fmaxf(m, swap_max(mx));
-    const float base = mx == -INFINITY ? 0.f : mx;
-    if (__any(mx != m)) {
-      const float f = __builtin_amdgcn_exp2f(m - base);
+    each([&](int b, int r) { mx = fmaxf(mx, s[b][r]); });
+    mx *= mul;
+    if (__any(mx > m + SLACK)) {
+      mx = fmaxf(m, swap_max(mx));
+      const float f = __builtin_amdgcn_exp2f(m - (mx == -INFINITY ? 0.f : mx));
       l *= f;
 #pragma unroll
       for (int i = 0; i < NACC; ++i)
@@ -257,14 +311,11 @@ struct Softmax {
         for (int r = 0; r < 4; ++r) acc[i][r] *= f;
       m = mx;
     }
-    const float from = base - W_SHIFT;
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s[b][r] = __builtin_amdgcn_exp2f(s[b][r] - from);
-        l += s[b][r];
-      }
+    const float from = (m == -INFINITY ? 0.f : m) - W_SHIFT;
+    each([&](int b, int r) {
+      s[b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], mul, -from));
+      l += s[b][r];
+    });
   }
   // factor of the sums, and the logarithm of the sum of exponentials
   __device__ __forceinline__ float finish(float& lse) {
@@ -274,77 +325,138 @@ struct Softmax {
   }
 };
 
-// Blocks in launch order go round the eight dies; this gives each die a contiguous part of the work, whose tiles share
-// keys in its L2.
-__device__ __forceinline__ int64_t die_order(int64_t total) {
-  const int64_t per = (total + 7) / 8;
-  return (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+// Blocks in launch order go round the eight dies; this gives each die runs of DIE_RUN neighbouring pieces of work, whose
+// tiles share keys in its L2.  Longer runs leave the dies with unequal work where rays are few and long.
+#ifndef DIE_RUN
+#define DIE_RUN 16
+#endif
+__device__ __forceinline__ int64_t die_order() {
+  const int64_t b = blockIdx.x >> 3;
+  return (b / DIE_RUN * 8 + (blockIdx.x & 7)) * DIE_RUN + b % DIE_RUN;
 }
 
-template <typename T, int DP>
+// the kept rows of a wavefront, NQ sets of 16: row number, what it sees, and the ranges over all of them
+template <int NQ>
+struct Kept {
+  int64_t row[NQ];
+  bool there[NQ];
+  Range seen[NQ];
+  Span span[NQ];
+  int lo, hi;
+  template <typename F>
+  __device__ __forceinline__ Kept(int64_t first, int64_t n, int c, F sees_of) {
+    lo = INT_MAX, hi = 0;
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      row[q] = first + 16 * q + c;
+      there[q] = row[q] < n;
+      seen[q] = sees_of(row[q]);
+      span[q] = span_of(seen[q]);
+      lo = min(lo, span[q].lo);
+      hi = max(hi, span[q].hi);
+    }
+  }
+};
+
+// Waits for the kept rows' fragments where it stands.  Without it their loads are still pending, as far as the compiler
+// knows, when the streaming loop begins, and their first use there waits for the rows asked for ahead as well.
+template <typename F, int N>
+__device__ __forceinline__ void arrived(F (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
+
+// [lo, hi) over the block's four wavefronts
+__device__ __forceinline__ Range block_range(int lo, int hi, int wave, int lane, int (&s)[8]) {
+  if (lane == 0) s[wave] = lo, s[4 + wave] = hi;
+  __syncthreads();
+  return {min(min(s[0], s[1]), min(s[2], s[3])), max(max(s[4], s[5]), max(s[6], s[7]))};
+}
+
+// NQ: sets of 16 queries a wavefront.  Two sets read each fragment of K and V once, which long rays are bound by; short
+// rays lose more to pieces that only one of the sets sees.
+template <typename T, int DP, int NQ, bool CAP>
 __global__ __launch_bounds__(AT_NT) void k_attn_fwd(ffn_ray_attn a, int64_t total) {
-  constexpr int KS = DP / 32, NB = DP / 16;
-  __shared__ T ks[AT_TILE * lds_row<T, DP>], vs[AT_TILE * lds_row<T, DP>];
-  __shared__ float ts[AT_TILE];
-  __shared__ int s_lo[4], s_hi[4], s_bad[4];
-  const int64_t work = die_order(total);
+  constexpr int KS = DP / 32, NB = DP / 16, TILE = AT_TILE * lds_row<T, DP>;
+  __shared__ __align__(16) T ks[2][TILE];
+  __shared__ __align__(16) T vs[2][TILE];
+  __shared__ __align__(16) float ts[2][AT_TILE];
+  __shared__ int s_range[8], s_bad[2][4];
+  const int64_t work = die_order();
   if (work >= total) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
   const int head = (int)(work % a.heads), kh = head / (a.heads / a.kv_heads);
-  const int64_t i = work / a.heads * AT_TILE + wave * 16 + c;
-  const bool there = i < a.q_rays.n;
-  const Range seen = keys_of(a, i);
-  const Span w = span_of(seen);
-  if (lane == 0) s_lo[wave] = w.lo, s_hi[wave] = w.hi;
-  typename Mat<T>::frag qf[KS];
-  load_frags<T, KS>(qf, (const T*)a.q + i * a.q_row + head * a.q_head, there, a.dim, g);
-  const Logits logits(a, head);
-  const float t = logits.bias && there ? a.t_q[i * a.t_q_row] : 0.f;
-  __syncthreads();
-  const int lo = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3])), hi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
+  const Kept<NQ> kept(work / a.heads * (64 * NQ) + wave * 16 * NQ, a.q_rays.n, c, [&](int64_t i) { return keys_of(a, i); });
+  const Logits<CAP> logits(a, head);
+  typename Mat<T>::frag qf[NQ][KS];
+  float t[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    load_frags<T, KS>(qf[q], (const T*)a.q + kept.row[q] * a.q_row + head * a.q_head, kept.there[q], a.dim, g);
+    t[q] = logits.bias && kept.there[q] ? a.t_q[kept.row[q] * a.t_q_row] : 0.f;
+  }
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) arrived(qf[q]);
+  arrived(t);
+  const Range range = block_range(kept.lo, kept.hi, wave, lane, s_range);
   const T* kb = (const T*)a.k + kh * a.k_head;
   const T* vb = (const T*)a.v + kh * a.v_head;
-  f32x4 acc[NB];
+  f32x4 acc[NQ][NB];
+  Softmax<T> sm[NQ];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-  Softmax sm;
+  for (int q = 0; q < NQ; ++q)
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[q][b] = f32x4{0.f, 0.f, 0.f, 0.f};
   Staged<T, DP> kst, vst;
   float tst = 0.f;
   auto fetch = [&](int row0) {
-    kst.load(kb, a.k_row, row0, hi, a.dim, tid);
-    vst.load(vb, a.v_row, row0, hi, a.dim, tid);
-    if (logits.bias && tid < AT_TILE && row0 + tid < hi) tst = a.t_k[(int64_t)(row0 + tid) * a.t_k_row];
+    kst.load(kb, a.k_row, row0, range.hi, a.dim, tid);
+    vst.load(vb, a.v_row, row0, range.hi, a.dim, tid);
+    if (logits.bias && tid < AT_TILE && row0 + tid < range.hi) tst = a.t_k[(int64_t)(row0 + tid) * a.t_k_row];
   };
-  if (lo < hi) fetch(lo);
-  for (int row0 = lo; row0 < hi; row0 += AT_TILE) {
-    kst.store(ks, tid);
-    const bool bad = __any(vst.store(vs, tid));
-    if (lane == 0) s_bad[wave] = bad;
-    if (tid < AT_TILE) ts[tid] = tst;
-    __syncthreads();
-    if (hi - row0 > AT_TILE) fetch(row0 + AT_TILE);
-    if (row0 < w.hi && row0 + AT_TILE > w.lo) {
-      f32x4 s[4], th[4];
-      products<T, DP>(s, ks, qf, lane);
-      logits(s, th, t, ts, g);
-      if (row0 < w.all_lo || row0 + AT_TILE > w.all_hi) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (!sees(row0 + 16 * b + 4 * g + r, seen)) s[b][r] = -INFINITY;
-      }
-      sm.step(s, acc);
-      add_weighted<T, DP>(acc, s, vs, s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3], row0, seen, lane);
-    }
-    __syncthreads();
+  auto put = [&](int to) {
+    kst.store(ks[to], tid);
+    vst.store(vs[to], tid);
+    const bool bad = __any(vst.nonfinite());
+    if (lane == 0) s_bad[to][wave] = bad;
+    if (tid < AT_TILE) ts[to][tid] = tst;
+  };
+  if (range.lo < range.hi) {
+    fetch(range.lo);
+    put(0);
   }
-  float lse;
-  const float by = sm.finish(lse);
-  if (there) {
-    const int64_t at = i * a.heads + head;
-    store_row<T, DP>((T*)a.o + at * a.dim, acc, by, a.dim, g);
-    if (g == 0) a.lse[at] = lse;
+  int at = 0;
+  for (int tile = range.lo; tile < range.hi; tile += AT_TILE, at ^= 1) {
+    __syncthreads();
+    const bool more = range.hi - tile > AT_TILE;
+    if (more) fetch(tile + AT_TILE);
+    const bool bad = s_bad[at][0] | s_bad[at][1] | s_bad[at][2] | s_bad[at][3];
+#pragma unroll
+    for (int p = 0; p < AT_TILE; p += PIECE) {
+      const int row0 = tile + p;
+      if (row0 >= kept.hi || row0 + PIECE <= kept.lo) continue;
+      Piece s[NQ];
+      products<T, DP, NQ>(s, ks[at] + p * lds_row<T, DP>, qf, lane);
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        Piece th;
+        logits(s[q], th, t[q], ts[at] + p, g);
+        mask(s[q], row0, kept.span[q], kept.seen[q], g, -INFINITY);
+        sm[q].step(s[q], logits.mul, acc[q]);
+      }
+      add_weighted<T, DP, NQ>(acc, s, vs[at] + p * lds_row<T, DP>, bad, row0, kept.seen, lane);
+    }
+    if (more) put(at ^ 1);
+  }
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    float lse;
+    const float by = sm[q].finish(lse);
+    if (kept.there[q]) {
+      const int64_t to = kept.row[q] * a.heads + head;
+      store_row<T, DP>((T*)a.o + to * a.dim, acc[q], by, a.dim, g);
+      if (g == 0) a.lse[to] = lse;
+    }
   }
 }
 
@@ -355,16 +467,13 @@ template <typename T>
 struct GradScale {
   float f = 0.f;
   template <int NACC>
-  __device__ __forceinline__ void apply(f32x4 (&s)[4], f32x4 (&acc)[NACC]) {
+  __device__ __forceinline__ void apply(Piece& s, f32x4 (&acc)[NACC]) {
     if constexpr (__is_same(T, _Float16)) {
       float mx = 0.f;
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, fabsf(s[b][r]));
-      mx = swap_max(mx);
-      const bool grow = mx > 0.f && (f == 0.f || mx * f > 32768.f);
-      if (__any(grow)) {
+      each([&](int b, int r) { mx = fmaxf(mx, fabsf(s[b][r])); });
+      if (__any(mx * f > 32768.f || (f == 0.f && mx > 0.f))) {
+        mx = swap_max(mx);
+        const bool grow = mx > 0.f && (f == 0.f || mx * f > 32768.f);
         const int e = min(max(140 - (int)(__float_as_uint(mx) >> 23), -100), 100);  // 13 - exponent
         const float to = __uint_as_float((unsigned)(127 + e) << 23);
         const float by = grow ? (f == 0.f ? 0.f : to / f) : 1.f;
@@ -374,10 +483,7 @@ struct GradScale {
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[i][r] *= by;
       }
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[b][r] *= f;
+      each([&](int b, int r) { s[b][r] *= f; });
     }
   }
   __device__ __forceinline__ float undo() const {
@@ -387,196 +493,226 @@ struct GradScale {
 };
 
 // dq; also leaves D = sum_d do o of its rows in the workspace for k_attn_dkv
-template <typename T, int DP>
+template <typename T, int DP, int NQ, bool CAP>
 __global__ __launch_bounds__(AT_NT) void k_attn_dq(ffn_ray_attn a, int64_t total) {
-  constexpr int KS = DP / 32, NB = DP / 16;
-  __shared__ T ks[AT_TILE * lds_row<T, DP>], vs[AT_TILE * lds_row<T, DP>];
-  __shared__ float ts[AT_TILE];
-  __shared__ int s_lo[4], s_hi[4], s_bad[4];
-  const int64_t work = die_order(total);
+  constexpr int KS = DP / 32, NB = DP / 16, TILE = AT_TILE * lds_row<T, DP>;
+  __shared__ __align__(16) T ks[2][TILE];
+  __shared__ __align__(16) T vs[2][TILE];
+  __shared__ __align__(16) float ts[2][AT_TILE];
+  __shared__ int s_range[8], s_bad[2][4];
+  const int64_t work = die_order();
   if (work >= total) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
   const int head = (int)(work % a.heads), kh = head / (a.heads / a.kv_heads);
-  const int64_t i = work / a.heads * AT_TILE + wave * 16 + c, at = i * a.heads + head;
-  const bool there = i < a.q_rays.n;
-  const Range seen = keys_of(a, i);
-  const Span w = span_of(seen);
-  if (lane == 0) s_lo[wave] = w.lo, s_hi[wave] = w.hi;
-  typename Mat<T>::frag qf[KS], df[KS];
-  load_frags<T, KS>(qf, (const T*)a.q + i * a.q_row + head * a.q_head, there, a.dim, g);
-  load_frags<T, KS>(df, (const T*)a.dout + i * a.do_row + head * a.do_head, there, a.dim, g);
-  float delta = 0.f;
-  {
+  const Kept<NQ> kept(work / a.heads * (64 * NQ) + wave * 16 * NQ, a.q_rays.n, c, [&](int64_t i) { return keys_of(a, i); });
+  const Logits<CAP> logits(a, head);
+  typename Mat<T>::frag qf[NQ][KS], df[NQ][KS];
+  float t[NQ], delta[NQ], from[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const int64_t i = kept.row[q], to = i * a.heads + head;
+    load_frags<T, KS>(qf[q], (const T*)a.q + i * a.q_row + head * a.q_head, kept.there[q], a.dim, g);
+    load_frags<T, KS>(df[q], (const T*)a.dout + i * a.do_row + head * a.do_head, kept.there[q], a.dim, g);
     typename Mat<T>::frag of[KS];
-    load_frags<T, KS>(of, (const T*)a.o + at * a.dim, there, a.dim, g);
+    load_frags<T, KS>(of, (const T*)a.o + to * a.dim, kept.there[q], a.dim, g);
+    float d = 0.f;
 #pragma unroll
     for (int k = 0; k < KS; ++k)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)of[k][j], (float)df[k][j], delta);
-    delta = swap_add(delta);
+      for (int j = 0; j < 8; ++j) d = __builtin_fmaf((float)of[k][j], (float)df[q][k][j], d);
+    delta[q] = swap_add(d);
+    t[q] = logits.bias && kept.there[q] ? a.t_q[i * a.t_q_row] : 0.f;
+    const float lse2 = kept.there[q] ? a.lse[to] * LOG2E : 0.f;
+    from[q] = (lse2 == -INFINITY ? 0.f : lse2) - W_SHIFT;
+    if (kept.there[q] && g == 0) ((float*)a.workspace)[to] = delta[q];
   }
-  const Logits logits(a, head);
-  const float t = logits.bias && there ? a.t_q[i * a.t_q_row] : 0.f;
-  float lse2 = there ? a.lse[at] * LOG2E : 0.f;
-  if (lse2 == -INFINITY) lse2 = 0.f;
-  const float from = lse2 - W_SHIFT;
-  if (there && g == 0) ((float*)a.workspace)[at] = delta;
-  __syncthreads();
-  const int lo = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3])), hi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    arrived(qf[q]);
+    arrived(df[q]);
+  }
+  arrived(t);
+  arrived(from);
+  const Range range = block_range(kept.lo, kept.hi, wave, lane, s_range);
   const T* kb = (const T*)a.k + kh * a.k_head;
   const T* vb = (const T*)a.v + kh * a.v_head;
-  f32x4 acc[NB];
+  f32x4 acc[NQ][NB];
+  GradScale<T> gs[NQ];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-  GradScale<T> gs;
+  for (int q = 0; q < NQ; ++q)
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[q][b] = f32x4{0.f, 0.f, 0.f, 0.f};
   Staged<T, DP> kst, vst;
   float tst = 0.f;
   auto fetch = [&](int row0) {
-    kst.load(kb, a.k_row, row0, hi, a.dim, tid);
-    vst.load(vb, a.v_row, row0, hi, a.dim, tid);
-    if (logits.bias && tid < AT_TILE && row0 + tid < hi) tst = a.t_k[(int64_t)(row0 + tid) * a.t_k_row];
+    kst.load(kb, a.k_row, row0, range.hi, a.dim, tid);
+    vst.load(vb, a.v_row, row0, range.hi, a.dim, tid);
+    if (logits.bias && tid < AT_TILE && row0 + tid < range.hi) tst = a.t_k[(int64_t)(row0 + tid) * a.t_k_row];
   };
-  if (lo < hi) fetch(lo);
-  for (int row0 = lo; row0 < hi; row0 += AT_TILE) {
-    const bool bad = __any(kst.store(ks, tid));
-    vst.store(vs, tid);
-    if (lane == 0) s_bad[wave] = bad;
-    if (tid < AT_TILE) ts[tid] = tst;
-    __syncthreads();
-    if (hi - row0 > AT_TILE) fetch(row0 + AT_TILE);
-    if (row0 < w.hi && row0 + AT_TILE > w.lo) {
-      f32x4 s[4], dp[4], th[4];
-      products<T, DP>(s, ks, qf, lane);
-      products<T, DP>(dp, vs, df, lane);
-      logits(s, th, t, ts, g);
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          s[b][r] = __builtin_amdgcn_exp2f(s[b][r] - from) * (dp[b][r] - delta);
-      if (logits.cap > 0.f) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[b][r] *= 1.f - th[b][r] * th[b][r];
-      }
-      if (row0 < w.all_lo || row0 + AT_TILE > w.all_hi) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (!sees(row0 + 16 * b + 4 * g + r, seen)) s[b][r] = 0.f;
-      }
-      gs.apply(s, acc);
-      add_weighted<T, DP>(acc, s, ks, s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3], row0, seen, lane);
-    }
-    __syncthreads();
+  auto put = [&](int to) {
+    kst.store(ks[to], tid);
+    vst.store(vs[to], tid);
+    const bool bad = __any(kst.nonfinite());
+    if (lane == 0) s_bad[to][wave] = bad;
+    if (tid < AT_TILE) ts[to][tid] = tst;
+  };
+  if (range.lo < range.hi) {
+    fetch(range.lo);
+    put(0);
   }
-  if (there) store_row<T, DP>((T*)a.dq + at * a.dim, acc, gs.undo() * (a.scale * W_UNSHIFT), a.dim, g);
+  int at = 0;
+  for (int tile = range.lo; tile < range.hi; tile += AT_TILE, at ^= 1) {
+    __syncthreads();
+    const bool more = range.hi - tile > AT_TILE;
+    if (more) fetch(tile + AT_TILE);
+    const bool bad = s_bad[at][0] | s_bad[at][1] | s_bad[at][2] | s_bad[at][3];
+#pragma unroll
+    for (int p = 0; p < AT_TILE; p += PIECE) {
+      const int row0 = tile + p;
+      if (row0 >= kept.hi || row0 + PIECE <= kept.lo) continue;
+      Piece s[NQ], dp[NQ];
+      products<T, DP, NQ>(s, ks[at] + p * lds_row<T, DP>, qf, lane);
+      products<T, DP, NQ>(dp, vs[at] + p * lds_row<T, DP>, df, lane);
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        Piece th;
+        logits(s[q], th, t[q], ts[at] + p, g);
+        each([&](int b, int r) {
+          s[q][b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[q][b][r], logits.mul, -from[q])) * (dp[q][b][r] - delta[q]);
+        });
+        if (CAP) each([&](int b, int r) { s[q][b][r] *= __builtin_fmaf(-th[b][r], th[b][r], 1.f); });
+        mask(s[q], row0, kept.span[q], kept.seen[q], g, 0.f);
+        gs[q].apply(s[q], acc[q]);
+      }
+      add_weighted<T, DP, NQ>(acc, s, ks[at] + p * lds_row<T, DP>, bad, row0, kept.seen, lane);
+    }
+    if (more) put(at ^ 1);
+  }
+#pragma unroll
+  for (int q = 0; q < NQ; ++q)
+    if (kept.there[q])
+      store_row<T, DP>((T*)a.dq + (kept.row[q] * a.heads + head) * a.dim, acc[q], gs[q].undo() * (a.scale * W_UNSHIFT), a.dim, g);
 }
 
-// dk and dv of 64 keys of one key head: the queries of the heads that share it stream past
-template <typename T, int DP>
+// dk and dv of the kept keys of one key head: the queries of the heads that share it stream past
+template <typename T, int DP, int NQ, bool CAP>
 __global__ __launch_bounds__(AT_NT) void k_attn_dkv(ffn_ray_attn a, int64_t total) {
-  constexpr int KS = DP / 32, NB = DP / 16;
-  __shared__ T qs[AT_TILE * lds_row<T, DP>], ds[AT_TILE * lds_row<T, DP>];
-  __shared__ float ts[AT_TILE], ls[AT_TILE], es[AT_TILE];
-  __shared__ int s_lo[4], s_hi[4], s_bad[8];
-  const int64_t work = die_order(total);
+  constexpr int KS = DP / 32, NB = DP / 16, TILE = AT_TILE * lds_row<T, DP>;
+  __shared__ __align__(16) T qs[2][TILE];
+  __shared__ __align__(16) T ds[2][TILE];
+  __shared__ __align__(16) float ts[2][AT_TILE], ls[2][AT_TILE], es[2][AT_TILE];
+  __shared__ int s_range[8], s_bad[2][8];
+  const int64_t work = die_order();
   if (work >= total) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
   const int kh = (int)(work % a.kv_heads), group = a.heads / a.kv_heads;
-  const int64_t j = work / a.kv_heads * AT_TILE + wave * 16 + c;
-  const bool there = j < a.k_rays.n;
-  const Range seen = queries_of(a, j);
-  const Span w = span_of(seen);
-  if (lane == 0) s_lo[wave] = w.lo, s_hi[wave] = w.hi;
-  typename Mat<T>::frag kf[KS], vf[KS];
-  load_frags<T, KS>(kf, (const T*)a.k + j * a.k_row + kh * a.k_head, there, a.dim, g);
-  load_frags<T, KS>(vf, (const T*)a.v + j * a.v_row + kh * a.v_head, there, a.dim, g);
+  const Kept<NQ> kept(work / a.kv_heads * (64 * NQ) + wave * 16 * NQ, a.k_rays.n, c, [&](int64_t j) { return queries_of(a, j); });
   const bool bias = a.slopes != nullptr;
-  const float t = bias && there ? a.t_k[j * a.t_k_row] : 0.f;
-  __syncthreads();
-  const int lo = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3])), hi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
-  f32x4 dk[NB], dv[NB];
+  typename Mat<T>::frag kf[NQ][KS], vf[NQ][KS];
+  float t[NQ];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) dk[b] = dv[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-  GradScale<T> gs;
+  for (int q = 0; q < NQ; ++q) {
+    const int64_t j = kept.row[q];
+    load_frags<T, KS>(kf[q], (const T*)a.k + j * a.k_row + kh * a.k_head, kept.there[q], a.dim, g);
+    load_frags<T, KS>(vf[q], (const T*)a.v + j * a.v_row + kh * a.v_head, kept.there[q], a.dim, g);
+    t[q] = bias && kept.there[q] ? a.t_k[j * a.t_k_row] : 0.f;
+  }
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    arrived(kf[q]);
+    arrived(vf[q]);
+  }
+  arrived(t);
+  const Range range = block_range(kept.lo, kept.hi, wave, lane, s_range);
+  f32x4 dk[NQ][NB], dv[NQ][NB];
+  GradScale<T> gs[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q)
+#pragma unroll
+    for (int b = 0; b < NB; ++b) dk[q][b] = dv[q][b] = f32x4{0.f, 0.f, 0.f, 0.f};
   Staged<T, DP> qst, dst;
   float tst = 0.f, lst = 0.f, est = 0.f;
   auto fetch = [&](int head, int row0) {
-    qst.load((const T*)a.q + head * a.q_head, a.q_row, row0, hi, a.dim, tid);
-    dst.load((const T*)a.dout + head * a.do_head, a.do_row, row0, hi, a.dim, tid);
-    if (tid < AT_TILE && row0 + tid < hi) {
+    qst.load((const T*)a.q + head * a.q_head, a.q_row, row0, range.hi, a.dim, tid);
+    dst.load((const T*)a.dout + head * a.do_head, a.do_row, row0, range.hi, a.dim, tid);
+    if (tid < AT_TILE && row0 + tid < range.hi) {
       const int64_t i = row0 + tid;
       if (bias) tst = a.t_q[i * a.t_q_row];
       lst = a.lse[i * a.heads + head] * LOG2E;
       est = ((const float*)a.workspace)[i * a.heads + head];
-      if (lst == -INFINITY) lst = 0.f;
+      lst = (lst == -INFINITY ? 0.f : lst) - W_SHIFT;
     }
   };
+  auto put = [&](int to) {
+    qst.store(qs[to], tid);
+    dst.store(ds[to], tid);
+    const bool bad_q = __any(qst.nonfinite()), bad_d = __any(dst.nonfinite());
+    if (lane == 0) s_bad[to][wave] = bad_q, s_bad[to][4 + wave] = bad_d;
+    if (tid < AT_TILE) ts[to][tid] = tst, ls[to][tid] = lst, es[to][tid] = est;
+  };
   const int first = kh * group, end = first + group;
-  if (lo < hi) fetch(first, lo);
-  for (int head = first; head < end && lo < hi; ++head) {
-    const Logits logits(a, head);
-    for (int row0 = lo; row0 < hi; row0 += AT_TILE) {
-      const bool bad_q = __any(qst.store(qs, tid)), bad_d = __any(dst.store(ds, tid));
-      if (lane == 0) s_bad[wave] = bad_q, s_bad[4 + wave] = bad_d;
-      if (tid < AT_TILE) ts[tid] = tst, ls[tid] = lst, es[tid] = est;
+  if (range.lo < range.hi) {
+    fetch(first, range.lo);
+    put(0);
+  }
+  int at = 0;
+  for (int head = first; head < end && range.lo < range.hi; ++head) {
+    const Logits<CAP> logits(a, head);
+    for (int tile = range.lo; tile < range.hi; tile += AT_TILE, at ^= 1) {
       __syncthreads();
-      if (hi - row0 > AT_TILE) fetch(head, row0 + AT_TILE);
-      else if (head + 1 < end) fetch(head + 1, lo);
-      if (row0 < w.hi && row0 + AT_TILE > w.lo) {
-        f32x4 s[4], dp[4], th[4];
-        products<T, DP>(s, qs, kf, lane);
-        products<T, DP>(dp, ds, vf, lane);
-        logits(s, th, t, ts, g);
-        const bool masked = row0 < w.all_lo || row0 + AT_TILE > w.all_hi;
+      const bool rest = range.hi - tile > AT_TILE, more = rest || head + 1 < end;
+      if (more) fetch(rest ? head : head + 1, rest ? tile + AT_TILE : range.lo);
+      const bool bad_q = s_bad[at][0] | s_bad[at][1] | s_bad[at][2] | s_bad[at][3];
+      const bool bad_d = s_bad[at][4] | s_bad[at][5] | s_bad[at][6] | s_bad[at][7];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const f32x4 l = *reinterpret_cast<const f32x4*>(ls + 16 * b + 4 * g);
-          const f32x4 e = *reinterpret_cast<const f32x4*>(es + 16 * b + 4 * g);
+      for (int p = 0; p < AT_TILE; p += PIECE) {
+        const int row0 = tile + p;
+        if (row0 >= kept.hi || row0 + PIECE <= kept.lo) continue;
+        Piece s[NQ], dp[NQ];
+        products<T, DP, NQ>(s, qs[at] + p * lds_row<T, DP>, kf, lane);
+        products<T, DP, NQ>(dp, ds[at] + p * lds_row<T, DP>, vf, lane);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            s[b][r] = __builtin_amdgcn_exp2f(s[b][r] - (l[r] - W_SHIFT));
-            dp[b][r] = s[b][r] * (dp[b][r] - e[r]);
+        for (int q = 0; q < NQ; ++q) {
+          Piece th;
+          logits(s[q], th, t[q], ts[at] + p, g);
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const f32x4 l = *reinterpret_cast<const f32x4*>(ls[at] + p + 16 * b + 4 * g);
+            const f32x4 e = *reinterpret_cast<const f32x4*>(es[at] + p + 16 * b + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              s[q][b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[q][b][r], logits.mul, -l[r]));
+              dp[q][b][r] = s[q][b][r] * (dp[q][b][r] - e[r]);
+            }
           }
+          if (CAP) each([&](int b, int r) { dp[q][b][r] *= __builtin_fmaf(-th[b][r], th[b][r], 1.f); });
+          mask(s[q], row0, kept.span[q], kept.seen[q], g, 0.f);
+          mask(dp[q], row0, kept.span[q], kept.seen[q], g, 0.f);
+          gs[q].apply(dp[q], dk[q]);
         }
-        if (logits.cap > 0.f) {
-#pragma unroll
-          for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) dp[b][r] *= 1.f - th[b][r] * th[b][r];
-        }
-        if (masked) {
-#pragma unroll
-          for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (!sees(row0 + 16 * b + 4 * g + r, seen)) s[b][r] = dp[b][r] = 0.f;
-        }
-        add_weighted<T, DP>(dv, s, ds, s_bad[4] | s_bad[5] | s_bad[6] | s_bad[7], row0, seen, lane);
-        gs.apply(dp, dk);
-        add_weighted<T, DP>(dk, dp, qs, s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3], row0, seen, lane);
+        add_weighted<T, DP, NQ>(dv, s, ds[at] + p * lds_row<T, DP>, bad_d, row0, kept.seen, lane);
+        add_weighted<T, DP, NQ>(dk, dp, qs[at] + p * lds_row<T, DP>, bad_q, row0, kept.seen, lane);
       }
-      __syncthreads();
+      if (more) put(at ^ 1);
     }
   }
-  if (there) {
-    const int64_t at = (j * a.kv_heads + kh) * a.dim;
-    store_row<T, DP>((T*)a.dk + at, dk, gs.undo() * (a.scale * W_UNSHIFT), a.dim, g);
-    store_row<T, DP>((T*)a.dv + at, dv, W_UNSHIFT, a.dim, g);
-  }
+#pragma unroll
+  for (int q = 0; q < NQ; ++q)
+    if (kept.there[q]) {
+      const int64_t to = (kept.row[q] * a.kv_heads + kh) * a.dim;
+      store_row<T, DP>((T*)a.dk + to, dk[q], gs[q].undo() * (a.scale * W_UNSHIFT), a.dim, g);
+      store_row<T, DP>((T*)a.dv + to, dv[q], W_UNSHIFT, a.dim, g);
+    }
 }
 
 // One query at a time: a wavefront takes query i, the heads of one key head along its columns, and part `split` of the
 // query's keys.  K comes straight into the operand's registers, V through the wavefront's own LDS rows (for the
 // transposing read).  Nothing is shared, so nothing waits.
-template <typename T, int DP>
+template <typename T, int DP, bool CAP>
 __global__ __launch_bounds__(AT_NT) void k_attn_row(ffn_ray_attn a, int splits, int64_t total) {
   constexpr int KS = DP / 32, NB = DP / 16;
-  __shared__ T vs_all[4][AT_TILE * lds_row<T, DP>];
-  __shared__ float ts_all[4][AT_TILE];
+  __shared__ __align__(16) T vs_all[4][AT_TILE * lds_row<T, DP>];
+  __shared__ __align__(16) float ts_all[4][AT_TILE];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
   const int64_t work = (int64_t)blockIdx.x * 4 + wave;
   if (work >= total) return;  // no barriers below
@@ -586,12 +722,15 @@ __global__ __launch_bounds__(AT_NT) void k_attn_row(ffn_ray_attn a, int splits, 
   const int kh = (int)(work % a.kv_heads);
   const int split = (int)(work / a.kv_heads % splits);
   const int64_t i = work / a.kv_heads / splits;
-  Range seen = keys_of(a, i);
+  Range seen[1] = {keys_of(a, i)};
+  seen[0].lo = __builtin_amdgcn_readfirstlane(seen[0].lo);
+  seen[0].hi = __builtin_amdgcn_readfirstlane(seen[0].hi);
   if (splits > 1) {  // whole tiles
-    const int tiles = (seen.hi - seen.lo + AT_TILE - 1) / AT_TILE;
+    const int tiles = (seen[0].hi - seen[0].lo + AT_TILE - 1) / AT_TILE;
     const int from = (int)((int64_t)tiles * split / splits), to = (int)((int64_t)tiles * (split + 1) / splits);
-    seen = {seen.lo + from * AT_TILE, min(seen.hi, seen.lo + to * AT_TILE)};
+    seen[0] = {seen[0].lo + from * AT_TILE, min(seen[0].hi, seen[0].lo + to * AT_TILE)};
   }
+  const int lo = seen[0].lo, hi = seen[0].hi;
   const T* kb = (const T*)a.k + kh * a.k_head;
   const T* vb = (const T*)a.v + kh * a.v_head;
   for (int h0 = 0; h0 < group; h0 += 16) {
@@ -599,12 +738,12 @@ __global__ __launch_bounds__(AT_NT) void k_attn_row(ffn_ray_attn a, int splits, 
     const int head = kh * group + min(h0 + c, group - 1);
     typename Mat<T>::frag qf[KS];
     load_frags<T, KS>(qf, (const T*)a.q + i * a.q_row + head * a.q_head, there, a.dim, g);
-    const Logits logits(a, head);
+    const Logits<CAP> logits(a, head);
     const float t = logits.bias ? a.t_q[i * a.t_q_row] : 0.f;
-    f32x4 acc[NB];
+    f32x4 acc[1][NB];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-    Softmax sm;
+    for (int b = 0; b < NB; ++b) acc[0][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Softmax<T> sm;
     Staged<T, DP, 64> vst;
     typename Mat<T>::frag kf[4][KS];
     float tst = 0.f;
@@ -612,34 +751,38 @@ __global__ __launch_bounds__(AT_NT) void k_attn_row(ffn_ray_attn a, int splits, 
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const int row = row0 + 16 * b + c;
-        load_frags<T, KS>(kf[b], kb + row * a.k_row, row < seen.hi, a.dim, g);
+        load_frags<T, KS>(kf[b], kb + row * a.k_row, row < hi, a.dim, g);
       }
-      vst.load(vb, a.v_row, row0, seen.hi, a.dim, lane);
-      if (logits.bias && row0 + lane < seen.hi) tst = a.t_k[(int64_t)(row0 + lane) * a.t_k_row];
+      vst.load(vb, a.v_row, row0, hi, a.dim, lane);
+      if (logits.bias && row0 + lane < hi) tst = a.t_k[(int64_t)(row0 + lane) * a.t_k_row];
     };
-    if (seen.lo < seen.hi) fetch(seen.lo);
-    for (int row0 = seen.lo; row0 < seen.hi; row0 += AT_TILE) {
-      f32x4 s[4], th[4];
+    if (lo < hi) fetch(lo);
+    for (int row0 = lo; row0 < hi; row0 += AT_TILE) {
+      Piece s[2];
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        s[b >> 1][b & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < KS; ++k) s[b] = Mat<T>::mma(kf[b][k], qf[k], s[b]);
+        for (int k = 0; k < KS; ++k) s[b >> 1][b & 1] = Mat<T>::mma(kf[b][k], qf[k], s[b >> 1][b & 1]);
       }
       vst.store(vs, lane);
       ts[lane] = tst;
-      if (seen.hi - row0 > AT_TILE) fetch(row0 + AT_TILE);
+      if (hi - row0 > AT_TILE) fetch(row0 + AT_TILE);
       wave_sync();
-      logits(s, th, t, ts, g);
-      if (seen.hi - row0 < AT_TILE) {
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (row0 + 16 * b + 4 * g + r >= seen.hi) s[b][r] = -INFINITY;
+      for (int p = 0; p < 2; ++p) {
+        const int from = row0 + PIECE * p;
+        if (from >= hi) break;
+        Piece th, w[1];
+        logits(s[p], th, t, ts + PIECE * p, g);
+        if (hi - from < PIECE)
+          each([&](int b, int r) {
+            if (from + 16 * b + 4 * g + r >= hi) s[p][b][r] = -INFINITY;
+          });
+        sm.step(s[p], logits.mul, acc[0]);
+        w[0][0] = s[p][0], w[0][1] = s[p][1];
+        add_weighted<T, DP, 1>(acc, w, vs + PIECE * p * lds_row<T, DP>, false, from, seen, lane);
       }
-      sm.step(s, acc);
-      add_weighted<T, DP>(acc, s, vs, false, row0, seen, lane);
       wave_sync();
     }
     if (splits == 1) {
@@ -647,7 +790,7 @@ __global__ __launch_bounds__(AT_NT) void k_attn_row(ffn_ray_attn a, int splits, 
       const float by = sm.finish(lse);
       if (there) {
         const int64_t at = i * a.heads + head;
-        store_row<T, DP>((T*)a.o + at * a.dim, acc, by, a.dim, g);
+        store_row<T, DP>((T*)a.o + at * a.dim, acc[0], by, a.dim, g);
         if (g == 0) a.lse[at] = lse;
       }
     } else {
@@ -655,7 +798,7 @@ __global__ __launch_bounds__(AT_NT) void k_attn_row(ffn_ray_attn a, int splits, 
       if (there) {
         const int64_t rows = (int64_t)a.q_rays.n * a.heads, at = split * rows + i * a.heads + head;
         float* part = (float*)a.workspace;
-        store_row<float, DP>(part + at * a.dim, acc, 1.f, a.dim, g);
+        store_row<float, DP>(part + at * a.dim, acc[0], 1.f, a.dim, g);
         if (g == 0) reinterpret_cast<float2*>(part + splits * rows * a.dim)[at] = make_float2(sm.m, l);
       }
     }
@@ -711,40 +854,60 @@ uint64_t attn_workspace(const ffn_ray_attn& a, bool backward) {
   return s > 1 ? s * rows * (a.dim + 2) * sizeof(float) : 0;
 }
 
-static unsigned die_grid(int64_t total) { return (unsigned)((total + 7) / 8 * 8); }
+static unsigned die_grid(int64_t total) { return (unsigned)((total + 8 * DIE_RUN - 1) / (8 * DIE_RUN) * (8 * DIE_RUN)); }
 
+// Sets of 16 kept rows a wavefront: two where rays are long on both sides and the registers hold them
+template <typename T, int DP> constexpr int MAX_SETS = sizeof(T) == 2 && DP <= 64 ? 2 : 1;
+#ifndef LONGRAY
+#define LONGRAY 256
+#endif
 template <typename T, int DP>
+static int sets(const ffn_ray_set& kept, const ffn_ray_set& streamed) {
+  const int64_t rays = kept.num_rays;
+  return kept.n >= LONGRAY * rays && streamed.n >= LONGRAY * rays ? MAX_SETS<T, DP> : 1;
+}
+
+template <typename T, int DP, bool CAP>
 static hipError_t fwd(const ffn_ray_attn& a, hipStream_t st) {
   if (by_row(a)) {
     const int splits = row_splits(a);
     const int64_t total = (int64_t)a.q_rays.n * a.kv_heads * splits;
-    k_attn_row<T, DP><<<(unsigned)((total + 3) / 4), AT_NT, 0, st>>>(a, splits, total);
+    k_attn_row<T, DP, CAP><<<(unsigned)((total + 3) / 4), AT_NT, 0, st>>>(a, splits, total);
     if (splits > 1) k_attn_join<T><<<(unsigned)(((int64_t)a.q_rays.n * a.heads + 3) / 4), AT_NT, 0, st>>>(a, splits);
   } else {
-    const int64_t total = ((int64_t)a.q_rays.n + AT_TILE - 1) / AT_TILE * a.heads;
-    k_attn_fwd<T, DP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
+    const int64_t rows = 64 * sets<T, DP>(a.q_rays, a.k_rays), total = ((int64_t)a.q_rays.n + rows - 1) / rows * a.heads;
+    if (rows > 64) k_attn_fwd<T, DP, MAX_SETS<T, DP>, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
+    else k_attn_fwd<T, DP, 1, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
+  }
+  return hipGetLastError();
+}
+
+template <typename T, int DP, bool CAP>
+static hipError_t bwd(const ffn_ray_attn& a, hipStream_t st) {
+  if (a.q_rays.n) {
+    const int64_t rows = 64 * sets<T, DP>(a.q_rays, a.k_rays), total = ((int64_t)a.q_rays.n + rows - 1) / rows * a.heads;
+    if (rows > 64) k_attn_dq<T, DP, MAX_SETS<T, DP>, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
+    else k_attn_dq<T, DP, 1, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
+  }
+  if (a.k_rays.n) {
+    const int64_t rows = 64 * sets<T, DP>(a.k_rays, a.q_rays), total = ((int64_t)a.k_rays.n + rows - 1) / rows * a.kv_heads;
+    if (rows > 64) k_attn_dkv<T, DP, MAX_SETS<T, DP>, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
+    else k_attn_dkv<T, DP, 1, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
   }
   return hipGetLastError();
 }
 
 template <typename T, int DP>
-static hipError_t bwd(const ffn_ray_attn& a, hipStream_t st) {
-  if (a.q_rays.n) {
-    const int64_t total = ((int64_t)a.q_rays.n + AT_TILE - 1) / AT_TILE * a.heads;
-    k_attn_dq<T, DP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
-  }
-  if (a.k_rays.n) {
-    const int64_t total = ((int64_t)a.k_rays.n + AT_TILE - 1) / AT_TILE * a.kv_heads;
-    k_attn_dkv<T, DP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
-  }
-  return hipGetLastError();
+static hipError_t by_cap(const ffn_ray_attn& a, bool backward, hipStream_t st) {
+  if (a.cap > 0.f) return backward ? bwd<T, DP, true>(a, st) : fwd<T, DP, true>(a, st);
+  return backward ? bwd<T, DP, false>(a, st) : fwd<T, DP, false>(a, st);
 }
 
 template <typename T>
 static hipError_t by_dim(const ffn_ray_attn& a, bool backward, hipStream_t st) {
-  if (a.dim <= 32) return backward ? bwd<T, 32>(a, st) : fwd<T, 32>(a, st);
-  if (a.dim <= 64) return backward ? bwd<T, 64>(a, st) : fwd<T, 64>(a, st);
-  return backward ? bwd<T, 128>(a, st) : fwd<T, 128>(a, st);
+  if (a.dim <= 32) return by_cap<T, 32>(a, backward, st);
+  if (a.dim <= 64) return by_cap<T, 64>(a, backward, st);
+  return by_cap<T, 128>(a, backward, st);
 }
 
 hipError_t launch_attn(const ffn_ray_attn& a, bool backward, hipStream_t st) {
