@@ -63,16 +63,23 @@ __device__ __forceinline__ float swap_max(float v) {
 struct Span {
   int lo, hi, all_lo, all_hi;
 };
+// v of the lane N further on among the same 16
+template <int N> __device__ __forceinline__ int turn16(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, 0x120 + N, 0xF, 0xF, true);  // row_ror:N
+}
+template <int N> __device__ __forceinline__ void span_step(Span& s) {
+  s.lo = min(s.lo, turn16<N>(s.lo));
+  s.hi = max(s.hi, turn16<N>(s.hi));
+  s.all_lo = max(s.all_lo, turn16<N>(s.all_lo));
+  s.all_hi = min(s.all_hi, turn16<N>(s.all_hi));
+}
 __device__ __forceinline__ Span span_of(const Range& r) {
   const bool none = r.hi <= r.lo;
   Span s{none ? INT_MAX : r.lo, none ? 0 : r.hi, none ? INT_MAX : r.lo, none ? 0 : r.hi};
-#pragma unroll
-  for (int m = 1; m < 16; m *= 2) {
-    s.lo = min(s.lo, __shfl_xor(s.lo, m));
-    s.hi = max(s.hi, __shfl_xor(s.hi, m));
-    s.all_lo = max(s.all_lo, __shfl_xor(s.all_lo, m));
-    s.all_hi = min(s.all_hi, __shfl_xor(s.all_hi, m));
-  }
+  span_step<8>(s);
+  span_step<4>(s);
+  span_step<2>(s);
+  span_step<1>(s);
   s.lo = __builtin_amdgcn_readfirstlane(s.lo);
   s.hi = __builtin_amdgcn_readfirstlane(s.hi);
   s.all_lo = __builtin_amdgcn_readfirstlane(s.all_lo);
@@ -83,32 +90,55 @@ __device__ __forceinline__ bool sees(int row, const Range& r) {
   return (unsigned)(row - r.lo) < (unsigned)(r.hi - r.lo);
 }
 
-// AT_TILE rows of one head on their way to LDS (rows outside [row0, end) and columns past dim as 0)
+// AT_TILE rows of one head on their way to LDS, tile after tile (rows outside [row, end) and columns past dim as 0)
 template <typename T, int DP, int NT = AT_NT>
 struct Staged {
-  static constexpr int EL = 16 / (int)sizeof(T), CPR = DP / EL, N = AT_TILE * CPR / NT;
+  static constexpr int EL = 16 / (int)sizeof(T), CPR = DP / EL, N = AT_TILE * CPR / NT, STEP = NT / CPR;
   uint4 v[N];
-  __device__ __forceinline__ void load(const T* __restrict__ base, int64_t stride, int row0, int end, int dim, int tid) {
+  const T* p;   // this thread's first 16 bytes of the next tile
+  int64_t row_step, tile_step;
+  int row;      // and their row; past any end where the column is past dim
+  __device__ __forceinline__ void begin(const T* __restrict__ base, int64_t stride, int row0, int dim, int tid) {
+    const int col = tid % CPR * EL;
+    row = col < dim ? row0 + tid / CPR : INT_MAX;
+    p = base + (int64_t)(row0 + tid / CPR) * stride + col;
+    row_step = STEP * stride;
+    tile_step = AT_TILE * stride;
+  }
+  __device__ __forceinline__ void load(int end) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = tid + i * NT, row = row0 + c / CPR, col = (c % CPR) * EL;
       v[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (row < end && col < dim) v[i] = *reinterpret_cast<const uint4*>(base + row * stride + col);
+      if (row < end - i * STEP) v[i] = *reinterpret_cast<const uint4*>(p + i * row_step);
     }
+    p += tile_step;
+    row += row == INT_MAX ? 0 : AT_TILE;
   }
   __device__ __forceinline__ void store(T* tile, int tid) const {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = tid + i * NT;
-      *reinterpret_cast<uint4*>(tile + (c / CPR) * lds_row<T, DP> + (c % CPR) * EL) = v[i];
-    }
+    for (int i = 0; i < N; ++i)
+      *reinterpret_cast<uint4*>(tile + (tid / CPR + i * STEP) * lds_row<T, DP> + (tid % CPR) * EL) = v[i];
   }
-  // whether any of this thread's values is infinite or NaN
+  // whether any of this thread's values is infinite or NaN: their largest magnitude, as integers
   __device__ __forceinline__ bool nonfinite() const {
-    bool bad = false;
+    if constexpr (sizeof(T) == 4) {
+      unsigned m = 0u;
 #pragma unroll
-    for (int i = 0; i < N; ++i) bad |= any_nonfinite<T>(v[i]);
-    return bad;
+      for (int i = 0; i < N; ++i)
+        m = max(max(m, max(v[i].x & 0x7FFFFFFFu, v[i].y & 0x7FFFFFFFu)), max(v[i].z & 0x7FFFFFFFu, v[i].w & 0x7FFFFFFFu));
+      return m >= 0x7F800000u;
+    } else {
+      typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+      u16x2 m = {0, 0};
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const unsigned w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[k] & 0x7FFF7FFFu));
+      }
+      constexpr unsigned short e = __is_same(T, __bf16) ? 0x7F80 : 0x7C00;
+      return max(m[0], m[1]) >= e;
+    }
   }
 };
 
@@ -125,12 +155,16 @@ __device__ __forceinline__ void load_frags(typename Mat<T>::frag (&f)[KS], const
   }
 }
 
-// tanh to single precision.  Pieces whose arguments all lie in [-1, 1], the usual ones, take the quotient of Lambert's
-// continued fraction (error 4e-8 at 1); others 1 - 2 / (1 + e^2x), and the odd series where that would cancel.
+// tanh to single precision.  Pieces whose arguments all lie within NEAR, the usual ones, take a minimax polynomial of
+// x^2 (relative error 3e-8); others 1 - 2 / (1 + e^2x), and the odd series where that would cancel.
+constexpr float NEAR = 0.75f;
 __device__ __forceinline__ float tanh_near(float x) {
   const float x2 = x * x;
-  const float n = __builtin_fmaf(x2, x2 + 105.f, 945.f), d = __builtin_fmaf(x2, __builtin_fmaf(x2, 15.f, 420.f), 945.f);
-  return x * n * __builtin_amdgcn_rcpf(d);
+  float p = __builtin_fmaf(x2, -0.004716258f, 0.019582909f);
+  p = __builtin_fmaf(x2, p, -0.053344432f);
+  p = __builtin_fmaf(x2, p, 0.13325407f);
+  p = __builtin_fmaf(x2, p, -0.33332959f);
+  return __builtin_fmaf(x * x2, p, x);
 }
 __device__ __forceinline__ float tanh_any(float x) {
   const float x2 = x * x;
@@ -177,7 +211,7 @@ struct Logits {
         th[b][r] = s[b][r] * inv_cap;
         top = fmaxf(top, fabsf(th[b][r]));
       });
-      if (__any(!(top <= 1.f))) each([&](int b, int r) { th[b][r] = tanh_any(th[b][r]); });
+      if (__any(!(top <= NEAR))) each([&](int b, int r) { th[b][r] = tanh_any(th[b][r]); });
       else each([&](int b, int r) { th[b][r] = tanh_near(th[b][r]); });
       each([&](int b, int r) { s[b][r] = cap2 * th[b][r]; });
     } else if (pre != 1.f) {
@@ -385,8 +419,9 @@ __global__ __launch_bounds__(AT_NT) void k_attn_fwd(ffn_ray_attn a, int64_t tota
   const int64_t work = die_order();
   if (work >= total) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
-  const int head = (int)(work % a.heads), kh = head / (a.heads / a.kv_heads);
-  const Kept<NQ> kept(work / a.heads * (64 * NQ) + wave * 16 * NQ, a.q_rays.n, c, [&](int64_t i) { return keys_of(a, i); });
+  const unsigned item = (unsigned)work;
+  const int head = (int)(item % (unsigned)a.heads), kh = head / (a.heads / a.kv_heads);
+  const Kept<NQ> kept((int64_t)(item / (unsigned)a.heads) * (64 * NQ) + wave * 16 * NQ, a.q_rays.n, c, [&](int64_t i) { return keys_of(a, i); });
   const Logits<CAP> logits(a, head);
   typename Mat<T>::frag qf[NQ][KS];
   float t[NQ];
@@ -399,8 +434,6 @@ __global__ __launch_bounds__(AT_NT) void k_attn_fwd(ffn_ray_attn a, int64_t tota
   for (int q = 0; q < NQ; ++q) arrived(qf[q]);
   arrived(t);
   const Range range = block_range(kept.lo, kept.hi, wave, lane, s_range);
-  const T* kb = (const T*)a.k + kh * a.k_head;
-  const T* vb = (const T*)a.v + kh * a.v_head;
   f32x4 acc[NQ][NB];
   Softmax<T> sm[NQ];
 #pragma unroll
@@ -408,10 +441,12 @@ __global__ __launch_bounds__(AT_NT) void k_attn_fwd(ffn_ray_attn a, int64_t tota
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[q][b] = f32x4{0.f, 0.f, 0.f, 0.f};
   Staged<T, DP> kst, vst;
+  kst.begin((const T*)a.k + kh * a.k_head, a.k_row, range.lo, a.dim, tid);
+  vst.begin((const T*)a.v + kh * a.v_head, a.v_row, range.lo, a.dim, tid);
   float tst = 0.f;
   auto fetch = [&](int row0) {
-    kst.load(kb, a.k_row, row0, range.hi, a.dim, tid);
-    vst.load(vb, a.v_row, row0, range.hi, a.dim, tid);
+    kst.load(range.hi);
+    vst.load(range.hi);
     if (logits.bias && tid < AT_TILE && row0 + tid < range.hi) tst = a.t_k[(int64_t)(row0 + tid) * a.t_k_row];
   };
   auto put = [&](int to) {
@@ -503,8 +538,9 @@ __global__ __launch_bounds__(AT_NT) void k_attn_dq(ffn_ray_attn a, int64_t total
   const int64_t work = die_order();
   if (work >= total) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
-  const int head = (int)(work % a.heads), kh = head / (a.heads / a.kv_heads);
-  const Kept<NQ> kept(work / a.heads * (64 * NQ) + wave * 16 * NQ, a.q_rays.n, c, [&](int64_t i) { return keys_of(a, i); });
+  const unsigned item = (unsigned)work;
+  const int head = (int)(item % (unsigned)a.heads), kh = head / (a.heads / a.kv_heads);
+  const Kept<NQ> kept((int64_t)(item / (unsigned)a.heads) * (64 * NQ) + wave * 16 * NQ, a.q_rays.n, c, [&](int64_t i) { return keys_of(a, i); });
   const Logits<CAP> logits(a, head);
   typename Mat<T>::frag qf[NQ][KS], df[NQ][KS];
   float t[NQ], delta[NQ], from[NQ];
@@ -534,8 +570,6 @@ __global__ __launch_bounds__(AT_NT) void k_attn_dq(ffn_ray_attn a, int64_t total
   arrived(t);
   arrived(from);
   const Range range = block_range(kept.lo, kept.hi, wave, lane, s_range);
-  const T* kb = (const T*)a.k + kh * a.k_head;
-  const T* vb = (const T*)a.v + kh * a.v_head;
   f32x4 acc[NQ][NB];
   GradScale<T> gs[NQ];
 #pragma unroll
@@ -543,10 +577,12 @@ __global__ __launch_bounds__(AT_NT) void k_attn_dq(ffn_ray_attn a, int64_t total
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[q][b] = f32x4{0.f, 0.f, 0.f, 0.f};
   Staged<T, DP> kst, vst;
+  kst.begin((const T*)a.k + kh * a.k_head, a.k_row, range.lo, a.dim, tid);
+  vst.begin((const T*)a.v + kh * a.v_head, a.v_row, range.lo, a.dim, tid);
   float tst = 0.f;
   auto fetch = [&](int row0) {
-    kst.load(kb, a.k_row, row0, range.hi, a.dim, tid);
-    vst.load(vb, a.v_row, row0, range.hi, a.dim, tid);
+    kst.load(range.hi);
+    vst.load(range.hi);
     if (logits.bias && tid < AT_TILE && row0 + tid < range.hi) tst = a.t_k[(int64_t)(row0 + tid) * a.t_k_row];
   };
   auto put = [&](int to) {
@@ -605,8 +641,9 @@ __global__ __launch_bounds__(AT_NT) void k_attn_dkv(ffn_ray_attn a, int64_t tota
   const int64_t work = die_order();
   if (work >= total) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
-  const int kh = (int)(work % a.kv_heads), group = a.heads / a.kv_heads;
-  const Kept<NQ> kept(work / a.kv_heads * (64 * NQ) + wave * 16 * NQ, a.k_rays.n, c, [&](int64_t j) { return queries_of(a, j); });
+  const unsigned item = (unsigned)work;
+  const int kh = (int)(item % (unsigned)a.kv_heads), group = a.heads / a.kv_heads;
+  const Kept<NQ> kept((int64_t)(item / (unsigned)a.kv_heads) * (64 * NQ) + wave * 16 * NQ, a.k_rays.n, c, [&](int64_t j) { return queries_of(a, j); });
   const bool bias = a.slopes != nullptr;
   typename Mat<T>::frag kf[NQ][KS], vf[NQ][KS];
   float t[NQ];
@@ -633,8 +670,12 @@ __global__ __launch_bounds__(AT_NT) void k_attn_dkv(ffn_ray_attn a, int64_t tota
   Staged<T, DP> qst, dst;
   float tst = 0.f, lst = 0.f, est = 0.f;
   auto fetch = [&](int head, int row0) {
-    qst.load((const T*)a.q + head * a.q_head, a.q_row, row0, range.hi, a.dim, tid);
-    dst.load((const T*)a.dout + head * a.do_head, a.do_row, row0, range.hi, a.dim, tid);
+    if (row0 == range.lo) {
+      qst.begin((const T*)a.q + head * a.q_head, a.q_row, row0, a.dim, tid);
+      dst.begin((const T*)a.dout + head * a.do_head, a.do_row, row0, a.dim, tid);
+    }
+    qst.load(range.hi);
+    dst.load(range.hi);
     if (tid < AT_TILE && row0 + tid < range.hi) {
       const int64_t i = row0 + tid;
       if (bias) tst = a.t_q[i * a.t_q_row];
@@ -732,7 +773,6 @@ __global__ __launch_bounds__(AT_NT) void k_attn_row(ffn_ray_attn a, int splits, 
   }
   const int lo = seen[0].lo, hi = seen[0].hi;
   const T* kb = (const T*)a.k + kh * a.k_head;
-  const T* vb = (const T*)a.v + kh * a.v_head;
   for (int h0 = 0; h0 < group; h0 += 16) {
     const bool there = h0 + c < group;
     const int head = kh * group + min(h0 + c, group - 1);
@@ -746,6 +786,7 @@ __global__ __launch_bounds__(AT_NT) void k_attn_row(ffn_ray_attn a, int splits, 
     Softmax<T> sm;
     Staged<T, DP, 64> vst;
     typename Mat<T>::frag kf[4][KS];
+    vst.begin((const T*)a.v + kh * a.v_head, a.v_row, lo, a.dim, lane);
     float tst = 0.f;
     auto fetch = [&](int row0) {
 #pragma unroll
@@ -753,7 +794,7 @@ __global__ __launch_bounds__(AT_NT) void k_attn_row(ffn_ray_attn a, int splits, 
         const int row = row0 + 16 * b + c;
         load_frags<T, KS>(kf[b], kb + row * a.k_row, row < hi, a.dim, g);
       }
-      vst.load(vb, a.v_row, row0, hi, a.dim, lane);
+      vst.load(hi);
       if (logits.bias && row0 + lane < hi) tst = a.t_k[(int64_t)(row0 + lane) * a.t_k_row];
     };
     if (lo < hi) fetch(lo);

@@ -93,21 +93,4 @@ __device__ __forceinline__ typename Mat<T>::frag product_frag(const f32x4& lo, c
   return __builtin_convertvector(both, typename Mat<T>::frag);
 }
 
-// whether 16 bytes of T hold an infinity or a NaN
-template <typename T> __device__ __forceinline__ bool any_nonfinite(const uint4& v) {
-  const unsigned w[4] = {v.x, v.y, v.z, v.w};
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (sizeof(T) == 4) {
-      bad |= (w[i] & 0x7F800000u) == 0x7F800000u;
-    } else {
-      constexpr unsigned e = __is_same(T, __bf16) ? 0x7F80u : 0x7C00u;
-      bad |= (w[i] & e) == e;
-      bad |= (w[i] & (e << 16)) == (e << 16);
-    }
-  }
-  return bad;
-}
-
 }  // namespace ffn
