@@ -14,6 +14,15 @@ namespace ffn {
 constexpr int AT_NT = 256, AT_TILE = 64;  // four wavefronts; rows of a streamed tile
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
+// Wavefronts a SIMD that the registers are held to: a wavefront waits more than it computes, so that one more is worth more
+// than a few registers (16 bits; dk and dv of 8192 short rays: 139 us with three, 117 with four).
+constexpr int least_waves(int size, int dim, int sets, bool cap) {
+  return size == 2 && dim == 32 ? 5 - sets : size == 2 && dim == 64 && sets == 2 && !cap ? 3 : 1;
+}
+constexpr int least_waves_dkv(int size, int dim, int sets, bool cap) {
+  return size == 2 && sets == 1 && dim == 32 ? 4 : size == 2 && sets == 1 && dim == 64 && !cap ? 3 : 1;
+}
+
 struct Range {
   int lo, hi;
 };
@@ -177,12 +186,13 @@ __device__ __forceinline__ float tanh_any(float x) {
   return fabsf(x) < 0.25f ? small : big;
 }
 
-// A piece of 32 streamed rows is what is scored, masked and skipped at once: two product tiles.
+// Streamed rows are scored, masked and skipped in pieces of 32: B = 2 product tiles at once (4 in k_attn_row).  Whole tiles
+// of 64 at once take a third more registers, and the wavefronts that costs are worth more: 108 us instead of 81 for the
+// forward of 8192 short rays, 692 instead of 594 for dk and dv of long ones.
 constexpr int PIECE = 32;
-typedef f32x4 Piece[2];
-template <typename F> __device__ __forceinline__ void each(F f) {
+template <int B, typename F> __device__ __forceinline__ void each(F f) {
 #pragma unroll
-  for (int b = 0; b < 2; ++b)
+  for (int b = 0; b < B; ++b)
 #pragma unroll
     for (int r = 0; r < 4; ++r) f(b, r);
 }
@@ -204,22 +214,23 @@ struct Logits {
     pre = bare ? 1.f : scale2;
     slope = bias ? a.slopes[head] * LOG2E / mul : 0.f;
   }
-  __device__ __forceinline__ void operator()(Piece& s, Piece& th, float t, const float* x, int g) const {
+  template <int B>
+  __device__ __forceinline__ void operator()(f32x4 (&s)[B], f32x4 (&th)[B], float t, const float* x, int g) const {
     if constexpr (CAP) {
       float top = 0.f;
-      each([&](int b, int r) {
+      each<B>([&](int b, int r) {
         th[b][r] = s[b][r] * inv_cap;
         top = fmaxf(top, fabsf(th[b][r]));
       });
-      if (__any(!(top <= NEAR))) each([&](int b, int r) { th[b][r] = tanh_any(th[b][r]); });
-      else each([&](int b, int r) { th[b][r] = tanh_near(th[b][r]); });
-      each([&](int b, int r) { s[b][r] = cap2 * th[b][r]; });
+      if (__any(!(top <= NEAR))) each<B>([&](int b, int r) { th[b][r] = tanh_any(th[b][r]); });
+      else each<B>([&](int b, int r) { th[b][r] = tanh_near(th[b][r]); });
+      each<B>([&](int b, int r) { s[b][r] = cap2 * th[b][r]; });
     } else if (pre != 1.f) {
-      each([&](int b, int r) { s[b][r] *= pre; });
+      each<B>([&](int b, int r) { s[b][r] *= pre; });
     }
     if (bias) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < B; ++b) {
         const f32x4 tx = *reinterpret_cast<const f32x4*>(x + 16 * b + 4 * g);
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[b][r] = __builtin_fmaf(-slope, fabsf(t - tx[r]), s[b][r]);
@@ -228,12 +239,12 @@ struct Logits {
   }
 };
 
-// s[q] = 32 tile rows . kept rows of set q
-template <typename T, int DP, int NQ>
-__device__ __forceinline__ void products(Piece (&s)[NQ], const T* tile, const typename Mat<T>::frag (&kept)[NQ][DP / 32],
+// s[q] = 16 B tile rows . kept rows of set q
+template <typename T, int DP, int NQ, int B>
+__device__ __forceinline__ void products(f32x4 (&s)[NQ][B], const T* tile, const typename Mat<T>::frag (&kept)[NQ][DP / 32],
                                          int lane) {
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
+  for (int b = 0; b < B; ++b) {
 #pragma unroll
     for (int q = 0; q < NQ; ++q) s[q][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -254,33 +265,36 @@ __device__ __forceinline__ typename Mat<T>::frag finite_frag(typename Mat<T>::fr
   return f;
 }
 
-// acc[q] += tile^T w[q]: the 32 tile rows are the K of the product.  Where the tile holds infinities or NaN (bad), pairs
+// acc[q] += tile^T w[q]: the 16 B tile rows are the K of the product.  Where the tile holds infinities or NaN (bad), pairs
 // that do not see each other must not meet, since a weight of 0 times them is not 0: the product takes them as 0, and the
 // pairs that do see each other are added one by one.
-template <typename T, int DP, int NQ>
-__device__ __forceinline__ void add_weighted(f32x4 (&acc)[NQ][DP / 16], const Piece (&w)[NQ], const T* tile, bool bad,
+template <typename T, int DP, int NQ, int B>
+__device__ __forceinline__ void add_weighted(f32x4 (&acc)[NQ][DP / 16], const f32x4 (&w)[NQ][B], const T* tile, bool bad,
                                              int row0, const Range (&seen)[NQ], int lane) {
-  typename Mat<T>::frag f[NQ], m[DP / 16];
 #pragma unroll
-  for (int db = 0; db < DP / 16; ++db) m[db] = col_frag<T, DP>(tile, 0, 16 * db, lane);
-  if (bad) {
+  for (int h = 0; h < B / 2; ++h) {
+    typename Mat<T>::frag f[NQ], m[DP / 16];
 #pragma unroll
-    for (int db = 0; db < DP / 16; ++db) m[db] = finite_frag<T>(m[db]);
+    for (int db = 0; db < DP / 16; ++db) m[db] = col_frag<T, DP>(tile, PIECE * h, 16 * db, lane);
+    if (bad) {
+#pragma unroll
+      for (int db = 0; db < DP / 16; ++db) m[db] = finite_frag<T>(m[db]);
+    }
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) f[q] = product_frag<T>(w[q][2 * h], w[q][2 * h + 1]);
+#pragma unroll
+    for (int db = 0; db < DP / 16; ++db)
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) acc[q][db] = Mat<T>::mma(m[db], f[q], acc[q][db]);
   }
-#pragma unroll
-  for (int q = 0; q < NQ; ++q) f[q] = product_frag<T>(w[q][0], w[q][1]);
-#pragma unroll
-  for (int db = 0; db < DP / 16; ++db)
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) acc[q][db] = Mat<T>::mma(m[db], f[q], acc[q][db]);
   if (bad) {
     const int g = lane >> 4, c = lane & 15;
 #pragma unroll 1
-    for (int row = 0; row < PIECE; ++row) {
+    for (int row = 0; row < 16 * B; ++row) {
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
         float mine = 0.f;
-        each([&](int b, int r) { mine = row >> 4 == b && (row & 3) == r ? w[q][b][r] : mine; });
+        each<B>([&](int b, int r) { mine = row >> 4 == b && (row & 3) == r ? w[q][b][r] : mine; });
         const float ww = __shfl(mine, 16 * ((row >> 2) & 3) + c);
         const bool see = sees(row0 + row, seen[q]);
 #pragma unroll
@@ -297,9 +311,10 @@ __device__ __forceinline__ void add_weighted(f32x4 (&acc)[NQ][DP / 16], const Pi
 }
 
 // what is not seen gets `v`
-__device__ __forceinline__ void mask(Piece& s, int row0, const Span& w, const Range& seen, int g, float v) {
-  if (row0 < w.all_lo || row0 + PIECE > w.all_hi)
-    each([&](int b, int r) {
+template <int B>
+__device__ __forceinline__ void mask(f32x4 (&s)[B], int row0, const Span& w, const Range& seen, int g, float v) {
+  if (row0 < w.all_lo || row0 + 16 * B > w.all_hi)
+    each<B>([&](int b, int r) {
       if (!sees(row0 + 16 * b + 4 * g + r, seen)) s[b][r] = v;
     });
 }
@@ -322,6 +337,12 @@ __device__ __forceinline__ void store_row(T* __restrict__ row, const f32x4 (&acc
 // numbers end at 2^-14, and the exponential's at 2^-126 (it gives 0 below).
 constexpr float W_SHIFT = 14.f, W_UNSHIFT = 1.f / 16384.f;
 
+// log(l 2^(m - W_SHIFT)); the exponent of l goes to m, so that the logarithm is not rounded at its size
+__device__ __forceinline__ float log_sum(float m, float l) {
+  const float e = (float)__builtin_amdgcn_frexp_expf(l);
+  return l == 0.f ? -INFINITY : (m + (e - W_SHIFT) + __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(l))) * LN2;
+}
+
 // Running softmax of one row, its sum still apart by lane group.  m is a maximum that lags: it is raised, and the sums are
 // rescaled, only when a logit passes it by more than SLACK (which fp16's weights, 2^14 and more, have room for), so that
 // most pieces need no exchange between lanes.
@@ -330,10 +351,10 @@ struct Softmax {
   static constexpr float SLACK = __is_same(T, _Float16) ? 1.f : 8.f;
   float m = -INFINITY, l = 0.f;
   // weights in place of the logits
-  template <int NACC>
-  __device__ __forceinline__ void step(Piece& s, float mul, f32x4 (&acc)[NACC]) {
+  template <int B, int NACC>
+  __device__ __forceinline__ void step(f32x4 (&s)[B], float mul, f32x4 (&acc)[NACC]) {
     float mx = s[0][0];
-    each([&](int b, int r) { mx = fmaxf(mx, s[b][r]); });
+    each<B>([&](int b, int r) { mx = fmaxf(mx, s[b][r]); });
     mx *= mul;
     if (__any(mx > m + SLACK)) {
       mx = fmaxf(m, swap_max(mx));
@@ -346,7 +367,7 @@ struct Softmax {
       m = mx;
     }
     const float from = (m == -INFINITY ? 0.f : m) - W_SHIFT;
-    each([&](int b, int r) {
+    each<B>([&](int b, int r) {
       s[b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], mul, -from));
       l += s[b][r];
     });
@@ -354,16 +375,14 @@ struct Softmax {
   // factor of the sums, and the logarithm of the sum of exponentials
   __device__ __forceinline__ float finish(float& lse) {
     l = swap_add(l);
-    lse = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l) - W_SHIFT) * LN2;
+    lse = log_sum(m, l);
     return l == 0.f ? 0.f : 1.f / l;
   }
 };
 
 // Blocks in launch order go round the eight dies; this gives each die runs of DIE_RUN neighbouring pieces of work, whose
 // tiles share keys in its L2.  Longer runs leave the dies with unequal work where rays are few and long.
-#ifndef DIE_RUN
-#define DIE_RUN 16
-#endif
+constexpr int DIE_RUN = 16;
 __device__ __forceinline__ int64_t die_order() {
   const int64_t b = blockIdx.x >> 3;
   return (b / DIE_RUN * 8 + (blockIdx.x & 7)) * DIE_RUN + b % DIE_RUN;
@@ -407,10 +426,18 @@ __device__ __forceinline__ Range block_range(int lo, int hi, int wave, int lane,
   return {min(min(s[0], s[1]), min(s[2], s[3])), max(max(s[4], s[5]), max(s[6], s[7]))};
 }
 
+// the pieces of a tile that the wavefront needs
+template <typename F>
+__device__ __forceinline__ void take_tile(F& take, int tile, int lo, int hi) {
+  const bool one = tile < hi && tile + PIECE > lo, two = tile + PIECE < hi && tile + AT_TILE > lo;
+  if (one) take(0);
+  if (two) take(PIECE);
+}
+
 // NQ: sets of 16 queries a wavefront.  Two sets read each fragment of K and V once, which long rays are bound by; short
 // rays lose more to pieces that only one of the sets sees.
 template <typename T, int DP, int NQ, bool CAP>
-__global__ __launch_bounds__(AT_NT) void k_attn_fwd(ffn_ray_attn a, int64_t total) {
+__global__ __launch_bounds__(AT_NT, least_waves(sizeof(T), DP, NQ, CAP)) void k_attn_fwd(ffn_ray_attn a, int64_t total) {
   constexpr int KS = DP / 32, NB = DP / 16, TILE = AT_TILE * lds_row<T, DP>;
   __shared__ __align__(16) T ks[2][TILE];
   __shared__ __align__(16) T vs[2][TILE];
@@ -466,21 +493,20 @@ __global__ __launch_bounds__(AT_NT) void k_attn_fwd(ffn_ray_attn a, int64_t tota
     const bool more = range.hi - tile > AT_TILE;
     if (more) fetch(tile + AT_TILE);
     const bool bad = s_bad[at][0] | s_bad[at][1] | s_bad[at][2] | s_bad[at][3];
-#pragma unroll
-    for (int p = 0; p < AT_TILE; p += PIECE) {
+    constexpr int B = PIECE / 16;
+    auto take = [&](int p) {
       const int row0 = tile + p;
-      if (row0 >= kept.hi || row0 + PIECE <= kept.lo) continue;
-      Piece s[NQ];
-      products<T, DP, NQ>(s, ks[at] + p * lds_row<T, DP>, qf, lane);
+      f32x4 s[NQ][B], th[B];
+      products<T, DP, NQ, B>(s, ks[at] + p * lds_row<T, DP>, qf, lane);
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
-        Piece th;
         logits(s[q], th, t[q], ts[at] + p, g);
         mask(s[q], row0, kept.span[q], kept.seen[q], g, -INFINITY);
         sm[q].step(s[q], logits.mul, acc[q]);
       }
-      add_weighted<T, DP, NQ>(acc, s, vs[at] + p * lds_row<T, DP>, bad, row0, kept.seen, lane);
-    }
+      add_weighted<T, DP, NQ, B>(acc, s, vs[at] + p * lds_row<T, DP>, bad, row0, kept.seen, lane);
+    };
+    take_tile(take, tile, kept.lo, kept.hi);
     if (more) put(at ^ 1);
   }
 #pragma unroll
@@ -501,11 +527,11 @@ __global__ __launch_bounds__(AT_NT) void k_attn_fwd(ffn_ray_attn a, int64_t tota
 template <typename T>
 struct GradScale {
   float f = 0.f;
-  template <int NACC>
-  __device__ __forceinline__ void apply(Piece& s, f32x4 (&acc)[NACC]) {
+  template <int B, int NACC>
+  __device__ __forceinline__ void apply(f32x4 (&s)[B], f32x4 (&acc)[NACC]) {
     if constexpr (__is_same(T, _Float16)) {
       float mx = 0.f;
-      each([&](int b, int r) { mx = fmaxf(mx, fabsf(s[b][r])); });
+      each<B>([&](int b, int r) { mx = fmaxf(mx, fabsf(s[b][r])); });
       if (__any(mx * f > 32768.f || (f == 0.f && mx > 0.f))) {
         mx = swap_max(mx);
         const bool grow = mx > 0.f && (f == 0.f || mx * f > 32768.f);
@@ -518,7 +544,7 @@ struct GradScale {
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[i][r] *= by;
       }
-      each([&](int b, int r) { s[b][r] *= f; });
+      each<B>([&](int b, int r) { s[b][r] *= f; });
     }
   }
   __device__ __forceinline__ float undo() const {
@@ -527,9 +553,12 @@ struct GradScale {
   }
 };
 
-// dq; also leaves D = sum_d do o of its rows in the workspace for k_attn_dkv
+// dq; also leaves D of its rows in the workspace for k_attn_dkv.  D = sum_d do o takes o's rounding in 16 bits, and a short
+// ray's dq was a fifth further off for it.  So there it is a first value D' only: the sums are those of P (dP - D'), the
+// exact D = sum_j P dP is formed beside them, and (D' - D) sum_j P k, whose fragments of K are there already, sets dq
+// right (102 -> 110 us for 8192 rays).  Long rays (NQ = 2) have an o far smaller than v, and keep D': 328 us instead of 472.
 template <typename T, int DP, int NQ, bool CAP>
-__global__ __launch_bounds__(AT_NT) void k_attn_dq(ffn_ray_attn a, int64_t total) {
+__global__ __launch_bounds__(AT_NT, least_waves(sizeof(T), DP, NQ, CAP)) void k_attn_dq(ffn_ray_attn a, int64_t total) {
   constexpr int KS = DP / 32, NB = DP / 16, TILE = AT_TILE * lds_row<T, DP>;
   __shared__ __align__(16) T ks[2][TILE];
   __shared__ __align__(16) T vs[2][TILE];
@@ -543,7 +572,7 @@ __global__ __launch_bounds__(AT_NT) void k_attn_dq(ffn_ray_attn a, int64_t total
   const Kept<NQ> kept((int64_t)(item / (unsigned)a.heads) * (64 * NQ) + wave * 16 * NQ, a.q_rays.n, c, [&](int64_t i) { return keys_of(a, i); });
   const Logits<CAP> logits(a, head);
   typename Mat<T>::frag qf[NQ][KS], df[NQ][KS];
-  float t[NQ], delta[NQ], from[NQ];
+  float t[NQ], delta[NQ], from[NQ], exact[NQ];
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
     const int64_t i = kept.row[q], to = i * a.heads + head;
@@ -556,11 +585,12 @@ __global__ __launch_bounds__(AT_NT) void k_attn_dq(ffn_ray_attn a, int64_t total
     for (int k = 0; k < KS; ++k)
 #pragma unroll
       for (int j = 0; j < 8; ++j) d = __builtin_fmaf((float)of[k][j], (float)df[q][k][j], d);
-    delta[q] = swap_add(d);
+    d = swap_add(d);
+    delta[q] = kept.seen[q].hi > kept.seen[q].lo ? d : 0.f;  // a row that sees nothing gets 0 whatever it holds
+    exact[q] = 0.f;
     t[q] = logits.bias && kept.there[q] ? a.t_q[i * a.t_q_row] : 0.f;
     const float lse2 = kept.there[q] ? a.lse[to] * LOG2E : 0.f;
     from[q] = (lse2 == -INFINITY ? 0.f : lse2) - W_SHIFT;
-    if (kept.there[q] && g == 0) ((float*)a.workspace)[to] = delta[q];
   }
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
@@ -569,13 +599,19 @@ __global__ __launch_bounds__(AT_NT) void k_attn_dq(ffn_ray_attn a, int64_t total
   }
   arrived(t);
   arrived(from);
+  arrived(delta);
   const Range range = block_range(kept.lo, kept.hi, wave, lane, s_range);
-  f32x4 acc[NQ][NB];
+  constexpr bool EXACT = sizeof(T) == 2 && NQ == 1;
+  constexpr int SETS = EXACT ? 2 * NQ : NQ;  // sums of P (dP - D') k, and of P k
+  f32x4 acc[SETS][NB];
   GradScale<T> gs[NQ];
+  Range seen[SETS];
 #pragma unroll
-  for (int q = 0; q < NQ; ++q)
+  for (int q = 0; q < SETS; ++q) {
+    seen[q] = kept.seen[q % NQ];
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[q][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   Staged<T, DP> kst, vst;
   kst.begin((const T*)a.k + kh * a.k_head, a.k_row, range.lo, a.dim, tid);
   vst.begin((const T*)a.v + kh * a.v_head, a.v_row, range.lo, a.dim, tid);
@@ -602,37 +638,51 @@ __global__ __launch_bounds__(AT_NT) void k_attn_dq(ffn_ray_attn a, int64_t total
     const bool more = range.hi - tile > AT_TILE;
     if (more) fetch(tile + AT_TILE);
     const bool bad = s_bad[at][0] | s_bad[at][1] | s_bad[at][2] | s_bad[at][3];
-#pragma unroll
-    for (int p = 0; p < AT_TILE; p += PIECE) {
+    constexpr int B = PIECE / 16;
+    auto take = [&](int p) {
       const int row0 = tile + p;
-      if (row0 >= kept.hi || row0 + PIECE <= kept.lo) continue;
-      Piece s[NQ], dp[NQ];
-      products<T, DP, NQ>(s, ks[at] + p * lds_row<T, DP>, qf, lane);
-      products<T, DP, NQ>(dp, vs[at] + p * lds_row<T, DP>, df, lane);
+      f32x4 dp[NQ][B], th[B], s[SETS][B];  // s: the products, then the weights; the sets' logits come last
+      f32x4(&x)[NQ][B] = *reinterpret_cast<f32x4(*)[NQ][B]>(&s[SETS - NQ]);
+      products<T, DP, NQ, B>(x, ks[at] + p * lds_row<T, DP>, qf, lane);
+      products<T, DP, NQ, B>(dp, vs[at] + p * lds_row<T, DP>, df, lane);
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
-        Piece th;
-        logits(s[q], th, t[q], ts[at] + p, g);
-        each([&](int b, int r) {
-          s[q][b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[q][b][r], logits.mul, -from[q])) * (dp[q][b][r] - delta[q]);
-        });
-        if (CAP) each([&](int b, int r) { s[q][b][r] *= __builtin_fmaf(-th[b][r], th[b][r], 1.f); });
-        mask(s[q], row0, kept.span[q], kept.seen[q], g, 0.f);
+        logits(x[q], th, t[q], ts[at] + p, g);
+        each<B>([&](int b, int r) { x[q][b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][b][r], logits.mul, -from[q])); });
+        if constexpr (EXACT) {
+          mask(x[q], row0, kept.span[q], kept.seen[q], g, 0.f);
+          mask(dp[q], row0, kept.span[q], kept.seen[q], g, 0.f);
+          each<B>([&](int b, int r) { exact[q] = __builtin_fmaf(x[q][b][r], dp[q][b][r], exact[q]); });
+        }
+        // the slope of the cap
+        if (CAP) each<B>([&](int b, int r) { x[q][b][r] *= __builtin_fmaf(-th[b][r], th[b][r], 1.f); });
+        each<B>([&](int b, int r) { s[q][b][r] = x[q][b][r] * (dp[q][b][r] - delta[q]); });
+        if constexpr (!EXACT) mask(s[q], row0, kept.span[q], kept.seen[q], g, 0.f);
         gs[q].apply(s[q], acc[q]);
       }
-      add_weighted<T, DP, NQ>(acc, s, ks[at] + p * lds_row<T, DP>, bad, row0, kept.seen, lane);
-    }
+      add_weighted<T, DP, SETS, B>(acc, s, ks[at] + p * lds_row<T, DP>, bad, row0, seen, lane);
+    };
+    take_tile(take, tile, kept.lo, kept.hi);
     if (more) put(at ^ 1);
   }
 #pragma unroll
-  for (int q = 0; q < NQ; ++q)
-    if (kept.there[q])
-      store_row<T, DP>((T*)a.dq + (kept.row[q] * a.heads + head) * a.dim, acc[q], gs[q].undo() * (a.scale * W_UNSHIFT), a.dim, g);
+  for (int q = 0; q < NQ; ++q) {
+    const int64_t to = kept.row[q] * a.heads + head;
+    const float D = EXACT ? swap_add(exact[q]) * W_UNSHIFT : delta[q], off = delta[q] - D, by = gs[q].undo();
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[q][b][r] = EXACT ? __builtin_fmaf(acc[q][b][r], by, off * acc[SETS - NQ + q][b][r]) : acc[q][b][r] * by;
+    if (kept.there[q]) {
+      store_row<T, DP>((T*)a.dq + to * a.dim, acc[q], a.scale * W_UNSHIFT, a.dim, g);
+      if (g == 0) ((float*)a.workspace)[to] = D;
+    }
+  }
 }
 
 // dk and dv of the kept keys of one key head: the queries of the heads that share it stream past
 template <typename T, int DP, int NQ, bool CAP>
-__global__ __launch_bounds__(AT_NT) void k_attn_dkv(ffn_ray_attn a, int64_t total) {
+__global__ __launch_bounds__(AT_NT, least_waves_dkv(sizeof(T), DP, NQ, CAP)) void k_attn_dkv(ffn_ray_attn a, int64_t total) {
   constexpr int KS = DP / 32, NB = DP / 16, TILE = AT_TILE * lds_row<T, DP>;
   __shared__ __align__(16) T qs[2][TILE];
   __shared__ __align__(16) T ds[2][TILE];
@@ -705,19 +755,17 @@ __global__ __launch_bounds__(AT_NT) void k_attn_dkv(ffn_ray_attn a, int64_t tota
       if (more) fetch(rest ? head : head + 1, rest ? tile + AT_TILE : range.lo);
       const bool bad_q = s_bad[at][0] | s_bad[at][1] | s_bad[at][2] | s_bad[at][3];
       const bool bad_d = s_bad[at][4] | s_bad[at][5] | s_bad[at][6] | s_bad[at][7];
-#pragma unroll
-      for (int p = 0; p < AT_TILE; p += PIECE) {
+      constexpr int B = PIECE / 16;
+    auto take = [&](int p) {
         const int row0 = tile + p;
-        if (row0 >= kept.hi || row0 + PIECE <= kept.lo) continue;
-        Piece s[NQ], dp[NQ];
-        products<T, DP, NQ>(s, qs[at] + p * lds_row<T, DP>, kf, lane);
-        products<T, DP, NQ>(dp, ds[at] + p * lds_row<T, DP>, vf, lane);
+        f32x4 s[NQ][B], dp[NQ][B], th[B];
+        products<T, DP, NQ, B>(s, qs[at] + p * lds_row<T, DP>, kf, lane);
+        products<T, DP, NQ, B>(dp, ds[at] + p * lds_row<T, DP>, vf, lane);
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
-          Piece th;
           logits(s[q], th, t[q], ts[at] + p, g);
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
+          for (int b = 0; b < B; ++b) {
             const f32x4 l = *reinterpret_cast<const f32x4*>(ls[at] + p + 16 * b + 4 * g);
             const f32x4 e = *reinterpret_cast<const f32x4*>(es[at] + p + 16 * b + 4 * g);
 #pragma unroll
@@ -726,14 +774,15 @@ __global__ __launch_bounds__(AT_NT) void k_attn_dkv(ffn_ray_attn a, int64_t tota
               dp[q][b][r] = s[q][b][r] * (dp[q][b][r] - e[r]);
             }
           }
-          if (CAP) each([&](int b, int r) { dp[q][b][r] *= __builtin_fmaf(-th[b][r], th[b][r], 1.f); });
+          if (CAP) each<B>([&](int b, int r) { dp[q][b][r] *= __builtin_fmaf(-th[b][r], th[b][r], 1.f); });
           mask(s[q], row0, kept.span[q], kept.seen[q], g, 0.f);
           mask(dp[q], row0, kept.span[q], kept.seen[q], g, 0.f);
           gs[q].apply(dp[q], dk[q]);
         }
-        add_weighted<T, DP, NQ>(dv, s, ds[at] + p * lds_row<T, DP>, bad_d, row0, kept.seen, lane);
-        add_weighted<T, DP, NQ>(dk, dp, qs[at] + p * lds_row<T, DP>, bad_q, row0, kept.seen, lane);
-      }
+        add_weighted<T, DP, NQ, B>(dv, s, ds[at] + p * lds_row<T, DP>, bad_d, row0, kept.seen, lane);
+        add_weighted<T, DP, NQ, B>(dk, dp, qs[at] + p * lds_row<T, DP>, bad_q, row0, kept.seen, lane);
+      };
+      take_tile(take, tile, kept.lo, kept.hi);
       if (more) put(at ^ 1);
     }
   }
@@ -799,31 +848,24 @@ __global__ __launch_bounds__(AT_NT) void k_attn_row(ffn_ray_attn a, int splits, 
     };
     if (lo < hi) fetch(lo);
     for (int row0 = lo; row0 < hi; row0 += AT_TILE) {
-      Piece s[2];
+      f32x4 s[1][4], th[4];
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        s[b >> 1][b & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        s[0][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < KS; ++k) s[b >> 1][b & 1] = Mat<T>::mma(kf[b][k], qf[k], s[b >> 1][b & 1]);
+        for (int k = 0; k < KS; ++k) s[0][b] = Mat<T>::mma(kf[b][k], qf[k], s[0][b]);
       }
       vst.store(vs, lane);
       ts[lane] = tst;
       if (hi - row0 > AT_TILE) fetch(row0 + AT_TILE);
       wave_sync();
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const int from = row0 + PIECE * p;
-        if (from >= hi) break;
-        Piece th, w[1];
-        logits(s[p], th, t, ts + PIECE * p, g);
-        if (hi - from < PIECE)
-          each([&](int b, int r) {
-            if (from + 16 * b + 4 * g + r >= hi) s[p][b][r] = -INFINITY;
-          });
-        sm.step(s[p], logits.mul, acc[0]);
-        w[0][0] = s[p][0], w[0][1] = s[p][1];
-        add_weighted<T, DP, 1>(acc, w, vs + PIECE * p * lds_row<T, DP>, false, from, seen, lane);
-      }
+      logits(s[0], th, t, ts, g);
+      if (hi - row0 < AT_TILE)
+        each<4>([&](int b, int r) {
+          if (row0 + 16 * b + 4 * g + r >= hi) s[0][b][r] = -INFINITY;
+        });
+      sm.step(s[0], logits.mul, acc[0]);
+      add_weighted<T, DP, 1, 4>(acc, s, vs, false, row0, seen, lane);
       wave_sync();
     }
     if (splits == 1) {
@@ -872,7 +914,7 @@ __global__ __launch_bounds__(AT_NT) void k_attn_join(ffn_ray_attn a, int splits)
     }
     ((T*)a.o)[at * a.dim + d] = (T)(o * by);
   }
-  if (lane == 0) a.lse[at] = l == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(l) - W_SHIFT) * LN2;
+  if (lane == 0) a.lse[at] = log_sum(base, l);
 }
 
 // Few rows are split over their keys until about this many wavefronts have work: 16 a CU
@@ -899,13 +941,10 @@ static unsigned die_grid(int64_t total) { return (unsigned)((total + 8 * DIE_RUN
 
 // Sets of 16 kept rows a wavefront: two where rays are long on both sides and the registers hold them
 template <typename T, int DP> constexpr int MAX_SETS = sizeof(T) == 2 && DP <= 64 ? 2 : 1;
-#ifndef LONGRAY
-#define LONGRAY 256
-#endif
 template <typename T, int DP>
 static int sets(const ffn_ray_set& kept, const ffn_ray_set& streamed) {
   const int64_t rays = kept.num_rays;
-  return kept.n >= LONGRAY * rays && streamed.n >= LONGRAY * rays ? MAX_SETS<T, DP> : 1;
+  return kept.n >= 256 * rays && streamed.n >= 256 * rays ? MAX_SETS<T, DP> : 1;
 }
 
 template <typename T, int DP, bool CAP>
