@@ -5,11 +5,11 @@
 namespace ffn {
 
 // ---------------------------------------------------------------------------
-// The grouping: a stable counting sort of row indices by expert.  Counts per block of 4096 rows, a scan per expert over
+// The grouping: a stable counting sort of row indices by expert.  Counts per block of 2048 rows, a scan per expert over
 // the blocks, and a move in which a row's place comes from ballots over the lanes that hold equal ids, so the order
 // depends on the ids alone.
 
-constexpr int PL_NT = 256, PL_ITEMS = 16, PL_BLOCK = PL_NT * PL_ITEMS, PL_BINS = FFN_MAX_EXPERTS + 1;
+constexpr int PL_NT = 256, PL_ITEMS = 8, PL_BLOCK = PL_NT * PL_ITEMS, PL_BINS = FFN_MAX_EXPERTS + 1;
 constexpr int EX_ROWS = 128;  // slots of a product tile
 
 // where the parts of a plan are, in words
@@ -71,20 +71,33 @@ __global__ __launch_bounds__(64) void k_plan_scan(uint32_t* __restrict__ block_c
                                                   uint32_t* __restrict__ plan, PlanView v) {
   const int lane = threadIdx.x;
   uint32_t* c = block_counts + (int64_t)blockIdx.x * blocks;
+  constexpr int PER = 8;
   uint32_t sum = 0u;
-  for (int b0 = 0; b0 < blocks; b0 += 64) {
-    const uint32_t x = b0 + lane < blocks ? c[b0 + lane] : 0u;
-    const uint32_t s = wave_scan(x, lane);
-    if (b0 + lane < blocks) c[b0 + lane] = sum + s - x;
+  for (int b0 = 0; b0 < blocks; b0 += 64 * PER) {
+    uint32_t x[PER], mine = 0u;
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+      const int b = b0 + lane * PER + q;
+      x[q] = b < blocks ? c[b] : 0u;
+      mine += x[q];
+    }
+    const uint32_t s = wave_scan(mine, lane);
+    uint32_t at = sum + s - mine;
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+      const int b = b0 + lane * PER + q;
+      if (b < blocks) c[b] = at;
+      at += x[q];
+    }
     sum += __shfl(s, 63);
   }
   if (lane == 0) plan[v.counts + blockIdx.x] = sum;
 }
 
 // out[b] = sum of f(in[a]) over a < b, for all bins and (out[bins]) the total; in may be global, out is in LDS
-template <typename F>
+template <int NT, typename F>
 __device__ __forceinline__ void bin_scan(const uint32_t* in, int bins, uint32_t* out, uint32_t* part, F f) {
-  constexpr int PER = (PL_BINS + PL_NT - 1) / PL_NT;
+  constexpr int PER = (PL_BINS + NT - 1) / NT;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   uint32_t x[PER], sum = 0u;
 #pragma unroll
@@ -108,9 +121,11 @@ __device__ __forceinline__ void bin_scan(const uint32_t* in, int bins, uint32_t*
   __syncthreads();
 }
 
-// entries {bin, index of the piece among its bin's} of a table of pieces of `size` slots
-__device__ __forceinline__ void fill_table(uint2* table, uint64_t n, uint64_t from, const uint32_t* first, int bins) {
-  for (uint64_t t = from + threadIdx.x; t < from + PL_BLOCK && t < n; t += PL_NT) {
+// entries {bin, index of the piece among its bin's} of a table of pieces, of which bin b has first[b + 1] - first[b]
+template <int NT>
+__device__ __forceinline__ void fill_table(uint2* table, uint64_t n, uint64_t from, uint64_t count, const uint32_t* first,
+                                           int bins) {
+  for (uint64_t t = from + threadIdx.x; t < from + count && t < n; t += NT) {
     uint2 e = make_uint2(0xFFFFFFFFu, 0u);
     if (t < first[bins]) {
       int lo = 0, hi = bins - 1;  // the last bin whose first piece is not past t
@@ -125,6 +140,75 @@ __device__ __forceinline__ void fill_table(uint2* table, uint64_t n, uint64_t fr
   }
 }
 
+// The bins of this wavefront's rows w0 + 64 q + lane, and how many rows of the same bin the wavefront has before each.
+// cnt: the wavefront's counts so far, 0 at first.
+template <int ITEMS>
+__device__ __forceinline__ void rank_rows(const int32_t* __restrict__ ids, const PlanView& v, int64_t w0, int bits,
+                                          uint32_t* cnt, uint32_t (&bin)[ITEMS], uint32_t (&rank)[ITEMS]) {
+  const int lane = threadIdx.x & 63;
+  const uint64_t below = (1ull << lane) - 1ull;
+#pragma unroll
+  for (int q = 0; q < ITEMS; ++q) {
+    const int64_t i = w0 + q * 64 + lane;
+    bin[q] = i < v.n ? bin_of(ids, i, v.bins) : 0u;
+  }
+#pragma unroll
+  for (int q = 0; q < ITEMS; ++q) {
+    const bool there = w0 + q * 64 + lane < v.n;
+    uint64_t same = __ballot(there);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t m = __ballot((bin[q] >> b) & 1u);
+      same &= ((bin[q] >> b) & 1u) ? m : ~m;
+    }
+    const uint32_t before = cnt[bin[q]];
+    rank[q] = before + (uint32_t)__popcll(same & below);
+    wave_sync();
+    if (there && (same & below) == 0ull) cnt[bin[q]] = before + (uint32_t)__popcll(same);
+    wave_sync();
+  }
+}
+
+// Few rows: the whole plan by one block, in one launch (3001 rows: 9 us instead of three launches of 14)
+constexpr int PS_NT = 1024, PS_ITEMS = 8, PS_ROWS = PS_NT * PS_ITEMS;
+__global__ __launch_bounds__(PS_NT) void k_plan_small(const int32_t* __restrict__ ids, PlanView v, int bits,
+                                                      uint32_t* __restrict__ plan) {
+  constexpr int NW = PS_NT / 64;
+  __shared__ uint32_t first[PL_BINS + 1], total[PL_BINS], part[NW], cnt[NW][PL_BINS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int b = lane; b < v.bins; b += 64) cnt[wave][b] = 0u;
+  wave_sync();
+  const int64_t w0 = (int64_t)wave * (PS_ROWS / NW);
+  uint32_t bin[PS_ITEMS], rank[PS_ITEMS];
+  rank_rows<PS_ITEMS>(ids, v, w0, bits, cnt[wave], bin, rank);
+  __syncthreads();
+  for (int b = tid; b < v.bins; b += PS_NT) {
+    uint32_t sum = 0u;
+    for (int w = 0; w < NW; ++w) {
+      const uint32_t c = cnt[w][b];
+      cnt[w][b] = sum;
+      sum += c;
+    }
+    total[b] = sum;
+    plan[v.counts + b] = sum;
+  }
+  __syncthreads();
+  bin_scan<PS_NT>(total, v.bins, first, part, [](uint32_t c) { return c; });
+  for (int b = tid; b < v.bins; b += PS_NT) plan[v.offsets + b] = first[b];
+#pragma unroll
+  for (int q = 0; q < PS_ITEMS; ++q) {
+    const int64_t i = w0 + q * 64 + lane;
+    if (i < v.n) plan[v.rows + first[bin[q]] + cnt[wave][bin[q]] + rank[q]] = (uint32_t)i;
+  }
+  __syncthreads();
+  bin_scan<PS_NT>(total, v.bins, first, part, [](uint32_t c) { return (c + EX_ROWS - 1) / EX_ROWS; });
+  fill_table<PS_NT>((uint2*)(plan + v.tiles), v.n_tiles, 0, v.n_tiles, first, v.bins);
+  __syncthreads();
+  const uint32_t size = v.chunk;
+  bin_scan<PS_NT>(total, v.bins, first, part, [size](uint32_t c) { return (c + size - 1) / size; });
+  fill_table<PS_NT>((uint2*)(plan + v.chunks), v.n_chunks, 0, v.n_chunks, first, v.bins);
+  for (int b = tid; b < v.bins; b += PS_NT) plan[v.chunk_first + b] = first[b];
+}
+
 __global__ __launch_bounds__(PL_NT) void k_plan_move(const int32_t* __restrict__ ids, PlanView v, int bits, int blocks,
                                                      int tile_blocks, const uint32_t* __restrict__ block_counts,
                                                      uint32_t* __restrict__ plan) {
@@ -135,43 +219,26 @@ __global__ __launch_bounds__(PL_NT) void k_plan_move(const int32_t* __restrict__
   if ((int)blockIdx.x >= blocks) {
     const int t = blockIdx.x - blocks;
     if (t < tile_blocks) {
-      bin_scan(counts, v.bins, first, part, [](uint32_t c) { return (c + EX_ROWS - 1) / EX_ROWS; });
-      fill_table((uint2*)(plan + v.tiles), v.n_tiles, (uint64_t)t * PL_BLOCK, first, v.bins);
+      bin_scan<PL_NT>(counts, v.bins, first, part, [](uint32_t c) { return (c + EX_ROWS - 1) / EX_ROWS; });
+      fill_table<PL_NT>((uint2*)(plan + v.tiles), v.n_tiles, (uint64_t)t * PL_BLOCK, PL_BLOCK, first, v.bins);
     } else {
       const uint32_t size = v.chunk;
-      bin_scan(counts, v.bins, first, part, [size](uint32_t c) { return (c + size - 1) / size; });
-      fill_table((uint2*)(plan + v.chunks), v.n_chunks, (uint64_t)(t - tile_blocks) * PL_BLOCK, first, v.bins);
+      bin_scan<PL_NT>(counts, v.bins, first, part, [size](uint32_t c) { return (c + size - 1) / size; });
+      fill_table<PL_NT>((uint2*)(plan + v.chunks), v.n_chunks, (uint64_t)(t - tile_blocks) * PL_BLOCK, PL_BLOCK, first, v.bins);
       if (t == tile_blocks)
         for (int b = tid; b < v.bins; b += PL_NT) plan[v.chunk_first + b] = first[b];
     }
     return;
   }
-  bin_scan(counts, v.bins, first, part, [](uint32_t c) { return c; });
+  bin_scan<PL_NT>(counts, v.bins, first, part, [](uint32_t c) { return c; });
   if (blockIdx.x == 0)
     for (int b = tid; b < v.bins; b += PL_NT) plan[v.offsets + b] = first[b];
-  if (v.n == 0) return;
   for (int b = tid; b < NW * PL_BINS; b += PL_NT) (&cnt[0][0])[b] = 0u;
   __syncthreads();
   // wavefront w holds rows [w PL_BLOCK / NW, ...) of the block, 64 consecutive ones per trip
   const int64_t w0 = (int64_t)blockIdx.x * PL_BLOCK + (int64_t)wave * (PL_BLOCK / NW);
-  const uint64_t below = (1ull << lane) - 1ull;
   uint32_t bin[PL_ITEMS], rank[PL_ITEMS];
-#pragma unroll
-  for (int q = 0; q < PL_ITEMS; ++q) {
-    const int64_t i = w0 + q * 64 + lane;
-    const bool there = i < v.n;
-    bin[q] = there ? bin_of(ids, i, v.bins) : 0u;
-    uint64_t same = __ballot(there);
-    for (int b = 0; b < bits; ++b) {
-      const uint64_t m = __ballot((bin[q] >> b) & 1u);
-      same &= ((bin[q] >> b) & 1u) ? m : ~m;
-    }
-    const uint32_t before = cnt[wave][bin[q]];
-    rank[q] = before + (uint32_t)__popcll(same & below);
-    wave_sync();
-    if (there && (same & below) == 0ull) cnt[wave][bin[q]] = before + (uint32_t)__popcll(same);
-    wave_sync();
-  }
+  rank_rows<PL_ITEMS>(ids, v, w0, bits, cnt[wave], bin, rank);
   __syncthreads();
   for (int b = tid; b < v.bins; b += PL_NT) {
     uint32_t at = first[b] + block_counts[(int64_t)b * blocks + blockIdx.x];
@@ -194,7 +261,7 @@ static int plan_blocks(uint32_t n) { return (int)(((uint64_t)n + PL_BLOCK - 1) /
 
 uint64_t expert_plan_words(uint32_t n, int experts) { return plan_view(n, experts).words; }
 uint64_t expert_plan_workspace(uint32_t n, int experts) {
-  return (uint64_t)plan_blocks(n) * (experts + 1) * sizeof(uint32_t);
+  return n <= PS_ROWS ? 0 : (uint64_t)plan_blocks(n) * (experts + 1) * sizeof(uint32_t);
 }
 
 hipError_t launch_expert_plan(const int32_t* ids, uint32_t n, int experts, uint32_t* plan, uint32_t* workspace,
@@ -203,11 +270,14 @@ hipError_t launch_expert_plan(const int32_t* ids, uint32_t n, int experts, uint3
   const int blocks = plan_blocks(n);
   int bits = 1;
   while ((1 << bits) < v.bins) ++bits;
-  if (blocks) k_plan_count<<<blocks, PL_NT, 0, st>>>(ids, v, workspace);
+  if (n <= PS_ROWS) {
+    k_plan_small<<<1, PS_NT, 0, st>>>(ids, v, bits, plan);
+    return hipGetLastError();
+  }
+  k_plan_count<<<blocks, PL_NT, 0, st>>>(ids, v, workspace);
   k_plan_scan<<<v.bins, 64, 0, st>>>(workspace, blocks, plan, v);
   const int tb = (int)((v.n_tiles + PL_BLOCK - 1) / PL_BLOCK), cb = (int)((v.n_chunks + PL_BLOCK - 1) / PL_BLOCK);
-  // without rows the offsets are written by no mover
-  k_plan_move<<<(blocks ? blocks : 1) + tb + cb, PL_NT, 0, st>>>(ids, v, bits, blocks ? blocks : 1, tb, workspace, plan);
+  k_plan_move<<<blocks + tb + cb, PL_NT, 0, st>>>(ids, v, bits, blocks, tb, workspace, plan);
   return hipGetLastError();
 }
 
@@ -244,14 +314,36 @@ struct StageW {
   }
 };
 
-// keeps the values whose y is positive
-template <typename V>
-__device__ __forceinline__ V where_positive(V g, const V& y) {
-  constexpr int N = sizeof(V) / sizeof(g[0]);
+// Keeps the values of g whose y is positive (16 bytes or a fragment of either type).  In 16 bits, two at a time on the
+// bits: y - 1 is below infinity's bits exactly where y is positive and no NaN; the saturating sum puts that into the sign.
+template <typename T, typename V>
+__device__ __forceinline__ V where_positive(const V& g, const V& y) {
+  constexpr int N = sizeof(V) / 4;
+  typedef uint32_t words __attribute__((ext_vector_type(N)));
+  words a = __builtin_bit_cast(words, g);
+  const words b = __builtin_bit_cast(words, y);
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int j = 0; j < N; ++j)
-    if (!((float)y[j] > 0.f)) g[j] = 0;
-  return g;
+    for (int i = 0; i < N; ++i) a[i] = __uint_as_float(b[i]) > 0.f ? a[i] : 0u;
+  } else {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    typedef short i16x2 __attribute__((ext_vector_type(2)));
+    constexpr unsigned short up = 0x8000 - (__is_same(T, __bf16) ? 0x7F80 : 0x7C00);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t word = b[i];
+      const u16x2 below = __builtin_bit_cast(u16x2, word) - (u16x2){1, 1};
+      const u16x2 sign = __builtin_elementwise_add_sat(below, (u16x2){up, up});
+      a[i] &= ~__builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, sign) >> (i16x2){15, 15});
+    }
+  }
+  return __builtin_bit_cast(V, a);
+}
+
+// row r of a tensor whose rows are `stride` bytes apart
+template <typename T>
+__device__ __forceinline__ const T* row_at(const T* base, uint32_t r, uint32_t stride) {
+  return reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + (uint64_t)r * stride);
 }
 
 // BACK = false: y = act(x W_e^T + b_e);  true: dx = (dy where y > 0) W_e.  128 slots by 16 NB columns a block, 32 slots a
@@ -293,9 +385,9 @@ __global__ __launch_bounds__(EX_NT, 2) void k_expert(ffn_experts a, PlanView v, 
     const T* gate[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int64_t r = in_slots ? slot[s] : row[s];
-      in[s] = (BACK ? (const T*)a.dy + r * a.dy_row : (const T*)a.x + r * a.x_row) + 8 * g;
-      gate[s] = BACK ? (const T*)a.y + r * a.out + 8 * g : nullptr;
+      const uint32_t r = in_slots ? slot[s] : row[s];
+      in[s] = row_at((const T*)(BACK ? a.dy : a.x), r, (uint32_t)(BACK ? a.dy_row : a.x_row) * sizeof(T)) + 8 * g;
+      gate[s] = BACK ? row_at((const T*)a.y, r, (uint32_t)a.out * sizeof(T)) + 8 * g : nullptr;
     }
     frag f[2][2];
     auto fetch = [&](int k0) {
@@ -311,7 +403,7 @@ __global__ __launch_bounds__(EX_NT, 2) void k_expert(ffn_experts a, PlanView v, 
           for (int j = 0; j < 8; ++j) x[j] = (T)0.f;
           if (there[s] && k + 8 * g < depth) {
             x = *reinterpret_cast<const frag*>(in[s] + k);
-            if (BACK && a.relu) x = where_positive(x, *reinterpret_cast<const frag*>(gate[s] + k));
+            if (BACK && a.relu) x = where_positive<T>(x, *reinterpret_cast<const frag*>(gate[s] + k));
           }
           f[s][ks] = x;
         }
@@ -391,39 +483,41 @@ __global__ __launch_bounds__(EX_NT) void k_expert_dw(ffn_experts a, PlanView v, 
   const int mw = (wave >> 1) * (TM / 2), kw = (wave & 1) * (TK / 2);
   const uint32_t off = a.plan[v.offsets + chunk.x], group = a.plan[v.counts + chunk.x];
   const uint32_t from = off + chunk.y * v.chunk, to = off + min(group, (chunk.y + merge) * v.chunk);
-  typedef T vec __attribute__((ext_vector_type(EL)));
-  vec gv[NG], yv[NG], xv[NX];
+  uint4 gv[NG], yv[NG], xv[NX];
   const bool x_slots = a.flags & FFN_EXPERTS_X_SLOTS, y_slots = a.flags & FFN_EXPERTS_Y_SLOTS;
   uint32_t gr[NG], xr[NX];  // the rows of the next step
   auto rows = [&](uint32_t s0) {
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
-      const uint32_t slot = s0 + (tid + i * EX_NT) / GC;
-      gr[i] = slot < to ? (y_slots ? slot : a.plan[v.rows + slot]) : 0u;
+      const uint32_t slot = min(s0 + (tid + i * EX_NT) / GC, to - 1);
+      gr[i] = y_slots ? slot : a.plan[v.rows + slot];
     }
 #pragma unroll
     for (int i = 0; i < NX; ++i) {
-      const uint32_t slot = s0 + (tid + i * EX_NT) / XC;
-      xr[i] = slot < to ? (x_slots ? slot : a.plan[v.rows + slot]) : 0u;
+      const uint32_t slot = min(s0 + (tid + i * EX_NT) / XC, to - 1);
+      xr[i] = x_slots ? slot : a.plan[v.rows + slot];
     }
   };
+  // this thread's columns; past the matrix, the last ones again (what comes of them is not stored)
+  const T* gp = (const T*)a.dy + min(m0 + tid % GC * EL, a.out - EL);
+  const T* yp = (const T*)a.y + min(m0 + tid % GC * EL, a.out - EL);
+  const T* xp = (const T*)a.x + min(k0 + tid % XC * EL, a.in - EL);
+  const uint32_t g_step = (uint32_t)a.dy_row * sizeof(T), y_step = (uint32_t)a.out * sizeof(T), x_step = (uint32_t)a.x_row * sizeof(T);
   auto fetch = [&](uint32_t s0) {
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
-      const int ch = tid + i * EX_NT, col = m0 + ch % GC * EL;
-#pragma unroll
-      for (int j = 0; j < EL; ++j) gv[i][j] = (T)0.f;
-      if (s0 + ch / GC < to && col < a.out) {
-        gv[i] = *reinterpret_cast<const vec*>((const T*)a.dy + gr[i] * a.dy_row + col);
-        if (a.relu) yv[i] = *reinterpret_cast<const vec*>((const T*)a.y + (int64_t)gr[i] * a.out + col);
-      }
+      gv[i] = *reinterpret_cast<const uint4*>(row_at(gp, gr[i], g_step));
+      if (a.relu) yv[i] = *reinterpret_cast<const uint4*>(row_at(yp, gr[i], y_step));
     }
 #pragma unroll
-    for (int i = 0; i < NX; ++i) {
-      const int ch = tid + i * EX_NT, col = k0 + ch % XC * EL;
+    for (int i = 0; i < NX; ++i) xv[i] = *reinterpret_cast<const uint4*>(row_at(xp, xr[i], x_step));
+    if (to - s0 < (uint32_t)S) {  // rows past the chunk (the last one again) as 0
 #pragma unroll
-      for (int j = 0; j < EL; ++j) xv[i][j] = (T)0.f;
-      if (s0 + ch / XC < to && col < a.in) xv[i] = *reinterpret_cast<const vec*>((const T*)a.x + xr[i] * a.x_row + col);
+      for (int i = 0; i < NG; ++i)
+        if (s0 + (tid + i * EX_NT) / GC >= to) gv[i] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int i = 0; i < NX; ++i)
+        if (s0 + (tid + i * EX_NT) / XC >= to) xv[i] = make_uint4(0u, 0u, 0u, 0u);
     }
   };
   f32x4 acc[NM][NK], sum[NM];
@@ -444,13 +538,13 @@ __global__ __launch_bounds__(EX_NT) void k_expert_dw(ffn_experts a, PlanView v, 
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
       const int ch = tid + i * EX_NT;
-      if (a.relu) gv[i] = where_positive(gv[i], yv[i]);
-      *reinterpret_cast<vec*>(gs + ch / GC * lds_row<T, TM> + ch % GC * EL) = gv[i];
+      if (a.relu) gv[i] = where_positive<T>(gv[i], yv[i]);
+      *reinterpret_cast<uint4*>(gs + ch / GC * lds_row<T, TM> + ch % GC * EL) = gv[i];
     }
 #pragma unroll
     for (int i = 0; i < NX; ++i) {
       const int ch = tid + i * EX_NT;
-      *reinterpret_cast<vec*>(xs + ch / XC * lds_row<T, TK> + ch % XC * EL) = xv[i];
+      *reinterpret_cast<uint4*>(xs + ch / XC * lds_row<T, TK> + ch % XC * EL) = xv[i];
     }
     __syncthreads();
     if (to - s0 > S) {

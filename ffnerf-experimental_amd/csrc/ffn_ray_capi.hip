@@ -120,6 +120,9 @@ int check_experts(const ffn_experts* a) {
     return fail(-1, "in=%d, out=%d must be multiples of 8, at most 4096", a->in, a->out);
   if (a->flags & ~(FFN_EXPERTS_X_SLOTS | FFN_EXPERTS_Y_SLOTS)) return fail(-1, "unknown flags %d", a->flags);
   if (!a->plan) return fail(-1, "NULL plan");
+  const int64_t far = (int64_t)(UINT32_MAX / elem(a->dtype));
+  if (a->x_row < 0 || a->x_row > far || a->dy_row < 0 || a->dy_row > far)
+    return fail(-1, "row strides must be 0 or more, and less than 4 GiB");
   return 0;
 }
 

@@ -27,30 +27,28 @@ def _dtype(x: torch.Tensor) -> int:
     return d
 
 
-def _want(x, name: str, shape, dtype, device, rows: int = -1) -> int | None:
-    """Pointer of x, which must have this shape, type and device; unit stride along the last `rows` of its axes that
-    a kernel takes as one (all of them: contiguous)."""
+def _want(x, name: str, shape: tuple, dtype, dev: int, rows: int = -1) -> int | None:
+    """Pointer of x, which must have this shape, type and device, and (rows -1) be contiguous, (1) have unit stride
+    along its last axis, or (0) any strides."""
     if x is None:
         return None
-    if not isinstance(x, torch.Tensor) or tuple(x.shape) != tuple(shape):
+    if (isinstance(x, torch.Tensor) and x.shape == shape and x.dtype is dtype and x.get_device() == dev
+            and (x.is_contiguous() if rows < 0 else not rows or x.stride(-1) == 1 or shape[-1] == 1)):
+        return x.data_ptr()
+    if not isinstance(x, torch.Tensor) or x.shape != shape:
         _refuse(f"{name} must be a tensor of shape {tuple(shape)}, not {tuple(getattr(x, 'shape', ()))}")
-    if x.dtype != dtype:
+    if x.dtype is not dtype:
         _refuse(f"{name} must be {dtype}, not {x.dtype}")
-    if x.device != device:
-        _refuse(f"{name} is on {x.device}, not on {device}")
-    if rows < 0:
-        if not x.is_contiguous():
-            _refuse(f"{name} must be contiguous")
-    elif rows and x.shape[-1] > 1 and x.stride(-1) != 1:
-        _refuse(f"{name} must have unit stride along its last axis")
-    return x.data_ptr()
+    if x.get_device() != dev:
+        _refuse(f"{name} is on {x.device}, not on cuda:{dev}")
+    _refuse(f"{name} must be contiguous" if rows < 0 else f"{name} must have unit stride along its last axis")
 
 
-def _index(x, name: str, device) -> int:
+def _index(x, name: str, dev: int) -> int:
     if not isinstance(x, torch.Tensor) or x.dim() != 1 or x.dtype not in (torch.int32, torch.uint32):
         _refuse(f"{name} must be a vector of int32")
-    if x.device != device:
-        _refuse(f"{name} is on {x.device}, not on {device}")
+    if x.get_device() != dev:
+        _refuse(f"{name} is on {x.device}, not on cuda:{dev}")
     if not x.is_contiguous():
         _refuse(f"{name} must be contiguous")
     return x.data_ptr()
@@ -63,10 +61,9 @@ class RaySet:
     def __init__(self, counts: torch.Tensor, offsets: torch.Tensor, ray_ids: torch.Tensor):
         if not isinstance(ray_ids, torch.Tensor) or not ray_ids.is_cuda:
             _refuse("ray_ids must be a tensor on the GPU")
-        self.device = ray_ids.device
-        c = self.c = fl.FfnRaySet()
-        c.counts, c.offsets = _index(counts, "counts", self.device), _index(offsets, "offsets", self.device)
-        c.ray_ids = _index(ray_ids, "ray_ids", self.device)
+        dev = self.device = ray_ids.get_device()
+        c = self.c = fl.FfnRaySet(_index(counts, "counts", dev), _index(offsets, "offsets", dev),
+                                  _index(ray_ids, "ray_ids", dev))
         if counts.shape != offsets.shape:
             _refuse(f"{counts.shape[0]} counts, {offsets.shape[0]} offsets")
         self.num_rays, self.n = counts.shape[0], ray_ids.shape[0]
@@ -76,37 +73,25 @@ class RaySet:
         self._keep = (counts, offsets, ray_ids)
 
 
-def _on(device):
-    """The device of the call, and its current stream."""
-    return torch.cuda.device(device) if device.index != torch.cuda.current_device() else _HERE
-
-
-class _Here:
-    def __enter__(self):
-        pass
-
-    def __exit__(self, *a):
-        pass
-
-
-_HERE = _Here()
-
-
-def _call(fn, args, device):
-    with _on(device):
-        rc = fn(C.byref(args), torch.cuda.current_stream(device).cuda_stream)
+def _call(fn, dev: int, *args):
+    """fn(*args, stream) on the current stream of device dev."""
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         fl.check(rc, fn.__name__)
 
 
-def _workspace(a, fn, device, *more):
+def _workspace(a, fn, dev: int, *more):
     n = C.c_uint64()
     rc = fn(C.byref(a), *more, C.byref(n))
     if rc:
         fl.check(rc, fn.__name__)
     if not n.value:
         return None
-    w = torch.empty(n.value, dtype=torch.uint8, device=device)
+    w = torch.empty(n.value, dtype=torch.uint8, device=dev)
     a.workspace, a.workspace_bytes = w.data_ptr(), n.value
     return w
 
@@ -119,16 +104,18 @@ def _attn_args(q, k, v, q_rays, k_rays, t_q, t_k, slopes, scale, cap, causal, pr
     if not isinstance(q, torch.Tensor) or q.dim() != 3 or not isinstance(k, torch.Tensor) or k.dim() != 3:
         _refuse("q and k must be tensors [rows, heads, dim]")
     a, dev = fl.FfnRayAttn(), q_rays.device
-    a.dtype, a.heads, a.kv_heads, a.dim = _dtype(q), q.shape[1], k.shape[1], q.shape[2]
-    a.q = _want(q, "q", (q_rays.n, q.shape[1], q.shape[2]), q.dtype, dev, 1)
-    shape = (k_rays.n, k.shape[1], q.shape[2])
-    a.k, a.v = _want(k, "k", shape, q.dtype, dev, 1), _want(v, "v", shape, q.dtype, dev, 1)
-    (a.q_row, a.q_head), (a.k_row, a.k_head), (a.v_row, a.v_head) = q.stride()[:2], k.stride()[:2], v.stride()[:2]
+    _, heads, dim = q.shape
+    dtype, kv_heads = q.dtype, k.shape[1]
+    a.dtype, a.heads, a.kv_heads, a.dim = _dtype(q), heads, kv_heads, dim
+    shape = (k_rays.n, kv_heads, dim)
+    a.q = _want(q, "q", (q_rays.n, heads, dim), dtype, dev, 1)
+    a.k, a.v = _want(k, "k", shape, dtype, dev, 1), _want(v, "v", shape, dtype, dev, 1)
+    (a.q_row, a.q_head, _), (a.k_row, a.k_head, _), (a.v_row, a.v_head, _) = q.stride(), k.stride(), v.stride()
     a.q_rays, a.k_rays = q_rays.c, k_rays.c
-    a.scale = q.shape[2] ** -0.5 if scale is None else scale
+    a.scale = dim ** -0.5 if scale is None else scale
     a.cap, a.causal = cap, 1 if causal else 0
     if slopes is not None:
-        a.slopes = _want(slopes, "slopes", (q.shape[1],), torch.float32, dev)
+        a.slopes = _want(slopes, "slopes", (heads,), torch.float32, dev)
         a.t_q = _want(t_q, "t_q", (q_rays.n,), torch.float32, dev, 0)
         a.t_k = _want(t_k, "t_k", (k_rays.n,), torch.float32, dev, 0)
         if t_q is None or t_k is None:
@@ -157,7 +144,7 @@ def ray_attention(q, k, v, q_rays: RaySet, k_rays: RaySet | None = None, *, t_q=
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev)
     a.o, a.lse = o.data_ptr(), lse.data_ptr()
     w = _workspace(a, lib.ffn_ray_attention_workspace, dev, 0)  # noqa: F841 (held until the launch)
-    _call(lib.ffn_ray_attention_fwd, a, dev)
+    _call(lib.ffn_ray_attention_fwd, dev, C.byref(a))
     return o, lse
 
 
@@ -173,7 +160,7 @@ def ray_attention_backward(do, q, k, v, o, lse, q_rays: RaySet, k_rays: RaySet |
     dq, dk, dv = (torch.empty(x.shape, dtype=q.dtype, device=dev) for x in (q, k, v))
     a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
     w = _workspace(a, lib.ffn_ray_attention_workspace, dev, 1)  # noqa: F841
-    _call(lib.ffn_ray_attention_bwd, a, dev)
+    _call(lib.ffn_ray_attention_bwd, dev, C.byref(a))
     return dq, dk, dv
 
 
@@ -231,7 +218,7 @@ def ray_scan(gate, x, rays: RaySet, *, h0=None, reverse: bool = False, marks: bo
         m = torch.empty(n.value // 4, dtype=torch.float32, device=dev)
         a.marks = m.data_ptr()
     w = _workspace(a, lib.ffn_ray_scan_workspace, dev, 0)  # noqa: F841
-    _call(lib.ffn_ray_scan_fwd, a, dev)
+    _call(lib.ffn_ray_scan_fwd, dev, C.byref(a))
     return h, last, m
 
 
@@ -249,7 +236,7 @@ def ray_scan_backward(dh, gate, x, marks, rays: RaySet, *, dlast=None, h0=None, 
     dh0 = torch.empty((rays.num_rays, x.shape[1]), dtype=torch.float32, device=dev)
     a.dgate, a.dx, a.dh0 = dgate.data_ptr(), dx.data_ptr(), dh0.data_ptr()
     w = _workspace(a, lib.ffn_ray_scan_workspace, dev, 1)  # noqa: F841
-    _call(lib.ffn_ray_scan_bwd, a, dev)
+    _call(lib.ffn_ray_scan_bwd, dev, C.byref(a))
     return dgate, dx, dh0
 
 
@@ -281,10 +268,19 @@ class ExpertPlan:
     offsets[e] + counts[e]], in the rows' own order; rows of no expert come last."""
 
     def __init__(self, words: torch.Tensor, n: int, n_experts: int):
-        self.words, self.n, self.n_experts = words, n, n_experts
-        self.counts = words[:n_experts]
-        self.offsets = words[n_experts + 1:2 * n_experts + 1]
-        self.rows = words[words.shape[0] - n:]
+        self.words, self.n, self.n_experts, self.device = words, n, n_experts, words.get_device()
+
+    @property
+    def counts(self) -> torch.Tensor:
+        return self.words[:self.n_experts]
+
+    @property
+    def offsets(self) -> torch.Tensor:
+        return self.words[self.n_experts + 1:2 * self.n_experts + 1]
+
+    @property
+    def rows(self) -> torch.Tensor:
+        return self.words[self.words.shape[0] - self.n:]
 
 
 def expert_plan(ids: torch.Tensor, n_experts: int) -> ExpertPlan:
@@ -292,25 +288,23 @@ def expert_plan(ids: torch.Tensor, n_experts: int) -> ExpertPlan:
     lib = fl.load()
     if not isinstance(ids, torch.Tensor) or not ids.is_cuda or ids.dim() != 1 or ids.dtype != torch.int32:
         _refuse("ids must be a vector of int32 on the GPU")
-    dev, n = ids.device, ids.shape[0]
+    dev, n = ids.get_device(), ids.shape[0]
     _index(ids, "ids", dev)
     if n >= 1 << 31:
         _refuse(f"{n} rows are too many")
     words, ws = C.c_uint64(), C.c_uint64()
     fl.check(lib.ffn_expert_plan_size(n, n_experts, C.byref(words), C.byref(ws)), "ffn_expert_plan_size")
     plan = torch.empty(words.value, dtype=torch.int32, device=dev)
-    w = torch.empty(max(ws.value, 1), dtype=torch.uint8, device=dev)
-    with _on(dev):
-        fl.check(lib.ffn_expert_plan(ids.data_ptr() if n else None, n, n_experts, plan.data_ptr(), words.value,
-                                     w.data_ptr(), ws.value, torch.cuda.current_stream(dev).cuda_stream),
-                 "ffn_expert_plan")
+    w = torch.empty(ws.value, dtype=torch.uint8, device=dev) if ws.value else None
+    _call(lib.ffn_expert_plan, dev, ids.data_ptr(), n, n_experts, plan.data_ptr(), words.value,
+          None if w is None else w.data_ptr(), ws.value)
     return ExpertPlan(plan, n, n_experts)
 
 
 def _expert_args(x, W, plan, relu, x_slots, y_slots):
     if not isinstance(x, torch.Tensor) or x.dim() != 2 or not isinstance(W, torch.Tensor) or W.dim() != 3:
         _refuse("x must be a tensor [rows, in], W a tensor [experts, out, in]")
-    a, dev = fl.FfnExperts(), plan.words.device
+    a, dev = fl.FfnExperts(), plan.device
     a.dtype, a.n_experts, a.d_in, a.d_out = _dtype(x), plan.n_experts, W.shape[2], W.shape[1]
     a.relu, a.flags = 1 if relu else 0, (1 if x_slots else 0) | (2 if y_slots else 0)
     a.n, a.plan = plan.n, plan.words.data_ptr()
@@ -330,7 +324,7 @@ def expert_linear(x, W, b, plan: ExpertPlan, *, relu: bool = False, x_slots: boo
     a.b = _want(b, "b", W.shape[:2], x.dtype, dev)
     y = torch.empty((plan.n, W.shape[1]), dtype=x.dtype, device=dev)
     a.y = y.data_ptr()
-    _call(lib.ffn_expert_linear_fwd, a, dev)
+    _call(lib.ffn_expert_linear_fwd, dev, C.byref(a))
     return y
 
 
@@ -347,7 +341,7 @@ def expert_linear_backward(dy, x, W, plan: ExpertPlan, *, y=None, x_slots: bool 
     db = torch.empty(W.shape[:2], dtype=torch.float32, device=dev) if need_dw else None
     a.dx, a.dW, a.db = (t.data_ptr() if t is not None else None for t in (dx, dW, db))
     w = _workspace(a, lib.ffn_expert_linear_workspace, dev)  # noqa: F841
-    _call(lib.ffn_expert_linear_bwd, a, dev)
+    _call(lib.ffn_expert_linear_bwd, dev, C.byref(a))
     return dx, dW, db
 
 

@@ -454,7 +454,7 @@ int ffn_expert_plan(const int32_t* ids, uint32_t n, int32_t n_experts, uint32_t*
 /* A layer of every expert on its own rows: y = x W_e^T + b_e, with relu
  * max(y, 0).  x [n][in] of dtype with row stride x_row, y [n][out] contiguous,
  * W [n_experts][out][in], b [n_experts][out] (NULL: 0) of dtype.  in and out
- * multiples of 8 up to 4096, rows 16-byte aligned.  Rows of x and y are the
+ * multiples of 8 up to 4096, rows 16-byte aligned and less than 4 GiB apart.  Rows of x and y are the
  * caller's rows, or the plan's slots where the flags say so (so that the layers
  * of a network stay in slot order between its first and its last).  Rows of no
  * expert give 0. */

@@ -20,7 +20,7 @@ def _ids(n, E, seed, none=0.1):
 
 
 @pytest.mark.parametrize("n,E", [(0, 3), (1, 1), (5, 1), (63, 2), (64, 64), (1000, 8), (4096, 5), (4097, 33),
-                                 (100003, 7), (50000, 1024)])
+                                 (100003, 7), (50000, 1024), (8192, 1024), (8193, 3)])
 def test_plan(n, E):
     import ray_ops
     ids = _ids(n, E, seed=n + E)
@@ -75,7 +75,8 @@ def _check(n, E, K, M, ty, seed, relu, bias=True, none=0.1):
 @pytest.mark.parametrize("ty", TYPES)
 @pytest.mark.parametrize("relu", [False, True])
 @pytest.mark.parametrize("n,E,K,M", [(1, 1, 8, 8), (130, 3, 32, 64), (777, 9, 24, 40), (1500, 4, 136, 72),
-                                     (3000, 70, 64, 64), (257, 2, 256, 8), (300, 1, 8, 256)])
+                                     (3000, 70, 64, 64), (257, 2, 256, 8), (300, 1, 8, 256),
+                                     (150, 2, 1024, 24), (150, 2, 16, 1024), (90, 1, 520, 512)])
 def test_layers(ty, relu, n, E, K, M):
     _check(n, E, K, M, TYPES[ty], seed=n + K, relu=relu)
 

@@ -96,7 +96,8 @@ def _experts(**kw):
     (dict(dtype=5), "dtype=5"), (dict(n_experts=0), "n_experts=0"), (dict(n_experts=1025), "n_experts=1025"),
     (dict(d_in=12), "in=12"), (dict(d_out=4104), "out=4104"), (dict(flags=4), "flags"), (dict(plan=None), "NULL plan"),
     (dict(x=None), "NULL buffer"), (dict(W=None), "NULL buffer"), (dict(y=None), "NULL buffer"),
-    (dict(x_row=65), "aligned"), (dict(W=P + 8), "aligned"), (dict(n=(1 << 31)), "exceed"),
+    (dict(x_row=65), "aligned"), (dict(x_row=-64), "row strides"), (dict(dy_row=1 << 31), "row strides"),
+    (dict(W=P + 8), "aligned"), (dict(n=(1 << 31)), "exceed"),
 ])
 def test_experts_refuse(kw, match):
     lib = fl.load()
@@ -109,7 +110,7 @@ def test_experts_refuse_what_only_one_call_needs():
     _refused(lib.ffn_expert_linear_bwd, C.byref(_experts(dy=None)), None, match="NULL buffer")
     _refused(lib.ffn_expert_linear_bwd, C.byref(_experts(workspace_bytes=16)), None, match="workspace of 16")
     _refused(lib.ffn_expert_plan, P, 100, 4, P, 10, P, 1 << 20, None, match="plan of 10 words")
-    _refused(lib.ffn_expert_plan, P, 100, 4, P, 1 << 20, P, 4, None, match="workspace of 4")
+    _refused(lib.ffn_expert_plan, P, 100000, 4, P, 1 << 20, P, 4, None, match="workspace of 4")
     _refused(lib.ffn_expert_plan, None, 100, 4, P, 1 << 20, P, 1 << 20, None, match="NULL ids")
     _refused(lib.ffn_expert_plan_size, 100, 0, C.byref(C.c_uint64()), C.byref(C.c_uint64()), match="n_experts=0")
 
