@@ -168,7 +168,8 @@ __device__ __forceinline__ void rank_rows(const int32_t* __restrict__ ids, const
   }
 }
 
-// Few rows: the whole plan by one block, in one launch (3001 rows: 9 us instead of three launches of 14)
+// Few rows: the whole plan by one block, in one launch, us, one / three launches: 2048 rows with 8 experts 9.1 / 11.0, with 256
+// 12.1 / 13.3; 8192 rows 11.4 / 11.4 and 15.8 / 14.0, where three still cost the host more.
 constexpr int PS_NT = 1024, PS_ITEMS = 8, PS_ROWS = PS_NT * PS_ITEMS;
 __global__ __launch_bounds__(PS_NT) void k_plan_small(const int32_t* __restrict__ ids, PlanView v, int bits,
                                                       uint32_t* __restrict__ plan) {
@@ -614,20 +615,28 @@ static void product(const ffn_experts& a, const PlanView& v, hipStream_t st) {
   const int64_t total = (int64_t)v.n_tiles * cols;
   k_expert<T, BACK, NB><<<(unsigned)((total + 7) / 8 * 8), EX_NT, 0, st>>>(a, v, total, cols);
 }
+// Columns a block: all of a row's, so that x is read once, but narrower ones while that leaves CUs without work.  64 / 128 /
+// 256 columns a block, us, forward in bf16: 300000 rows, 256 x 256 values 141 / 124 / 122 (dx 182 / 144 / 132); 65536 rows
+// 34 / 30 / 41; 4096 rows 8.6 / 12 / 19; 128 x 128 values, a million rows 173 / 156 / 233, 65536 rows 16.3 / 14.6 / -,
+// 4096 rows 6.5 / 9.0 / 12.6; 64 x 64 values, a million rows 65 / 85 / 151.
+constexpr int64_t FILL = 512;
 template <typename T, bool BACK>
 static void product(const ffn_experts& a, const PlanView& v, hipStream_t st) {
   const int width = BACK ? a.in : a.out;
-  if (width <= 64) product<T, BACK, 4>(a, v, st);
-  else if (width <= 128 || sizeof(T) == 4) product<T, BACK, 8>(a, v, st);  // float: 16 would not fit the registers
-  else if constexpr (sizeof(T) == 2) product<T, BACK, 16>(a, v, st);
+  const int64_t tiles = v.n_tiles;
+  if (width <= 64 || tiles * ((width + 127) / 128) < FILL) product<T, BACK, 4>(a, v, st);
+  else if (width <= 128 || sizeof(T) == 4 || tiles * ((width + 255) / 256) < 2 * FILL) product<T, BACK, 8>(a, v, st);
+  else if constexpr (sizeof(T) == 2) product<T, BACK, 16>(a, v, st);  // float: 16 would not fit the registers
 }
 
 template <typename T, int TM, int TK>
 static void weight_gradient(const ffn_experts& a, const PlanView& v, hipStream_t st) {
   const int mt = (a.out + TM - 1) / TM, kt = (a.in + TK - 1) / TK;
-  // as many chunks a block as there are blocks a chunk: about 512 of them share the slots, and the partials stay few
-  const int merge = mt * kt < 8 ? mt * kt : 8;
   const int64_t pieces = (int64_t)v.n_chunks * mt * kt, size = (int64_t)a.out * a.in + a.out;
+  // chunks a block: FILL blocks share the slots, and the partials stay few (300000 rows, 256 x 256 values, us with 256, 512,
+  // 1024 blocks: 171, 107, 121; 65536 rows 43, 47, 56)
+  const int64_t share = (pieces + FILL / 2) / FILL;
+  const int merge = (int)(share < 1 ? 1 : share > 8 ? 8 : share);
   k_expert_dw<T, TM, TK><<<(unsigned)((pieces + 7) / 8 * 8), EX_NT, 0, st>>>(a, v, pieces, mt, kt, merge);
   k_expert_join<<<dim3((unsigned)((size + EX_NT - 1) / EX_NT), a.n_experts), EX_NT, 0, st>>>(a, v, merge);
 }
@@ -641,7 +650,10 @@ static hipError_t run(const ffn_experts& a, bool backward, hipStream_t st) {
   }
   if (a.dx && a.n) product<T, true>(a, v, st);
   if (a.dW || a.db) {
-    const bool m = a.out > 64, k = a.in > 64;
+    // tiles of 128 read dy and x half as often, if enough of them have work (64 / 128, us: a million rows of 128 x 128 values
+    // 268 / 162, 4096 rows 9.8 / 14)
+    const bool many = (int64_t)v.n_chunks * ((a.out + 127) / 128) * ((a.in + 127) / 128) >= FILL / 2;
+    const bool m = many && a.out > 64, k = many && a.in > 64;
     if constexpr (sizeof(T) == 4) weight_gradient<T, 64, 64>(a, v, st);  // bound by its products, not by reads
     else if (m && k) weight_gradient<T, 128, 128>(a, v, st);
     else if (m) weight_gradient<T, 128, 64>(a, v, st);

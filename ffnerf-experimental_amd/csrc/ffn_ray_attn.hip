@@ -99,10 +99,10 @@ __device__ __forceinline__ bool sees(int row, const Range& r) {
   return (unsigned)(row - r.lo) < (unsigned)(r.hi - r.lo);
 }
 
-// AT_TILE rows of one head on their way to LDS, tile after tile (rows outside [row, end) and columns past dim as 0)
-template <typename T, int DP, int NT = AT_NT>
+// ROWS rows of one head on their way to LDS, tile after tile (rows outside [row, end) and columns past dim as 0)
+template <typename T, int DP, int NT = AT_NT, int ROWS = AT_TILE>
 struct Staged {
-  static constexpr int EL = 16 / (int)sizeof(T), CPR = DP / EL, N = AT_TILE * CPR / NT, STEP = NT / CPR;
+  static constexpr int EL = 16 / (int)sizeof(T), CPR = DP / EL, N = ROWS * CPR / NT, STEP = NT / CPR;
   uint4 v[N];
   const T* p;   // this thread's first 16 bytes of the next tile
   int64_t row_step, tile_step;
@@ -112,7 +112,7 @@ struct Staged {
     row = col < dim ? row0 + tid / CPR : INT_MAX;
     p = base + (int64_t)(row0 + tid / CPR) * stride + col;
     row_step = STEP * stride;
-    tile_step = AT_TILE * stride;
+    tile_step = ROWS * stride;
   }
   __device__ __forceinline__ void load(int end) {
 #pragma unroll
@@ -121,7 +121,7 @@ struct Staged {
       if (row < end - i * STEP) v[i] = *reinterpret_cast<const uint4*>(p + i * row_step);
     }
     p += tile_step;
-    row += row == INT_MAX ? 0 : AT_TILE;
+    row += row == INT_MAX ? 0 : ROWS;
   }
   __device__ __forceinline__ void store(T* tile, int tid) const {
 #pragma unroll
@@ -795,14 +795,25 @@ __global__ __launch_bounds__(AT_NT, least_waves_dkv(sizeof(T), DP, NQ, CAP)) voi
     }
 }
 
+// part `split` of one query's keys, in whole tiles
+template <int ROWS>
+__device__ __forceinline__ Range split_keys(Range r, int split, int splits) {
+  r = {__builtin_amdgcn_readfirstlane(r.lo), __builtin_amdgcn_readfirstlane(r.hi)};
+  if (splits == 1) return r;
+  const int tiles = (r.hi - r.lo + ROWS - 1) / ROWS;
+  const int from = (int)((int64_t)tiles * split / splits), to = (int)((int64_t)tiles * (split + 1) / splits);
+  return {r.lo + from * ROWS, min(r.hi, r.lo + to * ROWS)};
+}
+
 // One query at a time: a wavefront takes query i, the heads of one key head along its columns, and part `split` of the
 // query's keys.  K comes straight into the operand's registers, V through the wavefront's own LDS rows (for the
-// transposing read).  Nothing is shared, so nothing waits.
+// transposing read), 64 at a time where the registers hold them.  Nothing is shared, so nothing waits.
+template <typename T, int DP> constexpr int row_tile = sizeof(T) * DP > 256 ? 32 : 64;
 template <typename T, int DP, bool CAP>
 __global__ __launch_bounds__(AT_NT) void k_attn_row(ffn_ray_attn a, int splits, int64_t total) {
-  constexpr int KS = DP / 32, NB = DP / 16;
-  __shared__ __align__(16) T vs_all[4][AT_TILE * lds_row<T, DP>];
-  __shared__ __align__(16) float ts_all[4][AT_TILE];
+  constexpr int KS = DP / 32, NB = DP / 16, ROWS = row_tile<T, DP>, B = ROWS / 16;
+  __shared__ __align__(16) T vs_all[4][ROWS * lds_row<T, DP>];
+  __shared__ __align__(16) float ts_all[4][ROWS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
   const int64_t work = (int64_t)blockIdx.x * 4 + wave;
   if (work >= total) return;  // no barriers below
@@ -812,14 +823,7 @@ __global__ __launch_bounds__(AT_NT) void k_attn_row(ffn_ray_attn a, int splits, 
   const int kh = (int)(work % a.kv_heads);
   const int split = (int)(work / a.kv_heads % splits);
   const int64_t i = work / a.kv_heads / splits;
-  Range seen[1] = {keys_of(a, i)};
-  seen[0].lo = __builtin_amdgcn_readfirstlane(seen[0].lo);
-  seen[0].hi = __builtin_amdgcn_readfirstlane(seen[0].hi);
-  if (splits > 1) {  // whole tiles
-    const int tiles = (seen[0].hi - seen[0].lo + AT_TILE - 1) / AT_TILE;
-    const int from = (int)((int64_t)tiles * split / splits), to = (int)((int64_t)tiles * (split + 1) / splits);
-    seen[0] = {seen[0].lo + from * AT_TILE, min(seen[0].hi, seen[0].lo + to * AT_TILE)};
-  }
+  const Range seen[1] = {split_keys<ROWS>(keys_of(a, i), split, splits)};
   const int lo = seen[0].lo, hi = seen[0].hi;
   const T* kb = (const T*)a.k + kh * a.k_head;
   for (int h0 = 0; h0 < group; h0 += 16) {
@@ -833,39 +837,39 @@ __global__ __launch_bounds__(AT_NT) void k_attn_row(ffn_ray_attn a, int splits, 
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[0][b] = f32x4{0.f, 0.f, 0.f, 0.f};
     Softmax<T> sm;
-    Staged<T, DP, 64> vst;
-    typename Mat<T>::frag kf[4][KS];
+    Staged<T, DP, 64, ROWS> vst;
+    typename Mat<T>::frag kf[B][KS];
     vst.begin((const T*)a.v + kh * a.v_head, a.v_row, lo, a.dim, lane);
     float tst = 0.f;
     auto fetch = [&](int row0) {
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
+      for (int b = 0; b < B; ++b) {
         const int row = row0 + 16 * b + c;
         load_frags<T, KS>(kf[b], kb + row * a.k_row, row < hi, a.dim, g);
       }
       vst.load(hi);
-      if (logits.bias && row0 + lane < hi) tst = a.t_k[(int64_t)(row0 + lane) * a.t_k_row];
+      if (logits.bias && lane < ROWS && row0 + lane < hi) tst = a.t_k[(int64_t)(row0 + lane) * a.t_k_row];
     };
     if (lo < hi) fetch(lo);
-    for (int row0 = lo; row0 < hi; row0 += AT_TILE) {
-      f32x4 s[1][4], th[4];
+    for (int row0 = lo; row0 < hi; row0 += ROWS) {
+      f32x4 s[1][B], th[B];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
+      for (int b = 0; b < B; ++b) {
         s[0][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < KS; ++k) s[0][b] = Mat<T>::mma(kf[b][k], qf[k], s[0][b]);
       }
       vst.store(vs, lane);
-      ts[lane] = tst;
-      if (hi - row0 > AT_TILE) fetch(row0 + AT_TILE);
+      if (lane < ROWS) ts[lane] = tst;
+      if (hi - row0 > ROWS) fetch(row0 + ROWS);
       wave_sync();
       logits(s[0], th, t, ts, g);
-      if (hi - row0 < AT_TILE)
-        each<4>([&](int b, int r) {
+      if (hi - row0 < ROWS)
+        each<B>([&](int b, int r) {
           if (row0 + 16 * b + 4 * g + r >= hi) s[0][b][r] = -INFINITY;
         });
       sm.step(s[0], logits.mul, acc[0]);
-      add_weighted<T, DP, 1, 4>(acc, s, vs, false, row0, seen, lane);
+      add_weighted<T, DP, 1, B>(acc, s, vs, false, row0, seen, lane);
       wave_sync();
     }
     if (splits == 1) {
@@ -888,63 +892,266 @@ __global__ __launch_bounds__(AT_NT) void k_attn_row(ffn_ray_attn a, int splits, 
   }
 }
 
-// Joins the splits of k_attn_row: a wavefront a (query, head)
+// Sum over the splits s of factor[s] p[s step + 4 lane ..] by one wavefront: the lanes take four columns each of every G-th
+// split, and the G sums are added in order.  factor null: 1.
+__device__ __forceinline__ f32x4 sum_splits(const float* p, int64_t step, int splits, int dim, const float* factor, f32x4* sums,
+                                            int lane) {
+  const int quads = dim / 4, groups = 64 / quads, quad = lane % quads, group = lane / quads;
+  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (group < groups) {
+#pragma unroll 4
+    for (int s = group; s < splits; s += groups) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(p + s * step + 4 * quad);
+      const float f = factor ? factor[s] : 1.f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = __builtin_fmaf(x[r], f, o[r]);
+    }
+  }
+  sums[lane] = o;
+  wave_sync();
+  for (int s = 1; s < groups && lane < quads; ++s) {
+    const f32x4 x = sums[s * quads + lane];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] += x[r];
+  }
+  wave_sync();
+  return o;
+}
+
+// Joins the splits of k_attn_row: a wavefront a (query, head), its lanes the splits for the maximum and the sum.  An empty
+// split's sums are 0; where the others made its factor infinite or NaN, theirs already are.
+constexpr int MAX_SPLITS = 256;
 template <typename T>
 __global__ __launch_bounds__(AT_NT) void k_attn_join(ffn_ray_attn a, int splits) {
-  const int lane = threadIdx.x & 63;
-  const int64_t rows = (int64_t)a.q_rays.n * a.heads, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (at >= rows) return;
+  __shared__ float factor[4][MAX_SPLITS];
+  __shared__ f32x4 sums[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t rows = (int64_t)a.q_rays.n * a.heads, at = (int64_t)blockIdx.x * 4 + wave;
+  if (at >= rows) return;  // no barriers below
   const float* part = (const float*)a.workspace;
   const float2* ml = reinterpret_cast<const float2*>(part + splits * rows * a.dim);
-  float m = -INFINITY;
-  for (int s = 0; s < splits; ++s) m = fmaxf(m, ml[s * rows + at].x);
+  float m = -INFINITY, l = 0.f;
+  for (int s = lane; s < splits; s += 64) m = fmaxf(m, ml[s * rows + at].x);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
   const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  for (int s = 0; s < splits; ++s) {
+  for (int s = lane; s < splits; s += 64) {
     const float2 x = ml[s * rows + at];
-    l = __builtin_fmaf(x.y, __builtin_amdgcn_exp2f(x.x - base), l);
+    const float f = __builtin_amdgcn_exp2f(x.x - base);
+    factor[wave][s] = f;
+    l = __builtin_fmaf(x.y, f, l);
   }
-  const float by = l == 0.f ? 0.f : 1.f / l;
-  for (int d = lane; d < a.dim; d += 64) {
-    float o = 0.f;
-    for (int s = 0; s < splits; ++s) {
-      const float f = __builtin_amdgcn_exp2f(ml[s * rows + at].x - base);
-      // an empty split's sums are 0; where the others made f infinite or NaN, theirs already are
-      o = __builtin_fmaf(part[(s * rows + at) * a.dim + d], f, o);
-    }
-    ((T*)a.o)[at * a.dim + d] = (T)(o * by);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
+  wave_sync();
+  const f32x4 o = sum_splits(part + at * a.dim, rows * a.dim, splits, a.dim, factor[wave], sums[wave], lane);
+  if (lane < a.dim / 4) {
+    const float by = l == 0.f ? 0.f : 1.f / l;
+    typename Mat<T>::quad q;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) q[r] = (T)(o[r] * by);
+    *reinterpret_cast<typename Mat<T>::quad*>((T*)a.o + at * a.dim + 4 * lane) = q;
   }
   if (lane == 0) a.lse[at] = log_sum(base, l);
 }
 
-// Few rows are split over their keys until about this many wavefronts have work: 16 a CU
+// words of D before the parts, which are 16-byte aligned
+__host__ __device__ inline int64_t dq_parts(int64_t rows) { return (rows + 3) / 4 * 4; }
+
+// k_attn_dq for the queries that k_attn_row takes: K through the wavefront's LDS rows, V straight into the operand.  The
+// workspace holds D, then (splits) the sums of each part, and {sum P dP, D'}.
+template <typename T, int DP, bool CAP>
+__global__ __launch_bounds__(AT_NT) void k_attn_dq_row(ffn_ray_attn a, int splits, int64_t total) {
+  constexpr int KS = DP / 32, NB = DP / 16, ROWS = row_tile<T, DP>, B = ROWS / 16;
+  constexpr bool EXACT = sizeof(T) == 2;
+  constexpr int SETS = EXACT ? 2 : 1;
+  __shared__ __align__(16) T ks_all[4][ROWS * lds_row<T, DP>];
+  __shared__ __align__(16) float ts_all[4][ROWS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
+  const int64_t work = (int64_t)blockIdx.x * 4 + wave;
+  if (work >= total) return;  // no barriers below
+  T* ks = ks_all[wave];
+  float* ts = ts_all[wave];
+  const int group = a.heads / a.kv_heads;
+  const int kh = (int)(work % a.kv_heads);
+  const int split = (int)(work / a.kv_heads % splits);
+  const int64_t i = work / a.kv_heads / splits;
+  const Range all = keys_of(a, i), mine = split_keys<ROWS>(all, split, splits);
+  const Range seen[2] = {mine, mine};
+  const Range(&seen_by)[SETS] = *reinterpret_cast<const Range(*)[SETS]>(seen);
+  const int lo = mine.lo, hi = mine.hi;
+  const T* vb = (const T*)a.v + kh * a.v_head;
+  for (int h0 = 0; h0 < group; h0 += 16) {
+    const bool there = h0 + c < group;
+    const int head = kh * group + min(h0 + c, group - 1);
+    const int64_t at = i * a.heads + head;
+    typename Mat<T>::frag qf[KS], df[KS], of[KS];
+    load_frags<T, KS>(qf, (const T*)a.q + i * a.q_row + head * a.q_head, there, a.dim, g);
+    load_frags<T, KS>(df, (const T*)a.dout + i * a.do_row + head * a.do_head, there, a.dim, g);
+    load_frags<T, KS>(of, (const T*)a.o + at * a.dim, there, a.dim, g);
+    float delta = 0.f, exact = 0.f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)of[k][j], (float)df[k][j], delta);
+    delta = swap_add(delta);
+    if (all.hi <= all.lo) delta = 0.f;
+    const float lse2 = there ? a.lse[at] * LOG2E : 0.f, from = (lse2 == -INFINITY ? 0.f : lse2) - W_SHIFT;
+    const Logits<CAP> logits(a, head);
+    const float t = logits.bias ? a.t_q[i * a.t_q_row] : 0.f;
+    f32x4 acc[SETS][NB];
+#pragma unroll
+    for (int q = 0; q < SETS; ++q)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) acc[q][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    GradScale<T> gs;
+    Staged<T, DP, 64, ROWS> kst;
+    typename Mat<T>::frag vf[B][KS];
+    kst.begin((const T*)a.k + kh * a.k_head, a.k_row, lo, a.dim, lane);
+    float tst = 0.f;
+    auto fetch = [&](int row0) {
+      kst.load(hi);
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        const int row = row0 + 16 * b + c;
+        load_frags<T, KS>(vf[b], vb + row * a.v_row, row < hi, a.dim, g);
+      }
+      if (logits.bias && lane < ROWS && row0 + lane < hi) tst = a.t_k[(int64_t)(row0 + lane) * a.t_k_row];
+    };
+    if (lo < hi) fetch(lo);
+    for (int row0 = lo; row0 < hi; row0 += ROWS) {
+      f32x4 dp[B], th[B], s[SETS][B], x[1][B];
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        dp[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) dp[b] = Mat<T>::mma(vf[b][k], df[k], dp[b]);
+      }
+      kst.store(ks, lane);
+      if (lane < ROWS) ts[lane] = tst;
+      if (hi - row0 > ROWS) fetch(row0 + ROWS);
+      wave_sync();
+      const typename Mat<T>::frag(&q1)[1][KS] = *reinterpret_cast<const typename Mat<T>::frag(*)[1][KS]>(&qf);
+      products<T, DP, 1, B>(x, ks, q1, lane);
+      logits(x[0], th, t, ts, g);
+      const bool ends = hi - row0 < ROWS;
+      each<B>([&](int b, int r) {
+        float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[0][b][r], logits.mul, -from));
+        if (ends && row0 + 16 * b + 4 * g + r >= hi) w = 0.f;
+        if (EXACT) exact = __builtin_fmaf(w, dp[b][r], exact);
+        if (CAP) w *= __builtin_fmaf(-th[b][r], th[b][r], 1.f);
+        s[SETS - 1][b][r] = w;
+        s[0][b][r] = w * (dp[b][r] - delta);
+      });
+      gs.apply(s[0], acc[0]);
+      add_weighted<T, DP, SETS, B>(acc, s, ks, false, row0, seen_by, lane);
+      wave_sync();
+    }
+    const float by = gs.undo();
+    exact = swap_add(exact) * W_UNSHIFT;
+    if (splits == 1) {
+      const float D = EXACT ? exact : delta;
+      each<NB>([&](int b, int r) {
+        acc[0][b][r] = EXACT ? __builtin_fmaf(acc[0][b][r], by, (delta - D) * acc[SETS - 1][b][r]) : acc[0][b][r] * by;
+      });
+      if (there) {
+        store_row<T, DP>((T*)a.dq + at * a.dim, acc[0], a.scale * W_UNSHIFT, a.dim, g);
+        if (g == 0) ((float*)a.workspace)[at] = D;
+      }
+    } else if (there) {
+      const int64_t rows = (int64_t)a.q_rays.n * a.heads, to = split * rows + at;
+      float* part = (float*)a.workspace + dq_parts(rows);
+      store_row<float, DP>(part + to * (SETS * a.dim), acc[0], by, a.dim, g);
+      if (EXACT) store_row<float, DP>(part + to * (SETS * a.dim) + a.dim, acc[SETS - 1], 1.f, a.dim, g);
+      if (g == 0) reinterpret_cast<float2*>(part + splits * rows * (SETS * a.dim))[to] = make_float2(exact, delta);
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(AT_NT) void k_attn_dq_join(ffn_ray_attn a, int splits) {
+  constexpr bool EXACT = sizeof(T) == 2;
+  constexpr int SETS = EXACT ? 2 : 1;
+  __shared__ f32x4 sums[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t rows = (int64_t)a.q_rays.n * a.heads, at = (int64_t)blockIdx.x * 4 + wave;
+  if (at >= rows) return;  // no barriers below
+  const float* part = (const float*)a.workspace + dq_parts(rows);
+  const float2* ed = reinterpret_cast<const float2*>(part + splits * rows * (SETS * a.dim));
+  const float delta = ed[at].y;
+  float D = 0.f;
+  for (int s = lane; s < splits; s += 64) D += ed[s * rows + at].x;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) D += __shfl_xor(D, d);
+  if (!EXACT) D = delta;
+  const int64_t step = rows * (SETS * a.dim);
+  const float* p = part + at * (SETS * a.dim);
+  f32x4 o = sum_splits(p, step, splits, a.dim, nullptr, sums[wave], lane);
+  if (EXACT) {
+    const f32x4 x = sum_splits(p + a.dim, step, splits, a.dim, nullptr, sums[wave], lane);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = __builtin_fmaf(x[r], delta - D, o[r]);
+  }
+  if (lane < a.dim / 4) {
+    typename Mat<T>::quad q;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) q[r] = (T)(o[r] * (a.scale * W_UNSHIFT));
+    *reinterpret_cast<typename Mat<T>::quad*>((T*)a.dq + at * a.dim + 4 * lane) = q;
+  }
+  if (lane == 0) ((float*)a.workspace)[at] = D;
+}
+
+// Averages that the host knows: rays with queries, and the keys of one
+static int64_t rays_with_queries(const ffn_ray_attn& a) {
+  const int64_t rays = a.q_rays.num_rays < a.q_rays.n ? a.q_rays.num_rays : a.q_rays.n;
+  return rays < 1 ? 1 : rays;
+}
+
+// Whether one query at a time is the faster.  Its time is about 1.6 ns a (query, key head) and tile of keys, one more for
+// the start.  k_attn_fwd's is a chain over the keys of a block's 64 queries, 1.1 us a tile, or 1.6 ns a block and tile and
+// 10 ns a block if there are many blocks.  Measured, bf16, dim 64, 8 heads with 2 of keys, us (row / tile): 65536 rays of 8
+// keys and a query 303 / 154; 8192 of 128 102 / 202, with four queries each 257 / 213; 64 of 16384 106 / 17505, with four
+// 196 / 4395, with sixteen 782 / 1008, and 1642 / 1008 where each head has its own keys.  The backward (mostly dk and dv)
+// follows: 1001 / 489, 675 / 893, 1045 / 840, 618 / 22772, 699 / 6128, 1186 / 1701, 2061 / 1879.
+static bool by_row(const ffn_ray_attn& a) {
+  const double n = (double)a.q_rays.n, keys = (double)a.k_rays.n, mean = keys / rays_with_queries(a);
+  // 16 rows that share a few tiles of keys: k_attn_fwd's own case, though its chain may be a few us longer if all is small
+  if (n > 16. * rays_with_queries(a) && mean <= 16. * AT_TILE) return false;
+  const double row = 1.6 * n * a.kv_heads * (2. + floor(mean / AT_TILE));
+  const double blocks = ceil(n / AT_TILE) * a.heads;
+  const double a_block = (a.q_rays.n < AT_TILE ? keys : keys * AT_TILE / n) / AT_TILE;
+  const double tiles = fmax(a_block, mean / AT_TILE) + 1.;
+  return row < fmax(1100. * tiles, (1.6 * tiles + 10.) * blocks);
+}
+// Few rows are split over their keys until ROW_WAVES wavefronts have work, 16 a CU: 64 rays of 16384 keys, us with 512, 1024,
+// 2048 and 4096 of them: 126, 104, 104, 106; with four queries each 453, 325, 327, 195.
 constexpr int64_t ROW_WAVES = 4096;
-// one wavefront a row and no tile shared between rows, where rays have at most one query each (on average)
-static bool by_row(const ffn_ray_attn& a) { return a.q_rays.n <= a.q_rays.num_rays; }
 static int row_splits(const ffn_ray_attn& a) {
   const int64_t waves = (int64_t)a.q_rays.n * a.kv_heads;
-  const int64_t tiles = ((int64_t)a.k_rays.n / a.q_rays.n + AT_TILE - 1) / AT_TILE;  // of an average row
+  const int64_t tiles = (int64_t)a.k_rays.n / rays_with_queries(a) / AT_TILE + 1;
   int64_t s = (ROW_WAVES + waves - 1) / waves;
   s = s < tiles ? s : tiles;
-  return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+  return (int)(s < 1 ? 1 : s > MAX_SPLITS ? MAX_SPLITS : s);
 }
 
 uint64_t attn_workspace(const ffn_ray_attn& a, bool backward) {
   const uint64_t rows = (uint64_t)a.q_rays.n * a.heads;
-  if (backward) return rows * sizeof(float);
-  if (a.q_rays.n == 0 || !by_row(a)) return 0;
-  const uint64_t s = row_splits(a);
-  return s > 1 ? s * rows * (a.dim + 2) * sizeof(float) : 0;
+  const uint64_t splits = a.q_rays.n && by_row(a) ? row_splits(a) : 1;
+  const uint64_t sets = backward && a.dtype != FFN_F32 ? 2 : 1;
+  const uint64_t parts = splits > 1 ? splits * rows * (sets * a.dim + 2) : 0;
+  return ((backward ? (uint64_t)dq_parts(rows) : 0) + parts) * sizeof(float);
 }
 
 static unsigned die_grid(int64_t total) { return (unsigned)((total + 8 * DIE_RUN - 1) / (8 * DIE_RUN) * (8 * DIE_RUN)); }
 
-// Sets of 16 kept rows a wavefront: two where rays are long on both sides and the registers hold them
+// Sets of 16 kept rows a wavefront: two where rays are long on both sides and the registers hold them.  One set / two, us,
+// forward and backward of bf16, dim 64, 4 heads, causal: 400000 rows in rays of 48 189 + 483 / 194 + 499, of 96 192 + 486 /
+// 191 + 496; 262144 in rays of 128 124 + 351 / 120 + 325; 65536 in rays of 1024 114 + 361 / 105 + 267.
 template <typename T, int DP> constexpr int MAX_SETS = sizeof(T) == 2 && DP <= 64 ? 2 : 1;
 template <typename T, int DP>
 static int sets(const ffn_ray_set& kept, const ffn_ray_set& streamed) {
   const int64_t rays = kept.num_rays;
-  return kept.n >= 256 * rays && streamed.n >= 256 * rays ? MAX_SETS<T, DP> : 1;
+  return kept.n >= 128 * rays && streamed.n >= 128 * rays ? MAX_SETS<T, DP> : 1;
 }
 
 template <typename T, int DP, bool CAP>
@@ -964,7 +1171,12 @@ static hipError_t fwd(const ffn_ray_attn& a, hipStream_t st) {
 
 template <typename T, int DP, bool CAP>
 static hipError_t bwd(const ffn_ray_attn& a, hipStream_t st) {
-  if (a.q_rays.n) {
+  if (a.q_rays.n && by_row(a)) {
+    const int splits = row_splits(a);
+    const int64_t total = (int64_t)a.q_rays.n * a.kv_heads * splits;
+    k_attn_dq_row<T, DP, CAP><<<(unsigned)((total + 3) / 4), AT_NT, 0, st>>>(a, splits, total);
+    if (splits > 1) k_attn_dq_join<T><<<(unsigned)(((int64_t)a.q_rays.n * a.heads + 3) / 4), AT_NT, 0, st>>>(a, splits);
+  } else if (a.q_rays.n) {
     const int64_t rows = 64 * sets<T, DP>(a.q_rays, a.k_rays), total = ((int64_t)a.q_rays.n + rows - 1) / rows * a.heads;
     if (rows > 64) k_attn_dq<T, DP, MAX_SETS<T, DP>, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
     else k_attn_dq<T, DP, 1, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);

@@ -107,6 +107,42 @@ def test_few_queries_over_long_rays(ty, H, G, D):
     _check(q, k, v, do, qs, ks, backward=False, causal=True)
 
 
+FEW = [([2, 1, 0, 16, 3], [900, 64, 30, 1, 2049]), ([3, 2, 0, 5, 4, 2], [9, 60, 5, 33, 0, 64])]
+
+
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("H,G,D", [(4, 2, 32), (6, 2, 64), (20, 1, 16), (2, 1, 128), (3, 3, 24)])
+@pytest.mark.parametrize("nq,nk", FEW)
+def test_few_queries_a_ray(ty, H, G, D, nq, nk):
+    """A query at a time, split over long rays' keys and not, forward and backward."""
+    qs, ks = ray_set(nq, gap=2), ray_set(nk, gap=3)
+    q, k, v, do, t_q, t_k = _inputs(qs, ks, H, G, D, TYPES[ty], seed=16)
+    for option in ("bias", "all"):
+        _check(q, k, v, do, qs, ks, **_options(option, H, len(nq), t_q, t_k))
+
+
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("nq,nk", FEW)
+def test_few_queries_beside_a_sick_ray(ty, nq, nk):
+    """Keys, values and gradients of one ray that are infinite or NaN leave the others' results as they are."""
+    import ray_ops
+    qs, ks = ray_set(nq, gap=2), ray_set(nk, gap=3)
+    q, k, v, do, _, _ = _inputs(qs, ks, 4, 2, 32, TYPES[ty], seed=17)
+    rq, rk = _dev_set(qs), _dev_set(ks)
+    run = []
+    for sick in (False, True):
+        qd, kd, vd, dd = (x.clone() for x in (q, k, v, do))
+        if sick:
+            for x, ids in ((kd, ks[2]), (vd, ks[2]), (dd, qs[2])):
+                x[ids == 3] = torch.tensor([float("nan"), float("inf")], dtype=x.dtype)[torch.arange(int((ids == 3).sum())) % 2][:, None, None]
+        qd, kd, vd, dd = (x.cuda() for x in (qd, kd, vd, dd))
+        o, lse = ray_ops.ray_attention(qd, kd, vd, rq, rk)
+        run.append((o, lse, *ray_ops.ray_attention_backward(dd, qd, kd, vd, o, lse, rq, rk)))
+    for a, b, ids in zip(*run, (qs[2], qs[2], qs[2], ks[2], ks[2])):
+        well = (ids != 3).cuda()
+        assert torch.equal(a[well], b[well])
+
+
 @pytest.mark.parametrize("ty", ["bf16", "fp16"])
 def test_long_ray_with_its_gradients(ty):
     rays = ray_set([1000, 30])
