@@ -553,10 +553,11 @@ struct GradScale {
   }
 };
 
-// dq; also leaves D of its rows in the workspace for k_attn_dkv.  D = sum_d do o takes o's rounding in 16 bits, and a short
-// ray's dq was a fifth further off for it.  So there it is a first value D' only: the sums are those of P (dP - D'), the
-// exact D = sum_j P dP is formed beside them, and (D' - D) sum_j P k, whose fragments of K are there already, sets dq
-// right (102 -> 110 us for 8192 rays).  Long rays (NQ = 2) have an o far smaller than v, and keep D': 328 us instead of 472.
+// dq; also leaves D of its rows in the workspace for k_attn_dkv.  D = sum_d do o takes o's rounding in 16 bits, and dq was a
+// fifth further off for it on short rays, a twentieth on long ones of up to 32 columns.  So there it is a first value D'
+// only: the sums are those of P (dP - D'), the exact D = sum_j P dP is formed beside them, and (D' - D) sum_j P k, whose
+// fragments of K are there already, sets dq right (102 -> 110 us for 8192 rays; 65536 rows in rays of 2048, 32 columns,
+// backward 373 -> 437).  Long rays of more columns (NQ = 2) keep D', which does not show there: 328 us instead of 472.
 template <typename T, int DP, int NQ, bool CAP>
 __global__ __launch_bounds__(AT_NT, least_waves(sizeof(T), DP, NQ, CAP)) void k_attn_dq(ffn_ray_attn a, int64_t total) {
   constexpr int KS = DP / 32, NB = DP / 16, TILE = AT_TILE * lds_row<T, DP>;
@@ -1148,10 +1149,11 @@ static unsigned die_grid(int64_t total) { return (unsigned)((total + 8 * DIE_RUN
 // forward and backward of bf16, dim 64, 4 heads, causal: 400000 rows in rays of 48 189 + 483 / 194 + 499, of 96 192 + 486 /
 // 191 + 496; 262144 in rays of 128 124 + 351 / 120 + 325; 65536 in rays of 1024 114 + 361 / 105 + 267.
 template <typename T, int DP> constexpr int MAX_SETS = sizeof(T) == 2 && DP <= 64 ? 2 : 1;
-template <typename T, int DP>
+template <typename T, int DP> constexpr int DQ_SETS = DP > 32 ? MAX_SETS<T, DP> : 1;
+template <int MOST>
 static int sets(const ffn_ray_set& kept, const ffn_ray_set& streamed) {
   const int64_t rays = kept.num_rays;
-  return kept.n >= 128 * rays && streamed.n >= 128 * rays ? MAX_SETS<T, DP> : 1;
+  return kept.n >= 128 * rays && streamed.n >= 128 * rays ? MOST : 1;
 }
 
 template <typename T, int DP, bool CAP>
@@ -1162,7 +1164,7 @@ static hipError_t fwd(const ffn_ray_attn& a, hipStream_t st) {
     k_attn_row<T, DP, CAP><<<(unsigned)((total + 3) / 4), AT_NT, 0, st>>>(a, splits, total);
     if (splits > 1) k_attn_join<T><<<(unsigned)(((int64_t)a.q_rays.n * a.heads + 3) / 4), AT_NT, 0, st>>>(a, splits);
   } else {
-    const int64_t rows = 64 * sets<T, DP>(a.q_rays, a.k_rays), total = ((int64_t)a.q_rays.n + rows - 1) / rows * a.heads;
+    const int64_t rows = 64 * sets<MAX_SETS<T, DP>>(a.q_rays, a.k_rays), total = ((int64_t)a.q_rays.n + rows - 1) / rows * a.heads;
     if (rows > 64) k_attn_fwd<T, DP, MAX_SETS<T, DP>, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
     else k_attn_fwd<T, DP, 1, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
   }
@@ -1177,12 +1179,12 @@ static hipError_t bwd(const ffn_ray_attn& a, hipStream_t st) {
     k_attn_dq_row<T, DP, CAP><<<(unsigned)((total + 3) / 4), AT_NT, 0, st>>>(a, splits, total);
     if (splits > 1) k_attn_dq_join<T><<<(unsigned)(((int64_t)a.q_rays.n * a.heads + 3) / 4), AT_NT, 0, st>>>(a, splits);
   } else if (a.q_rays.n) {
-    const int64_t rows = 64 * sets<T, DP>(a.q_rays, a.k_rays), total = ((int64_t)a.q_rays.n + rows - 1) / rows * a.heads;
-    if (rows > 64) k_attn_dq<T, DP, MAX_SETS<T, DP>, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
+    const int64_t rows = 64 * sets<DQ_SETS<T, DP>>(a.q_rays, a.k_rays), total = ((int64_t)a.q_rays.n + rows - 1) / rows * a.heads;
+    if (rows > 64) k_attn_dq<T, DP, DQ_SETS<T, DP>, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
     else k_attn_dq<T, DP, 1, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
   }
   if (a.k_rays.n) {
-    const int64_t rows = 64 * sets<T, DP>(a.k_rays, a.q_rays), total = ((int64_t)a.k_rays.n + rows - 1) / rows * a.kv_heads;
+    const int64_t rows = 64 * sets<MAX_SETS<T, DP>>(a.k_rays, a.q_rays), total = ((int64_t)a.k_rays.n + rows - 1) / rows * a.kv_heads;
     if (rows > 64) k_attn_dkv<T, DP, MAX_SETS<T, DP>, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
     else k_attn_dkv<T, DP, 1, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
   }
