@@ -239,14 +239,14 @@ struct Logits {
   }
 };
 
-// s[q] = 16 B tile rows . kept rows of set q
-template <typename T, int DP, int NQ, int B>
+// s[q] = from(q, b) + 16 B tile rows . kept rows of set q
+template <typename T, int DP, int NQ, int B, typename F>
 __device__ __forceinline__ void products(f32x4 (&s)[NQ][B], const T* tile, const typename Mat<T>::frag (&kept)[NQ][DP / 32],
-                                         int lane) {
+                                         int lane, F from) {
 #pragma unroll
   for (int b = 0; b < B; ++b) {
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) s[q][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < NQ; ++q) s[q][b] = from(q, b);
 #pragma unroll
     for (int ks = 0; ks < DP / 32; ++ks) {
       const typename Mat<T>::frag f = row_frag<T, DP>(tile, 16 * b + (lane & 15), ks, lane);
@@ -254,6 +254,12 @@ __device__ __forceinline__ void products(f32x4 (&s)[NQ][B], const T* tile, const
       for (int q = 0; q < NQ; ++q) s[q][b] = Mat<T>::mma(f, kept[q][ks], s[q][b]);
     }
   }
+}
+
+template <typename T, int DP, int NQ, int B>
+__device__ __forceinline__ void products(f32x4 (&s)[NQ][B], const T* tile, const typename Mat<T>::frag (&kept)[NQ][DP / 32],
+                                         int lane) {
+  products<T, DP, NQ, B>(s, tile, kept, lane, [](int, int) { return f32x4{0.f, 0.f, 0.f, 0.f}; });
 }
 
 // a fragment with its infinities and NaN as 0
@@ -555,7 +561,8 @@ struct GradScale {
 
 // dq; also leaves D of its rows in the workspace for k_attn_dkv.  D = sum_d do o takes o's rounding in 16 bits, and dq was a
 // fifth further off for it on short rays, a twentieth on long ones of up to 32 columns.  So there it is a first value D'
-// only: the sums are those of P (dP - D'), the exact D = sum_j P dP is formed beside them, and (D' - D) sum_j P k, whose
+// only: the products begin at -D', the sums are those of P (dP - D'), D - D' = sum_j P (dP - D') is formed beside them, and
+// (D' - D) sum_j P k, whose
 // fragments of K are there already, sets dq right (102 -> 110 us for 8192 rays; 65536 rows in rays of 2048, 32 columns,
 // backward 373 -> 437).  Long rays of more columns (NQ = 2) keep D', which does not show there: 328 us instead of 472.
 template <typename T, int DP, int NQ, bool CAP>
@@ -645,7 +652,8 @@ __global__ __launch_bounds__(AT_NT, least_waves(sizeof(T), DP, NQ, CAP)) void k_
       f32x4 dp[NQ][B], th[B], s[SETS][B];  // s: the products, then the weights; the sets' logits come last
       f32x4(&x)[NQ][B] = *reinterpret_cast<f32x4(*)[NQ][B]>(&s[SETS - NQ]);
       products<T, DP, NQ, B>(x, ks[at] + p * lds_row<T, DP>, qf, lane);
-      products<T, DP, NQ, B>(dp, vs[at] + p * lds_row<T, DP>, df, lane);
+      products<T, DP, NQ, B>(dp, vs[at] + p * lds_row<T, DP>, df, lane,
+                             [&](int q, int) { return f32x4{-delta[q], -delta[q], -delta[q], -delta[q]}; });
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
         logits(x[q], th, t[q], ts[at] + p, g);
@@ -657,7 +665,7 @@ __global__ __launch_bounds__(AT_NT, least_waves(sizeof(T), DP, NQ, CAP)) void k_
         }
         // the slope of the cap
         if (CAP) each<B>([&](int b, int r) { x[q][b][r] *= __builtin_fmaf(-th[b][r], th[b][r], 1.f); });
-        each<B>([&](int b, int r) { s[q][b][r] = x[q][b][r] * (dp[q][b][r] - delta[q]); });
+        each<B>([&](int b, int r) { s[q][b][r] = x[q][b][r] * dp[q][b][r]; });
         if constexpr (!EXACT) mask(s[q], row0, kept.span[q], kept.seen[q], g, 0.f);
         gs[q].apply(s[q], acc[q]);
       }
@@ -669,7 +677,7 @@ __global__ __launch_bounds__(AT_NT, least_waves(sizeof(T), DP, NQ, CAP)) void k_
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
     const int64_t to = kept.row[q] * a.heads + head;
-    const float D = EXACT ? swap_add(exact[q]) * W_UNSHIFT : delta[q], off = delta[q] - D, by = gs[q].undo();
+    const float off = EXACT ? -swap_add(exact[q]) * W_UNSHIFT : 0.f, D = delta[q] - off, by = gs[q].undo();
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -731,7 +739,7 @@ __global__ __launch_bounds__(AT_NT, least_waves_dkv(sizeof(T), DP, NQ, CAP)) voi
       const int64_t i = row0 + tid;
       if (bias) tst = a.t_q[i * a.t_q_row];
       lst = a.lse[i * a.heads + head] * LOG2E;
-      est = ((const float*)a.workspace)[i * a.heads + head];
+      est = -((const float*)a.workspace)[i * a.heads + head];
       lst = (lst == -INFINITY ? 0.f : lst) - W_SHIFT;
     }
   };
@@ -761,18 +769,18 @@ __global__ __launch_bounds__(AT_NT, least_waves_dkv(sizeof(T), DP, NQ, CAP)) voi
         const int row0 = tile + p;
         f32x4 s[NQ][B], dp[NQ][B], th[B];
         products<T, DP, NQ, B>(s, qs[at] + p * lds_row<T, DP>, kf, lane);
-        products<T, DP, NQ, B>(dp, ds[at] + p * lds_row<T, DP>, vf, lane);
+        products<T, DP, NQ, B>(dp, ds[at] + p * lds_row<T, DP>, vf, lane,
+                               [&](int, int b) { return *reinterpret_cast<const f32x4*>(es[at] + p + 16 * b + 4 * g); });
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
           logits(s[q], th, t[q], ts[at] + p, g);
 #pragma unroll
           for (int b = 0; b < B; ++b) {
             const f32x4 l = *reinterpret_cast<const f32x4*>(ls[at] + p + 16 * b + 4 * g);
-            const f32x4 e = *reinterpret_cast<const f32x4*>(es[at] + p + 16 * b + 4 * g);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               s[q][b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[q][b][r], logits.mul, -l[r]));
-              dp[q][b][r] = s[q][b][r] * (dp[q][b][r] - e[r]);
+              dp[q][b][r] *= s[q][b][r];
             }
           }
           if (CAP) each<B>([&](int b, int r) { dp[q][b][r] *= __builtin_fmaf(-th[b][r], th[b][r], 1.f); });
@@ -960,7 +968,7 @@ __global__ __launch_bounds__(AT_NT) void k_attn_join(ffn_ray_attn a, int splits)
 __host__ __device__ inline int64_t dq_parts(int64_t rows) { return (rows + 3) / 4 * 4; }
 
 // k_attn_dq for the queries that k_attn_row takes: K through the wavefront's LDS rows, V straight into the operand.  The
-// workspace holds D, then (splits) the sums of each part, and {sum P dP, D'}.
+// workspace holds D, then (splits) the sums of each part, and {sum P (dP - D'), D'}.
 template <typename T, int DP, bool CAP>
 __global__ __launch_bounds__(AT_NT) void k_attn_dq_row(ffn_ray_attn a, int splits, int64_t total) {
   constexpr int KS = DP / 32, NB = DP / 16, ROWS = row_tile<T, DP>, B = ROWS / 16;
@@ -1024,7 +1032,7 @@ __global__ __launch_bounds__(AT_NT) void k_attn_dq_row(ffn_ray_attn a, int split
       f32x4 dp[B], th[B], s[SETS][B], x[1][B];
 #pragma unroll
       for (int b = 0; b < B; ++b) {
-        dp[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        dp[b] = f32x4{-delta, -delta, -delta, -delta};
 #pragma unroll
         for (int k = 0; k < KS; ++k) dp[b] = Mat<T>::mma(vf[b][k], df[k], dp[b]);
       }
@@ -1042,7 +1050,7 @@ __global__ __launch_bounds__(AT_NT) void k_attn_dq_row(ffn_ray_attn a, int split
         if (EXACT) exact = __builtin_fmaf(w, dp[b][r], exact);
         if (CAP) w *= __builtin_fmaf(-th[b][r], th[b][r], 1.f);
         s[SETS - 1][b][r] = w;
-        s[0][b][r] = w * (dp[b][r] - delta);
+        s[0][b][r] = w * dp[b][r];
       });
       gs.apply(s[0], acc[0]);
       add_weighted<T, DP, SETS, B>(acc, s, ks, false, row0, seen_by, lane);
@@ -1051,13 +1059,12 @@ __global__ __launch_bounds__(AT_NT) void k_attn_dq_row(ffn_ray_attn a, int split
     const float by = gs.undo();
     exact = swap_add(exact) * W_UNSHIFT;
     if (splits == 1) {
-      const float D = EXACT ? exact : delta;
       each<NB>([&](int b, int r) {
-        acc[0][b][r] = EXACT ? __builtin_fmaf(acc[0][b][r], by, (delta - D) * acc[SETS - 1][b][r]) : acc[0][b][r] * by;
+        acc[0][b][r] = EXACT ? __builtin_fmaf(acc[0][b][r], by, -exact * acc[SETS - 1][b][r]) : acc[0][b][r] * by;
       });
       if (there) {
         store_row<T, DP>((T*)a.dq + at * a.dim, acc[0], a.scale * W_UNSHIFT, a.dim, g);
-        if (g == 0) ((float*)a.workspace)[at] = D;
+        if (g == 0) ((float*)a.workspace)[at] = EXACT ? delta + exact : delta;
       }
     } else if (there) {
       const int64_t rows = (int64_t)a.q_rays.n * a.heads, to = split * rows + at;
@@ -1080,18 +1087,17 @@ __global__ __launch_bounds__(AT_NT) void k_attn_dq_join(ffn_ray_attn a, int spli
   const float* part = (const float*)a.workspace + dq_parts(rows);
   const float2* ed = reinterpret_cast<const float2*>(part + splits * rows * (SETS * a.dim));
   const float delta = ed[at].y;
-  float D = 0.f;
-  for (int s = lane; s < splits; s += 64) D += ed[s * rows + at].x;
+  float exact = 0.f;
+  for (int s = lane; EXACT && s < splits; s += 64) exact += ed[s * rows + at].x;
 #pragma unroll
-  for (int d = 32; d; d >>= 1) D += __shfl_xor(D, d);
-  if (!EXACT) D = delta;
+  for (int d = 32; d; d >>= 1) exact += __shfl_xor(exact, d);
   const int64_t step = rows * (SETS * a.dim);
   const float* p = part + at * (SETS * a.dim);
   f32x4 o = sum_splits(p, step, splits, a.dim, nullptr, sums[wave], lane);
   if (EXACT) {
     const f32x4 x = sum_splits(p + a.dim, step, splits, a.dim, nullptr, sums[wave], lane);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) o[r] = __builtin_fmaf(x[r], delta - D, o[r]);
+    for (int r = 0; r < 4; ++r) o[r] = __builtin_fmaf(x[r], -exact, o[r]);
   }
   if (lane < a.dim / 4) {
     typename Mat<T>::quad q;
@@ -1099,7 +1105,7 @@ __global__ __launch_bounds__(AT_NT) void k_attn_dq_join(ffn_ray_attn a, int spli
     for (int r = 0; r < 4; ++r) q[r] = (T)(o[r] * (a.scale * W_UNSHIFT));
     *reinterpret_cast<typename Mat<T>::quad*>((T*)a.dq + at * a.dim + 4 * lane) = q;
   }
-  if (lane == 0) ((float*)a.workspace)[at] = D;
+  if (lane == 0) ((float*)a.workspace)[at] = delta + exact;
 }
 
 // Averages that the host knows: rays with queries, and the keys of one
