@@ -15,24 +15,18 @@ constexpr int EX_ROWS = 128;  // slots of a product tile
 // where the parts of a plan are, in words
 struct PlanView {
   int bins;  // experts + 1: the last bin is that of the rows of no expert
-  uint32_t n, chunk;
-  uint64_t counts, offsets, rows, tiles, n_tiles, chunks, n_chunks, chunk_first, words;
+  uint32_t n;
+  uint64_t counts, offsets, rows, tiles, n_tiles, words;
 };
 __host__ __device__ inline PlanView plan_view(uint32_t n, int experts) {
   PlanView v;
   v.bins = experts + 1;
   v.n = n;
-  // slots of a weight-gradient partial: about 512 of them, of 256 to 8192 slots
-  uint64_t c = ((uint64_t)n / 512 + 63) / 64 * 64;
-  v.chunk = (uint32_t)(c < 256 ? 256 : c > 8192 ? 8192 : c);
   v.counts = 0;
   v.offsets = v.bins;
-  v.chunk_first = 2 * (uint64_t)v.bins;
-  v.tiles = (3 * (uint64_t)v.bins + 2) / 2 * 2;
+  v.tiles = 2 * (uint64_t)v.bins;
   v.n_tiles = ((uint64_t)n + EX_ROWS - 1) / EX_ROWS + v.bins;
-  v.chunks = v.tiles + 2 * v.n_tiles;
-  v.n_chunks = ((uint64_t)n + v.chunk - 1) / v.chunk + v.bins;
-  v.rows = v.chunks + 2 * v.n_chunks;
+  v.rows = v.tiles + 2 * v.n_tiles;
   v.words = v.rows + n;
   return v;
 }
@@ -203,32 +197,18 @@ __global__ __launch_bounds__(PS_NT) void k_plan_small(const int32_t* __restrict_
   __syncthreads();
   bin_scan<PS_NT>(total, v.bins, first, part, [](uint32_t c) { return (c + EX_ROWS - 1) / EX_ROWS; });
   fill_table<PS_NT>((uint2*)(plan + v.tiles), v.n_tiles, 0, v.n_tiles, first, v.bins);
-  __syncthreads();
-  const uint32_t size = v.chunk;
-  bin_scan<PS_NT>(total, v.bins, first, part, [size](uint32_t c) { return (c + size - 1) / size; });
-  fill_table<PS_NT>((uint2*)(plan + v.chunks), v.n_chunks, 0, v.n_chunks, first, v.bins);
-  for (int b = tid; b < v.bins; b += PS_NT) plan[v.chunk_first + b] = first[b];
 }
 
 __global__ __launch_bounds__(PL_NT) void k_plan_move(const int32_t* __restrict__ ids, PlanView v, int bits, int blocks,
-                                                     int tile_blocks, const uint32_t* __restrict__ block_counts,
+                                                     const uint32_t* __restrict__ block_counts,
                                                      uint32_t* __restrict__ plan) {
   constexpr int NW = PL_NT / 64;
   __shared__ uint32_t first[PL_BINS + 1], part[NW], cnt[NW][PL_BINS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t* counts = plan + v.counts;
   if ((int)blockIdx.x >= blocks) {
-    const int t = blockIdx.x - blocks;
-    if (t < tile_blocks) {
-      bin_scan<PL_NT>(counts, v.bins, first, part, [](uint32_t c) { return (c + EX_ROWS - 1) / EX_ROWS; });
-      fill_table<PL_NT>((uint2*)(plan + v.tiles), v.n_tiles, (uint64_t)t * PL_BLOCK, PL_BLOCK, first, v.bins);
-    } else {
-      const uint32_t size = v.chunk;
-      bin_scan<PL_NT>(counts, v.bins, first, part, [size](uint32_t c) { return (c + size - 1) / size; });
-      fill_table<PL_NT>((uint2*)(plan + v.chunks), v.n_chunks, (uint64_t)(t - tile_blocks) * PL_BLOCK, PL_BLOCK, first, v.bins);
-      if (t == tile_blocks)
-        for (int b = tid; b < v.bins; b += PL_NT) plan[v.chunk_first + b] = first[b];
-    }
+    bin_scan<PL_NT>(counts, v.bins, first, part, [](uint32_t c) { return (c + EX_ROWS - 1) / EX_ROWS; });
+    fill_table<PL_NT>((uint2*)(plan + v.tiles), v.n_tiles, (uint64_t)(blockIdx.x - blocks) * PL_BLOCK, PL_BLOCK, first, v.bins);
     return;
   }
   bin_scan<PL_NT>(counts, v.bins, first, part, [](uint32_t c) { return c; });
@@ -277,8 +257,8 @@ hipError_t launch_expert_plan(const int32_t* ids, uint32_t n, int experts, uint3
   }
   k_plan_count<<<blocks, PL_NT, 0, st>>>(ids, v, workspace);
   k_plan_scan<<<v.bins, 64, 0, st>>>(workspace, blocks, plan, v);
-  const int tb = (int)((v.n_tiles + PL_BLOCK - 1) / PL_BLOCK), cb = (int)((v.n_chunks + PL_BLOCK - 1) / PL_BLOCK);
-  k_plan_move<<<blocks + tb + cb, PL_NT, 0, st>>>(ids, v, bits, blocks, tb, workspace, plan);
+  const int tile_blocks = (int)((v.n_tiles + PL_BLOCK - 1) / PL_BLOCK);
+  k_plan_move<<<blocks + tile_blocks, PL_NT, 0, st>>>(ids, v, bits, blocks, workspace, plan);
   return hipGetLastError();
 }
 
@@ -318,7 +298,7 @@ struct StageW {
 // Keeps the values of g whose y is positive (16 bytes or a fragment of either type).  In 16 bits, two at a time on the
 // bits: y - 1 is below infinity's bits exactly where y is positive and no NaN; the saturating sum puts that into the sign.
 template <typename T, typename V>
-__device__ __forceinline__ V where_positive(const V& g, const V& y) {
+__device__ __forceinline__ V where_positive(V g, V y) {
   constexpr int N = sizeof(V) / 4;
   typedef uint32_t words __attribute__((ext_vector_type(N)));
   words a = __builtin_bit_cast(words, g);
@@ -463,12 +443,18 @@ __global__ __launch_bounds__(EX_NT, 2) void k_expert(ffn_experts a, PlanView v, 
   }
 }
 
-// Sum over `merge` chunks of an expert's slots of g^T x, g = dy where y > 0: TM x TK values a block in four
-// wavefronts.  The slots are the K of the product, so both operands are columns of their LDS tiles.  g against ones gives
-// db's share.
+// Shares of the weight gradient: `groups` runs of `len` slots, whatever experts they hold, so that all blocks have the same
+// work.  The part of run j and expert e has index j + e: parts follow each other with j, e or both one up.
+// (Equal pieces of each expert, eight to a block: 255 us instead of 204 for 500009 rows of 24 uneven experts.)
+struct Shares {
+  uint32_t groups, len;
+};
+
+// Sums over runs of an expert's slots of g^T x, g = dy where y > 0: TM x TK values a block in four wavefronts.  The slots
+// are the K of the product, so both operands are columns of their LDS tiles.  g against ones gives db's share.
 template <typename T, int TM, int TK>
 __global__ __launch_bounds__(EX_NT) void k_expert_dw(ffn_experts a, PlanView v, int64_t total, int m_tiles, int k_tiles,
-                                                     int merge) {
+                                                     Shares shares) {
   typedef typename Mat<T>::frag frag;
   constexpr int EL = 16 / (int)sizeof(T), S = 64;  // slots of a step
   constexpr int GC = TM / EL, XC = TK / EL, NG = S * GC / EX_NT, NX = S * XC / EX_NT, NM = TM / 32, NK = TK / 32;
@@ -476,14 +462,18 @@ __global__ __launch_bounds__(EX_NT) void k_expert_dw(ffn_experts a, PlanView v, 
   __shared__ __align__(16) T xs[S * lds_row<T, TK>];
   const int64_t per = (total + 7) / 8, work = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if (work >= total) return;
-  const int64_t piece = work / (m_tiles * k_tiles);
-  const uint2 chunk = reinterpret_cast<const uint2*>(a.plan + v.chunks)[piece];
-  if (chunk.x >= (uint32_t)v.bins - 1 || chunk.y % merge) return;
+  const uint32_t run = (uint32_t)(work / (m_tiles * k_tiles));
   const int k0 = (int)(work % k_tiles) * TK, m0 = (int)(work / k_tiles % m_tiles) * TM;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
   const int mw = (wave >> 1) * (TM / 2), kw = (wave & 1) * (TK / 2);
-  const uint32_t off = a.plan[v.offsets + chunk.x], group = a.plan[v.counts + chunk.x];
-  const uint32_t from = off + chunk.y * v.chunk, to = off + min(group, (chunk.y + merge) * v.chunk);
+  const uint32_t* offsets = a.plan + v.offsets;  // the last bin's: the end of the experts' slots
+  const int experts = v.bins - 1;
+  uint32_t from = run * shares.len, to = 0;
+  const uint32_t end = min(from + shares.len, offsets[experts]);
+  if (from >= end) return;
+  int e = -1;  // to the expert that holds `from`: the last one that does not begin past it
+  for (int b = 0; b < experts; b += 64)
+    e += (int)__popcll(__ballot(b + lane < experts && offsets[min(b + lane, experts)] <= from));
   uint4 gv[NG], yv[NG], xv[NX];
   const bool x_slots = a.flags & FFN_EXPERTS_X_SLOTS, y_slots = a.flags & FFN_EXPERTS_Y_SLOTS;
   uint32_t gr[NG], xr[NX];  // the rows of the next step
@@ -512,7 +502,7 @@ __global__ __launch_bounds__(EX_NT) void k_expert_dw(ffn_experts a, PlanView v, 
     }
 #pragma unroll
     for (int i = 0; i < NX; ++i) xv[i] = *reinterpret_cast<const uint4*>(row_at(xp, xr[i], x_step));
-    if (to - s0 < (uint32_t)S) {  // rows past the chunk (the last one again) as 0
+    if (to - s0 < (uint32_t)S) {  // rows past the part (the last one again) as 0
 #pragma unroll
       for (int i = 0; i < NG; ++i)
         if (s0 + (tid + i * EX_NT) / GC >= to) gv[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -521,82 +511,90 @@ __global__ __launch_bounds__(EX_NT) void k_expert_dw(ffn_experts a, PlanView v, 
         if (s0 + (tid + i * EX_NT) / XC >= to) xv[i] = make_uint4(0u, 0u, 0u, 0u);
     }
   };
-  f32x4 acc[NM][NK], sum[NM];
-#pragma unroll
-  for (int i = 0; i < NM; ++i) {
-    sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < NK; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
   const bool sums = k0 == 0 && kw == 0;
   frag ones;
 #pragma unroll
   for (int j = 0; j < 8; ++j) ones[j] = (T)1.f;
-  rows(from);
-  fetch(from);
-  rows(from + S);
-  for (uint32_t s0 = from; s0 < to; s0 += S) {
-#pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      const int ch = tid + i * EX_NT;
-      if (a.relu) gv[i] = where_positive<T>(gv[i], yv[i]);
-      *reinterpret_cast<uint4*>(gs + ch / GC * lds_row<T, TM> + ch % GC * EL) = gv[i];
-    }
-#pragma unroll
-    for (int i = 0; i < NX; ++i) {
-      const int ch = tid + i * EX_NT;
-      *reinterpret_cast<uint4*>(xs + ch / XC * lds_row<T, TK> + ch % XC * EL) = xv[i];
-    }
-    __syncthreads();
-    if (to - s0 > S) {
-      fetch(s0 + S);
-      rows(s0 + 2 * S);
-    }
-#pragma unroll
-    for (int h = 0; h < S / 32; ++h) {
-      frag gf[NM];
-#pragma unroll
-      for (int i = 0; i < NM; ++i) gf[i] = col_frag<T, TM>(gs, 32 * h, mw + 16 * i, lane);
-#pragma unroll
-      for (int j = 0; j < NK; ++j) {
-        const frag xf = col_frag<T, TK>(xs, 32 * h, kw + 16 * j, lane);
-#pragma unroll
-        for (int i = 0; i < NM; ++i) acc[i][j] = Mat<T>::mma(gf[i], xf, acc[i][j]);
-      }
-      if (sums) {
-#pragma unroll
-        for (int i = 0; i < NM; ++i) sum[i] = Mat<T>::mma(gf[i], ones, sum[i]);
-      }
-    }
-    __syncthreads();
-  }
   const int64_t size = (int64_t)a.out * a.in + a.out;
-  float* part = (float*)a.workspace + piece * size;
+  for (; from < end; from = to) {
+    while (offsets[e + 1] <= from) ++e;
+    to = min(offsets[e + 1], end);
+    f32x4 acc[NM][NK], sum[NM];
 #pragma unroll
-  for (int i = 0; i < NM; ++i)
+    for (int i = 0; i < NM; ++i) {
+      sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int m = m0 + mw + 16 * i + 4 * g + r;
-      if (m >= a.out) continue;
-#pragma unroll
-      for (int j = 0; j < NK; ++j) {
-        const int k = k0 + kw + 16 * j + c;
-        if (k < a.in) part[(int64_t)m * a.in + k] = acc[i][j][r];
-      }
-      if (sums && c == 0) part[(int64_t)a.out * a.in + m] = sum[i][r];
+      for (int j = 0; j < NK; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    rows(from);
+    fetch(from);
+    rows(from + S);
+    for (uint32_t s0 = from; s0 < to; s0 += S) {
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const int ch = tid + i * EX_NT;
+        if (a.relu) gv[i] = where_positive<T>(gv[i], yv[i]);
+        *reinterpret_cast<uint4*>(gs + ch / GC * lds_row<T, TM> + ch % GC * EL) = gv[i];
+      }
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        const int ch = tid + i * EX_NT;
+        *reinterpret_cast<uint4*>(xs + ch / XC * lds_row<T, TK> + ch % XC * EL) = xv[i];
+      }
+      __syncthreads();
+      if (to - s0 > S) {
+        fetch(s0 + S);
+        rows(s0 + 2 * S);
+      }
+#pragma unroll
+      for (int h = 0; h < S / 32; ++h) {
+        frag gf[NM];
+#pragma unroll
+        for (int i = 0; i < NM; ++i) gf[i] = col_frag<T, TM>(gs, 32 * h, mw + 16 * i, lane);
+#pragma unroll
+        for (int j = 0; j < NK; ++j) {
+          const frag xf = col_frag<T, TK>(xs, 32 * h, kw + 16 * j, lane);
+#pragma unroll
+          for (int i = 0; i < NM; ++i) acc[i][j] = Mat<T>::mma(gf[i], xf, acc[i][j]);
+        }
+        if (sums) {
+#pragma unroll
+          for (int i = 0; i < NM; ++i) sum[i] = Mat<T>::mma(gf[i], ones, sum[i]);
+        }
+      }
+      __syncthreads();
+    }
+    float* part = (float*)a.workspace + ((int64_t)run + e) * size;
+#pragma unroll
+    for (int i = 0; i < NM; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int m = m0 + mw + 16 * i + 4 * g + r;
+        if (m >= a.out) continue;
+#pragma unroll
+        for (int j = 0; j < NK; ++j) {
+          const int k = k0 + kw + 16 * j + c;
+          if (k < a.in) part[(int64_t)m * a.in + k] = acc[i][j][r];
+        }
+        if (sums && c == 0) part[(int64_t)a.out * a.in + m] = sum[i][r];
+      }
+  }
 }
 
-// dW and db: the partials of an expert's chunks, in order
-__global__ __launch_bounds__(EX_NT) void k_expert_join(ffn_experts a, PlanView v, int merge) {
+// dW and db: an expert's parts, in order
+__global__ __launch_bounds__(EX_NT) void k_expert_join(ffn_experts a, PlanView v, Shares shares) {
   const int64_t mk = (int64_t)a.out * a.in, size = mk + a.out;
   const int64_t at = (int64_t)blockIdx.x * EX_NT + threadIdx.x;
   if (at >= size) return;
   const int e = blockIdx.y;
-  const uint32_t first = a.plan[v.chunk_first + e], last = a.plan[v.chunk_first + e + 1];
-  const float* part = (const float*)a.workspace;
+  const uint32_t off = a.plan[v.offsets + e], end = off + a.plan[v.counts + e];
+  const float* part = (const float*)a.workspace + e * size + at;
   float s = 0.f;
-  for (uint32_t p = first; p < last; p += merge) s += part[p * size + at];
+  if (off < end) {
+    const uint32_t last = (end - 1) / shares.len;
+#pragma unroll 8
+    for (uint32_t run = off / shares.len; run <= last; ++run) s += part[run * size];
+  }
   if (at < mk) {
     if (a.dW) a.dW[e * mk + at] = s;
   } else if (a.db) {
@@ -604,9 +602,38 @@ __global__ __launch_bounds__(EX_NT) void k_expert_join(ffn_experts a, PlanView v
   }
 }
 
+// Blocks that fill the card: two a CU.  Runs for 384, 512, 768 and 1024 blocks: weight gradient of 500009 rows, 256 x 256 values,
+// 240, 204, 227, 217 us; a million rows of 128 x 128 131, 127, 139, 143.  Runs of less than 256 slots gain nothing.
+constexpr int64_t FILL = 512;
+
+// A block's part of dW, and the runs
+struct WeightGradient {
+  int tm, tk, m_tiles, k_tiles;
+  Shares shares;
+};
+static WeightGradient weight_gradient(const ffn_experts& a) {
+  WeightGradient w;
+  // Tiles of 128 read dy and x half as often, if there is work for enough of them (64 / 128, us: a million rows of 128 x 128
+  // values 268 / 125, 65536 rows 20 / 27; 16384 rows of 256 x 256 24 / 28); float is bound by its products, not by reads.
+  const int64_t large = (int64_t)((a.out + 127) / 128) * ((a.in + 127) / 128);
+  const bool many = a.dtype != FFN_F32 && a.n / 1024 * large >= FILL / 2;
+  w.tm = many && a.out > 64 ? 128 : 64;
+  w.tk = many && a.in > 64 ? 128 : 64;
+  w.m_tiles = (a.out + w.tm - 1) / w.tm;
+  w.k_tiles = (a.in + w.tk - 1) / w.tk;
+  const int64_t tiles = (int64_t)w.m_tiles * w.k_tiles, n = a.n;
+  int64_t groups = FILL / tiles;
+  groups = groups < n / 256 ? groups : n / 256;
+  groups = groups < 1 ? 1 : groups;
+  w.shares.len = (uint32_t)(((n + groups - 1) / groups + 63) / 64 * 64);
+  w.shares.groups = n ? (uint32_t)((n + w.shares.len - 1) / w.shares.len) : 0;
+  if (!n) w.shares.len = 64;
+  return w;
+}
+
 uint64_t expert_workspace(const ffn_experts& a) {
   if (!a.dW && !a.db) return 0;
-  return plan_view(a.n, a.n_experts).n_chunks * ((uint64_t)a.out * a.in + a.out) * sizeof(float);
+  return ((uint64_t)weight_gradient(a).shares.groups + a.n_experts) * ((uint64_t)a.out * a.in + a.out) * sizeof(float);
 }
 
 template <typename T, bool BACK, int NB>
@@ -619,7 +646,6 @@ static void product(const ffn_experts& a, const PlanView& v, hipStream_t st) {
 // 256 columns a block, us, forward in bf16: 300000 rows, 256 x 256 values 141 / 124 / 122 (dx 182 / 144 / 132); 65536 rows
 // 34 / 30 / 41; 4096 rows 8.6 / 12 / 19; 128 x 128 values, a million rows 173 / 156 / 233, 65536 rows 16.3 / 14.6 / -,
 // 4096 rows 6.5 / 9.0 / 12.6; 64 x 64 values, a million rows 65 / 85 / 151.
-constexpr int64_t FILL = 512;
 template <typename T, bool BACK>
 static void product(const ffn_experts& a, const PlanView& v, hipStream_t st) {
   const int width = BACK ? a.in : a.out;
@@ -630,15 +656,10 @@ static void product(const ffn_experts& a, const PlanView& v, hipStream_t st) {
 }
 
 template <typename T, int TM, int TK>
-static void weight_gradient(const ffn_experts& a, const PlanView& v, hipStream_t st) {
-  const int mt = (a.out + TM - 1) / TM, kt = (a.in + TK - 1) / TK;
-  const int64_t pieces = (int64_t)v.n_chunks * mt * kt, size = (int64_t)a.out * a.in + a.out;
-  // chunks a block: FILL blocks share the slots, and the partials stay few (300000 rows, 256 x 256 values, us with 256, 512,
-  // 1024 blocks: 171, 107, 121; 65536 rows 43, 47, 56)
-  const int64_t share = (pieces + FILL / 2) / FILL;
-  const int merge = (int)(share < 1 ? 1 : share > 8 ? 8 : share);
-  k_expert_dw<T, TM, TK><<<(unsigned)((pieces + 7) / 8 * 8), EX_NT, 0, st>>>(a, v, pieces, mt, kt, merge);
-  k_expert_join<<<dim3((unsigned)((size + EX_NT - 1) / EX_NT), a.n_experts), EX_NT, 0, st>>>(a, v, merge);
+static void parts(const ffn_experts& a, const PlanView& v, const WeightGradient& w, hipStream_t st) {
+  const int64_t total = (int64_t)w.shares.groups * w.m_tiles * w.k_tiles;
+  if (total)
+    k_expert_dw<T, TM, TK><<<(unsigned)((total + 7) / 8 * 8), EX_NT, 0, st>>>(a, v, total, w.m_tiles, w.k_tiles, w.shares);
 }
 
 template <typename T>
@@ -650,15 +671,17 @@ static hipError_t run(const ffn_experts& a, bool backward, hipStream_t st) {
   }
   if (a.dx && a.n) product<T, true>(a, v, st);
   if (a.dW || a.db) {
-    // tiles of 128 read dy and x half as often, if enough of them have work (64 / 128, us: a million rows of 128 x 128 values
-    // 268 / 162, 4096 rows 9.8 / 14)
-    const bool many = (int64_t)v.n_chunks * ((a.out + 127) / 128) * ((a.in + 127) / 128) >= FILL / 2;
-    const bool m = many && a.out > 64, k = many && a.in > 64;
-    if constexpr (sizeof(T) == 4) weight_gradient<T, 64, 64>(a, v, st);  // bound by its products, not by reads
-    else if (m && k) weight_gradient<T, 128, 128>(a, v, st);
-    else if (m) weight_gradient<T, 128, 64>(a, v, st);
-    else if (k) weight_gradient<T, 64, 128>(a, v, st);
-    else weight_gradient<T, 64, 64>(a, v, st);
+    const WeightGradient w = weight_gradient(a);
+    if constexpr (sizeof(T) == 4) {
+      parts<T, 64, 64>(a, v, w, st);
+    } else {
+      if (w.tm == 128 && w.tk == 128) parts<T, 128, 128>(a, v, w, st);
+      else if (w.tm == 128) parts<T, 128, 64>(a, v, w, st);
+      else if (w.tk == 128) parts<T, 64, 128>(a, v, w, st);
+      else parts<T, 64, 64>(a, v, w, st);
+    }
+    const int64_t size = (int64_t)a.out * a.in + a.out;
+    k_expert_join<<<dim3((unsigned)((size + EX_NT - 1) / EX_NT), a.n_experts), EX_NT, 0, st>>>(a, v, w.shares);
   }
   return hipGetLastError();
 }
