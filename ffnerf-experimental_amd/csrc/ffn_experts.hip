@@ -362,39 +362,45 @@ __global__ __launch_bounds__(EX_NT, 2) void k_expert(ffn_experts a, PlanView v, 
   if (!none) {
     const T* W = (const T*)a.W + (int64_t)tile.x * a.out * a.in;
     StageW<T, BACK ? EX_K : C, BACK ? C : EX_K, BACK> w;
-    const T* in[2];
-    const T* gate[2];
+    uint32_t r[2];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const uint32_t r = in_slots ? slot[s] : row[s];
-      in[s] = row_at((const T*)(BACK ? a.dy : a.x), r, (uint32_t)(BACK ? a.dy_row : a.x_row) * sizeof(T)) + 8 * g;
-      gate[s] = BACK ? row_at((const T*)a.y, r, (uint32_t)a.out * sizeof(T)) + 8 * g : nullptr;
-    }
-    frag f[2][2];
+    for (int s = 0; s < 2; ++s) r[s] = in_slots && there[s] ? slot[s] : row[s];
+    const T* in = (const T*)(BACK ? a.dy : a.x) + 8 * g;
+    const T* gate = (const T*)a.y + 8 * g;
+    const uint32_t in_step = (uint32_t)(BACK ? a.dy_row : a.x_row) * sizeof(T), gate_step = (uint32_t)a.out * sizeof(T);
+    // The rows of the next step as they are, without predicates (rows past the end are row 0, their results are not stored;
+    // past the last column, the last ones again), so that nothing waits for them here.
+    frag f[2][2], y[2][2];
+    const bool gated = BACK && a.relu;
     auto fetch = [&](int k0) {
       if (BACK) w.load(W, a.out, a.in, k0, col0);
       else w.load(W, a.out, a.in, col0, k0);
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < 2; ++s) {
+        asm("" : "+v"(r[s]));  // the addresses are formed again each time: registers are what is short
+        const T* row_in = row_at(in, r[s], in_step);
+        const T* row_gate = row_at(gate, r[s], gate_step);
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          const int k = k0 + 32 * ks;
-          frag x;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = (T)0.f;
-          if (there[s] && k + 8 * g < depth) {
-            x = *reinterpret_cast<const frag*>(in[s] + k);
-            if (BACK && a.relu) x = where_positive<T>(x, *reinterpret_cast<const frag*>(gate[s] + k));
+        for (int ks = 0; ks < 2; ++ks)
+          if (k0 + 32 * ks < depth) {
+            const int k = min(k0 + 32 * ks, depth - 8 - 8 * g);
+            f[s][ks] = *reinterpret_cast<const frag*>(row_in + k);
+            if (gated) y[s][ks] = *reinterpret_cast<const frag*>(row_gate + k);
           }
-          f[s][ks] = x;
-        }
+      }
     };
     fetch(0);
     for (int k0 = 0; k0 < depth; k0 += EX_K) {
       w.store(lds);
       frag x[2][2];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) x[s][0] = f[s][0], x[s][1] = f[s][1];
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          x[s][ks] = f[s][ks];
+          if (gated) x[s][ks] = where_positive<T>(x[s][ks], y[s][ks]);
+          if (depth - k0 < EX_K && k0 + 32 * ks + 8 * g >= depth) x[s][ks] = frag{};
+        }
       __syncthreads();
       if (k0 + EX_K < depth) fetch(k0 + EX_K);
 #pragma unroll
