@@ -649,9 +649,9 @@ static void product(const ffn_experts& a, const PlanView& v, hipStream_t st) {
   k_expert<T, BACK, NB><<<(unsigned)((total + 7) / 8 * 8), EX_NT, 0, st>>>(a, v, total, cols);
 }
 // Columns a block: all of a row's, so that x is read once, but narrower ones while that leaves CUs without work.  64 / 128 /
-// 256 columns a block, us, forward in bf16: 300000 rows, 256 x 256 values 141 / 124 / 122 (dx 182 / 144 / 132); 65536 rows
-// 34 / 30 / 41; 4096 rows 8.6 / 12 / 19; 128 x 128 values, a million rows 173 / 156 / 233, 65536 rows 16.3 / 14.6 / -,
-// 4096 rows 6.5 / 9.0 / 12.6; 64 x 64 values, a million rows 65 / 85 / 151.
+// 256 columns a block, us, forward in bf16: 300000 rows, 256 x 256 values 146 / 121 / 118 (dx 168 / 117 / 104); 65536 rows
+// 34 / 29 / 41; 4096 rows 8 / 11 / 18; 128 x 128 values, a million rows 171 / 150 / 219, 65536 rows 16 / 14 / 26, 4096 rows
+// 6 / 9 / 13; 64 x 64 values, a million rows 66 / 85 / 150.
 template <typename T, bool BACK>
 static void product(const ffn_experts& a, const PlanView& v, hipStream_t st) {
   const int width = BACK ? a.in : a.out;

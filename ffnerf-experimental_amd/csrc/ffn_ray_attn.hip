@@ -387,8 +387,10 @@ struct Softmax {
 };
 
 // Blocks in launch order go round the eight dies; this gives each die runs of DIE_RUN neighbouring pieces of work, whose
-// tiles share keys in its L2.  Longer runs leave the dies with unequal work where rays are few and long.
-constexpr int DIE_RUN = 16;
+// tiles share keys in its L2.  Longer runs leave the dies with unequal work where rays are few and long (forward and
+// backward, us, runs of 1, 4, 16: 65536 rows in rays of 4000 272 + 844, 266 + 788, 326 + 880; 131072 in rays of 1000, 8 heads
+// 318 + 972, 305 + 911, 301 + 862; 400000 in rays of 40 201 + 503, 195 + 492, 193 + 489).
+constexpr int DIE_RUN = 4;
 __device__ __forceinline__ int64_t die_order() {
   const int64_t b = blockIdx.x >> 3;
   return (b / DIE_RUN * 8 + (blockIdx.x & 7)) * DIE_RUN + b % DIE_RUN;

@@ -5,9 +5,8 @@
 //   * by rays: one whole ray.  One launch, every value read once.
 //   * by parts: a part of the packed rows of a fixed length, whatever rays it holds, so that few long rays fill the GPU
 //     too.  A part that begins inside a ray needs the state there: k_scan_ends composes, per part, the steps of the ray
-//     that leaves it (h -> A h + B), k_scan_groups those of neighbouring
-//     parts, in a fixed order.  That reads gate and x a second
-//     time, but only of rays that cross a part's end.
+//     that leaves it (h -> A h + B), k_scan_groups those of neighbouring parts, in a fixed order.  That reads gate and x a
+//     second time, but only of rays that cross a part's end.
 // The backward pass walks the other way with D_t = dh_t + (1 - z_{t+1}) D_{t+1}.
 #include "ffn_ray_common.h"
 #include "ffn_ray_kernels.h"

@@ -151,7 +151,7 @@ def test_other_stream_graph_and_repeats(lens):
 
 
 def test_in_pieces():
-    """A ray's rows in two calls, the second from the first's last state, are one call (new samples round by round)."""
+    """A ray's rows in two calls, the second from the first's last state, are one call (new samples chunk by chunk)."""
     import ray_ops
     rays = ray_set([40, 25])
     gate, x, _, _, _ = (y.cuda() for y in _inputs(rays, 16, torch.float32, seed=9))
