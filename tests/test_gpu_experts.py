@@ -93,6 +93,20 @@ def test_long_group():
     _check(60001, 3, 64, 32, torch.bfloat16, seed=4, relu=True)
 
 
+@pytest.mark.parametrize("ty", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,E,K,M", [(140001, 3, 72, 136), (140001, 2, 200, 40), (90001, 3, 24, 264)])
+def test_many_rows(ty, n, E, K, M):
+    """Enough rows for the widest tiles of every product."""
+    _check(n, E, K, M, TYPES[ty], seed=6, relu=True)
+
+
+@pytest.mark.parametrize("ty", ["bf16", "fp32"])
+@pytest.mark.parametrize("K,M", [(40, 136), (136, 104)])
+def test_many_experts(ty, K, M):
+    """About two rows an expert, many with none."""
+    _check(2500, 1020, K, M, TYPES[ty], seed=7, relu=True)
+
+
 @pytest.mark.parametrize("ty", ["bf16", "fp32"])
 def test_slot_order_and_strides(ty):
     """Two layers in slot order between are the layers in row order; x as columns of a wider tensor."""

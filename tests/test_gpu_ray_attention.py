@@ -201,6 +201,42 @@ def test_what_is_not_seen_does_not_matter(ty):
         assert (lse2[out.cuda()] == -float("inf")).all()
 
 
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("D", [32, 56])
+@pytest.mark.parametrize("option", ["plain", "prefix", "all"])
+def test_longer_rays(ty, D, option):
+    """Long rays on average, some of them short: wavefronts of 32 rows in 16 bits."""
+    lens = [400, 150, 1, 0, 333]
+    rays = ray_set(lens, gap=1)
+    q, k, v, do, t, _ = _inputs(rays, rays, 4, 2, D, TYPES[ty], seed=18)
+    _check(q, k, v, do, rays, rays, **_options(option, 4, len(lens), t, t))
+
+
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+def test_longer_rays_beside_a_sick_one(ty, causal):
+    """As test_what_is_not_seen_does_not_matter, where wavefronts take 32 rows."""
+    import ray_ops
+    rays = ray_set([300, 180, 7, 250], gap=4)
+    ids = rays[2]
+    q, k, v, do, _, _ = _inputs(rays, rays, 2, 1, 64, TYPES[ty], seed=19)
+    sick = (ids >= 4) | (ids == 1)
+    bad = torch.tensor([float("nan"), float("inf"), -float("inf")])
+    qs, ks, vs, ds = (x.clone() for x in (q, k, v, do))
+    for x in (qs, ks, vs, ds):
+        x[sick] = bad[torch.arange(int(sick.sum())) % 3].to(x.dtype)[:, None, None]
+    rd = _dev_set(rays)
+    a = [x.cuda() for x in (qs, ks, vs)]
+    o, lse = ray_ops.ray_attention(*a, rd, causal=causal)
+    got = ray_ops.ray_attention_backward(ds.cuda(), *a, o, lse, rd, causal=causal)
+    ref = Attention(q, k, v, seen_mask(rays, rays, causal, None), scale=64 ** -0.5)
+    well = ~sick
+    close(o[well], ref.o[well], ref.o_bound(q.dtype)[well], "o")
+    close(lse[well], ref.lse[well], ref.lse_bound()[well], "lse")
+    for x, (want, bound), name in zip(got, ref.backward(do, q.dtype), ("dq", "dk", "dv")):
+        close(x[well], want[well], bound[well], name)
+
+
 def test_infinite_value_that_is_seen():
     rays = ray_set([6, 40])
     q, k, v, do, _, _ = _inputs(rays, rays, 1, 1, 16, torch.bfloat16, seed=10)
