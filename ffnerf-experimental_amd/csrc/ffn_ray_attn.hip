@@ -386,14 +386,11 @@ struct Softmax {
   }
 };
 
-// Blocks in launch order go round the eight dies; this gives each die runs of DIE_RUN neighbouring pieces of work, whose
-// tiles share keys in its L2.  Longer runs leave the dies with unequal work where rays are few and long (forward and
-// backward, us, runs of 1, 4, 16: 65536 rows in rays of 4000 272 + 844, 266 + 788, 326 + 880; 131072 in rays of 1000, 8 heads
-// 318 + 972, 305 + 911, 301 + 862; 400000 in rays of 40 201 + 503, 195 + 492, 193 + 489).
-constexpr int DIE_RUN = 4;
-__device__ __forceinline__ int64_t die_order() {
+// Blocks in launch order go round the eight dies; this gives each die runs of 2^run neighbouring pieces of work, whose
+// tiles share keys in its L2.
+__device__ __forceinline__ int64_t die_order(int run) {
   const int64_t b = blockIdx.x >> 3;
-  return (b / DIE_RUN * 8 + (blockIdx.x & 7)) * DIE_RUN + b % DIE_RUN;
+  return (((b >> run) * 8 + (blockIdx.x & 7)) << run) + (b & ((1 << run) - 1));
 }
 
 // the kept rows of a wavefront, NQ sets of 16: row number, what it sees, and the ranges over all of them
@@ -448,13 +445,13 @@ __device__ __forceinline__ void take_tile(F& take, int tile, int lo, int hi) {
 // where rays are short, by the wavefronts' start.  24 rays of up to 4096 rows, 4 heads of 64 with 2 of keys, causal, bf16:
 // 310 us, 395 TFLOP/s; 8192 rays of 23, 4 heads of 32, every option: 82 us.
 template <typename T, int DP, int NQ, bool CAP>
-__global__ __launch_bounds__(AT_NT, least_waves(sizeof(T), DP, NQ, CAP)) void k_attn_fwd(ffn_ray_attn a, int64_t total) {
+__global__ __launch_bounds__(AT_NT, least_waves(sizeof(T), DP, NQ, CAP)) void k_attn_fwd(ffn_ray_attn a, int64_t total, int run) {
   constexpr int KS = DP / 32, NB = DP / 16, TILE = AT_TILE * lds_row<T, DP>;
   __shared__ __align__(16) T ks[2][TILE];
   __shared__ __align__(16) T vs[2][TILE];
   __shared__ __align__(16) float ts[2][AT_TILE];
   __shared__ int s_range[8], s_bad[2][4];
-  const int64_t work = die_order();
+  const int64_t work = die_order(run);
   if (work >= total) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
   const unsigned item = (unsigned)work;
@@ -572,13 +569,13 @@ struct GradScale {
 // backward 373 -> 437).  Long rays of more columns (NQ = 2) keep D', which does not show there: 328 us instead of 472.  Bound as k_attn_fwd is; on the rays named there
 // 335 us (550 TFLOP/s) and 108 us.
 template <typename T, int DP, int NQ, bool CAP>
-__global__ __launch_bounds__(AT_NT, least_waves(sizeof(T), DP, NQ, CAP)) void k_attn_dq(ffn_ray_attn a, int64_t total) {
+__global__ __launch_bounds__(AT_NT, least_waves(sizeof(T), DP, NQ, CAP)) void k_attn_dq(ffn_ray_attn a, int64_t total, int run) {
   constexpr int KS = DP / 32, NB = DP / 16, TILE = AT_TILE * lds_row<T, DP>;
   __shared__ __align__(16) T ks[2][TILE];
   __shared__ __align__(16) T vs[2][TILE];
   __shared__ __align__(16) float ts[2][AT_TILE];
   __shared__ int s_range[8], s_bad[2][4];
-  const int64_t work = die_order();
+  const int64_t work = die_order(run);
   if (work >= total) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
   const unsigned item = (unsigned)work;
@@ -700,13 +697,13 @@ __global__ __launch_bounds__(AT_NT, least_waves(sizeof(T), DP, NQ, CAP)) void k_
 // weights at two wavefronts a SIMD (vector ALU 46 %, matrix cores 27 % busy); on k_attn_fwd's rays 540 us (455 TFLOP/s) and
 // 118 us.
 template <typename T, int DP, int NQ, bool CAP>
-__global__ __launch_bounds__(AT_NT, least_waves_dkv(sizeof(T), DP, NQ, CAP)) void k_attn_dkv(ffn_ray_attn a, int64_t total) {
+__global__ __launch_bounds__(AT_NT, least_waves_dkv(sizeof(T), DP, NQ, CAP)) void k_attn_dkv(ffn_ray_attn a, int64_t total, int run) {
   constexpr int KS = DP / 32, NB = DP / 16, TILE = AT_TILE * lds_row<T, DP>;
   __shared__ __align__(16) T qs[2][TILE];
   __shared__ __align__(16) T ds[2][TILE];
   __shared__ __align__(16) float ts[2][AT_TILE], ls[2][AT_TILE], es[2][AT_TILE];
   __shared__ int s_range[8], s_bad[2][8];
-  const int64_t work = die_order();
+  const int64_t work = die_order(run);
   if (work >= total) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
   const unsigned item = (unsigned)work;
@@ -1159,17 +1156,23 @@ uint64_t attn_workspace(const ffn_ray_attn& a, bool backward) {
   return ((backward ? (uint64_t)dq_parts(rows) : 0) + parts) * sizeof(float);
 }
 
-static unsigned die_grid(int64_t total) { return (unsigned)((total + 8 * DIE_RUN - 1) / (8 * DIE_RUN) * (8 * DIE_RUN)); }
+// Runs of 16 pieces of work a die, of 4 where rays are so long that runs of 16 would leave the dies with unequal work (4 / 16,
+// forward + backward, us: 65536 rows in rays of 4000 266 + 788 / 326 + 880; 131072 in rays of 1000, 8 heads 305 + 911 /
+// 301 + 862; 131072 in rays of 512 119 + 346 / 93 + 287; 400000 in rays of 40 195 + 492 / 193 + 489)
+static int die_run(const ffn_ray_set& kept) { return kept.n >= 2048 * (int64_t)kept.num_rays ? 2 : 4; }
+static unsigned die_grid(int64_t total, int run) { return (unsigned)(((total + (8 << run) - 1) >> (3 + run)) << (3 + run)); }
 
-// Sets of 16 kept rows a wavefront: two where rays are long on both sides and the registers hold them.  One set / two, us,
-// forward and backward of bf16, dim 64, 4 heads, causal: 400000 rows in rays of 48 189 + 483 / 194 + 499, of 96 192 + 486 /
-// 191 + 496; 262144 in rays of 128 124 + 351 / 120 + 325; 65536 in rays of 1024 114 + 361 / 105 + 267.
+// Sets of 16 kept rows a wavefront: two where rays are long on both sides, the registers hold them and `least` blocks of 128
+// rows have work.  One set / two, us, forward and backward of bf16, dim 64, 4 heads, causal: 400000 rows in rays of 48
+// 189 + 483 / 194 + 499, of 96 192 + 486 / 191 + 496; 262144 in rays of 128 124 + 351 / 120 + 325; 65536 in rays of 1024
+// 114 + 361 / 105 + 267; in rays of 1500 72000 132 + 409 / 136 + 363, 36000 79 + 235 / 86 + 214, 18000 49 + 175 / 58 + 196.
+constexpr int64_t FWD_BLOCKS = 1536, DQ_BLOCKS = 1024, DKV_BLOCKS = 512;
 template <typename T, int DP> constexpr int MAX_SETS = sizeof(T) == 2 && DP <= 64 ? 2 : 1;
 template <typename T, int DP> constexpr int DQ_SETS = DP > 32 ? MAX_SETS<T, DP> : 1;
 template <int MOST>
-static int sets(const ffn_ray_set& kept, const ffn_ray_set& streamed) {
+static int sets(const ffn_ray_set& kept, const ffn_ray_set& streamed, int heads, int64_t least) {
   const int64_t rays = kept.num_rays;
-  return kept.n >= 128 * rays && streamed.n >= 128 * rays ? MOST : 1;
+  return kept.n >= 128 * rays && streamed.n >= 128 * rays && kept.n / 128 * heads >= least ? MOST : 1;
 }
 
 template <typename T, int DP, bool CAP>
@@ -1180,9 +1183,10 @@ static hipError_t fwd(const ffn_ray_attn& a, hipStream_t st) {
     k_attn_row<T, DP, CAP><<<(unsigned)((total + 3) / 4), AT_NT, 0, st>>>(a, splits, total);
     if (splits > 1) k_attn_join<T><<<(unsigned)(((int64_t)a.q_rays.n * a.heads + 3) / 4), AT_NT, 0, st>>>(a, splits);
   } else {
-    const int64_t rows = 64 * sets<MAX_SETS<T, DP>>(a.q_rays, a.k_rays), total = ((int64_t)a.q_rays.n + rows - 1) / rows * a.heads;
-    if (rows > 64) k_attn_fwd<T, DP, MAX_SETS<T, DP>, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
-    else k_attn_fwd<T, DP, 1, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
+    const int run = die_run(a.q_rays);
+    const int64_t rows = 64 * sets<MAX_SETS<T, DP>>(a.q_rays, a.k_rays, a.heads, FWD_BLOCKS), total = ((int64_t)a.q_rays.n + rows - 1) / rows * a.heads;
+    if (rows > 64) k_attn_fwd<T, DP, MAX_SETS<T, DP>, CAP><<<die_grid(total, run), AT_NT, 0, st>>>(a, total, run);
+    else k_attn_fwd<T, DP, 1, CAP><<<die_grid(total, run), AT_NT, 0, st>>>(a, total, run);
   }
   return hipGetLastError();
 }
@@ -1195,14 +1199,16 @@ static hipError_t bwd(const ffn_ray_attn& a, hipStream_t st) {
     k_attn_dq_row<T, DP, CAP><<<(unsigned)((total + 3) / 4), AT_NT, 0, st>>>(a, splits, total);
     if (splits > 1) k_attn_dq_join<T><<<(unsigned)(((int64_t)a.q_rays.n * a.heads + 3) / 4), AT_NT, 0, st>>>(a, splits);
   } else if (a.q_rays.n) {
-    const int64_t rows = 64 * sets<DQ_SETS<T, DP>>(a.q_rays, a.k_rays), total = ((int64_t)a.q_rays.n + rows - 1) / rows * a.heads;
-    if (rows > 64) k_attn_dq<T, DP, DQ_SETS<T, DP>, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
-    else k_attn_dq<T, DP, 1, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
+    const int run = die_run(a.q_rays);
+    const int64_t rows = 64 * sets<DQ_SETS<T, DP>>(a.q_rays, a.k_rays, a.heads, DQ_BLOCKS), total = ((int64_t)a.q_rays.n + rows - 1) / rows * a.heads;
+    if (rows > 64) k_attn_dq<T, DP, DQ_SETS<T, DP>, CAP><<<die_grid(total, run), AT_NT, 0, st>>>(a, total, run);
+    else k_attn_dq<T, DP, 1, CAP><<<die_grid(total, run), AT_NT, 0, st>>>(a, total, run);
   }
   if (a.k_rays.n) {
-    const int64_t rows = 64 * sets<MAX_SETS<T, DP>>(a.k_rays, a.q_rays), total = ((int64_t)a.k_rays.n + rows - 1) / rows * a.kv_heads;
-    if (rows > 64) k_attn_dkv<T, DP, MAX_SETS<T, DP>, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
-    else k_attn_dkv<T, DP, 1, CAP><<<die_grid(total), AT_NT, 0, st>>>(a, total);
+    const int run = die_run(a.k_rays);
+    const int64_t rows = 64 * sets<MAX_SETS<T, DP>>(a.k_rays, a.q_rays, a.kv_heads, DKV_BLOCKS), total = ((int64_t)a.k_rays.n + rows - 1) / rows * a.kv_heads;
+    if (rows > 64) k_attn_dkv<T, DP, MAX_SETS<T, DP>, CAP><<<die_grid(total, run), AT_NT, 0, st>>>(a, total, run);
+    else k_attn_dkv<T, DP, 1, CAP><<<die_grid(total, run), AT_NT, 0, st>>>(a, total, run);
   }
   return hipGetLastError();
 }

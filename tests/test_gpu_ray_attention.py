@@ -237,6 +237,41 @@ def test_longer_rays_beside_a_sick_one(ty, causal):
         close(x[well], want[well], bound[well], name)
 
 
+@pytest.mark.parametrize("ty", ["bf16", "fp16"])
+@pytest.mark.parametrize("D", [32, 56])
+@pytest.mark.parametrize("option,sick", [("plain", False), ("all", False), ("causal", True)])
+def test_longer_rays_of_many_heads(ty, D, option, sick):
+    """Enough heads for wavefronts of 32 rows; the first and the last heads are looked at."""
+    import ray_ops
+    lens, H, G = [400, 150, 1, 0, 349], 224, 112
+    rays = ray_set(lens, gap=1)
+    ids = rays[2]
+    q, k, v, do, t, _ = _inputs(rays, rays, H, G, D, TYPES[ty], seed=20)
+    opt = _options(option, H, len(lens), t, t)
+    given = [x.clone() for x in (q, k, v, do)]
+    well = torch.ones(rays[3], dtype=torch.bool)
+    if sick:
+        well = ids != 1
+        for x in given:
+            x[~well] = torch.tensor([float("nan"), float("inf")], dtype=x.dtype)[torch.arange(int((~well).sum())) % 2][:, None, None]
+    qd, kd, vd, dd = (x.cuda() for x in given)
+    on = {n: x.cuda() if isinstance(x, torch.Tensor) else x for n, x in opt.items()}
+    rd = _dev_set(rays)
+    o, lse = ray_ops.ray_attention(qd, kd, vd, rd, **on)
+    got = ray_ops.ray_attention_backward(dd, qd, kd, vd, o, lse, rd, **on)
+    for h in (0, H - 2):
+        hs, gs = slice(h, h + 2), slice(h // 2, h // 2 + 1)
+        some = dict(opt)
+        if "slopes" in some:
+            some["slopes"] = some["slopes"][hs]
+        mask = seen_mask(rays, rays, some.pop("causal", False), some.pop("prefix", None))
+        ref = Attention(q[:, hs], k[:, gs], v[:, gs], mask, scale=D ** -0.5, **some)
+        close(o[:, hs][well], ref.o[well], ref.o_bound(q.dtype)[well], "o")
+        close(lse[:, hs][well], ref.lse[well], ref.lse_bound()[well], "lse")
+        for x, at, (want, bound), name in zip(got, (hs, gs, gs), ref.backward(do[:, hs], q.dtype), ("dq", "dk", "dv")):
+            close(x[:, at][well], want[well], bound[well], name)
+
+
 def test_infinite_value_that_is_seen():
     rays = ray_set([6, 40])
     q, k, v, do, _, _ = _inputs(rays, rays, 1, 1, 16, torch.bfloat16, seed=10)
