@@ -664,6 +664,7 @@ __global__ __launch_bounds__(AT_NT, least_waves(sizeof(T), DP, NQ, CAP)) void k_
         if constexpr (EXACT) {
           mask(x[q], row0, kept.span[q], kept.seen[q], g, 0.f);
           mask(dp[q], row0, kept.span[q], kept.seen[q], g, 0.f);
+          if (CAP) mask(th, row0, kept.span[q], kept.seen[q], g, 0.f);  // a weight of 0 times a slope of NaN is NaN
           each<B>([&](int b, int r) { exact[q] = __builtin_fmaf(x[q][b][r], dp[q][b][r], exact[q]); });
         }
         // the slope of the cap
