@@ -280,8 +280,15 @@ struct Ends {
   float *A, *B, *run_A, *run_B;
 };
 
-// The ray that leaves each part in the direction of the walk: the part's steps of it as h -> A h + B, with A = 0 where
-// the ray begins (BACK: ends) in the part, so that B is the state.  A = B = 0 where none leaves.
+// h -> A h + B over some parts.  FORGET in the place of A: the walk of the ray that leaves them began in them, or none
+// leaves, and B is the state whatever entered; a factor of 0 would let another ray's infinity or NaN through.  Factors of
+// a ray's own steps are +0 or more, so that a product that underflows still multiplies, and the ray's own NaN stays in it.
+constexpr float FORGET = -0.f;
+__device__ __forceinline__ bool forgets(float A) { return __float_as_uint(A) == 0x80000000u; }
+__device__ __forceinline__ float over(float A, float B, float h) { return forgets(A) ? B : __builtin_fmaf(A, h, B); }
+
+// The ray that leaves each part in the direction of the walk: the part's steps of it, FORGET where the ray begins (BACK:
+// ends) in the part or none leaves.
 template <typename T, int V, bool BACK>
 __global__ __launch_bounds__(SC_NT) void k_scan_ends(ffn_ray_scan a, int size, int64_t parts, float* __restrict__ A_of,
                                                      float* __restrict__ B_of) {
@@ -295,18 +302,15 @@ __global__ __launch_bounds__(SC_NT) void k_scan_ends(ffn_ray_scan a, int size, i
   const int64_t p0 = part * size, p1 = min(p0 + size, (int64_t)a.rays.n);
   float A[V], B[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) A[v] = B[v] = 0.f;
+  for (int v = 0; v < V; ++v) A[v] = 1.f, B[v] = 0.f;
   Span64 s;
   const int64_t ray = ray_at(a, c.w, BACK ? p0 : p1 - 1, s);
+  bool whole = true;
   if (ray >= 0 && (BACK ? s.from < p0 : s.to > p1)) {
     const int64_t from = max(s.from, p0), to = min(s.to, p1);
-    const bool whole = BACK ? to == s.to : from == s.from;
+    whole = BACK ? to == s.to : from == s.from;
     const int len = (int)(to - from);
     if (whole) load_state<V>(B, BACK ? a.dlast : a.h0, ray, a.channels, c.ch);
-    else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) A[v] = 1.f;
-    }
     const int64_t row = c.w.row(BACK ? to - 1 : from), dir = BACK ? -1 : 1;
     const T* gp = c.gate + row * a.gate_row;
     const T* xp = BACK ? (const T*)a.dh + row * a.dh_row + c.ch : c.x + row * a.x_row;
@@ -339,7 +343,7 @@ __global__ __launch_bounds__(SC_NT) void k_scan_ends(ffn_ray_scan a, int size, i
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    A_of[part * a.channels + c.ch + v] = A[v];
+    A_of[part * a.channels + c.ch + v] = whole ? FORGET : A[v];
     B_of[part * a.channels + c.ch + v] = B[v];
   }
 }
@@ -362,8 +366,10 @@ __global__ __launch_bounds__(GR_C * GROUP) void k_scan_groups(int channels, int6
     float a = 1.f, b = 0.f;
     if (t >= d) a = sa[t - d][c], b = sb[t - d][c];
     __syncthreads();
-    B = __builtin_fmaf(A, b, B);
-    A *= a;
+    if (!forgets(A)) {
+      B = __builtin_fmaf(A, b, B);
+      A = forgets(a) ? FORGET : A * a;
+    }
     sa[t][c] = A;
     sb[t][c] = B;
     __syncthreads();
@@ -383,14 +389,14 @@ __device__ __forceinline__ void enter(float (&h)[V], const Ends& e, int64_t part
                                       int ch) {
   const int64_t r0 = (BACK ? parts - 1 - j0 : j0) / GROUP, r1 = (BACK ? parts - 1 - j : j) / GROUP;
 #pragma unroll
-  for (int v = 0; v < V; ++v) h[v] = 0.f;  // the run in which the walk began forgets it
+  for (int v = 0; v < V; ++v) h[v] = 0.f;  // the run, or the parts of it, in which the walk began forget it
 #pragma unroll 4
   for (int64_t r = r0; r < r1; ++r)
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      h[v] = __builtin_fmaf(e.run_A[r * channels + ch + v], h[v], e.run_B[r * channels + ch + v]);
+      h[v] = over(e.run_A[r * channels + ch + v], e.run_B[r * channels + ch + v], h[v]);
 #pragma unroll
-  for (int v = 0; v < V; ++v) h[v] = __builtin_fmaf(e.A[j * channels + ch + v], h[v], e.B[j * channels + ch + v]);
+  for (int v = 0; v < V; ++v) h[v] = over(e.A[j * channels + ch + v], e.B[j * channels + ch + v], h[v]);
 }
 
 // By parts of `size` places (a multiple of SC_MARK).  The blocks past part_blocks give the rays without rows their last
