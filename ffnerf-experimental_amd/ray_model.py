@@ -18,7 +18,7 @@ import numpy as np
 import torch
 
 import ffn_lib as fl
-from ray_ops import ExpertLinear, RayAttention, RayScan, RaySet, expert_plan
+from ray_ops import ExpertLinear, RayAttention, RayScan, RaySet, expert_plan, once
 
 
 class HashEncode(torch.autograd.Function):
@@ -37,11 +37,15 @@ class HashEncode(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         xyz, = ctx.saved_tensors
-        grad = torch.zeros_like(ctx.nerf.t["table"])
-        fl.check(ctx.nerf.handle.lib.ffn_hash_encode_bwd(ctx.nerf.handle.h, fl.ptr(xyz), fl.ptr(g.contiguous()),
-                                                         xyz.shape[0], fl.ptr(grad), fl.stream_ptr()),
-                 "ffn_hash_encode_bwd")
-        return grad, None, None
+        nerf = ctx.nerf
+
+        def grad():
+            to, rows = torch.zeros_like(nerf.t["table"]), g.contiguous()
+            fl.check(nerf.handle.lib.ffn_hash_encode_bwd(nerf.handle.h, fl.ptr(xyz), fl.ptr(rows), xyz.shape[0],
+                                                         fl.ptr(to), fl.stream_ptr()), "ffn_hash_encode_bwd")
+            return to
+
+        return once(grad, g), None, None
 
 
 def march_samples(nerf, rays, bits, res: int, dt: float, max_steps: int):

@@ -2,8 +2,9 @@
 
 They take the packed samples that `ffn_march` leaves.  `RaySet` names them; `ray_attention`, `ray_scan` and
 `expert_linear` compute, their `*_backward` give gradients, and `RayAttention`, `RayScan`, `ExpertLinear` are the same
-as differentiable functions of torch.  Every call runs on the current stream of its tensors' device, allocates its
-results and scratch from torch, and never waits.  A wrong argument is an FfnError before anything is launched.
+as functions of torch that can be differentiated once; a second time is an error.  Every call runs on the current stream
+of its tensors' device, allocates its results and scratch from torch, and never waits.  A wrong argument is an FfnError
+before anything is launched.
 """
 from __future__ import annotations
 
@@ -96,6 +97,24 @@ def _workspace(a, fn, dev: int, *more):
     return w
 
 
+class _Once(torch.autograd.Function):
+    """What fn gives, as a function of `inputs` that cannot be differentiated."""
+
+    @staticmethod
+    def forward(ctx, fn, *inputs):
+        return fn()
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("the operators' gradients can be differentiated once only: their own gradients are not implemented")
+
+
+def once(fn, *inputs):
+    """fn() of a backward pass that depends on `inputs`.  Under create_graph the results are tied to them, so that a second
+    gradient through them is an error, whichever tensors it is asked for; else it would silently lack them."""
+    return _Once.apply(fn, *inputs) if torch.is_grad_enabled() else fn()
+
+
 # ---------------------------------------------------------------------------
 # attention
 
@@ -180,7 +199,8 @@ class RayAttention(torch.autograd.Function):
         q, k, v, o, lse = ctx.saved_tensors
         if do.stride(-1) != 1 or any(s * do.element_size() % 16 for s in do.stride()[:2]) or do.data_ptr() % 16:
             do = do.contiguous()
-        return ray_attention_backward(do, q, k, v, o, lse, *ctx.rays, **ctx.options) + (None, None, None)
+        grads = once(lambda: ray_attention_backward(do, q, k, v, o, lse, *ctx.rays, **ctx.options), do, q, k, v)
+        return (*grads, None, None, None)
 
 
 # ---------------------------------------------------------------------------
@@ -254,8 +274,8 @@ class RayScan(torch.autograd.Function):
     def backward(ctx, dh, dlast):
         gate, x, marks, h0 = ctx.saved_tensors
         dh = dh if dh.stride(-1) == 1 else dh.contiguous()
-        dgate, dx, dh0 = ray_scan_backward(dh, gate, x, marks, ctx.rays, dlast=dlast.contiguous(), h0=h0,
-                                           reverse=ctx.reverse)
+        dgate, dx, dh0 = once(lambda: ray_scan_backward(dh, gate, x, marks, ctx.rays, dlast=dlast.contiguous(), h0=h0,
+                                                        reverse=ctx.reverse), dh, dlast, gate, x, h0)
         return dgate, dx, None, (dh0 if h0 is not None else None), None
 
 
@@ -361,7 +381,7 @@ class ExpertLinear(torch.autograd.Function):
         if dy.stride(-1) != 1 or dy.stride(0) * dy.element_size() % 16 or dy.data_ptr() % 16:
             dy = dy.contiguous()
         need_dw = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        dx, dW, db = expert_linear_backward(dy, x, W, ctx.plan, y=y, need_dx=ctx.needs_input_grad[0], need_dw=need_dw,
-                                            **ctx.order)
+        dx, dW, db = once(lambda: expert_linear_backward(dy, x, W, ctx.plan, y=y, need_dx=ctx.needs_input_grad[0],
+                                                         need_dw=need_dw, **ctx.order), dy, x, W)
         return (dx, dW.to(W.dtype) if need_dw else None, db.to(W.dtype) if need_dw and ctx.bias else None, None, None,
                 None, None)
