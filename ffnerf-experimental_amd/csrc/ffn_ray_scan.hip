@@ -75,20 +75,37 @@ template <typename T, int V> __device__ __forceinline__ typename Chan<T, V>::vec
   }
 }
 
-__device__ __forceinline__ float sigmoid_f(float g) {
-  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
+// z = sigmoid(g) and 1 - z, each to its own size: with e = exp(-|g|) they are 1 / (1 + e) and e / (1 + e), whichever is
+// which.  1 - z by subtraction would be off by 5e-4 of itself at g = 10, and 0 from 17 on.
+__device__ __forceinline__ void gates(float g, float& z, float& keep) {
+  const float e = __builtin_amdgcn_exp2f(fabsf(g) * -1.4426950408889634f);
+  const float most = __builtin_amdgcn_rcpf(1.f + e), least = e * most;
+  z = g < 0.f ? least : most;
+  keep = g < 0.f ? most : least;
 }
 
-// N rows from p on, `step` bytes apart, of which `left` are there: the last one again for the others, so that no lane
-// branches
+// N rows from p on, `step` bytes apart.  Addresses are opaque to the compiler: else all N are formed, and held, before the
+// first load.
 template <typename T, int V, int N>
-__device__ __forceinline__ void load_rows(typename Chan<T, V>::vec (&to)[N], const T* p, int step, int left) {
-  int off = 0;
+__device__ __forceinline__ void load_rows(typename Chan<T, V>::vec (&to)[N], const T* p, int step) {
+  const char* at = reinterpret_cast<const char*>(p);
 #pragma unroll
   for (int u = 0; u < N; ++u) {
+    to[u] = *reinterpret_cast<const typename Chan<T, V>::vec*>(at);
+    at += step;
+    asm volatile("" : "+v"(at));
+  }
+}
+// the same where `left` of them are there: the last one again for the others, so that no lane branches
+template <typename T, int V, int N>
+__device__ __forceinline__ void load_rows(typename Chan<T, V>::vec (&to)[N], const T* p, int step, int left) {
+  const int last = (min(left, N) - 1) * step;
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    // between 0 and the last row, whichever way the rows go
+    int off = max(min(u * step, last), min(max(u * step, last), 0));
+    if (u) asm volatile("" : "+v"(off));
     to[u] = *reinterpret_cast<const typename Chan<T, V>::vec*>(reinterpret_cast<const char*>(p) + off);
-    off += u + 1 < left ? step : 0;
-    asm volatile("" : "+v"(off));  // opaque: else all N addresses are formed, and held, before the first load
   }
 }
 
@@ -140,8 +157,9 @@ __device__ __forceinline__ void walk_fwd(const ffn_ray_scan& a, const Cols<T, V>
       if (k + u < len) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float z = sigmoid_f(get<T, V>(gc[u], v));
-          h[v] = __builtin_fmaf(1.f - z, h[v], z * get<T, V>(xc[u], v));
+          float z, keep;
+          gates(get<T, V>(gc[u], v), z, keep);
+          h[v] = __builtin_fmaf(keep, h[v], z * get<T, V>(xc[u], v));
         }
         *reinterpret_cast<vec*>(hp) = pack<T, V>(h);
       }
@@ -151,8 +169,8 @@ __device__ __forceinline__ void walk_fwd(const ffn_ray_scan& a, const Cols<T, V>
 }
 
 // Gradients over `len` > 0 places from `from` on, last to first, in pieces of SC_MARK: a piece's states come again from
-// the mark before it, so that the backward pass neither reads h nor takes its rounding.  Of them it keeps z and
-// q = (x - h_{t-1}) z (1 - z):  dx = z D, dgate = q D, and D goes on as (1 - z) D.  start: the state before a walk
+// the mark before it, so that the backward pass neither reads h nor takes its rounding.  Of them it keeps z, 1 - z
+// and q = (x - h_{t-1}) z (1 - z):  dx = z D, dgate = q D, and D goes on as (1 - z) D.  start: the state before a walk
 // whose first piece has no mark (NULL: 0).
 template <typename T, int V>
 __device__ __forceinline__ void walk_bwd(const ffn_ray_scan& a, const Cols<T, V>& c, int64_t from, int len, bool mark0,
@@ -172,7 +190,7 @@ __device__ __forceinline__ void walk_bwd(const ffn_ray_scan& a, const Cols<T, V>
   load_rows<T, V, L>(dh, dp, (int)(ds * sizeof(T)), len - k);
   for (; k >= 0; k -= L) {
     const float* m = k || mark0 ? a.marks + (from + k) / L * a.channels + c.ch : start;
-    float h[V], z[L][V], q[L][V];
+    float h[V], z[L][V], keep[L][V], q[L][V];
     vec dc[L];
 #pragma unroll
     for (int v = 0; v < V; ++v) h[v] = m ? m[v] : 0.f;
@@ -181,13 +199,15 @@ __device__ __forceinline__ void walk_bwd(const ffn_ray_scan& a, const Cols<T, V>
       dc[u] = dh[u];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float zz = sigmoid_f(get<T, V>(g[u], v)), keep = 1.f - zz, xx = get<T, V>(x[u], v);
+        const float xx = get<T, V>(x[u], v);
+        float zz, kk;
+        gates(get<T, V>(g[u], v), zz, kk);
         z[u][v] = zz;
-        q[u][v] = (xx - h[v]) * (zz * keep);
-        h[v] = __builtin_fmaf(keep, h[v], zz * xx);
-        // opaque: formed here, before the next piece's rows are asked for (else both pieces' rows are held), and 1 - z
-        // formed again below instead of kept
-        asm volatile("" : "+v"(z[u][v]), "+v"(q[u][v]));
+        keep[u][v] = kk;
+        q[u][v] = (xx - h[v]) * (zz * kk);
+        h[v] = __builtin_fmaf(kk, h[v], zz * xx);
+        // opaque: formed here, before the next piece's rows are asked for (else both pieces' rows are held)
+        asm volatile("" : "+v"(z[u][v]), "+v"(keep[u][v]), "+v"(q[u][v]));
       }
     }
     const int left = len - k;
@@ -195,9 +215,9 @@ __device__ __forceinline__ void walk_bwd(const ffn_ray_scan& a, const Cols<T, V>
     if (k > 0) {
       gp -= L * c.gs, xp -= L * c.xs, dp -= L * ds;
       og -= L * os, ox -= L * os;
-      load_rows<T, V, L>(g, gp, c.gb, L);
-      load_rows<T, V, L>(x, xp, c.xb, L);
-      load_rows<T, V, L>(dh, dp, (int)(ds * sizeof(T)), L);
+      load_rows<T, V, L>(g, gp, c.gb);
+      load_rows<T, V, L>(x, xp, c.xb);
+      load_rows<T, V, L>(dh, dp, (int)(ds * sizeof(T)));
     }
 #pragma unroll
     for (int u = L - 1; u >= 0; --u) {
@@ -208,7 +228,7 @@ __device__ __forceinline__ void walk_bwd(const ffn_ray_scan& a, const Cols<T, V>
           const float D = get<T, V>(dc[u], v) + d[v];
           vx[v] = z[u][v] * D;
           vg[v] = q[u][v] * D;
-          d[v] = (1.f - z[u][v]) * D;
+          d[v] = keep[u][v] * D;
         }
         *reinterpret_cast<vec*>(wx) = pack<T, V>(vx);
         *reinterpret_cast<vec*>(wg) = pack<T, V>(vg);
@@ -333,7 +353,8 @@ __global__ __launch_bounds__(SC_NT) void k_scan_ends(ffn_ray_scan a, int size, i
         if (k + u < len) {
 #pragma unroll
           for (int v = 0; v < V; ++v) {
-            const float z = sigmoid_f(get<T, V>(gc[u], v)), keep = 1.f - z;
+            float z, keep;
+            gates(get<T, V>(gc[u], v), z, keep);
             A[v] *= keep;
             // BACK: the D that leaves a step is (1 - z) (dh + D)
             B[v] = BACK ? keep * (B[v] + get<T, V>(xc[u], v)) : __builtin_fmaf(keep, B[v], z * get<T, V>(xc[u], v));
@@ -402,9 +423,10 @@ __device__ __forceinline__ void enter(float (&h)[V], const Ends& e, int64_t part
 // By parts of `size` places (a multiple of SC_MARK).  The blocks past part_blocks give the rays without rows their last
 // state.  Large inputs: parts in falling order, since k_scan_ends has just read the last ones (they are still in the
 // last-level cache).  710137 rows of three rays, 128 channels, fp16: 94 us for k_scan_ends, 5 and 102, where one read of
-// gate and x and one write would take 116.
+// gate and x and one write would take 116.  Registers are held for four wavefronts a SIMD (backward of 200,000 rows of 37
+// float channels: 41 us, with three 44).
 template <typename T, int V, bool BACK>
-__global__ __launch_bounds__(SC_NT) void k_scan_parts(ffn_ray_scan a, int size, int64_t parts, int64_t part_blocks,
+__global__ __launch_bounds__(SC_NT, 4) void k_scan_parts(ffn_ray_scan a, int size, int64_t parts, int64_t part_blocks,
                                                       Ends e) {
   const int lanes = a.channels / V;
   if (blockIdx.x >= part_blocks) {
