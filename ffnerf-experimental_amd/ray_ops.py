@@ -144,6 +144,10 @@ def _attn_args(q, k, v, q_rays, k_rays, t_q, t_k, slopes, scale, cap, causal, pr
         if prefix.shape[0] != q_rays.num_rays:
             _refuse(f"{prefix.shape[0]} prefixes for {q_rays.num_rays} rays")
         a.prefix = _index(prefix, "prefix", dev)
+        if prefix.dtype == torch.uint32:  # the library's are signed: what is past their end is past any ray's too
+            p = prefix.view(torch.int32)
+            a.held = torch.where(p < 0, 2 ** 31 - 1, p)  # kept until the launch
+            a.prefix = a.held.data_ptr()
     return a, dev
 
 
@@ -154,7 +158,8 @@ def ray_attention(q, k, v, q_rays: RaySet, k_rays: RaySet | None = None, *, t_q=
     q [n_q, heads, dim], k and v [n_k, kv_heads, dim] (float32, float16 or bfloat16, any strides with unit stride along
     dim and 16-byte aligned rows; heads a multiple of kv_heads, which share), dim a multiple of 8 up to 128.  Scores are
     scale q.k (scale: 1/sqrt(dim)), with cap > 0 cap tanh(score / cap), less slopes[head] |t_q - t_k|; causal: a query
-    sees no key behind it (places counted from the ray's end where the sets differ), and always the first prefix[ray].
+    sees no key behind it (places counted from the ray's end where the sets differ), and always the first prefix[ray]
+    (int32, below 0 as 0; or uint32).
     k_rays None: q's own set.  o as q, lse [n_q, heads] float32; a row that sees nothing has 0 and -inf."""
     k_rays = q_rays if k_rays is None else k_rays
     lib = fl.load()

@@ -383,7 +383,7 @@ typedef struct ffn_ray_attn {
   const float* slopes;                  /* [heads] or NULL */
   const float *t_q, *t_k;               /* with slopes: depths, strides in elements */
   int64_t t_q_row, t_k_row;
-  const uint32_t* prefix;               /* [num_rays] or NULL; used if causal */
+  const int32_t* prefix;                /* [num_rays] or NULL; used if causal; a negative one is as 0 */
   void* o;
   float* lse;
   /* backward only: dout as q (strides do_row, do_head), dq, dk, dv contiguous */
