@@ -28,21 +28,40 @@ def _dtype(x: torch.Tensor) -> int:
     return d
 
 
-def _want(x, name: str, shape: tuple, dtype, dev: int, rows: int = -1) -> int | None:
+def _want(x, name: str, shape: tuple, dtype, dev: int, rows: int = -1) -> int:
     """Pointer of x, which must have this shape, type and device, and (rows -1) be contiguous, (1) have unit stride
     along its last axis, or (0) any strides."""
-    if x is None:
-        return None
     if (isinstance(x, torch.Tensor) and x.shape == shape and x.dtype is dtype and x.get_device() == dev
             and (x.is_contiguous() if rows < 0 else not rows or x.stride(-1) == 1 or shape[-1] == 1)):
         return x.data_ptr()
     if not isinstance(x, torch.Tensor) or x.shape != shape:
-        _refuse(f"{name} must be a tensor of shape {tuple(shape)}, not {tuple(getattr(x, 'shape', ()))}")
+        _refuse(f"{name} must be a tensor of shape {tuple(shape)}, not "
+                f"{tuple(x.shape) if isinstance(x, torch.Tensor) else type(x).__name__}")
     if x.dtype is not dtype:
         _refuse(f"{name} must be {dtype}, not {x.dtype}")
     if x.get_device() != dev:
         _refuse(f"{name} is on {x.device}, not on cuda:{dev}")
     _refuse(f"{name} must be contiguous" if rows < 0 else f"{name} must have unit stride along its last axis")
+
+
+def _may(x, *args) -> int | None:
+    """_want of a tensor that may be left out."""
+    return None if x is None else _want(x, *args)
+
+
+def _is(x, kind, name: str):
+    if not isinstance(x, kind):
+        _refuse(f"{name} must be a {kind.__name__}, not {type(x).__name__}")
+    return x
+
+
+def _number(x, name: str) -> float:
+    if not isinstance(x, str):
+        try:
+            return float(x)
+        except (TypeError, ValueError):
+            pass
+    _refuse(f"{name} must be a number, not {type(x).__name__}")
 
 
 def _index(x, name: str, dev: int) -> int:
@@ -122,7 +141,8 @@ def once(fn, *inputs):
 def _attn_args(q, k, v, q_rays, k_rays, t_q, t_k, slopes, scale, cap, causal, prefix):
     if not isinstance(q, torch.Tensor) or q.dim() != 3 or not isinstance(k, torch.Tensor) or k.dim() != 3:
         _refuse("q and k must be tensors [rows, heads, dim]")
-    a, dev = fl.FfnRayAttn(), q_rays.device
+    a, dev = fl.FfnRayAttn(), _is(q_rays, RaySet, "q_rays").device
+    _is(k_rays, RaySet, "k_rays")
     _, heads, dim = q.shape
     dtype, kv_heads = q.dtype, k.shape[1]
     a.dtype, a.heads, a.kv_heads, a.dim = _dtype(q), heads, kv_heads, dim
@@ -131,19 +151,19 @@ def _attn_args(q, k, v, q_rays, k_rays, t_q, t_k, slopes, scale, cap, causal, pr
     a.k, a.v = _want(k, "k", shape, dtype, dev, 1), _want(v, "v", shape, dtype, dev, 1)
     (a.q_row, a.q_head, _), (a.k_row, a.k_head, _), (a.v_row, a.v_head, _) = q.stride(), k.stride(), v.stride()
     a.q_rays, a.k_rays = q_rays.c, k_rays.c
-    a.scale = dim ** -0.5 if scale is None else scale
-    a.cap, a.causal = cap, 1 if causal else 0
+    a.scale = dim ** -0.5 if scale is None else _number(scale, "scale")
+    a.cap, a.causal = _number(cap, "cap"), 1 if causal else 0
     if slopes is not None:
+        if t_q is None or t_k is None:
+            _refuse("slopes need t_q and t_k")
         a.slopes = _want(slopes, "slopes", (heads,), torch.float32, dev)
         a.t_q = _want(t_q, "t_q", (q_rays.n,), torch.float32, dev, 0)
         a.t_k = _want(t_k, "t_k", (k_rays.n,), torch.float32, dev, 0)
-        if t_q is None or t_k is None:
-            _refuse("slopes need t_q and t_k")
         a.t_q_row, a.t_k_row = t_q.stride(0), t_k.stride(0)
     if prefix is not None:
+        a.prefix = _index(prefix, "prefix", dev)
         if prefix.shape[0] != q_rays.num_rays:
             _refuse(f"{prefix.shape[0]} prefixes for {q_rays.num_rays} rays")
-        a.prefix = _index(prefix, "prefix", dev)
         if prefix.dtype == torch.uint32:  # the library's are signed: what is past their end is past any ray's too
             p = prefix.view(torch.int32)
             a.held = torch.where(p < 0, 2 ** 31 - 1, p)  # kept until the launch
@@ -215,13 +235,13 @@ class RayAttention(torch.autograd.Function):
 def _scan_args(gate, x, rays, h0, reverse):
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         _refuse("x must be a tensor [rows, channels]")
-    a, dev = fl.FfnRayScan(), rays.device
+    a, dev = fl.FfnRayScan(), _is(rays, RaySet, "rays").device
     shape = (rays.n, x.shape[1])
     a.dtype, a.channels, a.reverse = _dtype(x), x.shape[1], 1 if reverse else 0
     a.rays = rays.c
     a.gate, a.x = _want(gate, "gate", shape, x.dtype, dev, 1), _want(x, "x", shape, x.dtype, dev, 1)
     a.gate_row, a.x_row = gate.stride(0), x.stride(0)
-    a.h0 = _want(h0, "h0", (rays.num_rays, x.shape[1]), torch.float32, dev)
+    a.h0 = _may(h0, "h0", (rays.num_rays, x.shape[1]), torch.float32, dev)
     return a, dev
 
 
@@ -253,10 +273,10 @@ def ray_scan_backward(dh, gate, x, marks, rays: RaySet, *, dlast=None, h0=None, 
     a, dev = _scan_args(gate, x, rays, h0, reverse)
     a.dh = _want(dh, "dh", x.shape, x.dtype, dev, 1)
     a.dh_row = dh.stride(0)
-    a.dlast = _want(dlast, "dlast", (rays.num_rays, x.shape[1]), torch.float32, dev)
+    a.dlast = _may(dlast, "dlast", (rays.num_rays, x.shape[1]), torch.float32, dev)
     n = C.c_uint64()
     fl.check(lib.ffn_ray_scan_marks(C.byref(a), C.byref(n)), "ffn_ray_scan_marks")
-    a.marks = _want(marks, "marks", (n.value // 4,), torch.float32, dev)
+    a.marks = _may(marks, "marks", (n.value // 4,), torch.float32, dev)
     dgate, dx = torch.empty(x.shape, dtype=x.dtype, device=dev), torch.empty(x.shape, dtype=x.dtype, device=dev)
     dh0 = torch.empty((rays.num_rays, x.shape[1]), dtype=torch.float32, device=dev)
     a.dgate, a.dx, a.dh0 = dgate.data_ptr(), dx.data_ptr(), dh0.data_ptr()
@@ -313,6 +333,8 @@ def expert_plan(ids: torch.Tensor, n_experts: int) -> ExpertPlan:
     lib = fl.load()
     if not isinstance(ids, torch.Tensor) or not ids.is_cuda or ids.dim() != 1 or ids.dtype != torch.int32:
         _refuse("ids must be a vector of int32 on the GPU")
+    if not hasattr(n_experts, "__index__") or not 1 <= n_experts <= fl.MAX_EXPERTS:
+        _refuse(f"n_experts={n_experts!r} must be a whole number of 1 to {fl.MAX_EXPERTS}")
     dev, n = ids.get_device(), ids.shape[0]
     _index(ids, "ids", dev)
     if n >= 1 << 31:
@@ -329,7 +351,7 @@ def expert_plan(ids: torch.Tensor, n_experts: int) -> ExpertPlan:
 def _expert_args(x, W, plan, relu, x_slots, y_slots):
     if not isinstance(x, torch.Tensor) or x.dim() != 2 or not isinstance(W, torch.Tensor) or W.dim() != 3:
         _refuse("x must be a tensor [rows, in], W a tensor [experts, out, in]")
-    a, dev = fl.FfnExperts(), plan.device
+    a, dev = fl.FfnExperts(), _is(plan, ExpertPlan, "plan").device
     a.dtype, a.n_experts, a.d_in, a.d_out = _dtype(x), plan.n_experts, W.shape[2], W.shape[1]
     a.relu, a.flags = 1 if relu else 0, (1 if x_slots else 0) | (2 if y_slots else 0)
     a.n, a.plan = plan.n, plan.words.data_ptr()
@@ -346,7 +368,7 @@ def expert_linear(x, W, b, plan: ExpertPlan, *, relu: bool = False, x_slots: boo
     order instead of the rows' own.  y [n, out]; rows of no expert give 0."""
     lib = fl.load()
     a, dev = _expert_args(x, W, plan, relu, x_slots, y_slots)
-    a.b = _want(b, "b", W.shape[:2], x.dtype, dev)
+    a.b = _may(b, "b", W.shape[:2], x.dtype, dev)
     y = torch.empty((plan.n, W.shape[1]), dtype=x.dtype, device=dev)
     a.y = y.data_ptr()
     _call(lib.ffn_expert_linear_fwd, dev, C.byref(a))
@@ -360,7 +382,7 @@ def expert_linear_backward(dy, x, W, plan: ExpertPlan, *, y=None, x_slots: bool 
     lib = fl.load()
     a, dev = _expert_args(x, W, plan, y is not None, x_slots, y_slots)
     shape = (plan.n, W.shape[1])
-    a.y, a.dy, a.dy_row = _want(y, "y", shape, x.dtype, dev), _want(dy, "dy", shape, x.dtype, dev, 1), dy.stride(0)
+    a.y, a.dy, a.dy_row = _may(y, "y", shape, x.dtype, dev), _want(dy, "dy", shape, x.dtype, dev, 1), dy.stride(0)
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_dx else None
     dW = torch.empty(W.shape, dtype=torch.float32, device=dev) if need_dw else None
     db = torch.empty(W.shape[:2], dtype=torch.float32, device=dev) if need_dw else None
