@@ -30,6 +30,9 @@ int elem(int32_t dtype) { return dtype == FFN_F32 ? 4 : dtype == FFN_F16 || dtyp
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 bool aligned(const void* p, int64_t stride, int size) { return aligned(p) && stride * size % 16 == 0; }
 
+// the stride of an axis of `count`: that of one place, or none, is any number and leads nowhere
+int64_t step(int64_t count, int64_t stride) { return count > 1 ? stride : 0; }
+
 int check_set(const ffn_ray_set& s, const char* name, bool ids) {
   if (s.n > MAX_ROWS) return fail(-1, "%s: %u rows exceed %u", name, s.n, MAX_ROWS);
   if (s.num_rays && (!s.counts || !s.offsets)) return fail(-1, "%s: NULL counts or offsets", name);
@@ -57,14 +60,16 @@ int check_attn(const ffn_ray_attn* a, bool backward) {
   const int b = elem(a->dtype);
   const bool nq = a->q_rays.n > 0, nk = a->k_rays.n > 0;
   if ((nq && (!a->q || !a->o || !a->lse)) || (nk && (!a->k || !a->v))) return fail(-1, "NULL buffer");
-  if (!aligned(a->q, a->q_row, b) || !aligned(a->q, a->q_head, b) || !aligned(a->k, a->k_row, b) ||
-      !aligned(a->k, a->k_head, b) || !aligned(a->v, a->v_row, b) || !aligned(a->v, a->v_head, b) || !aligned(a->o))
+  const int64_t qn = a->q_rays.n, kn = a->k_rays.n, qh = nq ? a->heads : 0, kh = nk ? a->kv_heads : 0;
+  if (!aligned(a->q, step(qn, a->q_row), b) || !aligned(a->q, step(qh, a->q_head), b) ||
+      !aligned(a->k, step(kn, a->k_row), b) || !aligned(a->k, step(kh, a->k_head), b) ||
+      !aligned(a->v, step(kn, a->v_row), b) || !aligned(a->v, step(kh, a->v_head), b) || !aligned(a->o))
     return fail(-1, "rows and heads of q, k, v and o must be 16-byte aligned");
   if (a->slopes && ((nq && !a->t_q) || (nk && !a->t_k))) return fail(-1, "slopes without t_q and t_k");
   if (backward) {
     if ((nq && (!a->dout || !a->dq)) || (nk && (!a->dk || !a->dv))) return fail(-1, "NULL gradient buffer");
-    if (!aligned(a->dout, a->do_row, b) || !aligned(a->dout, a->do_head, b) || !aligned(a->dq) || !aligned(a->dk) ||
-        !aligned(a->dv))
+    if (!aligned(a->dout, step(qn, a->do_row), b) || !aligned(a->dout, step(qh, a->do_head), b) || !aligned(a->dq) ||
+        !aligned(a->dk) || !aligned(a->dv))
       return fail(-1, "rows and heads of the gradients must be 16-byte aligned");
   }
   const uint64_t need = ffn::attn_workspace(*a, backward);
@@ -95,8 +100,8 @@ int check_scan(const ffn_ray_scan* a, bool backward) {
     return fail(-1, "misaligned gradient buffer");
   // the kernels step through a few rows with 32-bit offsets
   const int64_t far = (int64_t)MAX_SCAN_STRIDE / elem(a->dtype);
-  if (a->gate_row > far || a->gate_row < -far || a->x_row > far || a->x_row < -far ||
-      (backward && (a->dh_row > far || a->dh_row < -far)))
+  if (a->rays.n > 1 && (a->gate_row > far || a->gate_row < -far || a->x_row > far || a->x_row < -far ||
+                        (backward && (a->dh_row > far || a->dh_row < -far))))
     return fail(-1, "rows more than %d bytes apart", MAX_SCAN_STRIDE);
   const uint64_t need = ffn::scan_workspace(*a, backward);
   if (need && (!a->workspace || !aligned(a->workspace) || a->workspace_bytes < need))
@@ -121,7 +126,7 @@ int check_experts(const ffn_experts* a) {
   if (a->flags & ~(FFN_EXPERTS_X_SLOTS | FFN_EXPERTS_Y_SLOTS)) return fail(-1, "unknown flags %d", a->flags);
   if (!a->plan) return fail(-1, "NULL plan");
   const int64_t far = (int64_t)(UINT32_MAX / elem(a->dtype));
-  if (a->x_row < 0 || a->x_row > far || a->dy_row < 0 || a->dy_row > far)
+  if (a->n > 1 && (a->x_row < 0 || a->x_row > far || a->dy_row < 0 || a->dy_row > far))
     return fail(-1, "row strides must be 0 or more, and less than 4 GiB");
   return 0;
 }
@@ -199,7 +204,7 @@ int ffn_expert_linear_fwd(const ffn_experts* a, void* stream) {
   const int b = elem(a->dtype);
   if (a->n == 0) return 0;
   if (!a->x || !a->W || !a->y) return fail(-1, "NULL buffer");
-  if (!aligned(a->x, a->x_row, b) || !aligned(a->W) || !aligned(a->b) || !aligned(a->y))
+  if (!aligned(a->x, step(a->n, a->x_row), b) || !aligned(a->W) || !aligned(a->b) || !aligned(a->y))
     return fail(-1, "rows of x, W, b and y must be 16-byte aligned");
   return launched(ffn::launch_experts(*a, false, (hipStream_t)stream), "ffn_expert_linear_fwd");
 }
@@ -216,7 +221,7 @@ int ffn_expert_linear_bwd(const ffn_experts* a, void* stream) {
   const int b = elem(a->dtype);
   if (a->n && (!a->dy || (a->relu && !a->y) || (a->dx && !a->W) || ((a->dW || a->db) && !a->x)))
     return fail(-1, "NULL buffer");
-  if (!aligned(a->dy, a->dy_row, b) || !aligned(a->y) || !aligned(a->W) || !aligned(a->x, a->x_row, b) ||
+  if (!aligned(a->dy, step(a->n, a->dy_row), b) || !aligned(a->y) || !aligned(a->W) || !aligned(a->x, step(a->n, a->x_row), b) ||
       !aligned(a->dx) || !aligned(a->dW) || !aligned(a->db))
     return fail(-1, "rows of dy, y, W, x and the gradients must be 16-byte aligned");
   const uint64_t need = ffn::expert_workspace(*a);

@@ -32,7 +32,7 @@ def _want(x, name: str, shape: tuple, dtype, dev: int, rows: int = -1) -> int:
     """Pointer of x, which must have this shape, type and device, and (rows -1) be contiguous, (1) have unit stride
     along its last axis, or (0) any strides."""
     if (isinstance(x, torch.Tensor) and x.shape == shape and x.dtype is dtype and x.get_device() == dev
-            and (x.is_contiguous() if rows < 0 else not rows or x.stride(-1) == 1 or shape[-1] == 1)):
+            and (x.is_contiguous() if rows < 0 else not rows or x.stride(-1) == 1 or shape[-1] == 1 or not x.numel())):
         return x.data_ptr()
     if not isinstance(x, torch.Tensor) or x.shape != shape:
         _refuse(f"{name} must be a tensor of shape {tuple(shape)}, not "
