@@ -72,7 +72,7 @@ class RayModel(torch.nn.Module):
         super().__init__()
         if width % (8 * heads):
             raise ValueError(f"width={width} must be a multiple of 8 heads={heads}")
-        self.heads, self.cells, self.dtype, experts = heads, cells, dtype, cells ** 3
+        self.width, self.heads, self.cells, self.dtype, experts = width, heads, cells, dtype, cells ** 3
 
         def weight(*shape):
             return torch.nn.Parameter(torch.randn(shape) * shape[-1] ** -0.5)
@@ -94,10 +94,10 @@ class RayModel(torch.nn.Module):
         """Colour [num_rays, 3] of each ray on a black background."""
         t, n, ty = samples[:, 3], samples.shape[0], self.dtype
         x = (features @ self.W_in.t()).to(ty)
-        qkv = (x @ self.W_qkv.to(ty).t()).view(n, 3, self.heads, -1)
+        qkv = (x @ self.W_qkv.to(ty).t()).view(n, 3, self.heads, self.width // self.heads)
         o = RayAttention.apply(qkv[:, 0], qkv[:, 1], qkv[:, 2], rays, None,
                                dict(t_q=t, t_k=t, slopes=self.slopes, cap=30.0, causal=True))
-        x = x + o.reshape(n, -1) @ self.W_o.to(ty).t()
+        x = x + o.reshape(n, self.width) @ self.W_o.to(ty).t()
         gate, carry = (x @ self.W_scan.to(ty).t()).chunk(2, 1)
         x = x + RayScan.apply(gate, carry, rays)[0]
         plan = expert_plan(self.regions(samples), self.cells ** 3)
