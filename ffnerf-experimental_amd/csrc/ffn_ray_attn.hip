@@ -1123,20 +1123,25 @@ static int64_t rays_with_queries(const ffn_ray_attn& a) {
 }
 
 // Whether one query at a time is the faster.  Its time is about 1.6 ns a (query, key head) and tile of keys, one more for
-// the start.  k_attn_fwd's is a chain over the keys of a block's 64 queries, 1.1 us a tile, or 1.6 ns a block and tile and
-// 10 ns a block if there are many blocks.  Measured, bf16, dim 64, 8 heads with 2 of keys, us (row / tile): 65536 rays of 8
-// keys and a query 303 / 154; 8192 of 128 102 / 202, with four queries each 257 / 213; 64 of 16384 106 / 17505, with four
-// 196 / 4395, with sixteen 782 / 1008, and 1642 / 1008 where each head has its own keys.  The backward (mostly dk and dv)
-// follows: 1001 / 489, 675 / 893, 1045 / 840, 618 / 22772, 699 / 6128, 1186 / 1701, 2061 / 1879.
-static bool by_row(const ffn_ray_attn& a) {
+// the start, for every 16 heads that share the key head: k_attn_row passes over the keys once for each.  k_attn_fwd's is a
+// chain over the keys of a block's 64 queries, 1.1 us a tile, or 1.6 ns a block and tile and 10 ns a block if there are many
+// blocks; k_attn_dq's is 1.4 times that, where k_attn_dq_row's is hardly more than k_attn_row's.  Measured, bf16, dim 64, 8
+// heads with 2 of keys, us (row / tile): 65536 rays of 8 keys and a query 303 / 154; 8192 of 128 102 / 202, with four
+// queries each 257 / 213; 64 of 16384 106 / 17505, with four 196 / 4395, with sixteen 782 / 1008, and 1642 / 1008 where each
+// head has its own keys.  Backward, mostly dk and dv: 1001 / 489, 675 / 893, 1045 / 840, 618 / 22772, 699 / 6128, 1186 / 1701,
+// 2061 / 1879.  64 heads on one key head, forward and backward: 24 rays of 2500 among themselves 10138 + 28308 / 3672 +
+// 20712; 64 of 8192 with 16 queries 778 + 2001 / 692 + 2420, with 32 1332 + 2539 / 748 + 2211; 64 of 16384 with one query
+// 177 + 2559 (32 heads 92 + 1350).
+static bool by_row(const ffn_ray_attn& a, bool backward) {
   const double n = (double)a.q_rays.n, keys = (double)a.k_rays.n, mean = keys / rays_with_queries(a);
   // 16 rows that share a few tiles of keys: k_attn_fwd's own case, though its chain may be a few us longer if all is small
   if (n > 16. * rays_with_queries(a) && mean <= 16. * AT_TILE) return false;
-  const double row = 1.6 * n * a.kv_heads * (2. + floor(mean / AT_TILE));
+  const int passes = (a.heads / a.kv_heads + 15) / 16;  // over the keys, 16 heads a pass
+  const double row = 1.6 * n * a.kv_heads * passes * (2. + floor(mean / AT_TILE));
   const double blocks = ceil(n / AT_TILE) * a.heads;
   const double a_block = (a.q_rays.n < AT_TILE ? keys : keys * AT_TILE / n) / AT_TILE;
   const double tiles = fmax(a_block, mean / AT_TILE) + 1.;
-  return row < fmax(1100. * tiles, (1.6 * tiles + 10.) * blocks);
+  return row < (backward ? 1.4 : 1.) * fmax(1100. * tiles, (1.6 * tiles + 10.) * blocks);
 }
 // Few rows are split over their keys until ROW_WAVES wavefronts have work, 16 a CU: 64 rays of 16384 keys, us with 512, 1024,
 // 2048 and 4096 of them: 126, 104, 104, 106; with four queries each 453, 325, 327, 195.
@@ -1151,7 +1156,7 @@ static int row_splits(const ffn_ray_attn& a) {
 
 uint64_t attn_workspace(const ffn_ray_attn& a, bool backward) {
   const uint64_t rows = (uint64_t)a.q_rays.n * a.heads;
-  const uint64_t splits = a.q_rays.n && by_row(a) ? row_splits(a) : 1;
+  const uint64_t splits = a.q_rays.n && by_row(a, backward) ? row_splits(a) : 1;
   const uint64_t sets = backward && a.dtype != FFN_F32 ? 2 : 1;
   const uint64_t parts = splits > 1 ? splits * rows * (sets * a.dim + 2) : 0;
   return ((backward ? (uint64_t)dq_parts(rows) : 0) + parts) * sizeof(float);
@@ -1178,7 +1183,7 @@ static int sets(const ffn_ray_set& kept, const ffn_ray_set& streamed, int heads,
 
 template <typename T, int DP, bool CAP>
 static hipError_t fwd(const ffn_ray_attn& a, hipStream_t st) {
-  if (by_row(a)) {
+  if (by_row(a, false)) {
     const int splits = row_splits(a);
     const int64_t total = (int64_t)a.q_rays.n * a.kv_heads * splits;
     k_attn_row<T, DP, CAP><<<(unsigned)((total + 3) / 4), AT_NT, 0, st>>>(a, splits, total);
@@ -1194,7 +1199,7 @@ static hipError_t fwd(const ffn_ray_attn& a, hipStream_t st) {
 
 template <typename T, int DP, bool CAP>
 static hipError_t bwd(const ffn_ray_attn& a, hipStream_t st) {
-  if (a.q_rays.n && by_row(a)) {
+  if (a.q_rays.n && by_row(a, true)) {
     const int splits = row_splits(a);
     const int64_t total = (int64_t)a.q_rays.n * a.kv_heads * splits;
     k_attn_dq_row<T, DP, CAP><<<(unsigned)((total + 3) / 4), AT_NT, 0, st>>>(a, splits, total);
