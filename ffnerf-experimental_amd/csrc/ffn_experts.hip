@@ -343,8 +343,8 @@ __global__ __launch_bounds__(EX_NT, ex_waves(sizeof(T), NB)) void k_expert(ffn_e
   constexpr int C = 16 * NB, EL = 16 / (int)sizeof(T);
   constexpr int W_SIZE = BACK ? EX_K * lds_row<T, C> : C * lds_row<T, EX_K>, OUT_SIZE = 4 * 16 * lds_row<T, C>;
   __shared__ __align__(16) T lds[W_SIZE > OUT_SIZE ? W_SIZE : OUT_SIZE];
-  const int64_t per = (total + 7) / 8, work = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if (work >= total) return;
+  const int64_t block = block_number(), per = (total + 7) / 8, work = (block & 7) * per + (block >> 3);
+  if (block >= 8 * per || work >= total) return;
   const uint2 tile = reinterpret_cast<const uint2*>(a.plan + v.tiles)[work / col_tiles];
   if (tile.x >= (uint32_t)v.bins) return;
   const int col0 = (int)(work % col_tiles) * C;
@@ -655,7 +655,7 @@ template <typename T, bool BACK, int NB>
 static void product(const ffn_experts& a, const PlanView& v, hipStream_t st) {
   const int width = BACK ? a.in : a.out, cols = (width + 16 * NB - 1) / (16 * NB);
   const int64_t total = (int64_t)v.n_tiles * cols;
-  k_expert<T, BACK, NB><<<(unsigned)((total + 7) / 8 * 8), EX_NT, 0, st>>>(a, v, total, cols);
+  k_expert<T, BACK, NB><<<grid_of((total + 7) / 8 * 8), EX_NT, 0, st>>>(a, v, total, cols);
 }
 // Columns a block: all of a row's, so that x is read once, but narrower ones while that leaves CUs without work.  64 / 128 /
 // 256 columns a block, us, forward in bf16: 300000 rows, 256 x 256 values 146 / 121 / 118 (dx 168 / 117 / 104); 65536 rows

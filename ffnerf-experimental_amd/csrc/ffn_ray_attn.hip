@@ -389,8 +389,8 @@ struct Softmax {
 // Blocks in launch order go round the eight dies; this gives each die runs of 2^run neighbouring pieces of work, whose
 // tiles share keys in its L2.
 __device__ __forceinline__ int64_t die_order(int run) {
-  const int64_t b = blockIdx.x >> 3;
-  return (((b >> run) * 8 + (blockIdx.x & 7)) << run) + (b & ((1 << run) - 1));
+  const int64_t n = block_number(), b = n >> 3;
+  return (((b >> run) * 8 + (n & 7)) << run) + (b & ((1 << run) - 1));
 }
 
 // the kept rows of a wavefront, NQ sets of 16: row number, what it sees, and the ranges over all of them
@@ -832,7 +832,7 @@ __global__ __launch_bounds__(AT_NT) void k_attn_row(ffn_ray_attn a, int splits, 
   __shared__ __align__(16) T vs_all[4][ROWS * lds_row<T, DP>];
   __shared__ __align__(16) float ts_all[4][ROWS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
-  const int64_t work = (int64_t)blockIdx.x * 4 + wave;
+  const int64_t work = block_number() * 4 + wave;
   if (work >= total) return;  // no barriers below
   T* vs = vs_all[wave];
   float* ts = ts_all[wave];
@@ -985,7 +985,7 @@ __global__ __launch_bounds__(AT_NT) void k_attn_dq_row(ffn_ray_attn a, int split
   __shared__ __align__(16) T ks_all[4][ROWS * lds_row<T, DP>];
   __shared__ __align__(16) float ts_all[4][ROWS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
-  const int64_t work = (int64_t)blockIdx.x * 4 + wave;
+  const int64_t work = block_number() * 4 + wave;
   if (work >= total) return;  // no barriers below
   T* ks = ks_all[wave];
   float* ts = ts_all[wave];
@@ -1166,7 +1166,7 @@ uint64_t attn_workspace(const ffn_ray_attn& a, bool backward) {
 // forward + backward, us: 65536 rows in rays of 4000 266 + 788 / 326 + 880; 131072 in rays of 1000, 8 heads 305 + 911 /
 // 301 + 862; 131072 in rays of 512 119 + 346 / 93 + 287; 400000 in rays of 40 195 + 492 / 193 + 489)
 static int die_run(const ffn_ray_set& kept) { return kept.n >= 2048 * (int64_t)kept.num_rays ? 2 : 4; }
-static unsigned die_grid(int64_t total, int run) { return (unsigned)(((total + (8 << run) - 1) >> (3 + run)) << (3 + run)); }
+static dim3 die_grid(int64_t total, int run) { return grid_of(((total + (8 << run) - 1) >> (3 + run)) << (3 + run)); }
 
 // Sets of 16 kept rows a wavefront: two where rays are long on both sides, the registers hold them and `least` blocks of 128
 // rows have work.  One set / two, us, forward and backward of bf16, dim 64, 4 heads, causal: 400000 rows in rays of 48
@@ -1186,7 +1186,7 @@ static hipError_t fwd(const ffn_ray_attn& a, hipStream_t st) {
   if (by_row(a, false)) {
     const int splits = row_splits(a);
     const int64_t total = (int64_t)a.q_rays.n * a.kv_heads * splits;
-    k_attn_row<T, DP, CAP><<<(unsigned)((total + 3) / 4), AT_NT, 0, st>>>(a, splits, total);
+    k_attn_row<T, DP, CAP><<<grid_of((total + 3) / 4), AT_NT, 0, st>>>(a, splits, total);
     if (splits > 1) k_attn_join<T><<<(unsigned)(((int64_t)a.q_rays.n * a.heads + 3) / 4), AT_NT, 0, st>>>(a, splits);
   } else {
     const int run = die_run(a.q_rays);
@@ -1202,7 +1202,7 @@ static hipError_t bwd(const ffn_ray_attn& a, hipStream_t st) {
   if (a.q_rays.n && by_row(a, true)) {
     const int splits = row_splits(a);
     const int64_t total = (int64_t)a.q_rays.n * a.kv_heads * splits;
-    k_attn_dq_row<T, DP, CAP><<<(unsigned)((total + 3) / 4), AT_NT, 0, st>>>(a, splits, total);
+    k_attn_dq_row<T, DP, CAP><<<grid_of((total + 3) / 4), AT_NT, 0, st>>>(a, splits, total);
     if (splits > 1) k_attn_dq_join<T><<<(unsigned)(((int64_t)a.q_rays.n * a.heads + 3) / 4), AT_NT, 0, st>>>(a, splits);
   } else if (a.q_rays.n) {
     const int run = die_run(a.q_rays);

@@ -25,6 +25,8 @@ constexpr uint32_t MAX_ROWS = 0x7FFFFF00u;
 
 constexpr int MAX_SCAN_STRIDE = 1 << 27;
 
+constexpr uint64_t MAX_SCAN_STATES = 1ull << 46;  // channels of all rays: what one launch can count
+
 int elem(int32_t dtype) { return dtype == FFN_F32 ? 4 : dtype == FFN_F16 || dtype == FFN_BF16 ? 2 : 0; }
 
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -103,6 +105,8 @@ int check_scan(const ffn_ray_scan* a, bool backward) {
   if (a->rays.n > 1 && (a->gate_row > far || a->gate_row < -far || a->x_row > far || a->x_row < -far ||
                         (backward && (a->dh_row > far || a->dh_row < -far))))
     return fail(-1, "rows more than %d bytes apart", MAX_SCAN_STRIDE);
+  if ((uint64_t)a->rays.num_rays * a->channels > MAX_SCAN_STATES)
+    return fail(-1, "%d channels of %u rays exceed 2^46", a->channels, a->rays.num_rays);
   const uint64_t need = ffn::scan_workspace(*a, backward);
   if (need && (!a->workspace || !aligned(a->workspace) || a->workspace_bytes < need))
     return fail(-1, "workspace of %llu bytes, %llu wanted", (unsigned long long)(a->workspace ? a->workspace_bytes : 0),

@@ -8,6 +8,14 @@
 
 namespace ffn {
 
+// A launch counts an axis's threads in 32 bits, and one of more does a part of its work without an error.  So blocks go on
+// along y after GRID_X of them (a multiple of the dies, 2^31 threads of 256 a block); those past the last one find no work.
+constexpr int64_t GRID_X = 1 << 23;
+inline dim3 grid_of(int64_t blocks) {
+  return blocks <= GRID_X ? dim3((unsigned)blocks) : dim3((unsigned)GRID_X, (unsigned)((blocks + GRID_X - 1) / GRID_X));
+}
+__device__ __forceinline__ int64_t block_number() { return (int64_t)blockIdx.y * GRID_X + blockIdx.x; }
+
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8), aligned(16)));  // loaded as two 16-byte halves
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));

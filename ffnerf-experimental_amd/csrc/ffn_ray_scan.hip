@@ -269,14 +269,15 @@ __device__ void clear_outside(const ffn_ray_scan& a, int64_t i, T* p0, T* p1) {
 // rows of 2^18 rays, 64 channels, bf16: forward 411 us (4.4 TB/s), backward 800 (3.8 TB/s; the marks are read too).
 template <typename T, int V, bool BACK>
 __global__ __launch_bounds__(SC_NT) void k_scan_rays(ffn_ray_scan a, int64_t ray_blocks) {
-  if (blockIdx.x >= ray_blocks) {
-    const int64_t i = (blockIdx.x - ray_blocks) * SC_NT + threadIdx.x;
+  const int64_t block = block_number();
+  if (block >= ray_blocks) {
+    const int64_t i = (block - ray_blocks) * SC_NT + threadIdx.x;
     if (BACK) clear_outside<T>(a, i, (T*)a.dgate, (T*)a.dx);
     else clear_outside<T>(a, i, (T*)a.h, nullptr);
     return;
   }
   const int lanes = a.channels / V;
-  const int64_t id = (int64_t)blockIdx.x * SC_NT + threadIdx.x;
+  const int64_t id = block * SC_NT + threadIdx.x;
   const int64_t ray = id / lanes;
   if (ray >= a.rays.num_rays) return;
   const Cols<T, V> c(a, (int)(id % lanes) * V);
@@ -315,7 +316,7 @@ __global__ __launch_bounds__(SC_NT) void k_scan_ends(ffn_ray_scan a, int size, i
   constexpr int U = 8;
   typedef typename Chan<T, V>::vec vec;
   const int lanes = a.channels / V;
-  const int64_t id = (int64_t)blockIdx.x * SC_NT + threadIdx.x;
+  const int64_t id = block_number() * SC_NT + threadIdx.x;
   const int64_t part = id / lanes;
   if (part >= parts) return;
   const Cols<T, V> c(a, (int)(id % lanes) * V);
@@ -429,8 +430,9 @@ template <typename T, int V, bool BACK>
 __global__ __launch_bounds__(SC_NT, 4) void k_scan_parts(ffn_ray_scan a, int size, int64_t parts, int64_t part_blocks,
                                                       Ends e) {
   const int lanes = a.channels / V;
-  if (blockIdx.x >= part_blocks) {
-    const int64_t id = (blockIdx.x - part_blocks) * SC_NT + threadIdx.x, ray = id / lanes;
+  const int64_t block = block_number();
+  if (block >= part_blocks) {
+    const int64_t id = (block - part_blocks) * SC_NT + threadIdx.x, ray = id / lanes;
     if (ray >= a.rays.num_rays) return;
     const Span64 s = places_of(a, (uint32_t)ray);
     if (s.to > s.from) return;
@@ -440,7 +442,7 @@ __global__ __launch_bounds__(SC_NT, 4) void k_scan_parts(ffn_ray_scan a, int siz
     store_state<V>(BACK ? a.dh0 : a.last, ray, a.channels, ch, h);
     return;
   }
-  const int64_t id = (part_blocks - 1 - blockIdx.x) * SC_NT + threadIdx.x;
+  const int64_t id = (part_blocks - 1 - block) * SC_NT + threadIdx.x;
   const int64_t part = id / lanes;
   if (part >= parts) return;
   const Cols<T, V> c(a, (int)(id % lanes) * V);
@@ -504,7 +506,7 @@ static hipError_t run(const ffn_ray_scan& a, hipStream_t st) {
   const int64_t lanes = a.channels / V;
   if (by_rays(a)) {
     const int64_t rb = (a.rays.num_rays * lanes + SC_NT - 1) / SC_NT, cb = ((int64_t)a.rays.n + SC_NT - 1) / SC_NT;
-    if (rb + cb) k_scan_rays<T, V, BACK><<<(unsigned)(rb + cb), SC_NT, 0, st>>>(a, rb);
+    if (rb + cb) k_scan_rays<T, V, BACK><<<grid_of(rb + cb), SC_NT, 0, st>>>(a, rb);
     return hipGetLastError();
   }
   const int size = part_size(a);
@@ -513,11 +515,11 @@ static hipError_t run(const ffn_ray_scan& a, hipStream_t st) {
   const Ends e{w, w + parts * a.channels, w + 2 * parts * a.channels, w + (2 * parts + runs) * a.channels};
   const int64_t pb = (parts * lanes + SC_NT - 1) / SC_NT, rb = (a.rays.num_rays * lanes + SC_NT - 1) / SC_NT;
   if (parts) {
-    k_scan_ends<T, V, BACK><<<(unsigned)pb, SC_NT, 0, st>>>(a, size, parts, e.A, e.B);
+    k_scan_ends<T, V, BACK><<<grid_of(pb), SC_NT, 0, st>>>(a, size, parts, e.A, e.B);
     k_scan_groups<BACK><<<dim3((unsigned)runs, (a.channels + GR_C - 1) / GR_C), GR_C * GROUP, 0, st>>>(
         a.channels, parts, e.A, e.B, e.run_A, e.run_B);
   }
-  if (pb + rb) k_scan_parts<T, V, BACK><<<(unsigned)(pb + rb), SC_NT, 0, st>>>(a, size, parts, pb, e);
+  if (pb + rb) k_scan_parts<T, V, BACK><<<grid_of(pb + rb), SC_NT, 0, st>>>(a, size, parts, pb, e);
   return hipGetLastError();
 }
 

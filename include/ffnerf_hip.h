@@ -409,8 +409,9 @@ int ffn_ray_attention_bwd(const ffn_ray_attn* a, void* stream);
  * (1), from h0[ray] (NULL: 0).  It is the compositing recurrence for any number
  * of feature channels: back to front, with opacity 1 - exp(-softplus(gate)) =
  * sigmoid(gate).  gate and x [n][channels] of dtype with unit stride along the
- * channels, rows at most 2^27 bytes apart; h [n][channels] of dtype, contiguous; h0, last, dlast, dh0
- * [num_rays][channels] float: last is the state after a ray's last step (h0 for
+ * channels (up to 65536), rows at most 2^27 bytes apart; h [n][channels] of
+ * dtype, contiguous; h0, last, dlast, dh0 [num_rays][channels] float (up to
+ * 2^46 values): last is the state after a ray's last step (h0 for
  * a ray without rows).  marks (NULL without a backward pass): states the
  * forward keeps for the backward, of ffn_ray_scan_marks bytes. */
 typedef struct ffn_ray_scan {
