@@ -351,7 +351,8 @@ __device__ __forceinline__ float log_sum(float m, float l) {
 
 // Running softmax of one row, its sum still apart by lane group.  m is a maximum that lags: it is raised, and the sums are
 // rescaled, only when a logit passes it by more than SLACK (which fp16's weights, 2^14 and more, have room for), so that
-// most pieces need no exchange between lanes.
+// most pieces need no exchange between lanes.  The rows of a wavefront are raised together, so that a row's last bits depend on
+// its neighbours (each by its own logits alone: forward of 24 long rays 297 us instead of 278).
 template <typename T>
 struct Softmax {
   static constexpr float SLACK = __is_same(T, _Float16) ? 1.f : 8.f;
@@ -561,13 +562,12 @@ struct GradScale {
   }
 };
 
-// dq; also leaves D of its rows in the workspace for k_attn_dkv.  D = sum_d do o takes o's rounding in 16 bits, and dq was a
-// fifth further off for it on short rays, a twentieth on long ones of up to 32 columns.  So there it is a first value D'
-// only: the products begin at -D', the sums are those of P (dP - D'), D - D' = sum_j P (dP - D') is formed beside them, and
-// (D' - D) sum_j P k, whose
-// fragments of K are there already, sets dq right (102 -> 110 us for 8192 rays; 65536 rows in rays of 2048, 32 columns,
-// backward 373 -> 437).  Long rays of more columns (NQ = 2) keep D', which does not show there: 328 us instead of 472.  Bound as k_attn_fwd is; on the rays named there
-// 335 us (550 TFLOP/s) and 108 us.
+// dq; also leaves D of its rows in the workspace for k_attn_dkv.  D = sum_d do o takes o's rounding in 16 bits, which puts dq of
+// short rays a fifth further off, of long ones of up to 32 columns a twentieth.  There it is only a first value D': the
+// products begin at -D', the sums are those of P (dP - D'), and beside them sum_j P (dP - D') = D - D' and sum_j P k, whose
+// fragments of K are there already, set dq right (102 -> 110 us for 8192 rays; 65536 rows in rays of 2048, 32 columns,
+// backward 373 -> 437).  Long rays of more columns (two sets of rows) keep D', which does not show there: 328 us instead of
+// 472.  Bound as k_attn_fwd is; on the rays named there 335 us (550 TFLOP/s) and 109 us.
 template <typename T, int DP, int NQ, bool CAP>
 __global__ __launch_bounds__(AT_NT, least_waves(sizeof(T), DP, NQ, CAP)) void k_attn_dq(ffn_ray_attn a, int64_t total, int run) {
   constexpr int KS = DP / 32, NB = DP / 16, TILE = AT_TILE * lds_row<T, DP>;
@@ -772,7 +772,7 @@ __global__ __launch_bounds__(AT_NT, least_waves_dkv(sizeof(T), DP, NQ, CAP)) voi
       const bool bad_q = s_bad[at][0] | s_bad[at][1] | s_bad[at][2] | s_bad[at][3];
       const bool bad_d = s_bad[at][4] | s_bad[at][5] | s_bad[at][6] | s_bad[at][7];
       constexpr int B = PIECE / 16;
-    auto take = [&](int p) {
+      auto take = [&](int p) {
         const int row0 = tile + p;
         f32x4 s[NQ][B], dp[NQ][B], th[B];
         products<T, DP, NQ, B>(s, qs[at] + p * lds_row<T, DP>, kf, lane);

@@ -265,8 +265,9 @@ __device__ void clear_outside(const ffn_ray_scan& a, int64_t i, T* p0, T* p1) {
   }
 }
 
-// By rays: a thread a ray and V channels; the blocks past ray_blocks clear the rows of no ray.  Bound by memory: 4.7 million
-// rows of 2^18 rays, 64 channels, bf16: forward 411 us (4.4 TB/s), backward 800 (3.8 TB/s; the marks are read too).
+// By rays: a thread a ray and V channels; the blocks past ray_blocks clear the rows of no ray.  Bound by memory, with the
+// vector ALU 89 % busy beside it: 4.7 million rows of 2^18 rays, 64 channels, bf16, repeated: forward 387 us (4.7 TB/s),
+// backward 690 (4.4 TB/s; the marks are read too); by turns they take 1075.
 template <typename T, int V, bool BACK>
 __global__ __launch_bounds__(SC_NT) void k_scan_rays(ffn_ray_scan a, int64_t ray_blocks) {
   const int64_t block = block_number();
@@ -422,9 +423,9 @@ __device__ __forceinline__ void enter(float (&h)[V], const Ends& e, int64_t part
 }
 
 // By parts of `size` places (a multiple of SC_MARK).  The blocks past part_blocks give the rays without rows their last
-// state.  Large inputs: parts in falling order, since k_scan_ends has just read the last ones (they are still in the
-// last-level cache).  710137 rows of three rays, 128 channels, fp16: 94 us for k_scan_ends, 5 and 102, where one read of
-// gate and x and one write would take 116.  Registers are held for four wavefronts a SIMD (backward of 200,000 rows of 37
+// state.  Parts in falling order, since k_scan_ends has just read the last ones: 204 us for all three launches instead of
+// 209 in rising order, with 710137 rows of three rays, 128 channels, fp16; 94 us of them k_scan_ends, 5 and 102, where one
+// read of gate and x and one write would take 116.  Registers are held for four wavefronts a SIMD (backward of 200,000 rows of 37
 // float channels: 41 us, with three 44).
 template <typename T, int V, bool BACK>
 __global__ __launch_bounds__(SC_NT, 4) void k_scan_parts(ffn_ray_scan a, int size, int64_t parts, int64_t part_blocks,

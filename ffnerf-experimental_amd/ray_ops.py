@@ -76,7 +76,8 @@ def _index(x, name: str, dev: int) -> int:
 
 class RaySet:
     """Packed rows of rays: ray r has rows offsets[r] .. offsets[r] + counts[r] - 1, ray_ids[i] is row i's ray (all
-    int32, as ffn_march leaves them; ray_ids cut to the rows in use)."""
+    int32, as ffn_march leaves them; ray_ids cut to the rows in use).  Rays do not overlap, and all rows of a ray have
+    its id; other rows are in no ray."""
 
     def __init__(self, counts: torch.Tensor, offsets: torch.Tensor, ray_ids: torch.Tensor):
         if not isinstance(ray_ids, torch.Tensor) or not ray_ids.is_cuda:

@@ -345,9 +345,11 @@ enum { FFN_F32 = 0, FFN_F16 = 1, FFN_BF16 = 2 };                    /* element t
 
 /* Rows of rays, packed: ray r has rows offsets[r] .. offsets[r] + counts[r] - 1
  * of n (< 2^31 - 256), and ray_ids[i] is the ray of row i (ffn_march's counts,
- * offsets and ray_ids).  Rays must not overlap.  A row that is in no ray (its
- * id is no ray, or its place is outside that ray's rows) sees nothing, and
- * what a call writes for it is 0. */
+ * offsets and ray_ids).  Rays must not overlap, and all rows of a ray must
+ * have its id (else that ray's results are undefined).  A row that is in no ray
+ * (its id is no ray, or its place is outside that ray's rows) sees nothing, and
+ * what a call writes for it is 0.  The strides of an axis of one place are not
+ * looked at. */
 typedef struct ffn_ray_set {
   const uint32_t* counts;               /* [num_rays] */
   const uint32_t* offsets;              /* [num_rays] */
@@ -364,9 +366,11 @@ typedef struct ffn_ray_set {
  *   seen: same ray and, if causal, b <= a + nk - nq or b < prefix[ray]
  *   o_i = sum_j softmax_j(l_ij) v_j,   lse_i = log sum_j exp(l_ij)
  * A query that sees nothing has o = 0 and lse = -infinity; what a key that is
- * not seen holds (infinities and NaN too) changes nothing.  The queries may be
- * the keys' own set (all samples attend) or another set of the same rays (one
- * query a ray; a ray's new samples against all of them).
+ * not seen holds (infinities and NaN too) does not reach it, but for last bits:
+ * rows that are worked on together share the moment at which their sums are
+ * rescaled and, with a cap, the form of the tanh.  The queries may be the keys'
+ * own set (all samples attend) or another set of the same rays (one query a
+ * ray; a ray's new samples against all of them).
  * q [n_q][heads][dim], k and v [n_k][kv_heads][dim] of dtype with unit stride
  * along dim; other strides in elements.  dim a multiple of 8, at most 128;
  * rows 16-byte aligned.  o [n_q][heads][dim] of dtype, lse [n_q][heads] float,
