@@ -370,7 +370,10 @@ typedef struct ffn_ray_set {
  * rows that are worked on together share the moment at which their sums are
  * rescaled and, with a cap, the form of the tanh.  The queries may be the keys'
  * own set (all samples attend) or another set of the same rays (one query a
- * ray; a ray's new samples against all of them).
+ * ray; a ray's new samples against all of them).  Both sets should then hold
+ * the rays in the same order: 64 neighbouring rows walk all that lies between
+ * the first and the last row they see, so that the time of shuffled rays grows
+ * with the square of their number.
  * q [n_q][heads][dim], k and v [n_k][kv_heads][dim] of dtype with unit stride
  * along dim; other strides in elements.  dim a multiple of 8, at most 128;
  * rows 16-byte aligned.  o [n_q][heads][dim] of dtype, lse [n_q][heads] float,
