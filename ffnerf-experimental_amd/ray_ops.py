@@ -181,7 +181,8 @@ def ray_attention(q, k, v, q_rays: RaySet, k_rays: RaySet | None = None, *, t_q=
     scale q.k (scale: 1/sqrt(dim)), with cap > 0 cap tanh(score / cap), less slopes[head] |t_q - t_k|; causal: a query
     sees no key behind it (places counted from the ray's end where the sets differ), and always the first prefix[ray]
     (int32, below 0 as 0; or uint32).
-    k_rays None: q's own set; another one is fast where it holds the rays in the same order.  o as q, lse [n_q, heads] float32; a row that sees nothing has 0 and -inf."""
+    k_rays None: q's own set; another one is fast where it holds the rays in the same order.  o as q, lse [n_q, heads]
+    float32; a row that sees nothing has 0 and -inf."""
     k_rays = q_rays if k_rays is None else k_rays
     lib = fl.load()
     a, dev = _attn_args(q, k, v, q_rays, k_rays, t_q, t_k, slopes, scale, cap, causal, prefix)
