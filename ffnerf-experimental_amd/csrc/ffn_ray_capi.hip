@@ -135,6 +135,37 @@ int check_experts(const ffn_experts* a) {
   return 0;
 }
 
+int check_norm(const ffn_norm* a) {
+  if (!a) return fail(-1, "NULL arguments");
+  if (!elem(a->dtype)) return fail(-1, "dtype=%d is not FFN_F32, FFN_F16 or FFN_BF16", a->dtype);
+  if (a->param_dtype != FFN_F32 && a->param_dtype != a->dtype)
+    return fail(-1, "param_dtype=%d must be FFN_F32 or dtype=%d", a->param_dtype, a->dtype);
+  if (a->width < 1 || a->width > FFN_NORM_MAX_WIDTH)
+    return fail(-1, "width=%d must be 1 to %d", a->width, FFN_NORM_MAX_WIDTH);
+  if (a->n > MAX_ROWS) return fail(-1, "%u rows exceed %u", a->n, MAX_ROWS);
+  if (!(a->eps >= 0.f) || a->eps > 3e38f) return fail(-1, "eps=%g must be 0 or positive", a->eps);
+  const uintptr_t odd = elem(a->dtype) - 1, podd = elem(a->param_dtype) - 1;
+  if (((uintptr_t)a->x | (uintptr_t)a->y | (uintptr_t)a->dy | (uintptr_t)a->dx) & odd) return fail(-1, "misaligned buffer");
+  if (((uintptr_t)a->weight | (uintptr_t)a->bias) & podd) return fail(-1, "misaligned parameters");
+  return 0;
+}
+
+int check_route(const ffn_route* a) {
+  if (!a) return fail(-1, "NULL arguments");
+  if (!elem(a->dtype)) return fail(-1, "dtype=%d is not FFN_F32, FFN_F16 or FFN_BF16", a->dtype);
+  if (a->k < 1 || a->k > FFN_MAX_EXPERTS) return fail(-1, "k=%d must be 1 to %d", a->k, FFN_MAX_EXPERTS);
+  if (a->width < 1 || a->width > 65536) return fail(-1, "width=%d must be 1 to 65536", a->width);
+  const uint64_t places = (uint64_t)a->n * a->k;
+  if (places > MAX_ROWS) return fail(-1, "%llu places exceed %u", (unsigned long long)places, MAX_ROWS);
+  if (int rc = check_plan_sizes((uint32_t)places, a->n_experts)) return rc;
+  if (a->n && (!a->plan || !a->slots)) return fail(-1, "NULL plan or slots");
+  if (a->rows_stride < 0 || a->slots_stride < 0) return fail(-1, "row strides must be 0 or more");
+  const uintptr_t odd = elem(a->dtype) - 1;
+  if (((uintptr_t)a->rows_in | (uintptr_t)a->slots_in | (uintptr_t)a->rows_out | (uintptr_t)a->slots_out) & odd)
+    return fail(-1, "misaligned buffer");
+  return 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -233,6 +264,54 @@ int ffn_expert_linear_bwd(const ffn_experts* a, void* stream) {
     return fail(-1, "workspace of %llu bytes, %llu wanted", (unsigned long long)(a->workspace ? a->workspace_bytes : 0),
                 (unsigned long long)need);
   return launched(ffn::launch_experts(*a, true, (hipStream_t)stream), "ffn_expert_linear_bwd");
+}
+
+int ffn_layer_norm_fwd(const ffn_norm* a, void* stream) {
+  if (int rc = check_norm(a)) return rc;
+  if (a->n == 0) return 0;
+  if (!a->x || !a->y || !a->mean || !a->rstd) return fail(-1, "NULL buffer");
+  return launched(ffn::launch_norm(*a, false, (hipStream_t)stream), "ffn_layer_norm_fwd");
+}
+
+int ffn_layer_norm_workspace(const ffn_norm* a, uint64_t* bytes) {
+  if (int rc = check_norm(a)) return rc;
+  if (!bytes) return fail(-1, "NULL bytes");
+  *bytes = ffn::norm_workspace(*a);
+  return 0;
+}
+
+int ffn_layer_norm_bwd(const ffn_norm* a, void* stream) {
+  if (int rc = check_norm(a)) return rc;
+  if (a->n && (!a->x || !a->dy || !a->mean || !a->rstd)) return fail(-1, "NULL buffer");
+  const uint64_t need = a->dweight || a->dbias ? ffn::norm_workspace(*a) : 0;
+  if (need && (!a->workspace || !aligned(a->workspace) || a->workspace_bytes < need))
+    return fail(-1, "workspace of %llu bytes, %llu wanted", (unsigned long long)(a->workspace ? a->workspace_bytes : 0),
+                (unsigned long long)need);
+  return launched(ffn::launch_norm(*a, true, (hipStream_t)stream), "ffn_layer_norm_bwd");
+}
+
+int ffn_expert_slots(const uint32_t* plan, uint32_t places, int32_t n_experts, uint32_t* slots, void* stream) {
+  if (int rc = check_plan_sizes(places, n_experts)) return rc;
+  if (places && (!plan || !slots)) return fail(-1, "NULL plan or slots");
+  return launched(ffn::launch_route_slots(plan, places, n_experts, slots, (hipStream_t)stream), "ffn_expert_slots");
+}
+
+int ffn_expert_dispatch(const ffn_route* a, void* stream) {
+  if (int rc = check_route(a)) return rc;
+  if (a->n && (!a->rows_in || !a->slots_out)) return fail(-1, "NULL buffer");
+  return launched(ffn::launch_dispatch(*a, (hipStream_t)stream), "ffn_expert_dispatch");
+}
+
+int ffn_expert_combine(const ffn_route* a, void* stream) {
+  if (int rc = check_route(a)) return rc;
+  if (a->n && (!a->slots_in || !a->rows_out)) return fail(-1, "NULL buffer");
+  return launched(ffn::launch_combine(*a, (hipStream_t)stream), "ffn_expert_combine");
+}
+
+int ffn_expert_combine_bwd(const ffn_route* a, void* stream) {
+  if (int rc = check_route(a)) return rc;
+  if (a->n && (!a->rows_in || !a->slots_out || (a->dweights && !a->slots_in))) return fail(-1, "NULL buffer");
+  return launched(ffn::launch_combine_bwd(*a, (hipStream_t)stream), "ffn_expert_combine_bwd");
 }
 
 }  // extern "C"

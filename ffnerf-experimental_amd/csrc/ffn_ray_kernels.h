@@ -21,6 +21,14 @@ hipError_t launch_expert_plan(const int32_t* ids, uint32_t n, int experts, uint3
 uint64_t expert_workspace(const ffn_experts& a);
 hipError_t launch_experts(const ffn_experts& a, bool backward, hipStream_t st);
 
+uint64_t norm_workspace(const ffn_norm& a);
+hipError_t launch_norm(const ffn_norm& a, bool backward, hipStream_t st);
+
+hipError_t launch_route_slots(const uint32_t* plan, uint32_t places, int n_experts, uint32_t* slots, hipStream_t st);
+hipError_t launch_dispatch(const ffn_route& a, hipStream_t st);
+hipError_t launch_combine(const ffn_route& a, hipStream_t st);
+hipError_t launch_combine_bwd(const ffn_route& a, hipStream_t st);
+
 // the message of ffn_last_error; returns code
 int set_error(int code, const char* msg);
 

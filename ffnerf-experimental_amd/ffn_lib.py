@@ -30,6 +30,8 @@ EXPORTS = [
     "ffn_ray_attention_workspace", "ffn_ray_attention_fwd", "ffn_ray_attention_bwd", "ffn_ray_scan_marks",
     "ffn_ray_scan_workspace", "ffn_ray_scan_fwd", "ffn_ray_scan_bwd", "ffn_expert_plan_size", "ffn_expert_plan",
     "ffn_expert_linear_fwd", "ffn_expert_linear_workspace", "ffn_expert_linear_bwd",
+    "ffn_layer_norm_fwd", "ffn_layer_norm_workspace", "ffn_layer_norm_bwd", "ffn_expert_slots",
+    "ffn_expert_dispatch", "ffn_expert_combine", "ffn_expert_combine_bwd",
 ]
 ABI_VERSION = 3  # FFN_ABI_VERSION of the header these structures and signatures follow
 MARCH_NOALLOC_MAX_RAYS = 1 << 20
@@ -131,6 +133,27 @@ class FfnExperts(C.Structure):
     ]
 
 
+NORM_MAX_WIDTH = 16384  # FFN_NORM_MAX_WIDTH
+
+
+class FfnNorm(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("param_dtype", C.c_int32), ("width", C.c_int32), ("n", C.c_uint32),
+        ("eps", C.c_float), ("reserved", C.c_uint32), ("x", _vp), ("x_row", C.c_int64), ("weight", _vp),
+        ("bias", _vp), ("y", _vp), ("mean", _vp), ("rstd", _vp), ("dy", _vp), ("dy_row", C.c_int64), ("dx", _vp),
+        ("dweight", _vp), ("dbias", _vp), ("workspace", _vp), ("workspace_bytes", C.c_uint64),
+    ]
+
+
+class FfnRoute(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("n_experts", C.c_int32), ("k", C.c_int32), ("width", C.c_int32), ("n", C.c_uint32),
+        ("reserved", C.c_uint32), ("plan", _vp), ("slots", _vp), ("weights", _vp), ("rows_in", _vp),
+        ("rows_stride", C.c_int64), ("slots_in", _vp), ("slots_stride", C.c_int64), ("rows_out", _vp),
+        ("slots_out", _vp), ("dweights", _vp),
+    ]
+
+
 def march_params(res, dt, max_steps, T_stop=1e-4, chunk=32, sh_multiplier=1.0, sample_capacity=0,
                  flags=0) -> FfnMarchParams:
     m = FfnMarchParams()
@@ -203,6 +226,12 @@ def load(path: Path | str | None = None) -> C.CDLL:
     lib.ffn_expert_linear_workspace.argtypes = [C.POINTER(FfnExperts), u64p]
     lib.ffn_expert_linear_fwd.argtypes = [C.POINTER(FfnExperts), _vp]
     lib.ffn_expert_linear_bwd.argtypes = [C.POINTER(FfnExperts), _vp]
+    lib.ffn_layer_norm_workspace.argtypes = [C.POINTER(FfnNorm), u64p]
+    lib.ffn_layer_norm_fwd.argtypes = [C.POINTER(FfnNorm), _vp]
+    lib.ffn_layer_norm_bwd.argtypes = [C.POINTER(FfnNorm), _vp]
+    lib.ffn_expert_slots.argtypes = [_vp, C.c_uint32, C.c_int32, _vp, _vp]
+    for name in ("ffn_expert_dispatch", "ffn_expert_combine", "ffn_expert_combine_bwd"):
+        getattr(lib, name).argtypes = [C.POINTER(FfnRoute), _vp]
     for name in EXPORTS:
         if name != "ffn_last_error":
             getattr(lib, name).restype = C.c_int

@@ -1,10 +1,10 @@
 """Operators along rays and expert layers on torch tensors (C ABI: the second half of include/ffnerf_hip.h).
 
-They take the packed samples that `ffn_march` leaves.  `RaySet` names them; `ray_attention`, `ray_scan` and
-`expert_linear` compute, their `*_backward` give gradients, and `RayAttention`, `RayScan`, `ExpertLinear` are the same
-as functions of torch that can be differentiated once; a second time is an error.  Every call runs on the current stream
-of its tensors' device, allocates its results and scratch from torch, and never waits.  A wrong argument is an FfnError
-before anything is launched.
+They take the packed samples that `ffn_march` leaves.  `RaySet` names them; `ray_attention`, `ray_scan`, `expert_linear`,
+`layer_norm`, `expert_dispatch` and `expert_combine` compute, their `*_backward` give gradients, and `RayAttention`,
+`RayScan`, `ExpertLinear`, `LayerNorm`, `ExpertDispatch`, `ExpertCombine` are the same as functions of torch that can be
+differentiated once; a second time is an error.  Every call runs on the current stream of its tensors' device, allocates
+its results and scratch from torch, and never waits.  A wrong argument is an FfnError before anything is launched.
 """
 from __future__ import annotations
 
@@ -414,3 +414,191 @@ class ExpertLinear(torch.autograd.Function):
                                                          need_dw=need_dw, **ctx.order), dy, x, W)
         return (dx, dW.to(W.dtype) if need_dw else None, db.to(W.dtype) if need_dw and ctx.bias else None, None, None,
                 None, None)
+
+
+# ---------------------------------------------------------------------------
+# rows to several experts and back
+
+
+class ExpertRoute:
+    """Rows that go to k experts each.  plan: the ExpertPlan of the n k places, place i k + j being row i's j-th expert;
+    slots [n, k] (int32): the plan's slot of each place.  Arrays "of slots" have n k rows in the plan's order, as
+    expert_linear takes and gives them with x_slots and y_slots; slots of no expert come last."""
+
+    def __init__(self, plan: ExpertPlan, slots: torch.Tensor):
+        self.plan, self.slots, self.device = plan, slots, plan.device
+        self.n, self.k = slots.shape
+
+
+def expert_route(ids: torch.Tensor, n_experts: int) -> ExpertRoute:
+    """The route of rows with expert ids [n, k] (int32); an id outside [0, n_experts) leaves its place without an expert."""
+    if not isinstance(ids, torch.Tensor) or not ids.is_cuda or ids.dim() != 2 or ids.dtype != torch.int32:
+        _refuse("ids must be a matrix [rows, k] of int32 on the GPU")
+    if not ids.is_contiguous():
+        _refuse("ids must be contiguous")
+    if not 1 <= ids.shape[1] <= fl.MAX_EXPERTS:
+        _refuse(f"k={ids.shape[1]} must be 1 to {fl.MAX_EXPERTS}")
+    lib = fl.load()
+    plan = expert_plan(ids.view(-1), n_experts)
+    slots = torch.empty(ids.shape, dtype=torch.int32, device=plan.device)
+    _call(lib.ffn_expert_slots, plan.device, plan.words.data_ptr(), plan.n, plan.n_experts, slots.data_ptr())
+    return ExpertRoute(plan, slots)
+
+
+def _route_args(x, name, route, slots: bool, weights=None):
+    """Arguments with the width and type of x, an array of rows or of slots."""
+    dev = _is(route, ExpertRoute, "route").device
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        _refuse(f"{name} must be a tensor [{'slots' if slots else 'rows'}, width]")
+    a = fl.FfnRoute()
+    a.dtype, a.n_experts, a.k, a.width, a.n = _dtype(x), route.plan.n_experts, route.k, x.shape[1], route.n
+    a.plan, a.slots = route.plan.words.data_ptr(), route.slots.data_ptr()
+    at = _want(x, name, (route.n * route.k if slots else route.n, x.shape[1]), x.dtype, dev, 1)
+    if slots:
+        a.slots_in, a.slots_stride = at, x.stride(0)
+    else:
+        a.rows_in, a.rows_stride = at, x.stride(0)
+    a.weights = _may(weights, "weights", (route.n, route.k), torch.float32, dev)
+    return a, dev
+
+
+def expert_dispatch(x, route: ExpertRoute):
+    """Rows of x [n, width] (float32, float16 or bfloat16, unit stride along the columns) in the slots' order [n k, width];
+    slots of no expert are 0."""
+    a, dev = _route_args(x, "x", route, False)
+    out = torch.empty((route.n * route.k, x.shape[1]), dtype=x.dtype, device=dev)
+    a.slots_out = out.data_ptr()
+    _call(fl.load().ffn_expert_dispatch, dev, C.byref(a))
+    return out
+
+
+def expert_dispatch_backward(dxs, route: ExpertRoute):
+    """dx [n, width] of expert_dispatch from the gradient of its slots: each row's slots, summed."""
+    return expert_combine(dxs, route)
+
+
+def expert_combine(y, route: ExpertRoute, weights=None):
+    """Sums back to rows [n, width]: sum_j weights[i, j] y[slot of row i's j-th expert].
+
+    y [n k, width] of slots (float32, float16 or bfloat16, unit stride along the columns), weights [n, k] float32 (None:
+    1).  Sums are float32; a place of no expert adds nothing, whatever y and weights hold there."""
+    a, dev = _route_args(y, "y", route, True, weights)
+    out = torch.empty((route.n, y.shape[1]), dtype=y.dtype, device=dev)
+    a.rows_out = out.data_ptr()
+    _call(fl.load().ffn_expert_combine, dev, C.byref(a))
+    return out
+
+
+def expert_combine_backward(dout, y, route: ExpertRoute, weights=None, *, need_dweights: bool = True):
+    """(dy, dweights) of expert_combine: dy of slots (0 in those of no expert), dweights [n, k] float32 (0 at places of no
+    expert; None if not needed)."""
+    a, dev = _route_args(dout, "dout", route, False, weights)
+    if need_dweights:
+        a.slots_in = _want(y, "y", (route.n * route.k, dout.shape[1]), dout.dtype, dev, 1)
+        a.slots_stride = y.stride(0)
+    dy = torch.empty((route.n * route.k, dout.shape[1]), dtype=dout.dtype, device=dev)
+    dw = torch.empty((route.n, route.k), dtype=torch.float32, device=dev) if need_dweights else None
+    a.slots_out, a.dweights = dy.data_ptr(), (dw.data_ptr() if need_dweights else None)
+    _call(fl.load().ffn_expert_combine_bwd, dev, C.byref(a))
+    return dy, dw
+
+
+class ExpertDispatch(torch.autograd.Function):
+    """expert_dispatch; differentiable in x."""
+
+    @staticmethod
+    def forward(ctx, x, route):
+        ctx.route = route
+        return expert_dispatch(x, route)
+
+    @staticmethod
+    def backward(ctx, dxs):
+        dxs = dxs if dxs.stride(-1) == 1 else dxs.contiguous()
+        return once(lambda: expert_dispatch_backward(dxs, ctx.route), dxs), None
+
+
+class ExpertCombine(torch.autograd.Function):
+    """expert_combine; differentiable in y and weights."""
+
+    @staticmethod
+    def forward(ctx, y, route, weights=None):
+        ctx.route = route
+        ctx.save_for_backward(y, weights)
+        return expert_combine(y, route, weights)
+
+    @staticmethod
+    def backward(ctx, dout):
+        y, weights = ctx.saved_tensors
+        dout = dout if dout.stride(-1) == 1 else dout.contiguous()
+        need = ctx.needs_input_grad[2]
+        dy, dw = once(lambda: expert_combine_backward(dout, y, ctx.route, weights, need_dweights=need), dout, y, weights)
+        return dy, None, dw
+
+
+# ---------------------------------------------------------------------------
+# layer norm
+
+
+def _norm_args(x, weight, bias, eps):
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() != 2:
+        _refuse("x must be a tensor [rows, width] on the GPU")
+    a, dev = fl.FfnNorm(), x.get_device()
+    if x.shape[0] >= 1 << 31:
+        _refuse(f"{x.shape[0]} rows are too many")
+    given = [p for p in (weight, bias) if isinstance(p, torch.Tensor)]
+    kind = torch.float32 if any(p.dtype is torch.float32 for p in given) else x.dtype
+    a.dtype, a.param_dtype, a.width, a.n, a.eps = _dtype(x), DTYPES[kind], x.shape[1], x.shape[0], _number(eps, "eps")
+    a.x, a.x_row = _want(x, "x", tuple(x.shape), x.dtype, dev, 1), x.stride(0)
+    a.weight = _may(weight, "weight", (x.shape[1],), kind, dev)
+    a.bias = _may(bias, "bias", (x.shape[1],), kind, dev)
+    return a, dev
+
+
+def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5):
+    """(y, mean, rstd): y = (x - mean) rstd weight + bias by rows, rstd = 1 / sqrt(var + eps).
+
+    x [n, width] (float32, float16 or bfloat16, unit stride along the columns; fastest where rows start on 16 bytes), width
+    up to 16384; weight and bias [width] both float32 or both of x's type (None: 1 and 0).  y as x; mean and rstd [n]
+    float32."""
+    a, dev = _norm_args(x, weight, bias, eps)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    mean, rstd = (torch.empty(x.shape[0], dtype=torch.float32, device=dev) for _ in range(2))
+    a.y, a.mean, a.rstd = y.data_ptr(), mean.data_ptr(), rstd.data_ptr()
+    _call(fl.load().ffn_layer_norm_fwd, dev, C.byref(a))
+    return y, mean, rstd
+
+
+def layer_norm_backward(dy, x, weight, mean, rstd, *, need_dx: bool = True, need_dw: bool = True):
+    """(dx, dweight, dbias) of layer_norm, with its mean and rstd.  dx as x, dweight and dbias [width] float32; None for
+    those not needed."""
+    a, dev = _norm_args(x, weight, None, 0.0)
+    a.dy, a.dy_row = _want(dy, "dy", tuple(x.shape), x.dtype, dev, 1), dy.stride(0)
+    a.mean = _want(mean, "mean", (x.shape[0],), torch.float32, dev)
+    a.rstd = _want(rstd, "rstd", (x.shape[0],), torch.float32, dev)
+    lib = fl.load()
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_dx else None
+    dw, db = (torch.empty(x.shape[1], dtype=torch.float32, device=dev) if need_dw else None for _ in range(2))
+    a.dx, a.dweight, a.dbias = (t.data_ptr() if t is not None else None for t in (dx, dw, db))
+    w = _workspace(a, lib.ffn_layer_norm_workspace, dev) if need_dw else None  # noqa: F841
+    _call(lib.ffn_layer_norm_bwd, dev, C.byref(a))
+    return dx, dw, db
+
+
+class LayerNorm(torch.autograd.Function):
+    """y of layer_norm; differentiable in x, weight and bias."""
+
+    @staticmethod
+    def forward(ctx, x, weight=None, bias=None, eps=1e-5):
+        y, mean, rstd = layer_norm(x, weight, bias, eps=eps)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        dy = dy if dy.stride(-1) == 1 else dy.contiguous()
+        need_w, need_b = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
+        dx, dw, db = once(lambda: layer_norm_backward(dy, x, weight, mean, rstd, need_dx=ctx.needs_input_grad[0],
+                                                      need_dw=need_w or need_b), dy, x, weight)
+        return dx, dw.to(weight.dtype) if need_w else None, db.to(ctx.bias_dtype) if need_b else None, None

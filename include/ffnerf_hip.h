@@ -494,6 +494,73 @@ int ffn_expert_linear_workspace(const ffn_experts* a, uint64_t* bytes);  /* of t
  * Experts without rows get 0.  No atomics: two calls give the same bits. */
 int ffn_expert_linear_bwd(const ffn_experts* a, void* stream);
 
+/* Layer norm of rows, y = (x - mean) rstd weight + bias with rstd = 1 /
+ * sqrt(var + eps), statistics in float.  x [n][width] of dtype with unit stride
+ * along the columns and row stride x_row, 1 <= width <= FFN_NORM_MAX_WIDTH;
+ * weight and bias [width] of param_dtype (FFN_F32 or dtype; NULL: 1 and 0); y
+ * [n][width] of dtype, mean and rstd [n] float, contiguous.  Rows of 16-byte
+ * alignment are fastest. */
+#define FFN_NORM_MAX_WIDTH 16384
+typedef struct ffn_norm {
+  int32_t dtype, param_dtype, width;
+  uint32_t n;
+  float eps;
+  uint32_t reserved;
+  const void* x;
+  int64_t x_row;
+  const void *weight, *bias;
+  void* y;
+  float *mean, *rstd;                   /* the backward reads the forward's */
+  /* backward only: dy as y with row stride dy_row; dx [n][width] contiguous of dtype; dweight, dbias [width] float;
+     any of dx, dweight, dbias may be NULL */
+  const void* dy;
+  int64_t dy_row;
+  void* dx;
+  float *dweight, *dbias;
+  void* workspace;
+  uint64_t workspace_bytes;
+} ffn_norm;
+
+int ffn_layer_norm_fwd(const ffn_norm* a, void* stream);
+int ffn_layer_norm_workspace(const ffn_norm* a, uint64_t* bytes);  /* of the backward, with dweight or dbias */
+/* No atomics: two calls give the same bits. */
+int ffn_layer_norm_bwd(const ffn_norm* a, void* stream);
+
+/* Rows to several experts and back.  With a plan (ffn_expert_plan) over the
+ * n k ids of n rows' k experts, place i k + j being row i's j-th:
+ * ffn_expert_slots gives the inverse of the plan's rows, slots[place] = the
+ * slot that holds it (places = n k).  An array "of slots" is [n k][width] in the
+ * plan's slot order, what the expert layers take and give under
+ * FFN_EXPERTS_X_SLOTS and FFN_EXPERTS_Y_SLOTS.
+ *   dispatch     slots_out[slot] = rows_in[i] for each of row i's slots
+ *   combine      rows_out[i] = sum_j weights[i][j] slots_in[slot of (i, j)]
+ *   combine_bwd  of sum(rows_out rows_in): slots_out[slot] = weights rows_in[i],
+ *                dweights[i][j] = rows_in[i] . slots_in[slot] (NULL: not wanted,
+ *                and slots_in is not read)
+ * The gradient of dispatch is combine without weights (NULL: 1).  A place of no
+ * expert has a slot of 0, adds nothing whatever slots_in and weights hold there,
+ * and has a dweight of 0.  rows_in [n][width] and slots_in [n k][width] have
+ * unit stride along the columns and strides of 0 or more between rows; the
+ * outputs are contiguous, weights and dweights [n][k] float.  1 <= width <= 65536, 1 <= k <=
+ * FFN_MAX_EXPERTS, n k < 2^31 - 256.  Sums are held in float, in the order of j. */
+typedef struct ffn_route {
+  int32_t dtype, n_experts, k, width;
+  uint32_t n, reserved;
+  const uint32_t *plan, *slots;
+  const float* weights;                 /* or NULL */
+  const void* rows_in;
+  int64_t rows_stride;                  /* elements */
+  const void* slots_in;
+  int64_t slots_stride;
+  void *rows_out, *slots_out;
+  float* dweights;
+} ffn_route;
+
+int ffn_expert_slots(const uint32_t* plan, uint32_t places, int32_t n_experts, uint32_t* slots, void* stream);
+int ffn_expert_dispatch(const ffn_route* a, void* stream);
+int ffn_expert_combine(const ffn_route* a, void* stream);
+int ffn_expert_combine_bwd(const ffn_route* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
