@@ -26,6 +26,7 @@ constexpr uint32_t MAX_ROWS = 0x7FFFFF00u;
 constexpr int MAX_SCAN_STRIDE = 1 << 27;
 
 constexpr uint64_t MAX_SCAN_STATES = 1ull << 46;  // channels of all rays: what one launch can count
+constexpr uint64_t MAX_DELTA_STATES = 1ull << 36; // heads of all rays: a block each
 
 int elem(int32_t dtype) { return dtype == FFN_F32 ? 4 : dtype == FFN_F16 || dtype == FFN_BF16 ? 2 : 0; }
 
@@ -135,6 +136,57 @@ int check_experts(const ffn_experts* a) {
   return 0;
 }
 
+int check_delta_sizes(const ffn_ray_delta* a) {
+  if (!a) return fail(-1, "NULL arguments");
+  if (!elem(a->dtype)) return fail(-1, "dtype=%d is not FFN_F32, FFN_F16 or FFN_BF16", a->dtype);
+  if (a->heads < 1 || a->v_heads < 1 || a->v_heads > 1024 || a->v_heads % a->heads)
+    return fail(-1, "v_heads=%d, heads=%d: v_heads must be a multiple of heads, at most 1024", a->v_heads, a->heads);
+  if (a->key_dim < 8 || a->key_dim > 128 || a->key_dim % 8 || a->val_dim < 8 || a->val_dim > 128 || a->val_dim % 8)
+    return fail(-1, "key_dim=%d, val_dim=%d must be multiples of 8, at most 128", a->key_dim, a->val_dim);
+  if (a->reverse != 0 && a->reverse != 1) return fail(-1, "reverse=%d must be 0 or 1", a->reverse);
+  if (a->rays.n > MAX_ROWS) return fail(-1, "rays: %u rows exceed %u", a->rays.n, MAX_ROWS);
+  return 0;
+}
+
+int check_delta(const ffn_ray_delta* a, bool backward) {
+  if (int rc = check_delta_sizes(a)) return rc;
+  if (int rc = check_set(a->rays, "rays", true)) return rc;
+  if (!(a->scale == a->scale) || a->scale > 3e38f || a->scale < -3e38f) return fail(-1, "scale=%g is not finite", a->scale);
+  if ((uint64_t)a->rays.num_rays * a->v_heads > MAX_DELTA_STATES)
+    return fail(-1, "%d heads of %u rays exceed 2^36", a->v_heads, a->rays.num_rays);
+  const bool n = a->rays.n > 0;
+  const int b = elem(a->dtype);
+  const int64_t rows = a->rays.n, h = n ? a->heads : 0, vh = n ? a->v_heads : 0;
+  if (n && (!a->q || !a->k || !a->v || !a->decay || !a->beta)) return fail(-1, "NULL buffer");
+  const int64_t steps[] = {step(rows, a->q_row),     step(h, a->q_head),       step(rows, a->k_row),    step(h, a->k_head),
+                           step(rows, a->v_row),     step(vh, a->v_head),      step(rows, a->decay_row), step(vh, a->decay_head),
+                           step(rows, a->beta_row),  step(vh, a->beta_head),   backward ? step(rows, a->do_row) : 0,
+                           backward ? step(vh, a->do_head) : 0};
+  for (int64_t s : steps)
+    if (s < 0) return fail(-1, "strides must be 0 or more");
+  if (!aligned(a->q, step(rows, a->q_row), b) || !aligned(a->q, step(h, a->q_head), b) || !aligned(a->k, step(rows, a->k_row), b) ||
+      !aligned(a->k, step(h, a->k_head), b) || !aligned(a->v, step(rows, a->v_row), b) || !aligned(a->v, step(vh, a->v_head), b))
+    return fail(-1, "rows and heads of q, k and v must be 16-byte aligned");
+  if (((uintptr_t)a->decay | (uintptr_t)a->beta) & (b - 1)) return fail(-1, "misaligned decay or beta");
+  if (!aligned(a->h0)) return fail(-1, "h0 must be 16-byte aligned");
+  if (!backward) {
+    if (n && !a->o) return fail(-1, "NULL output");
+    if (!aligned(a->o) || !aligned(a->last) || !aligned(a->marks)) return fail(-1, "o, last and marks must be 16-byte aligned");
+    return 0;
+  }
+  if (n && (!a->dout || !a->dq || !a->dk || !a->dv || !a->ddecay || !a->dbeta || !a->marks))
+    return fail(-1, "NULL gradient buffer or marks");
+  if (!aligned(a->dout, step(rows, a->do_row), b) || !aligned(a->dout, step(vh, a->do_head), b) || !aligned(a->dq) ||
+      !aligned(a->dk) || !aligned(a->dv) || !aligned(a->ddecay) || !aligned(a->dbeta) || !aligned(a->dlast) || !aligned(a->dh0) ||
+      !aligned(a->marks))
+    return fail(-1, "rows and heads of the gradients, the states' gradients and marks must be 16-byte aligned");
+  const uint64_t need = ffn::delta_workspace(*a);
+  if (need && (!a->workspace || !aligned(a->workspace) || a->workspace_bytes < need))
+    return fail(-1, "workspace of %llu bytes, %llu wanted", (unsigned long long)(a->workspace ? a->workspace_bytes : 0),
+                (unsigned long long)need);
+  return 0;
+}
+
 int check_norm(const ffn_norm* a) {
   if (!a) return fail(-1, "NULL arguments");
   if (!elem(a->dtype)) return fail(-1, "dtype=%d is not FFN_F32, FFN_F16 or FFN_BF16", a->dtype);
@@ -210,6 +262,30 @@ int ffn_ray_scan_fwd(const ffn_ray_scan* a, void* stream) {
 int ffn_ray_scan_bwd(const ffn_ray_scan* a, void* stream) {
   if (int rc = check_scan(a, true)) return rc;
   return launched(ffn::launch_scan(*a, true, (hipStream_t)stream), "ffn_ray_scan_bwd");
+}
+
+int ffn_ray_delta_marks(const ffn_ray_delta* a, uint64_t* bytes) {
+  if (int rc = check_delta_sizes(a)) return rc;
+  if (!bytes) return fail(-1, "NULL bytes");
+  *bytes = ffn::delta_marks(*a);
+  return 0;
+}
+
+int ffn_ray_delta_workspace(const ffn_ray_delta* a, int32_t backward, uint64_t* bytes) {
+  if (int rc = check_delta_sizes(a)) return rc;
+  if (!bytes) return fail(-1, "NULL bytes");
+  *bytes = backward ? ffn::delta_workspace(*a) : 0;
+  return 0;
+}
+
+int ffn_ray_delta_fwd(const ffn_ray_delta* a, void* stream) {
+  if (int rc = check_delta(a, false)) return rc;
+  return launched(ffn::launch_delta(*a, false, (hipStream_t)stream), "ffn_ray_delta_fwd");
+}
+
+int ffn_ray_delta_bwd(const ffn_ray_delta* a, void* stream) {
+  if (int rc = check_delta(a, true)) return rc;
+  return launched(ffn::launch_delta(*a, true, (hipStream_t)stream), "ffn_ray_delta_bwd");
 }
 
 int ffn_expert_plan_size(uint32_t n, int32_t n_experts, uint64_t* plan_words, uint64_t* workspace_bytes) {

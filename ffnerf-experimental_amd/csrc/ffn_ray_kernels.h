@@ -14,6 +14,10 @@ uint64_t scan_marks(const ffn_ray_scan& a);
 uint64_t scan_workspace(const ffn_ray_scan& a, bool backward);
 hipError_t launch_scan(const ffn_ray_scan& a, bool backward, hipStream_t st);
 
+uint64_t delta_marks(const ffn_ray_delta& a);
+uint64_t delta_workspace(const ffn_ray_delta& a);
+hipError_t launch_delta(const ffn_ray_delta& a, bool backward, hipStream_t st);
+
 uint64_t expert_plan_words(uint32_t n, int experts);
 uint64_t expert_plan_workspace(uint32_t n, int experts);
 hipError_t launch_expert_plan(const int32_t* ids, uint32_t n, int experts, uint32_t* plan, uint32_t* workspace,

@@ -31,7 +31,8 @@ EXPORTS = [
     "ffn_ray_scan_workspace", "ffn_ray_scan_fwd", "ffn_ray_scan_bwd", "ffn_expert_plan_size", "ffn_expert_plan",
     "ffn_expert_linear_fwd", "ffn_expert_linear_workspace", "ffn_expert_linear_bwd",
     "ffn_layer_norm_fwd", "ffn_layer_norm_workspace", "ffn_layer_norm_bwd", "ffn_expert_slots",
-    "ffn_expert_dispatch", "ffn_expert_combine", "ffn_expert_combine_bwd",
+    "ffn_expert_dispatch", "ffn_expert_combine", "ffn_expert_combine_bwd", "ffn_ray_delta_marks",
+    "ffn_ray_delta_workspace", "ffn_ray_delta_fwd", "ffn_ray_delta_bwd",
 ]
 ABI_VERSION = 3  # FFN_ABI_VERSION of the header these structures and signatures follow
 MARCH_NOALLOC_MAX_RAYS = 1 << 20
@@ -117,6 +118,19 @@ class FfnRayScan(C.Structure):
         ("h0", _vp), ("h", _vp), ("last", _vp), ("marks", _vp), ("dh", _vp), ("dh_row", C.c_int64),
         ("dlast", _vp), ("dgate", _vp), ("dx", _vp), ("dh0", _vp), ("workspace", _vp),
         ("workspace_bytes", C.c_uint64),
+    ]
+
+
+class FfnRayDelta(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("heads", C.c_int32), ("v_heads", C.c_int32), ("key_dim", C.c_int32),
+        ("val_dim", C.c_int32), ("reverse", C.c_int32), ("scale", C.c_float), ("reserved", C.c_int32),
+        ("rays", FfnRaySet), ("q", _vp), ("k", _vp), ("v", _vp), ("q_row", C.c_int64), ("q_head", C.c_int64),
+        ("k_row", C.c_int64), ("k_head", C.c_int64), ("v_row", C.c_int64), ("v_head", C.c_int64), ("decay", _vp),
+        ("beta", _vp), ("decay_row", C.c_int64), ("decay_head", C.c_int64), ("beta_row", C.c_int64),
+        ("beta_head", C.c_int64), ("h0", _vp), ("o", _vp), ("last", _vp), ("marks", _vp), ("dout", _vp),
+        ("do_row", C.c_int64), ("do_head", C.c_int64), ("dlast", _vp), ("dq", _vp), ("dk", _vp), ("dv", _vp),
+        ("ddecay", _vp), ("dbeta", _vp), ("dh0", _vp), ("workspace", _vp), ("workspace_bytes", C.c_uint64),
     ]
 
 
@@ -216,11 +230,12 @@ def load(path: Path | str | None = None) -> C.CDLL:
     lib.ffn_set_profiling.argtypes = [_vp, C.c_int32]
     lib.ffn_stage_times.argtypes = [_vp, _fp, C.POINTER(C.c_int32), C.c_int32]
     u64p = C.POINTER(C.c_uint64)
-    for op, args in (("attention", FfnRayAttn), ("scan", FfnRayScan)):
+    for op, args in (("attention", FfnRayAttn), ("scan", FfnRayScan), ("delta", FfnRayDelta)):
         getattr(lib, f"ffn_ray_{op}_workspace").argtypes = [C.POINTER(args), C.c_int32, u64p]
         getattr(lib, f"ffn_ray_{op}_fwd").argtypes = [C.POINTER(args), _vp]
         getattr(lib, f"ffn_ray_{op}_bwd").argtypes = [C.POINTER(args), _vp]
     lib.ffn_ray_scan_marks.argtypes = [C.POINTER(FfnRayScan), u64p]
+    lib.ffn_ray_delta_marks.argtypes = [C.POINTER(FfnRayDelta), u64p]
     lib.ffn_expert_plan_size.argtypes = [C.c_uint32, C.c_int32, u64p, u64p]
     lib.ffn_expert_plan.argtypes = [_vp, C.c_uint32, C.c_int32, _vp, C.c_uint64, _vp, C.c_uint64, _vp]
     lib.ffn_expert_linear_workspace.argtypes = [C.POINTER(FfnExperts), u64p]

@@ -1,9 +1,9 @@
 """Operators along rays and expert layers on torch tensors (C ABI: the second half of include/ffnerf_hip.h).
 
-They take the packed samples that `ffn_march` leaves.  `RaySet` names them; `ray_attention`, `ray_scan`, `expert_linear`,
-`layer_norm`, `expert_dispatch` and `expert_combine` compute, their `*_backward` give gradients, and `RayAttention`,
-`RayScan`, `ExpertLinear`, `LayerNorm`, `ExpertDispatch`, `ExpertCombine` are the same as functions of torch that can be
-differentiated once; a second time is an error.  Every call runs on the current stream of its tensors' device, allocates
+They take the packed samples that `ffn_march` leaves.  `RaySet` names them; `ray_attention`, `ray_scan`, `ray_delta`,
+`expert_linear`, `expert_dispatch`, `expert_combine` and `layer_norm` compute, their `*_backward` give gradients, and
+`RayAttention`, `RayScan`, `RayDelta`, `ExpertLinear`, `ExpertDispatch`, `ExpertCombine`, `LayerNorm` are the same as
+functions of torch that can be differentiated once; a second time is an error.  Every call runs on the current stream of its tensors' device, allocates
 its results and scratch from torch, and never waits.  A wrong argument is an FfnError before anything is launched.
 """
 from __future__ import annotations
@@ -304,6 +304,105 @@ class RayScan(torch.autograd.Function):
         dgate, dx, dh0 = once(lambda: ray_scan_backward(dh, gate, x, marks, ctx.rays, dlast=dlast.contiguous(), h0=h0,
                                                         reverse=ctx.reverse), dh, dlast, gate, x, h0)
         return dgate, dx, None, (dh0 if h0 is not None else None), None
+
+
+# ---------------------------------------------------------------------------
+# the delta rule
+
+
+def _delta_args(q, k, v, decay, beta, rays, h0, scale, reverse):
+    if not isinstance(q, torch.Tensor) or q.dim() != 3 or not isinstance(v, torch.Tensor) or v.dim() != 3:
+        _refuse("q and v must be tensors [rows, heads, dim]")
+    a, dev = fl.FfnRayDelta(), _is(rays, RaySet, "rays").device
+    n, dtype = rays.n, q.dtype
+    (_, heads, dk), (_, v_heads, dv) = q.shape, v.shape
+    a.dtype, a.heads, a.v_heads, a.key_dim, a.val_dim = _dtype(q), heads, v_heads, dk, dv
+    a.reverse, a.rays = 1 if reverse else 0, rays.c
+    a.scale = dk ** -0.5 if scale is None and dk else _number(scale, "scale")
+    a.q, a.k = _want(q, "q", (n, heads, dk), dtype, dev, 1), _want(k, "k", (n, heads, dk), dtype, dev, 1)
+    a.v = _want(v, "v", (n, v_heads, dv), dtype, dev, 1)
+    a.decay = _want(decay, "decay", (n, v_heads), dtype, dev, 0)
+    a.beta = _want(beta, "beta", (n, v_heads), dtype, dev, 0)
+    (a.q_row, a.q_head, _), (a.k_row, a.k_head, _), (a.v_row, a.v_head, _) = q.stride(), k.stride(), v.stride()
+    (a.decay_row, a.decay_head), (a.beta_row, a.beta_head) = decay.stride(), beta.stride()
+    state = (rays.num_rays, v_heads, dk, dv)
+    a.h0 = _may(h0, "h0", state, torch.float32, dev)
+    return a, dev, state
+
+
+def ray_delta(q, k, v, decay, beta, rays: RaySet, *, h0=None, scale: float | None = None, reverse: bool = False,
+              last=False, marks: bool = False):
+    """(o, last, marks): a matrix state a ray and value head, S_t = a_t S_{t-1} + k_t n_t^T with a_t = exp(decay_t) and
+    n_t = beta_t (v_t - a_t S_{t-1}^T k_t), read as o_t = scale S_t^T q_t (scale: 1/sqrt(key dim)).
+
+    q and k [n, heads, key_dim], v [n, v_heads, val_dim] (float32, float16 or bfloat16, unit stride along the dims, rows
+    and heads on 16 bytes; v_heads a multiple of heads, which are shared; dims multiples of 8 up to 128), decay (at most 0;
+    -inf forgets what was before) and beta [n, v_heads] of the same type; stable where beta |k|^2 <= 2.  From h0 [num_rays,
+    v_heads, key_dim, val_dim] float32 (None: 0); reverse: from each ray's last row to its first.  o [n, v_heads, val_dim];
+    last: True for the state after each ray, or a tensor that takes it (h0 itself: in place), as h0; marks: what
+    ray_delta_backward needs.  Both None unless asked."""
+    lib = fl.load()
+    a, dev, state = _delta_args(q, k, v, decay, beta, rays, h0, scale, reverse)
+    o = torch.empty(v.shape, dtype=v.dtype, device=dev)
+    if isinstance(last, torch.Tensor):
+        a.last = _want(last, "last", state, torch.float32, dev)
+    else:
+        last = torch.empty(state, dtype=torch.float32, device=dev) if last else None
+        a.last = last.data_ptr() if last is not None else None
+    a.o, m = o.data_ptr(), None
+    if marks:
+        n = C.c_uint64()
+        fl.check(lib.ffn_ray_delta_marks(C.byref(a), C.byref(n)), "ffn_ray_delta_marks")
+        m = torch.empty(n.value // 4, dtype=torch.float32, device=dev)
+        a.marks = m.data_ptr()
+    _call(lib.ffn_ray_delta_fwd, dev, C.byref(a))
+    return o, last, m
+
+
+def ray_delta_backward(do, q, k, v, decay, beta, marks, rays: RaySet, *, dlast=None, h0=None, scale: float | None = None,
+                       reverse: bool = False):
+    """(dq, dk, dv, ddecay, dbeta, dh0) of ray_delta's o (do) and last (dlast, None: 0), with its marks and options.  Of the
+    inputs' type; dh0 float32, None without h0."""
+    lib = fl.load()
+    a, dev, state = _delta_args(q, k, v, decay, beta, rays, h0, scale, reverse)
+    a.dout = _want(do, "do", v.shape, v.dtype, dev, 1)
+    a.do_row, a.do_head = do.stride()[:2]
+    a.dlast = _may(dlast, "dlast", state, torch.float32, dev)
+    n = C.c_uint64()
+    fl.check(lib.ffn_ray_delta_marks(C.byref(a), C.byref(n)), "ffn_ray_delta_marks")
+    a.marks = _want(marks, "marks", (n.value // 4,), torch.float32, dev)
+    out = [torch.empty(x.shape, dtype=q.dtype, device=dev) for x in (q, k, v, decay, beta)]
+    a.dq, a.dk, a.dv, a.ddecay, a.dbeta = (x.data_ptr() for x in out)
+    dh0 = torch.empty(state, dtype=torch.float32, device=dev) if h0 is not None else None
+    a.dh0 = dh0.data_ptr() if h0 is not None else None
+    w = _workspace(a, lib.ffn_ray_delta_workspace, dev, 1)  # noqa: F841
+    _call(lib.ffn_ray_delta_bwd, dev, C.byref(a))
+    return (*out, dh0)
+
+
+class RayDelta(torch.autograd.Function):
+    """(o, last) of ray_delta; differentiable in q, k, v, decay, beta and h0.  options: a dict of scale and reverse, and
+    last=False where the state after the rays is not wanted (None)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, decay, beta, rays, h0=None, options=None):
+        ctx.options = dict(options or {})
+        wanted = ctx.options.pop("last", True)
+        o, last, marks = ray_delta(q, k, v, decay, beta, rays, h0=h0, last=bool(wanted), marks=True, **ctx.options)
+        ctx.save_for_backward(q, k, v, decay, beta, marks, h0)
+        ctx.rays = rays
+        return o, last
+
+    @staticmethod
+    def backward(ctx, do, dlast):
+        q, k, v, decay, beta, marks, h0 = ctx.saved_tensors
+        if do.stride(-1) != 1 or any(s < 0 or s * do.element_size() % 16 for s in do.stride()[:2]) or do.data_ptr() % 16:
+            do = do.contiguous()
+        dlast = None if dlast is None else dlast.contiguous()
+        dq, dk, dv, dg, db, dh0 = once(
+            lambda: ray_delta_backward(do, q, k, v, decay, beta, marks, ctx.rays, dlast=dlast, h0=h0, **ctx.options),
+            do, dlast, q, k, v, decay, beta, h0)
+        return dq, dk, dv, dg, db, None, dh0, None
 
 
 # ---------------------------------------------------------------------------

@@ -447,6 +447,56 @@ int ffn_ray_scan_fwd(const ffn_ray_scan* a, void* stream);
  * marks of the same sizes. */
 int ffn_ray_scan_bwd(const ffn_ray_scan* a, void* stream);
 
+/* A matrix state a ray and value head, written by the delta rule with decay:
+ *   S_t = a_t S_{t-1} + k_t n_t^T,  a_t = exp(decay_t)
+ *   n_t = beta_t (v_t - a_t S_{t-1}^T k_t),  o_t = scale S_t^T q_t
+ * over a ray's rows in order (reverse = 0) or from its last row to its first
+ * (1), from h0[ray] (NULL: 0), in float.  Where ffn_ray_scan carries a value a
+ * channel, this carries what was written under a key until it is read, replaced
+ * or decayed.  It is stable where beta |k|^2 <= 2 and decay <= 0; a decay of
+ * -infinity forgets what was before the row.  What a row holds, infinities and
+ * NaN too, does not reach the o of rows before it.
+ * q and k [n][heads][key_dim], v [n][v_heads][val_dim] of dtype with unit stride
+ * along the dims; value head h uses key head h / (v_heads / heads).  decay and
+ * beta [n][v_heads] of dtype.  Strides in elements, 0 or more.  key_dim and
+ * val_dim multiples of 8, at most 128; rows and heads of q, k, v 16-byte aligned.
+ * o [n][v_heads][val_dim] of dtype; h0, last, dlast, dh0
+ * [num_rays][v_heads][key_dim][val_dim] float; all contiguous and 16-byte aligned.  last (NULL: not
+ * wanted) is the state after a ray's last row, h0 for a ray without rows, and
+ * may be h0 itself.  marks (NULL without a backward pass): states the forward
+ * keeps for the backward, of ffn_ray_delta_marks bytes. */
+typedef struct ffn_ray_delta {
+  int32_t dtype, heads, v_heads, key_dim, val_dim, reverse;
+  float scale;
+  int32_t reserved;
+  ffn_ray_set rays;
+  const void *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  const void *decay, *beta;
+  int64_t decay_row, decay_head, beta_row, beta_head;
+  const float* h0;                      /* or NULL */
+  void* o;
+  float* last;                          /* or NULL */
+  float* marks;
+  /* backward only; dout as o (strides do_row, do_head); dq, dk [n][heads][key_dim], dv [n][v_heads][val_dim], ddecay and
+     dbeta [n][v_heads] of dtype, contiguous */
+  const void* dout;
+  int64_t do_row, do_head;
+  const float* dlast;                   /* or NULL */
+  void *dq, *dk, *dv, *ddecay, *dbeta;
+  float* dh0;                           /* or NULL */
+  void* workspace;
+  uint64_t workspace_bytes;
+} ffn_ray_delta;
+
+int ffn_ray_delta_marks(const ffn_ray_delta* a, uint64_t* bytes);
+int ffn_ray_delta_workspace(const ffn_ray_delta* a, int32_t backward, uint64_t* bytes);
+int ffn_ray_delta_fwd(const ffn_ray_delta* a, void* stream);
+/* Gradients of sum(o dout) + sum(last dlast), from q, k, v, decay, beta, h0 and
+ * the forward's marks of the same sizes; dq and dk summed over the value heads
+ * of a key head.  scale gets none.  No atomics: two calls give the same bits. */
+int ffn_ray_delta_bwd(const ffn_ray_delta* a, void* stream);
+
 #define FFN_MAX_EXPERTS 1024
 /* Rows grouped by expert.  ids [n]: the expert of each row; an id outside
  * [0, n_experts) gives the row to none.  plan (ffn_expert_plan_size words of 4

@@ -1,4 +1,4 @@
-"""Wrong arguments of layer norm and of routing: refused with a message, before any launch (nothing here reaches the
+"""Wrong arguments of layer norm, of routing and of the delta rule: refused with a message, before any launch (nothing here reaches the
 GPU; pointers are never read)."""
 import ctypes as C
 
@@ -89,3 +89,43 @@ def test_python_entry_points_refuse():
         ray_ops.expert_route(torch.zeros(4, 2, dtype=torch.int32), 3)
     with pytest.raises(fl.FfnError, match="route must be a ExpertRoute"):
         ray_ops.expert_dispatch(x, None)
+
+
+def _delta(**kw):
+    s = dict(counts=P, offsets=P, ray_ids=P, num_rays=4, n=64)
+    a = fl.FfnRayDelta(dtype=2, heads=2, v_heads=4, key_dim=32, val_dim=64, scale=0.2, rays=fl.FfnRaySet(**s), q=P, k=P, v=P,
+                       q_row=64, q_head=32, k_row=64, k_head=32, v_row=256, v_head=64, decay=P, beta=P, decay_row=4,
+                       decay_head=1, beta_row=4, beta_head=1, h0=P, o=P, last=P, marks=P, dout=P, do_row=256, do_head=64,
+                       dlast=P, dq=P, dk=P, dv=P, ddecay=P, dbeta=P, dh0=P, workspace=P, workspace_bytes=1 << 30)
+    for k, v in kw.items():
+        setattr(a, k, fl.FfnRaySet(**{**s, **v}) if k == "rays" else v)
+    return a
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(dtype=3), "dtype=3"), (dict(heads=3), "multiple of heads"), (dict(heads=0), "heads=0"),
+    (dict(v_heads=1026), "v_heads=1026"), (dict(key_dim=12), "key_dim=12"), (dict(key_dim=136), "key_dim=136"),
+    (dict(val_dim=0), "val_dim=0"), (dict(reverse=2), "reverse=2"), (dict(scale=float("nan")), "scale="),
+    (dict(scale=float("inf")), "scale="), (dict(rays=dict(n=1 << 31)), "exceed"), (dict(rays=dict(counts=None)), "NULL counts"),
+    (dict(rays=dict(ray_ids=None)), "NULL ray_ids"), (dict(rays=dict(num_rays=(1 << 32) - 1), v_heads=32), "2^36"),
+    (dict(q=None), "NULL buffer"), (dict(beta=None), "NULL buffer"), (dict(q=P + 2), "aligned"), (dict(k_row=65), "aligned"),
+    (dict(v_head=4), "aligned"), (dict(q_row=-64), "strides"), (dict(decay_head=-1), "strides"), (dict(decay=P + 1), "misaligned"),
+    (dict(h0=P + 4), "h0 must"), (dict(marks=P + 4), "16-byte aligned"),
+])
+def test_delta_refuses(kw, match):
+    lib = fl.load()
+    _refused(lib.ffn_ray_delta_fwd, C.byref(_delta(**kw)), None, match=match)
+    _refused(lib.ffn_ray_delta_bwd, C.byref(_delta(**kw)), None, match=match)
+
+
+def test_delta_refuses_what_only_one_direction_needs():
+    lib = fl.load()
+    _refused(lib.ffn_ray_delta_fwd, C.byref(_delta(o=None)), None, match="NULL output")
+    _refused(lib.ffn_ray_delta_fwd, C.byref(_delta(last=P + 8)), None, match="16-byte aligned")
+    for kw, match in ((dict(dout=None), "NULL gradient"), (dict(ddecay=None), "NULL gradient"), (dict(marks=None), "marks"),
+                      (dict(do_row=4), "aligned"), (dict(dq=P + 8), "aligned"), (dict(do_row=-8), "strides"),
+                      (dict(workspace_bytes=8), "workspace of 8"), (dict(workspace=None), "workspace of 0")):
+        _refused(lib.ffn_ray_delta_bwd, C.byref(_delta(**kw)), None, match=match)
+    _refused(lib.ffn_ray_delta_fwd, None, None, match="NULL arguments")
+    _refused(lib.ffn_ray_delta_marks, C.byref(_delta()), None, match="NULL bytes")
+    _refused(lib.ffn_ray_delta_workspace, C.byref(_delta()), 1, None, match="NULL bytes")
