@@ -170,10 +170,13 @@ __global__ __launch_bounds__(BLOCK ? 1024 : NM_NT) void k_norm_fwd(const ffn_nor
 
 // g = dy w, xhat = (x - mean) rstd:  dx = rstd (g - mean(g) - xhat mean(g xhat)), dw = sum of dy xhat, db = sum of dy.
 // The saved mean is rounded: what the row's x - mean still has as its mean is taken off as well.
-template <typename T, int EL, int P, bool BLOCK>
-__global__ __launch_bounds__(BLOCK ? 1024 : NM_NT) void k_norm_bwd(const ffn_norm a, int team) {
+// BT: threads of a block that takes a row, 0 where a wavefront's team does.  Blocks of 1024 leave a lane 128 registers: the
+// next row then waits for the last one, and the weights are read again for every row.
+template <typename T, int EL, int P, int BT>
+__global__ __launch_bounds__(BT ? BT : NM_NT) void k_norm_bwd(const ffn_norm a, int team) {
   __shared__ float part[16][4];
   constexpr int N = P * EL;
+  constexpr bool BLOCK = BT > 0, AHEAD = BT < 1024;
   const Team t = Team::of<BLOCK>(team);
   const int width = a.width;
   const float inv = 1.f / (float)width;
@@ -191,13 +194,17 @@ __global__ __launch_bounds__(BLOCK ? 1024 : NM_NT) void k_norm_bwd(const ffn_nor
     nmean = a.mean[at];
     nrstd = a.rstd[at];
   };
-  if (trips) fetch(t.first);
+  if (AHEAD && trips) fetch(t.first);
   for (int64_t k = 0; k < trips; ++k) {
     const int64_t row = t.first + k * t.step;
+    if (!AHEAD) {
+      fetch(row);
+      load_params<T, EL, P>(a.weight, a.param_dtype == FFN_F32, 1.f, t.lane, team, width, w);
+    }
     RowPart<T, EL, P> x = nx;
     const RowPart<T, EL, P> y = ny;
     const float mean = nmean, rstd = nrstd;
-    if (k + 1 < trips) fetch(row + t.step);
+    if (AHEAD && k + 1 < trips) fetch(row + t.step);
     float s[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -265,8 +272,15 @@ __global__ __launch_bounds__(NM_NT) void k_norm_join(const float* __restrict__ p
   __shared__ float sums[16][17];
   const int col = threadIdx.x & 15, from = threadIdx.x >> 4, c = blockIdx.x * 16 + col;
   float s = 0.f;
-  if (c < 2 * width)
-    for (int b = from; b < blocks; b += 16) s += part[(int64_t)b * 2 * width + c];
+  if (c < 2 * width) {
+    for (int b = from; b < blocks; b += 128) {
+      float x[8];  // on their way at once
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = b + 16 * i < blocks ? part[(int64_t)(b + 16 * i) * 2 * width + c] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += x[i];
+    }
+  }
   sums[from][col] = s;
   __syncthreads();
   if (from || c >= 2 * width) return;
@@ -321,11 +335,12 @@ void start(const ffn_norm& a, bool backward, const Shape& s, hipStream_t st) {
   const dim3 grid(backward ? grad_blocks(a, s) : (int)std::min<int64_t>(NM_BLOCKS, (a.n + rows - 1) / rows));
   if (s.block) {
     if constexpr (P * EL == NM_BLOCK_COLS) {
-      if (backward) k_norm_bwd<T, EL, P, true><<<grid, s.threads, 0, st>>>(a, s.team);
+      if (backward && s.threads <= 512) k_norm_bwd<T, EL, P, 512><<<grid, s.threads, 0, st>>>(a, s.team);
+      else if (backward) k_norm_bwd<T, EL, P, 1024><<<grid, s.threads, 0, st>>>(a, s.team);
       else k_norm_fwd<T, EL, P, 1, true><<<grid, s.threads, 0, st>>>(a, s.team);
     }
   } else if (backward) {
-    k_norm_bwd<T, EL, P, false><<<grid, s.threads, 0, st>>>(a, s.team);
+    k_norm_bwd<T, EL, P, 0><<<grid, s.threads, 0, st>>>(a, s.team);
   } else {
     // short parts take several rows at once, so that a lane has 64 bytes on their way
     constexpr int U = P * EL * sizeof(T) >= 64 ? 1 : P * EL * sizeof(T) >= 32 ? 2 : 4;

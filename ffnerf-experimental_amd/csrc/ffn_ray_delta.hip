@@ -27,6 +27,7 @@ constexpr int DL_SEG = 2;             // chunks between two states that are kept
 constexpr int DL_MARK = DL_C * DL_SEG;
 constexpr int DL_LD = 20;             // LDS row of a 16 x 16 matrix
 constexpr int DL_VEC = 64;            // a chunk's b, e, D_15 and (first of the last 16) e_15
+constexpr float DL_RESET = -1e30f;    // stands for a decay of -infinity, which must not meet a zero in a product
 constexpr int DL_CLEAR = 1024;        // rows that one block looks through for those of no ray
 
 __device__ __forceinline__ f32x4 mma4(float a, float b, const f32x4& c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
@@ -71,7 +72,7 @@ __device__ __forceinline__ f32x4 sum16(f32x4 x) {
   return x;
 }
 
-// The rows of a ray in the order of the recurrence.
+// the rows of a ray in the order of the recurrence.
 struct Chain {
   int64_t from;  // row of place 0
   int64_t first; // lowest row
@@ -86,40 +87,71 @@ __device__ __forceinline__ Chain chain_of(const ffn_ray_delta& a, int64_t ray) {
 // overlap, never share a slot
 __device__ __forceinline__ int64_t mark_slot(const Chain& ch, int p) { return (ch.first + p) / DL_MARK; }
 
+// Loads go to the last row, or the first columns, where a place is past the ray's end or the columns, and their values are
+// dropped then: under a branch each would wait for the one before it.
+
 // this lane's part of a chunk's rows p0 + c: four values of every 16 columns, 0 past the ray's end or the columns
 template <typename T, int N>
 __device__ __forceinline__ void load_rows(f32x4 (&to)[N], const T* base, int64_t row_stride, const Chain& ch, int p0, int c,
                                           int g, int cols) {
+  typedef T tvec __attribute__((ext_vector_type(4)));
+  const T* p = base + ch.row(min(p0 + c, ch.count - 1)) * row_stride;
   const bool there = p0 + c < ch.count;
-  const T* p = base + (there ? ch.row(p0 + c) : ch.from) * row_stride + 4 * g;
+  tvec x[N];
+#pragma unroll
+  for (int t = 0; t < N; ++t) x[t] = *reinterpret_cast<const tvec*>(p + (16 * t + 4 * g < cols ? 16 * t + 4 * g : 0));
 #pragma unroll
   for (int t = 0; t < N; ++t) {
-    to[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (there && 16 * t + 4 * g < cols) to[t] = load4(p + 16 * t);
+    const f32x4 f = __builtin_convertvector(x[t], f32x4), zero = {0.f, 0.f, 0.f, 0.f};
+    to[t] = there && 16 * t + 4 * g < cols ? f : zero;
   }
 }
 // column `col` of the chunk's rows 4 g + r
 template <typename T>
 __device__ __forceinline__ f32x4 load_col(const T* base, int64_t row_stride, const Chain& ch, int p0, int g, int col, int cols) {
-  f32x4 x;
+  T x[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) x[r] = base[ch.row(min(p0 + 4 * g + r, ch.count - 1)) * row_stride + (col < cols ? col : 0)];
+  f32x4 y;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) y[r] = p0 + 4 * g + r < ch.count && col < cols ? (float)x[r] : 0.f;
+  return y;
+}
+
+// the decays of the chunk's rows 4 g + r and the strength of its row c
+template <typename T>
+__device__ __forceinline__ void load_gates(const ffn_ray_delta& a, int h, const Chain& ch, int p0, int c, int g, f32x4& decay,
+                                           float& beta) {
+  const T *d = (const T*)a.decay + h * a.decay_head, *b = (const T*)a.beta + h * a.beta_head;
+  const T bx = b[ch.row(min(p0 + c, ch.count - 1)) * a.beta_row];
+  T dx[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) dx[r] = d[ch.row(min(p0 + 4 * g + r, ch.count - 1)) * a.decay_row];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    const int p = p0 + 4 * g + r;
-    x[r] = p < ch.count && col < cols ? (float)base[ch.row(p) * row_stride + col] : 0.f;
+    const float x = p0 + 4 * g + r < ch.count ? (float)dx[r] : 0.f;
+    decay[r] = x < DL_RESET ? DL_RESET : x;
   }
-  return x;
+  beta = p0 + c < ch.count ? (float)bx : 0.f;
 }
 
 // A state's 16 columns from `w16` on, in product layout, from or to [dk][dv].
 template <int NT>
 __device__ __forceinline__ void load_state(f32x4 (&S)[NT], const float* from, const ffn_ray_delta& a, int c, int g, int w16) {
 #pragma unroll
+  for (int t = 0; t < NT; ++t) S[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (!from) return;
+  const int v = min(w16 + c, a.val_dim - 1);
+#pragma unroll
   for (int t = 0; t < NT; ++t) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int k = 16 * t + 4 * g + r, v = w16 + c;
-      S[t][r] = from && k < a.key_dim && v < a.val_dim ? from[(int64_t)k * a.val_dim + v] : 0.f;
-    }
+    for (int r = 0; r < 4; ++r) S[t][r] = from[(int64_t)min(16 * t + 4 * g + r, a.key_dim - 1) * a.val_dim + v];
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (16 * t + 4 * g + r >= a.key_dim || w16 + c >= a.val_dim) S[t][r] = 0.f;
   }
 }
 template <int NT>
@@ -134,63 +166,70 @@ __device__ __forceinline__ void store_state(float* to, const f32x4 (&S)[NT], con
   }
 }
 
+// x of lane L of this lane's group of 16
+template <int L> __device__ __forceinline__ float of_lane(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x150 + L, 0xF, 0xF, true));
+}
+
+// exp(x): the product with log2(e) in two parts, so that the result is as accurate as the hardware's 2^x
+__device__ __forceinline__ float exp_of(float x) {
+  const float hi = x * 1.442695041f, lo = __builtin_fmaf(x, 1.442695041f, -hi);
+  const float y = __builtin_amdgcn_exp2f(hi);
+  return __builtin_fmaf(y, lo * 0.6931471806f, y);
+}
+
+// Column c of X with (I + A) X = I: x[J] is done when the rows before it have been taken off.  a[j] = A[c][j].  (By rows of X
+// a NaN in a row of A would meet the zeros of the rows before it.)
+template <int J, int I> __device__ __forceinline__ void take_off_row(const float (&a)[DL_C], float (&x)[DL_C]) {
+  x[I] = __builtin_fmaf(-of_lane<I>(a[J]), x[J], x[I]);
+  if constexpr (I + 1 < DL_C) take_off_row<J, I + 1>(a, x);
+}
+template <int J> __device__ __forceinline__ void take_off(const float (&a)[DL_C], float (&x)[DL_C]) {
+  take_off_row<J, J + 1>(a, x);
+  if constexpr (J + 2 < DL_C) take_off<J + 1>(a, x);
+}
+
 // What a chunk's rows do to each other, by one wavefront: T, P and (if Dm) D as [row i][column j], and the rows' vectors.
-// decay and beta: those of row c.
+// decay: those of rows 4 g + r (at least DL_RESET), beta: that of row c.  Sums of decays are products with zeros and ones.
 template <int NT>
-__device__ __forceinline__ void prepare_chunk(const f32x4 (&kf)[NT], const f32x4 (&qf)[NT], float decay, float beta, float scale,
-                                              int c, int g, float* Tm, float* Pm, float* Dm, float* vec) {
-  const f32x4 kk = dot_tiles(kf, kf), kq = dot_tiles(kf, qf);  // k_j.k_i and k_j.q_i: row j = 4 g + r, column i = c
-  // sums of decays from j + 1 to c, from the start to c, and from c + 1 to the end
-  float run = 0.f, after = 0.f;
-  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+__device__ __forceinline__ void prepare_chunk(const f32x4 (&kf)[NT], const f32x4 (&qf)[NT], const f32x4& decay, float beta,
+                                              float scale, int c, int g, float* Tm, float* Pm, float* Dm, float* vec) {
+  // row j = 4 g + r, column i = c: the sum of decays from j + 1 to i
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int l = DL_C - 1; l > 0; --l) {
-    const float d = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, decay), l));
-    run = l <= c ? run + d : run;
-    after = l > c ? after + d : after;
-    s[(l - 1) & 3] = g == (l - 1) >> 2 ? run : s[(l - 1) & 3];
-  }
-  run += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, decay), 0));
-  f32x4 D, P;
+  for (int s = 0; s < 4; ++s) sum = mma4(4 * g + s > c ? 1.f : 0.f, 4 * g + s <= c ? decay[s] : 0.f, sum);
+  const f32x4 kk = dot_tiles(kf, kf), kq = dot_tiles(kf, qf);
+  f32x4 D, P, A;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int j = 4 * g + r;
-    D[r] = j <= c ? expf(s[r]) : 0.f;
-    P[r] = j <= c ? scale * D[r] * kq[r] : 0.f;
-    Tm[j * DL_LD + c] = j < c ? beta * D[r] * kk[r] : 0.f;  // A^T, until T takes its place
+    const float d = exp_of(sum[r]);
+    D[r] = j <= c ? d : 0.f;
+    P[r] = j <= c ? scale * d * kq[r] : 0.f;
+    A[r] = j < c ? beta * d * kk[r] : 0.f;
   }
+  *reinterpret_cast<f32x4*>(Tm + c * DL_LD + 4 * g) = A;
   *reinterpret_cast<f32x4*>(Pm + c * DL_LD + 4 * g) = P;
   if (Dm) *reinterpret_cast<f32x4*>(Dm + c * DL_LD + 4 * g) = D;
+  const float e = exp_of(decay[0] + sum[0]);  // in the first group, from the chunk's start to row c
   if (g == 0) {
     vec[c] = beta;
-    vec[16 + c] = expf(run);
-    vec[32 + c] = expf(after);
-    if (c == DL_C - 1) vec[48] = expf(run);
+    vec[16 + c] = e;
+    if (c == DL_C - 1) vec[48] = e;
   }
+  if (c == DL_C - 1) *reinterpret_cast<f32x4*>(vec + 32 + 4 * g) = D;
   wave_sync();
-  // column c of T, from the top: row j is done when the rows before it have been taken off
-  float t[DL_C];
+  float a[DL_C], x[DL_C];
 #pragma unroll
-  for (int i = 0; i < DL_C; ++i) t[i] = i == c ? 1.f : 0.f;
-  f32x4 next[DL_C / 4];
+  for (int i = 0; i < DL_C; i += 4) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(Tm + c * DL_LD + i);
 #pragma unroll
-  for (int i4 = 0; i4 < DL_C / 4; ++i4) next[i4] = *reinterpret_cast<const f32x4*>(Tm + 4 * i4);
-#pragma unroll
-  for (int j = 0; j < DL_C - 1; ++j) {
-    f32x4 A[DL_C / 4];
-#pragma unroll
-    for (int i4 = (j + 1) / 4; i4 < DL_C / 4; ++i4) A[i4] = next[i4];
-#pragma unroll
-    for (int i4 = (j + 2) / 4; i4 < DL_C / 4; ++i4) next[i4] = *reinterpret_cast<const f32x4*>(Tm + (j + 1) * DL_LD + 4 * i4);
-    __builtin_amdgcn_sched_barrier(0);  // one row ahead, not all of them
-#pragma unroll
-    for (int i = j + 1; i < DL_C; ++i) t[i] = __builtin_fmaf(-A[i / 4][i % 4], t[j], t[i]);
-    __builtin_amdgcn_sched_barrier(0);
+    for (int r = 0; r < 4; ++r) a[i + r] = v[r], x[i + r] = i + r == c ? 1.f : 0.f;
   }
+  take_off<0>(a, x);
   wave_sync();
 #pragma unroll
-  for (int i = 0; i < DL_C; ++i)
-    if (g == i >> 2) Tm[i * DL_LD + c] = t[i];
+  for (int r = 0; r < 4; ++r) Tm[(4 * g + r) * DL_LD + c] = g == 0 ? x[r] : g == 1 ? x[4 + r] : g == 2 ? x[8 + r] : x[12 + r];
 }
 
 __device__ __forceinline__ bool finite4(const f32x4& x) {
@@ -241,7 +280,8 @@ __global__ __launch_bounds__(512) void k_delta_fwd(const ffn_ray_delta a) {
   }
   const int64_t ray = block / a.v_heads;
   const int h = (int)(block - ray * a.v_heads), hk = h / (a.v_heads / a.heads);
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, W = blockDim.x >> 6, c = lane & 15, g = lane >> 4, w16 = 16 * w;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, W = blockDim.x >> 6, w16 = 16 * w;
+  int c = lane & 15, g = lane >> 4;
   const Chain ch = chain_of(a, ray);
   const T* q = (const T*)a.q + hk * a.q_head;
   const T* k = (const T*)a.k + hk * a.k_head;
@@ -255,13 +295,13 @@ __global__ __launch_bounds__(512) void k_delta_fwd(const ffn_ray_delta a) {
     for (int i = w; i < CH; i += W) {
       const int p = p0 + DL_C * i;
       if (p >= ch.count) break;
+      asm volatile("" : "+v"(c), "+v"(g));  // opaque: else all that goes by the lane alone is formed ahead, and held
       f32x4 kf[NT], qf[NT];
       load_rows(kf, k, a.k_row, ch, p, c, g, a.key_dim);
       load_rows(qf, q, a.q_row, ch, p, c, g, a.key_dim);
-      const bool there = p + c < ch.count;
-      const int64_t row = there ? ch.row(p + c) : ch.from;
-      const float decay = there ? (float)((const T*)a.decay)[row * a.decay_row + h * a.decay_head] : 0.f;
-      const float beta = there ? (float)((const T*)a.beta)[row * a.beta_row + h * a.beta_head] : 0.f;
+      f32x4 decay;
+      float beta;
+      load_gates<T>(a, h, ch, p, c, g, decay, beta);
 #pragma unroll
       for (int t = 0; t < NT; ++t) store4(&Kl[(DL_C * i + c) * LDK + 16 * t + 4 * g], kf[t]);
       prepare_chunk(kf, qf, decay, beta, a.scale, c, g, Tm[i], Pm[i], (float*)nullptr, vec[i]);
@@ -271,6 +311,7 @@ __global__ __launch_bounds__(512) void k_delta_fwd(const ffn_ray_delta a) {
     for (int i = 0; i < CH; ++i) {
       const int p = p0 + DL_C * i;
       if (p >= ch.count) break;
+      asm volatile("" : "+v"(c), "+v"(g));
       if (a.marks && p && p % DL_MARK == 0)
         store_state(a.marks + (mark_slot(ch, p) * a.v_heads + h) * size, S, a, c, g, w16);
       const T* Kc = Kl + DL_C * i * LDK;
@@ -420,7 +461,8 @@ __global__ __launch_bounds__(512) void k_delta_bwd(const ffn_ray_delta a) {
   }
   const int64_t ray = block / a.v_heads;
   const int h = (int)(block - ray * a.v_heads), hk = h / (a.v_heads / a.heads);
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, W = blockDim.x >> 6, c = lane & 15, g = lane >> 4, w16 = 16 * w;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, W = blockDim.x >> 6, w16 = 16 * w;
+  int c = lane & 15, g = lane >> 4;
   const int LDV = 16 * W + 4, vcol = w16 + c;
   float* Tm = lds;
   float* Pm = Tm + DL_SEG * SQ;
@@ -450,13 +492,13 @@ __global__ __launch_bounds__(512) void k_delta_bwd(const ffn_ray_delta a) {
     for (int i = w; i < DL_SEG; i += W) {
       const int p = p0 + DL_C * i;
       if (p >= ch.count) break;
+      asm volatile("" : "+v"(c), "+v"(g));  // opaque: else all that goes by the lane alone is formed ahead, and held
       f32x4 kf[NT], qf[NT];
       load_rows(kf, k, a.k_row, ch, p, c, g, a.key_dim);
       load_rows(qf, q, a.q_row, ch, p, c, g, a.key_dim);
-      const bool there = p + c < ch.count;
-      const int64_t row = there ? ch.row(p + c) : ch.from;
-      const float decay = there ? (float)((const T*)a.decay)[row * a.decay_row + h * a.decay_head] : 0.f;
-      const float beta = there ? (float)((const T*)a.beta)[row * a.beta_row + h * a.beta_head] : 0.f;
+      f32x4 decay;
+      float beta;
+      load_gates<T>(a, h, ch, p, c, g, decay, beta);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         store4(&Kl[(DL_C * i + c) * LDK + 16 * t + 4 * g], kf[t]);
@@ -500,6 +542,7 @@ __global__ __launch_bounds__(512) void k_delta_bwd(const ffn_ray_delta a) {
     for (int i = DL_SEG - 1; i >= 0; --i) {
       const int p = p0 + DL_C * i;
       if (p >= ch.count) continue;
+      asm volatile("" : "+v"(c), "+v"(g));
       const T *Kc = Kl + DL_C * i * LDK, *Qc = Ql + DL_C * i * LDK;
       const float *vec = vecs + i * DL_VEC, *Tc = Tm + i * SQ, *Pc = Pm + i * SQ, *Dc = Dm + i * SQ;
       const f32x4 beta = *reinterpret_cast<const f32x4*>(vec + 4 * g), e = *reinterpret_cast<const f32x4*>(vec + 16 + 4 * g);
