@@ -19,8 +19,8 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["ffn_capi.hip", "ffn_sample.hip", "ffn_hash.hip", "ffn_mlp.hip", "ffn_optim.hip", "ffn_march.hip",
            "ffn_mlp16.hip", "ffn_batch.hip", "ffn_order.hip", "ffn_mlp_fwd.hip", "ffn_ray_attn.hip",
-           "ffn_ray_scan.hip", "ffn_ray_delta.hip", "ffn_experts.hip", "ffn_norm.hip", "ffn_route.hip",
-           "ffn_ray_capi.hip"]
+           "ffn_ray_scan.hip", "ffn_ray_delta_f32.hip", "ffn_ray_delta_f16.hip", "ffn_ray_delta_bf16.hip",
+           "ffn_experts.hip", "ffn_norm.hip", "ffn_route.hip", "ffn_ray_capi.hip"]
 
 FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",

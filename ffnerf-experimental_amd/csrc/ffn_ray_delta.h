@@ -1,0 +1,1043 @@
+// ffn_ray_delta.h -- a matrix state a ray and head, written by the delta rule with decay, and its gradients: the kernels, which
+// ffn_ray_delta_f32.hip, _f16.hip and _bf16.hip make for their types.
+//
+//   S_t = a_t S_{t-1} + k_t n_t^T,  n_t = b_t (v_t - a_t S_{t-1}^T k_t),  a_t = exp(decay_t),  o_t = scale S_t^T q_t
+//
+// In chunks of 16 rows, one matrix tile.  Inside a chunk, with D_ij = exp(decay_{j+1} + .. + decay_i) and e_i the same
+// from the chunk's start, the rows' writes n solve a unit triangular system, and everything else is a matrix product:
+//   A_ij = b_i D_ij k_i.k_j (j < i),  T = (I + A)^-1,  n = T R,  R_i = b_i (v_i - e_i S^T k_i)
+//   P_ij = scale D_ij q_i.k_j (j <= i),  o_i = scale e_i S^T q_i + sum_j P_ij n_j,  S' = e_15 S + sum_j D_15,j k_j n_j^T
+// Marched rays are short: a chunk of 16 wastes less of their last tile than a longer one, and its triangle is solved by
+// substitution (sums of powers of A would cancel where neighbouring keys are alike, as they are along a ray).  Sums of
+// decays are taken anew for every pair, so that neither a reset (decay = -infinity) nor a strong decay before a row costs
+// the pairs after it their accuracy.
+//
+// A block is a ray and head; its wavefronts each hold 16 columns of S, whose columns do not touch each other, in product
+// layout (lane c + 16 g: column c, rows 4 g + r of each 16), which is that of a product's second operand as well.  T and P
+// belong to the rows alone: the wavefronts make those of a segment's chunks side by side and share them through LDS.
+//
+// Products: in float, by the K = 4 instruction.  Of bfloat16 inputs the rows are exact operands of the 16-bit instruction,
+// and what they meet (S, n, dS: float) goes as three bfloat16 parts, which together are the float itself: three products
+// at 16 times the rate (K = 32; 8 times at K = 16), to the same accuracy.
+#pragma once
+#include <algorithm>
+
+#include "ffn_ray_common.h"
+#include "ffn_ray_kernels.h"
+
+namespace ffn {
+
+constexpr int DL_C = 16;              // rows of a chunk
+constexpr int DL_SEG = 2;             // chunks between two states that are kept for the backward pass
+constexpr int DL_MARK = DL_C * DL_SEG;
+constexpr int DL_LD = 20;             // LDS row of a 16 x 16 matrix
+constexpr int DL_VEC = 64;            // a chunk's b, e, D_15 and (first of the last 16) e_15
+constexpr float DL_RESET = -1e30f;    // stands for a decay of -infinity, which must not meet a zero in a product
+constexpr int DL_CLEAR = 1024;        // rows that one block looks through for those of no ray
+
+// ---------------------------------------------------------------------------
+// products
+
+__device__ __forceinline__ f32x4 mma4(float a, float b, const f32x4& c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma16(const b16x4& a, const b16x4& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma32(const b16x4& a0, const b16x4& a1, const b16x4& b0, const b16x4& b1, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7),
+                                                 __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7), c, 0, 0, 0);
+}
+// A b for a 16 x 16 A, this lane's four values of its row c and columns 4 g + s, on a product
+__device__ __forceinline__ f32x4 mul16(const f32x4& a, const f32x4& b, f32x4 to) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s) to = mma4(a[s], b[s], to);
+  return to;
+}
+
+// Four floats as N bfloat16 parts by cutting: 8 bits of the 24 each, so that three are the float itself and two are off by
+// 2^-16 of it.
+template <int N> struct Parts {
+  b16x4 p[N];
+};
+template <int N> __device__ __forceinline__ Parts<N> parts_of(f32x4 x) {
+  Parts<N> y;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    const u32x4 w = __builtin_bit_cast(u32x4, x);
+    const u32x2 up = {__builtin_amdgcn_perm(w[1], w[0], 0x07060302u), __builtin_amdgcn_perm(w[3], w[2], 0x07060302u)};
+    y.p[i] = __builtin_bit_cast(b16x4, up);
+    if (i + 1 < N) x = x - __builtin_bit_cast(f32x4, w & 0xFFFF0000u);
+  }
+  return y;
+}
+
+// How a type's rows enter products.  Row: four neighbouring values of a row.  Two: a float operand where the result is
+// rounded to the type (bfloat16: two parts).
+template <typename T> struct Delta {
+  static constexpr bool EXACT = false;
+  typedef f32x4 Row;
+  typedef f32x4 Full;
+  typedef f32x4 Two;
+  static __device__ __forceinline__ Full full(const f32x4& x) { return x; }
+  static __device__ __forceinline__ Two two(const f32x4& x) { return x; }
+  static __device__ __forceinline__ Row row(const f32x4& x) { return x; }
+  static __device__ __forceinline__ f32x4 value(const Row& x) { return x; }
+  // on a product: 16 values of K from each operand's lane parts, then 32
+  template <typename A, typename B> static __device__ __forceinline__ f32x4 mul(const A& a, const B& b, const f32x4& c) { return mul16(a, b, c); }
+  template <typename A, typename B>
+  static __device__ __forceinline__ f32x4 mul(const A& a0, const A& a1, const B& b0, const B& b1, const f32x4& c) {
+    return mul16(a1, b1, mul16(a0, b0, c));
+  }
+};
+template <> struct Delta<__bf16> {
+  static constexpr bool EXACT = true;
+  typedef b16x4 Row;
+  typedef Parts<3> Full;
+  typedef Parts<2> Two;
+  static __device__ __forceinline__ Full full(const f32x4& x) { return parts_of<3>(x); }
+  static __device__ __forceinline__ Two two(const f32x4& x) { return parts_of<2>(x); }
+  static __device__ __forceinline__ f32x4 value(const Row& x) { return __builtin_convertvector(x, f32x4); }
+  static __device__ __forceinline__ f32x4 mul(const Row& a, const Row& b, const f32x4& c) { return mma16(a, b, c); }
+  template <int N> static __device__ __forceinline__ f32x4 mul(const Row& a, const Parts<N>& b, f32x4 c) {
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i) c = mma16(a, b.p[i], c);
+    return c;
+  }
+  template <int N> static __device__ __forceinline__ f32x4 mul(const Parts<N>& a, const Row& b, f32x4 c) {
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i) c = mma16(a.p[i], b, c);
+    return c;
+  }
+  static __device__ __forceinline__ f32x4 mul(const Two& a, const Two& b, const f32x4& c) {
+    return mma16(a.p[0], b.p[0], mma16(a.p[0], b.p[1], mma16(a.p[1], b.p[0], c)));
+  }
+  static __device__ __forceinline__ f32x4 mul(const Row& a0, const Row& a1, const Row& b0, const Row& b1, const f32x4& c) {
+    return mma32(a0, a1, b0, b1, c);
+  }
+  template <int N>
+  static __device__ __forceinline__ f32x4 mul(const Row& a0, const Row& a1, const Parts<N>& b0, const Parts<N>& b1, f32x4 c) {
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i) c = mma32(a0, a1, b0.p[i], b1.p[i], c);
+    return c;
+  }
+  template <int N>
+  static __device__ __forceinline__ f32x4 mul(const Parts<N>& a0, const Parts<N>& a1, const Row& b0, const Row& b1, f32x4 c) {
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i) c = mma32(a0.p[i], a1.p[i], b0, b1, c);
+    return c;
+  }
+  static __device__ __forceinline__ f32x4 mul(const Two& a0, const Two& a1, const Two& b0, const Two& b1, const f32x4& c) {
+    return mma32(a0.p[0], a1.p[0], b0.p[0], b1.p[0],
+                 mma32(a0.p[0], a1.p[0], b0.p[1], b1.p[1], mma32(a0.p[1], a1.p[1], b0.p[0], b1.p[0], c)));
+  }
+};
+
+// sum over the tiles of a and b, an even number
+template <typename T, int N, typename A, typename B>
+__device__ __forceinline__ f32x4 mul_tiles(const A (&a)[N], const B (&b)[N], f32x4 c) {
+  if constexpr (Delta<T>::EXACT) {
+#pragma unroll
+    for (int t = 0; t < N; t += 2) c = Delta<T>::mul(a[t], a[t + 1], b[t], b[t + 1], c);
+    return c;
+  } else {
+    f32x4 d = {0.f, 0.f, 0.f, 0.f};  // two chains
+#pragma unroll
+    for (int t = 0; t < N; t += 2) {
+      c = Delta<T>::mul(a[t], b[t], c);
+      d = Delta<T>::mul(a[t + 1], b[t + 1], d);
+    }
+    return c + d;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// rows and states
+
+template <typename T> __device__ __forceinline__ f32x4 load4(const T* p) {
+  typedef T tvec __attribute__((ext_vector_type(4)));
+  return __builtin_convertvector(*reinterpret_cast<const tvec*>(p), f32x4);
+}
+template <typename T> __device__ __forceinline__ void store4(T* p, const f32x4& x) {
+  typedef T tvec __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<tvec*>(p) = __builtin_convertvector(x, tvec);
+}
+// four values of an LDS row as a product's operand
+template <typename T> __device__ __forceinline__ typename Delta<T>::Row row_of(const T* p) {
+  if constexpr (Delta<T>::EXACT) return *reinterpret_cast<const b16x4*>(p);
+  else return load4(p);
+}
+// column c of the rows 4 g .. 4 g + 3 from `tile` on, LD apart: the transposed operand
+template <typename T, int LD> __device__ __forceinline__ typename Delta<T>::Row col_of(const T* tile, int c, int g) {
+  if constexpr (Delta<T>::EXACT) {
+    typedef __attribute__((address_space(3))) s16x4* lds_quad;
+    return __builtin_bit_cast(b16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad)(tile + (4 * g + (c >> 2)) * LD + 4 * (c & 3))));
+  } else {
+    f32x4 x;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) x[s] = (float)tile[(4 * g + s) * LD + c];
+    return x;
+  }
+}
+
+// sum over the 16 lanes of a group
+__device__ __forceinline__ f32x4 sum16(f32x4 x) {
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] += __shfl_xor(x[r], d);
+  }
+  return x;
+}
+
+// The rows of a ray in the order of the recurrence.
+struct Chain {
+  int64_t first;  // lowest row
+  int count;
+  bool back;
+};
+__device__ __forceinline__ Chain chain_of(const ffn_ray_delta& a, int64_t ray) {
+  const int64_t n = a.rays.n, o = min((int64_t)a.rays.offsets[ray], n), c = min((int64_t)a.rays.counts[ray], n - o);
+  return {o, (int)c, a.reverse != 0};
+}
+// where the state before place p (a multiple of DL_MARK above 0) is kept: places of one ray, and of rays that do not
+// overlap, never share a slot
+__device__ __forceinline__ int64_t mark_slot(const Chain& ch, int p) { return (ch.first + p) / DL_MARK; }
+
+// The rows of the chunk at place p0: `many` of them from row `low` on.  Place i's row is low + at(i); past the ray's end it
+// is that of the last place, whose values are then dropped: under a branch each load would wait for the one before it.
+struct Chunk {
+  int64_t low;
+  int many;
+  bool back;
+  __device__ __forceinline__ Chunk(const Chain& ch, int p0)
+      : low(0), many(min(DL_C, ch.count - p0)), back(ch.back) {
+    low = back ? ch.first + ch.count - p0 - many : ch.first + p0;
+  }
+  __device__ __forceinline__ uint32_t at(int i) const {
+    const int j = min(i, many - 1);
+    return back ? many - 1 - j : j;
+  }
+};
+
+// element `at` rows on from the row at p, rows `stride` < 2^27 bytes apart
+template <typename T> __device__ __forceinline__ const T* row_ptr(const T* p, uint32_t at, int64_t stride) {
+  return reinterpret_cast<const T*>(reinterpret_cast<const char*>(p) + at * (uint32_t)(stride * (int64_t)sizeof(T)));
+}
+
+// this lane's part of a chunk's row c: four values of every 16 columns, as they lie in memory
+template <typename T, int N> struct RawRow {
+  typedef T tvec __attribute__((ext_vector_type(4)));
+  tvec v[N];
+  __device__ __forceinline__ void load(const T* base, int64_t stride, const Chunk& ck, int c, int g, int cols) {
+    const T* p = row_ptr(base + ck.low * stride, ck.at(c), stride);
+    if (cols == 16 * N) {
+#pragma unroll
+      for (int t = 0; t < N; ++t) v[t] = *reinterpret_cast<const tvec*>(p + 16 * t + 4 * g);
+    } else {
+#pragma unroll
+      for (int t = 0; t < N; ++t) v[t] = *reinterpret_cast<const tvec*>(p + (16 * t + 4 * g < cols ? 16 * t + 4 * g : 0));
+    }
+  }
+  // 0 past the ray's end or the columns
+  __device__ __forceinline__ void trim(const Chunk& ck, int c, int g, int cols) {
+    if (ck.many == DL_C && cols == 16 * N) return;
+#pragma unroll
+    for (int t = 0; t < N; ++t) v[t] = c < ck.many && 16 * t + 4 * g < cols ? v[t] : tvec{};
+  }
+  __device__ __forceinline__ void operands(typename Delta<T>::Row (&to)[N]) const {
+#pragma unroll
+    for (int t = 0; t < N; ++t) {
+      if constexpr (Delta<T>::EXACT) to[t] = v[t];
+      else to[t] = __builtin_convertvector(v[t], f32x4);
+    }
+  }
+};
+// column `col` of the chunk's rows 4 g + r
+template <typename T> struct RawCol {
+  T v[4];
+  __device__ __forceinline__ void load(const T* base, int64_t stride, const Chunk& ck, int g, int col, int cols) {
+    const T* p = base + ck.low * stride + (col < cols ? col : 0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = *row_ptr(p, ck.at(4 * g + r), stride);
+  }
+  __device__ __forceinline__ f32x4 value(const Chunk& ck, int g, int col, int cols) const {
+    f32x4 x;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = (float)v[r];
+    if (ck.many < DL_C || cols % 16) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = 4 * g + r < ck.many && col < cols ? x[r] : 0.f;
+    }
+    return x;
+  }
+};
+// the decays of the chunk's rows 4 g + r and the strength of its row c
+template <typename T> struct RawGates {
+  T d[4], b;
+  __device__ __forceinline__ void load(const ffn_ray_delta& a, int h, const Chunk& ck, int c, int g) {
+    const T *dp = (const T*)a.decay + ck.low * a.decay_row + h * a.decay_head, *bp = (const T*)a.beta + ck.low * a.beta_row + h * a.beta_head;
+    b = *row_ptr(bp, ck.at(c), a.beta_row);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) d[r] = *row_ptr(dp, ck.at(4 * g + r), a.decay_row);
+  }
+  __device__ __forceinline__ f32x4 decay(const Chunk& ck, int g) const {
+    f32x4 y;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float x = 4 * g + r < ck.many ? (float)d[r] : 0.f;
+      y[r] = x < DL_RESET ? DL_RESET : x;
+    }
+    return y;
+  }
+  __device__ __forceinline__ float beta(const Chunk& ck, int c) const { return c < ck.many ? (float)b : 0.f; }
+};
+
+// A state's 16 columns from `w16` on, in product layout, from or to [dk][dv].
+template <int NT>
+__device__ __forceinline__ void load_state(f32x4 (&S)[NT], const float* from, const ffn_ray_delta& a, int c, int g, int w16) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t) S[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (!from) return;
+  const int v = min(w16 + c, a.val_dim - 1);
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) S[t][r] = from[(int64_t)min(16 * t + 4 * g + r, a.key_dim - 1) * a.val_dim + v];
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (16 * t + 4 * g + r >= a.key_dim || w16 + c >= a.val_dim) S[t][r] = 0.f;
+  }
+}
+template <int NT>
+__device__ __forceinline__ void store_state(float* to, const f32x4 (&S)[NT], const ffn_ray_delta& a, int c, int g, int w16) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int k = 16 * t + 4 * g + r, v = w16 + c;
+      if (k < a.key_dim && v < a.val_dim) to[(int64_t)k * a.val_dim + v] = S[t][r];
+    }
+  }
+}
+
+// exp(x): the product with log2(e) in two parts, so that the result is as accurate as the hardware's 2^x
+__device__ __forceinline__ float exp_of(float x) {
+  const float hi = x * 1.442695041f, lo = __builtin_fmaf(x, 1.442695041f, -hi);
+  const float y = __builtin_amdgcn_exp2f(hi);
+  return __builtin_fmaf(y, lo * 0.6931471806f, y);
+}
+
+// x[I] += a of lane I of this lane's 16, times x[J], for all I > J in a row of instructions.  The two waits are for the
+// lanes' values of a, which a vector instruction may just have written.
+#define DL_TAKE(I) "v_fmac_f32_dpp %" #I ", %16, %17 row_newbcast:" #I " row_mask:0xf bank_mask:0xf\n"
+template <int J> __device__ __forceinline__ void take_off(float a, float (&x)[DL_C]) {
+  const float y = x[J];
+#define DL_X "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]), "+v"(x[6]), "+v"(x[7]), "+v"(x[8]), \
+    "+v"(x[9]), "+v"(x[10]), "+v"(x[11]), "+v"(x[12]), "+v"(x[13]), "+v"(x[14]), "+v"(x[15])
+#define DL_STEP(N, CODE) \
+  if constexpr (J == N) asm("s_nop 1\n" CODE : DL_X : "v"(a), "v"(y));
+  DL_STEP(14, DL_TAKE(15))
+  DL_STEP(13, DL_TAKE(14) DL_TAKE(15))
+  DL_STEP(12, DL_TAKE(13) DL_TAKE(14) DL_TAKE(15))
+  DL_STEP(11, DL_TAKE(12) DL_TAKE(13) DL_TAKE(14) DL_TAKE(15))
+#define DL_12 DL_TAKE(12) DL_TAKE(13) DL_TAKE(14) DL_TAKE(15)
+  DL_STEP(10, DL_TAKE(11) DL_12)
+  DL_STEP(9, DL_TAKE(10) DL_TAKE(11) DL_12)
+  DL_STEP(8, DL_TAKE(9) DL_TAKE(10) DL_TAKE(11) DL_12)
+#define DL_8 DL_TAKE(8) DL_TAKE(9) DL_TAKE(10) DL_TAKE(11) DL_12
+  DL_STEP(7, DL_8)
+  DL_STEP(6, DL_TAKE(7) DL_8)
+  DL_STEP(5, DL_TAKE(6) DL_TAKE(7) DL_8)
+  DL_STEP(4, DL_TAKE(5) DL_TAKE(6) DL_TAKE(7) DL_8)
+#define DL_4 DL_TAKE(4) DL_TAKE(5) DL_TAKE(6) DL_TAKE(7) DL_8
+  DL_STEP(3, DL_4)
+  DL_STEP(2, DL_TAKE(3) DL_4)
+  DL_STEP(1, DL_TAKE(2) DL_TAKE(3) DL_4)
+  DL_STEP(0, DL_TAKE(1) DL_TAKE(2) DL_TAKE(3) DL_4)
+#undef DL_TAKE
+#undef DL_X
+#undef DL_STEP
+#undef DL_12
+#undef DL_8
+#undef DL_4
+}
+// Column c of X with (I + A) X = I: x[J] is done when the rows before it have been taken off.  a[j] = -A[c][j].  (By rows of
+// X a NaN in a row of A would meet the zeros of the rows before it.)
+template <int J> __device__ __forceinline__ void solve(const float (&a)[DL_C], float (&x)[DL_C]) {
+  take_off<J>(a[J], x);
+  if constexpr (J + 2 < DL_C) solve<J + 1>(a, x);
+}
+
+// What a chunk's rows do to each other, by one wavefront: T, P and (if Dm) D as [row i][column j], and the rows' vectors.
+// decay: those of rows 4 g + r (at least DL_RESET), beta: that of row c.  Sums of decays are products with zeros and ones.
+template <typename T, int NT>
+__device__ __forceinline__ void prepare_chunk(const typename Delta<T>::Row (&kf)[NT], const typename Delta<T>::Row (&qf)[NT],
+                                              const f32x4& decay, float beta, float scale, int c, int g, float* Tm, float* Pm,
+                                              float* Dm, float* vec) {
+  // row j = 4 g + r, column i = c: the sum of decays from j + 1 to i, k_j.k_i and k_j.q_i
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  f32x4 sum = zero;
+#pragma unroll
+  for (int s = 0; s < 4; ++s) sum = mma4(4 * g + s > c ? 1.f : 0.f, 4 * g + s <= c ? decay[s] : 0.f, sum);
+  const f32x4 kk = mul_tiles<T>(kf, kf, zero), kq = mul_tiles<T>(kf, qf, zero);
+  f32x4 D, P, A;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int j = 4 * g + r;
+    const float d = exp_of(sum[r]);
+    D[r] = j <= c ? d : 0.f;
+    P[r] = j <= c ? scale * d * kq[r] : 0.f;
+    A[r] = j < c ? -beta * d * kk[r] : 0.f;
+  }
+  *reinterpret_cast<f32x4*>(Tm + c * DL_LD + 4 * g) = A;
+  *reinterpret_cast<f32x4*>(Pm + c * DL_LD + 4 * g) = P;
+  if (Dm) *reinterpret_cast<f32x4*>(Dm + c * DL_LD + 4 * g) = D;
+  const float e = exp_of(decay[0] + sum[0]);  // in the first group, from the chunk's start to row c
+  if (g == 0) {
+    vec[c] = beta;
+    vec[16 + c] = e;
+    if (c == DL_C - 1) vec[48] = e;
+  }
+  if (c == DL_C - 1) *reinterpret_cast<f32x4*>(vec + 32 + 4 * g) = D;
+  wave_sync();
+  float a[DL_C], x[DL_C];
+#pragma unroll
+  for (int i = 0; i < DL_C; i += 4) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(Tm + c * DL_LD + i);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) a[i + r] = v[r], x[i + r] = i + r == c ? 1.f : 0.f;
+  }
+  solve<0>(a, x);
+  wave_sync();
+#pragma unroll
+  for (int r = 0; r < 4; ++r) Tm[(4 * g + r) * DL_LD + c] = g == 0 ? x[r] : g == 1 ? x[4 + r] : g == 2 ? x[8 + r] : x[12 + r];
+}
+
+__device__ __forceinline__ bool finite4(const f32x4& x) {
+  return fabsf(x[0]) <= 3.4e38f && fabsf(x[1]) <= 3.4e38f && fabsf(x[2]) <= 3.4e38f && fabsf(x[3]) <= 3.4e38f;
+}
+// A x for a lower triangular A where x holds infinities or NaN: they must not meet the zeros above the diagonal, so they
+// are left out, and the rows from the first of them on are NaN.
+__device__ __forceinline__ f32x4 mul16_sick(const f32x4& A, f32x4 x, const f32x4& to, int g) {
+  int first = DL_C;
+#pragma unroll
+  for (int r = 3; r >= 0; --r) {
+    if (!(fabsf(x[r]) <= 3.4e38f)) {
+      first = 4 * g + r;
+      x[r] = 0.f;
+    }
+  }
+  first = min(first, __shfl_xor(first, 16));
+  first = min(first, __shfl_xor(first, 32));
+  f32x4 y = mul16(A, x, to);
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (4 * g + r >= first) y[r] = __builtin_nanf("");
+  return y;
+}
+
+// rows of no ray: 0 in `heads` x `cols` of each output
+template <typename T>
+__device__ __forceinline__ void clear_rows(const ffn_ray_delta& a, int64_t block, T* p, int64_t width) {
+  for (int64_t i = block * DL_CLEAR + threadIdx.x; i < min((block + 1) * DL_CLEAR, (int64_t)a.rays.n); i += blockDim.x) {
+    const uint32_t r = a.rays.ray_ids[i];
+    if (r < a.rays.num_rays) {
+      const int64_t o = a.rays.offsets[r];
+      if (i >= o && i - o < (int64_t)a.rays.counts[r]) continue;
+    }
+    for (int64_t j = 0; j < width; ++j) p[i * width + j] = (T)0.f;
+  }
+}
+
+// a / b of a block's number: both fit 32 bits in nearly every call
+__device__ __forceinline__ int64_t quotient(int64_t a, int b) {
+  return a >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+
+template <typename T, int DK, int W>
+__global__ __launch_bounds__(64 * W) void k_delta_fwd(const ffn_ray_delta a) {
+  constexpr int NT = DK / 16, LDK = DK + 16 / (int)sizeof(T), CH = W < 4 ? W : 4;
+  typedef Delta<T> Ops;
+  typedef typename Ops::Row Row;
+  __shared__ float Tm[CH][DL_C * DL_LD], Pm[CH][DL_C * DL_LD], vec[CH][DL_VEC];
+  __shared__ __align__(16) T Kl[CH * DL_C * LDK], Ql[CH * DL_C * LDK];
+  const int64_t block = block_number(), teams = (int64_t)a.rays.num_rays * a.v_heads;
+  if (block >= teams) {
+    clear_rows(a, block - teams, (T*)a.o, (int64_t)a.v_heads * a.val_dim);
+    return;
+  }
+  const int64_t ray = quotient(block, a.v_heads);
+  const int h = (int)(block - ray * a.v_heads), hk = h / (a.v_heads / a.heads);
+  const Chain ch = chain_of(a, ray);
+  const int lane = threadIdx.x & 63, w = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w16 = 16 * w;
+  int c = lane & 15, g = lane >> 4;
+  const T* q = (const T*)a.q + hk * a.q_head;
+  const T* k = (const T*)a.k + hk * a.k_head;
+  const T* v = (const T*)a.v + h * a.v_head;
+  const int64_t size = (int64_t)a.key_dim * a.val_dim;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  // the next segment's rows are on their way while a segment is worked on
+  RawRow<T, NT> kr, qr;
+  RawGates<T> gates;
+  const auto fetch = [&](int p) {
+    if (w < CH && p < ch.count) {
+      const Chunk ck(ch, p);
+      kr.load(k, a.k_row, ck, c, g, a.key_dim);
+      qr.load(q, a.q_row, ck, c, g, a.key_dim);
+      gates.load(a, h, ck, c, g);
+    }
+  };
+  fetch(DL_C * w);
+  f32x4 S[NT];
+  load_state(S, a.h0 ? a.h0 + block * size : nullptr, a, c, g, w16);
+#pragma unroll 1
+  for (int p0 = 0; p0 < ch.count; p0 += CH * DL_C) {
+    asm volatile("" : "+v"(c), "+v"(g));  // opaque: else all that goes by the lane alone is formed ahead, and held
+    RawCol<T> vr[CH];
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+      if (p0 + DL_C * i < ch.count) vr[i].load(v, a.v_row, Chunk(ch, p0 + DL_C * i), g, w16 + c, a.val_dim);
+    if (w < CH && p0 + DL_C * w < ch.count) {
+      const Chunk ck(ch, p0 + DL_C * w);
+      kr.trim(ck, c, g, a.key_dim);
+      qr.trim(ck, c, g, a.key_dim);
+      Row kf[NT], qf[NT];
+      kr.operands(kf);
+      qr.operands(qf);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        typedef typename RawRow<T, NT>::tvec tvec;
+        *reinterpret_cast<tvec*>(&Kl[(DL_C * w + c) * LDK + 16 * t + 4 * g]) = kr.v[t];
+        *reinterpret_cast<tvec*>(&Ql[(DL_C * w + c) * LDK + 16 * t + 4 * g]) = qr.v[t];
+      }
+      prepare_chunk<T>(kf, qf, gates.decay(ck, g), gates.beta(ck, c), a.scale, c, g, Tm[w], Pm[w], (float*)nullptr, vec[w]);
+      fetch(p0 + DL_C * (CH + w));
+    }
+    if constexpr (W > 1) __syncthreads();
+    else wave_sync();
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int p = p0 + DL_C * i;
+      if (p < ch.count) {
+        const Chunk ck(ch, p);
+        if (a.marks && p && p % DL_MARK == 0) store_state(a.marks + (mark_slot(ch, p) * a.v_heads + h) * size, S, a, c, g, w16);
+        const T *Kc = Kl + DL_C * i * LDK, *Qc = Ql + DL_C * i * LDK;
+        Row kf[NT], qf[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          kf[t] = row_of(Kc + c * LDK + 16 * t + 4 * g);
+          qf[t] = row_of(Qc + c * LDK + 16 * t + 4 * g);
+        }
+        const f32x4 beta = *reinterpret_cast<const f32x4*>(&vec[i][4 * g]);
+        const f32x4 e = *reinterpret_cast<const f32x4*>(&vec[i][16 + 4 * g]);
+        const f32x4 left = *reinterpret_cast<const f32x4*>(&vec[i][32 + 4 * g]);
+        const float all = vec[i][48];
+        const f32x4 Tr = *reinterpret_cast<const f32x4*>(&Tm[i][c * DL_LD + 4 * g]);
+        const f32x4 Pr = *reinterpret_cast<const f32x4*>(&Pm[i][c * DL_LD + 4 * g]);
+        typename Ops::Full full[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) full[t] = Ops::full(S[t]);
+        const f32x4 R = beta * (vr[i].value(ck, g, w16 + c, a.val_dim) - e * mul_tiles<T>(kf, full, zero));
+        const f32x4 qs = a.scale * e * mul_tiles<T>(qf, full, zero);
+        f32x4 n = mul16(Tr, R, zero), y;
+        if (__any(!finite4(n))) {
+          n = mul16_sick(Tr, R, zero, g);
+          y = mul16_sick(Pr, n, qs, g);
+        } else {
+          y = mul16(Pr, n, qs);
+        }
+        T* o = (T*)a.o + (ck.low * a.v_heads + h) * a.val_dim;
+        const int64_t stride = (int64_t)a.v_heads * a.val_dim;
+        if (w16 + c < a.val_dim) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (4 * g + r < ck.many) *const_cast<T*>(row_ptr(o + w16 + c, ck.at(4 * g + r), stride)) = (T)y[r];
+        }
+        const typename Ops::Full nl = Ops::full(left * n);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) S[t] = Ops::mul(col_of<T, LDK>(Kc + 16 * t, c, g), nl, all * S[t]);
+      }
+    }
+    if constexpr (W > 1) __syncthreads();
+    else wave_sync();
+  }
+  if (a.last) store_state(a.last + block * size, S, a, c, g, w16);
+}
+
+// Few rows a ray (one more sample of each): the state goes through once, row by row on the vector ALU, and memory bounds
+// it.  A wavefront takes 32 columns of a state: 8 lanes of four columns, 8 groups of rows dk = 8 i + group.
+template <typename T, int DK>
+__global__ __launch_bounds__(256) void k_delta_step(const ffn_ray_delta a) {
+  constexpr int N = DK / 8;
+  const int parts = (a.val_dim + 31) / 32;
+  const int64_t teams = (int64_t)a.rays.num_rays * a.v_heads * parts, blocks = (teams + 3) / 4;
+  if (block_number() >= blocks) {
+    clear_rows(a, block_number() - blocks, (T*)a.o, (int64_t)a.v_heads * a.val_dim);
+    return;
+  }
+  const int64_t team = block_number() * 4 + (threadIdx.x >> 6);
+  if (team >= teams) return;
+  const int64_t state = quotient(team, parts), ray = quotient(state, a.v_heads);
+  const int h = (int)(state - ray * a.v_heads), hk = h / (a.v_heads / a.heads);
+  const int lane = threadIdx.x & 63, rg = lane >> 3, col = (int)(team - state * parts) * 32 + 4 * (lane & 7);
+  const bool in = col < a.val_dim;
+  const Chain ch = chain_of(a, ray);
+  const int64_t at = state * a.key_dim * a.val_dim;
+  f32x4 S[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int kd = 8 * i + rg;
+    S[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (a.h0 && in && kd < a.key_dim) S[i] = load4(a.h0 + at + (int64_t)kd * a.val_dim + col);
+  }
+  for (int p = 0; p < ch.count; ++p) {
+    const int64_t row = ch.back ? ch.first + ch.count - 1 - p : ch.first + p;
+    const T* q = (const T*)a.q + row * a.q_row + hk * a.q_head;
+    const T* k = (const T*)a.k + row * a.k_row + hk * a.k_head;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (in) v = load4((const T*)a.v + row * a.v_row + h * a.v_head + col);
+    const float decay = expf((float)((const T*)a.decay)[row * a.decay_row + h * a.decay_head]);
+    const float beta = (float)((const T*)a.beta)[row * a.beta_row + h * a.beta_head];
+    float kk[N], qq[N], qk = 0.f;
+    f32x4 ks = {0.f, 0.f, 0.f, 0.f}, qs = ks;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int kd = 8 * i + rg;
+      kk[i] = kd < a.key_dim ? (float)k[kd] : 0.f;
+      qq[i] = kd < a.key_dim ? (float)q[kd] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      S[i] = decay * S[i];
+      qk = __builtin_fmaf(qq[i], kk[i], qk);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        ks[e] = __builtin_fmaf(kk[i], S[i][e], ks[e]);
+        qs[e] = __builtin_fmaf(qq[i], S[i][e], qs[e]);
+      }
+    }
+#pragma unroll
+    for (int d = 8; d < 64; d *= 2) {
+      qk += __shfl_xor(qk, d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        ks[e] += __shfl_xor(ks[e], d);
+        qs[e] += __shfl_xor(qs[e], d);
+      }
+    }
+    const f32x4 n = beta * (v - ks);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[i][e] = __builtin_fmaf(kk[i], n[e], S[i][e]);
+    }
+    if (rg == 0 && in) store4((T*)a.o + (row * a.v_heads + h) * a.val_dim + col, a.scale * (qs + qk * n));
+  }
+  if (!a.last) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int kd = 8 * i + rg;
+    if (in && kd < a.key_dim) store4(a.last + at + (int64_t)kd * a.val_dim + col, S[i]);
+  }
+}
+
+// The backward pass.  Segments of two chunks from the ray's end, each from the state that the forward kept: its chunks'
+// states and writes again, then the chunks back to front.  With dS the gradient of the state after a chunk:
+//   dn = P^T do + D_15 K dS,  dR = T^T dn,  dv = b dR,  X = D (do n^T) (j <= i),  Y = -D (dR n^T) (j < i)
+//   dq_i = scale (e_i S do_i + sum_j X_ij k_j),  left_i = -e_i S dR_i + sum_j Y_ij k_j
+//   right_j = D_15,j dS n_j + sum_i (scale X_ij q_i + b_i Y_ij k_i),  dk = b left + right,  db_i = k_i.left_i + v_i.dR_i
+//   dS' = e_15 dS + sum_i (scale e_i q_i do_i^T - b_i e_i k_i dR_i^T)
+// Every factor e or D a row i was multiplied with gives its sum of products to the decays up to i:
+//   ddecay = sums, from each row to the chunk's end, of q.dq + b k.left - k.right, and at the end dS.S
+// dn, dR, dv and dS go by columns, as S does; dq and dk are sums over the columns: S, dS, n and dR pass through LDS, and a
+// wavefront takes 16 columns of dq and dk.
+
+// An LDS array of float rows as operands of products whose result is rounded to the type: floats, or two parts each.
+template <typename T, int LD> struct Plane {
+  static constexpr int WORDS = 1;  // a value's four bytes
+  float* p;
+  __device__ __forceinline__ void set(int row, int col, float x) {
+    if constexpr (Delta<T>::EXACT) {
+      __bf16* q = (__bf16*)p;
+      const uint32_t w = __builtin_bit_cast(uint32_t, x);
+      q[row * 2 * LD + col] = __builtin_bit_cast(__bf16, (uint16_t)(w >> 16));
+      const float rest = x - __builtin_bit_cast(float, w & 0xFFFF0000u);
+      q[row * 2 * LD + LD + col] = __builtin_bit_cast(__bf16, (uint16_t)(__builtin_bit_cast(uint32_t, rest) >> 16));
+    } else {
+      p[row * LD + col] = x;
+    }
+  }
+  __device__ __forceinline__ typename Delta<T>::Two get(int row, int col) const {
+    if constexpr (Delta<T>::EXACT) {
+      const __bf16* q = (const __bf16*)p + row * 2 * LD + col;
+      return {{*reinterpret_cast<const b16x4*>(q), *reinterpret_cast<const b16x4*>(q + LD)}};
+    } else {
+      return *reinterpret_cast<const f32x4*>(p + row * LD + col);
+    }
+  }
+};
+
+// sum over the W tiles of 16 columns of the operands that a and b give for a column
+template <typename T, int W, typename A, typename B>
+__device__ __forceinline__ f32x4 mul_cols(A a, B b, f32x4 c) {
+#pragma unroll
+  for (int u = 0; u + 1 < W; u += 2) c = Delta<T>::mul(a(16 * u), a(16 * u + 16), b(16 * u), b(16 * u + 16), c);
+  // the last odd one in sums of its own: a product of K = 16 right behind one of K = 32 on the same sums gave wrong results
+  if constexpr (W % 2) c = c + Delta<T>::mul(a(16 * W - 16), b(16 * W - 16), f32x4{0.f, 0.f, 0.f, 0.f});
+  return c;
+}
+
+template <typename T, int DK, int W> struct DeltaLds {
+  static constexpr int LDV = 16 * W + (Delta<T>::EXACT ? 8 : 4), LDK = DK + 16 / (int)sizeof(T), SQ = DL_C * DL_LD;
+  static constexpr int WORDS = DL_SEG * (3 * SQ + DL_VEC) + 2 * SQ + (2 * DL_C + DK) * LDV + W * 32;
+  static constexpr int BYTES = WORDS * 4 + (2 * DL_MARK * LDK + DL_C * (16 * W + 8)) * (int)sizeof(T);
+};
+
+template <typename T, int DK, int W>
+__global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
+  typedef Delta<T> Ops;
+  typedef typename Ops::Row Row;
+  typedef DeltaLds<T, DK, W> L;
+  constexpr int NT = DK / 16, TP = (NT + W - 1) / W, LDK = L::LDK, LDV = L::LDV, LDG = 16 * W + 8, SQ = L::SQ;
+  extern __shared__ __align__(16) float lds[];
+  const int64_t block = block_number(), teams = (int64_t)a.rays.num_rays * a.v_heads;
+  const bool shared = a.heads != a.v_heads;
+  if (block >= teams) {
+    clear_rows(a, block - teams, (T*)a.dq, (int64_t)a.heads * a.key_dim);
+    clear_rows(a, block - teams, (T*)a.dk, (int64_t)a.heads * a.key_dim);
+    clear_rows(a, block - teams, (T*)a.dv, (int64_t)a.v_heads * a.val_dim);
+    clear_rows(a, block - teams, (T*)a.ddecay, (int64_t)a.v_heads);
+    clear_rows(a, block - teams, (T*)a.dbeta, (int64_t)a.v_heads);
+    return;
+  }
+  const int64_t ray = quotient(block, a.v_heads);
+  const int h = (int)(block - ray * a.v_heads), hk = h / (a.v_heads / a.heads);
+  const Chain ch = chain_of(a, ray);
+  const int lane = threadIdx.x & 63, w = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w16 = 16 * w;
+  int c = lane & 15, g = lane >> 4;
+  float* Tm = lds;
+  float* Pm = Tm + DL_SEG * SQ;
+  float* Dm = Pm + DL_SEG * SQ;
+  float* vecs = Dm + DL_SEG * SQ;
+  float* Xm = vecs + DL_SEG * DL_VEC;
+  float* Ym = Xm + SQ;
+  Plane<T, LDV> Nl{Ym + SQ}, Rl{Ym + SQ + DL_C * LDV}, Sl{Ym + SQ + 2 * DL_C * LDV};
+  float* sums = Sl.p + DK * LDV;
+  T* Kl = (T*)(sums + W * 32);
+  T* Ql = Kl + DL_MARK * LDK;
+  T* Gl = Ql + DL_MARK * LDK;  // do
+  const T* q = (const T*)a.q + hk * a.q_head;
+  const T* k = (const T*)a.k + hk * a.k_head;
+  const T* v = (const T*)a.v + h * a.v_head;
+  const T* dout = (const T*)a.dout + h * a.do_head;
+  const int64_t size = (int64_t)a.key_dim * a.val_dim;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  const auto sync = [] {
+    if constexpr (W > 1) __syncthreads();
+    else wave_sync();
+  };
+  f32x4 dS[NT];
+  load_state(dS, a.dlast ? a.dlast + block * size : nullptr, a, c, g, w16);
+#pragma unroll 1
+  for (int p0 = ch.count ? (ch.count - 1) / DL_MARK * DL_MARK : -1; p0 >= 0; p0 -= DL_MARK) {
+    asm volatile("" : "+v"(c), "+v"(g));
+    RawCol<T> vr[DL_SEG], gr[DL_SEG];
+#pragma unroll
+    for (int i = 0; i < DL_SEG; ++i) {
+      if (p0 + DL_C * i < ch.count) {
+        const Chunk ck(ch, p0 + DL_C * i);
+        vr[i].load(v, a.v_row, ck, g, w16 + c, a.val_dim);
+        gr[i].load(dout, a.do_row, ck, g, w16 + c, a.val_dim);
+      }
+    }
+    f32x4 S[DL_SEG + 1][NT], n[DL_SEG];
+    const float* from = p0 ? a.marks + (mark_slot(ch, p0) * a.v_heads + h) * size : a.h0 ? a.h0 + block * size : nullptr;
+    load_state(S[0], from, a, c, g, w16);
+    for (int i = w; i < DL_SEG; i += W) {
+      const int p = p0 + DL_C * i;
+      if (p >= ch.count) break;
+      const Chunk ck(ch, p);
+      RawRow<T, NT> kr, qr;
+      RawGates<T> gates;
+      kr.load(k, a.k_row, ck, c, g, a.key_dim);
+      qr.load(q, a.q_row, ck, c, g, a.key_dim);
+      gates.load(a, h, ck, c, g);
+      kr.trim(ck, c, g, a.key_dim);
+      qr.trim(ck, c, g, a.key_dim);
+      Row kf[NT], qf[NT];
+      kr.operands(kf);
+      qr.operands(qf);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        typedef typename RawRow<T, NT>::tvec tvec;
+        *reinterpret_cast<tvec*>(&Kl[(DL_C * i + c) * LDK + 16 * t + 4 * g]) = kr.v[t];
+        *reinterpret_cast<tvec*>(&Ql[(DL_C * i + c) * LDK + 16 * t + 4 * g]) = qr.v[t];
+      }
+      prepare_chunk<T>(kf, qf, gates.decay(ck, g), gates.beta(ck, c), a.scale, c, g, Tm + i * SQ, Pm + i * SQ, Dm + i * SQ,
+                       vecs + i * DL_VEC);
+    }
+    sync();
+    // the segment's states S[0] .. S[DL_SEG] and writes n
+#pragma unroll
+    for (int i = 0; i < DL_SEG; ++i) {
+      if (p0 + DL_C * i < ch.count) {
+        const Chunk ck(ch, p0 + DL_C * i);
+        const T* Kc = Kl + DL_C * i * LDK;
+        const float* vec = vecs + i * DL_VEC;
+        Row kf[NT];
+        typename Ops::Full full[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          kf[t] = row_of(Kc + c * LDK + 16 * t + 4 * g);
+          full[t] = Ops::full(S[i][t]);
+        }
+        const f32x4 beta = *reinterpret_cast<const f32x4*>(vec + 4 * g), e = *reinterpret_cast<const f32x4*>(vec + 16 + 4 * g);
+        const f32x4 R = beta * (vr[i].value(ck, g, w16 + c, a.val_dim) - e * mul_tiles<T>(kf, full, zero));
+        n[i] = mul16(*reinterpret_cast<const f32x4*>(Tm + i * SQ + c * DL_LD + 4 * g), R, zero);
+        const typename Ops::Full nl = Ops::full(*reinterpret_cast<const f32x4*>(vec + 32 + 4 * g) * n[i]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) S[i + 1][t] = Ops::mul(col_of<T, LDK>(Kc + 16 * t, c, g), nl, vec[48] * S[i][t]);
+      }
+    }
+#pragma unroll
+    for (int i = DL_SEG - 1; i >= 0; --i) {
+      const int p = p0 + DL_C * i;
+      if (p < ch.count) {
+        asm volatile("" : "+v"(c), "+v"(g));
+        const Chunk ck(ch, p);
+        const T *Kc = Kl + DL_C * i * LDK, *Qc = Ql + DL_C * i * LDK;
+        const float *vec = vecs + i * DL_VEC, *Tc = Tm + i * SQ, *Pc = Pm + i * SQ, *Dc = Dm + i * SQ;
+        const int vcol = w16 + c;
+        const f32x4 beta = *reinterpret_cast<const f32x4*>(vec + 4 * g), e = *reinterpret_cast<const f32x4*>(vec + 16 + 4 * g);
+        const f32x4 left = *reinterpret_cast<const f32x4*>(vec + 32 + 4 * g);
+        // by columns: dn, dR, dv
+        const f32x4 go = gr[i].value(ck, g, vcol, a.val_dim), vv = vr[i].value(ck, g, vcol, a.val_dim);
+        f32x4 dn, dR, col;
+        {
+          Row kf[NT];
+          typename Ops::Full full[NT];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            kf[t] = row_of(Kc + c * LDK + 16 * t + 4 * g);
+            full[t] = Ops::full(dS[t]);
+          }
+          dn = left * mul_tiles<T>(kf, full, zero);
+        }
+        Row gow;
+        if constexpr (Ops::EXACT) gow = __builtin_convertvector(go, b16x4);
+        else gow = go;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) col[s] = Pc[(4 * g + s) * DL_LD + c];
+        dn = Ops::mul(Ops::full(col), gow, dn);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) col[s] = Tc[(4 * g + s) * DL_LD + c];
+        dR = mul16(col, dn, zero);
+        f32x4 to_beta = vv * dR, to_decay = zero;
+        {
+          T* dv = (T*)a.dv + (ck.low * a.v_heads + h) * a.val_dim;
+          const int64_t stride = (int64_t)a.v_heads * a.val_dim;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (4 * g + r < ck.many && vcol < a.val_dim)
+              *const_cast<T*>(row_ptr(dv + vcol, ck.at(4 * g + r), stride)) = (T)(beta[r] * dR[r]);
+            Nl.set(4 * g + r, vcol, n[i][r]);
+            Rl.set(4 * g + r, vcol, dR[r]);
+            Gl[(4 * g + r) * LDG + vcol] = (T)go[r];
+          }
+        }
+        float inner = 0.f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            inner = __builtin_fmaf(dS[t][r], S[i + 1][t][r], inner);
+            Sl.set(16 * t + 4 * g + r, vcol, S[i][t][r]);
+          }
+        }
+        inner += __shfl_xor(inner, 16);
+        inner += __shfl_xor(inner, 32);
+        if (g == 3) to_decay[3] = inner;  // the chunk's last row
+        sync();
+        const auto g_row = [&](int col) { return row_of(Gl + c * LDG + col + 4 * g); };
+        const auto n_row = [&](int col) { return Nl.get(c, col + 4 * g); };
+        const auto r_row = [&](int col) { return Rl.get(c, col + 4 * g); };
+        // X and Y (the first and the second wavefront, where there are two); products with S
+        if (w == 0 || w == 1) {
+          const f32x4 D = *reinterpret_cast<const f32x4*>(Dc + c * DL_LD + 4 * g);
+          if (w == 0) {
+            f32x4 x = mul_cols<T, W>(n_row, g_row, zero);  // rows j, column i
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = 4 * g + r <= c ? D[r] * x[r] : 0.f;
+            *reinterpret_cast<f32x4*>(Xm + c * DL_LD + 4 * g) = x;
+          }
+          if (w == 1 || W == 1) {
+            f32x4 y = mul_cols<T, W>(n_row, r_row, zero);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[r] = 4 * g + r < c ? -D[r] * y[r] : 0.f;
+            *reinterpret_cast<f32x4*>(Ym + c * DL_LD + 4 * g) = y;
+          }
+        }
+        f32x4 dq[TP], lf[TP];
+#pragma unroll
+        for (int j = 0; j < TP; ++j) {
+          const int t = w + j * W;
+          if (t < NT) {
+            const auto s_row = [&](int col) { return Sl.get(16 * t + c, col + 4 * g); };
+            dq[j] = mul_cols<T, W>(g_row, s_row, zero);
+            lf[j] = mul_cols<T, W>(r_row, s_row, zero);
+          }
+        }
+        sync();
+        // dS out, and back to the chunk's start
+        const typename Ops::Full fo = Ops::full(a.scale * e * go), fr = Ops::full(-(beta * e) * dR);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) Sl.set(16 * t + 4 * g + r, vcol, dS[t][r]);
+          dS[t] = Ops::mul(col_of<T, LDK>(Kc + 16 * t, c, g), fr, Ops::mul(col_of<T, LDK>(Qc + 16 * t, c, g), fo, vec[48] * dS[t]));
+        }
+        sync();
+        f32x4 xc, yc;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          xc[s] = a.scale * Xm[(4 * g + s) * DL_LD + c];
+          yc[s] = beta[s] * Ym[(4 * g + s) * DL_LD + c];
+        }
+        const typename Ops::Two xr = Ops::two(*reinterpret_cast<const f32x4*>(Xm + c * DL_LD + 4 * g)),
+                                yr = Ops::two(*reinterpret_cast<const f32x4*>(Ym + c * DL_LD + 4 * g)), xt = Ops::two(xc), yt = Ops::two(yc);
+#pragma unroll
+        for (int j = 0; j < TP; ++j) {
+          const int t = w + j * W, kcol = 16 * t + c;
+          if (t < NT) {
+            const auto s_row = [&](int col) { return Sl.get(kcol, col + 4 * g); };
+            const Row kt = col_of<T, LDK>(Kc + 16 * t, c, g), qt = col_of<T, LDK>(Qc + 16 * t, c, g);
+            const f32x4 kv = Ops::value(kt), qv = Ops::value(qt);
+            const f32x4 gq = a.scale * Ops::mul(xr, kt, e * dq[j]);
+            const f32x4 gl = Ops::mul(yr, kt, -(e * lf[j]));
+            const f32x4 right = Ops::mul(yt, kt, Ops::mul(xt, qt, left * mul_cols<T, W>(n_row, s_row, zero)));
+            const f32x4 gk = beta * gl + right;
+            to_beta += kv * gl;
+            to_decay += qv * gq + beta * (kv * gl) - kv * right;
+            if (kcol < a.key_dim) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                if (4 * g + r < ck.many) {
+                  if (shared) {
+                    const int64_t to = ((ck.low + ck.at(4 * g + r)) * a.v_heads + h) * a.key_dim + kcol;
+                    ((float*)a.workspace)[to] = gq[r];
+                    ((float*)a.workspace)[to + (int64_t)a.rays.n * a.v_heads * a.key_dim] = gk[r];
+                  } else {
+                    const int64_t low = (ck.low * a.heads + h) * a.key_dim + kcol, stride = (int64_t)a.heads * a.key_dim;
+                    *const_cast<T*>(row_ptr((T*)a.dq + low, ck.at(4 * g + r), stride)) = (T)gq[r];
+                    *const_cast<T*>(row_ptr((T*)a.dk + low, ck.at(4 * g + r), stride)) = (T)gk[r];
+                  }
+                }
+              }
+            }
+          }
+        }
+        to_beta = sum16(to_beta);
+        to_decay = sum16(to_decay);
+        if (c == 0) {
+          *reinterpret_cast<f32x4*>(sums + w * 32 + 4 * g) = to_beta;
+          *reinterpret_cast<f32x4*>(sums + w * 32 + 16 + 4 * g) = to_decay;
+        }
+        sync();
+        if (w == 0 && g == 0) {
+          float db = 0.f, dd = 0.f;
+#pragma unroll
+          for (int u = 0; u < W; ++u) {
+            db += sums[u * 32 + c];
+            dd += sums[u * 32 + 16 + c];
+          }
+#pragma unroll
+          for (int d = 1; d < DL_C; d *= 2) {
+            const float x = __shfl_down(dd, d);
+            dd += c + d < DL_C ? x : 0.f;
+          }
+          if (c < ck.many) {
+            const int64_t to = (ck.low + ck.at(c)) * a.v_heads + h;
+            ((T*)a.ddecay)[to] = (T)dd;
+            ((T*)a.dbeta)[to] = (T)db;
+          }
+        }
+      }
+    }
+  }
+  if (a.dh0) store_state(a.dh0 + block * size, dS, a, c, g, w16);
+}
+
+// dq and dk of key heads that value heads share, in a fixed order
+template <typename T>
+__global__ __launch_bounds__(256) void k_delta_join(const ffn_ray_delta a) {
+  const int64_t all = (int64_t)a.rays.n * a.heads * a.key_dim, i = block_number() * 256 + threadIdx.x;
+  if (i >= 2 * all) return;
+  const int64_t j = i < all ? i : i - all, row = j / ((int64_t)a.heads * a.key_dim);
+  const uint32_t r = a.rays.ray_ids[row];
+  if (r >= a.rays.num_rays) return;  // written as 0
+  const int64_t o = a.rays.offsets[r];
+  if (row < o || row - o >= (int64_t)a.rays.counts[r]) return;
+  const int x = (int)(j - row * a.heads * a.key_dim), hk = x / a.key_dim, col = x - hk * a.key_dim, per = a.v_heads / a.heads;
+  const float* from = (const float*)a.workspace + (i < all ? 0 : (int64_t)a.rays.n * a.v_heads * a.key_dim) +
+                      (row * a.v_heads + hk * per) * a.key_dim + col;
+  float s = 0.f;
+  for (int u = 0; u < per; ++u) s += from[(int64_t)u * a.key_dim];
+  ((T*)(i < all ? a.dq : a.dk))[j] = (T)s;
+}
+
+// ---------------------------------------------------------------------------
+// launches
+
+inline int64_t delta_clear_blocks(const ffn_ray_delta& a) { return ((int64_t)a.rays.n + DL_CLEAR - 1) / DL_CLEAR; }
+
+template <typename T, int DK, int W>
+hipError_t start_delta(const ffn_ray_delta& a, bool back, hipStream_t st) {
+  const dim3 grid = grid_of((int64_t)a.rays.num_rays * a.v_heads + delta_clear_blocks(a));
+  if (!back) {
+    k_delta_fwd<T, DK, W><<<grid, 64 * W, 0, st>>>(a);
+    return hipGetLastError();
+  }
+  constexpr int bytes = DeltaLds<T, DK, W>::BYTES;
+  static_assert(bytes <= 160 * 1024, "LDS");
+  if (bytes > 64 * 1024) {  // has to be allowed, on the device that is current
+    const hipError_t e = hipFuncSetAttribute((const void*)k_delta_bwd<T, DK, W>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) return e;
+  }
+  k_delta_bwd<T, DK, W><<<grid, 64 * W, bytes, st>>>(a);
+  return hipGetLastError();
+}
+
+template <typename T, int DK>
+hipError_t delta_by_columns(const ffn_ray_delta& a, bool back, hipStream_t st) {
+  if (!back && !a.marks && a.rays.n <= 4ull * a.rays.num_rays) {
+    const int64_t teams = (int64_t)a.rays.num_rays * a.v_heads * ((a.val_dim + 31) / 32);
+    k_delta_step<T, DK><<<grid_of((teams + 3) / 4 + delta_clear_blocks(a)), 256, 0, st>>>(a);
+    return hipGetLastError();
+  }
+  hipError_t e;
+  if (a.val_dim <= 16) e = start_delta<T, DK, 1>(a, back, st);
+  else if (a.val_dim <= 32) e = start_delta<T, DK, 2>(a, back, st);
+  else if (a.val_dim <= 48) e = start_delta<T, DK, 3>(a, back, st);
+  else if (a.val_dim <= 64) e = start_delta<T, DK, 4>(a, back, st);
+  else e = start_delta<T, DK, 8>(a, back, st);
+  if (!back || e != hipSuccess || a.heads == a.v_heads || !a.rays.n) return e;
+  k_delta_join<T><<<grid_of((2 * (int64_t)a.rays.n * a.heads * a.key_dim + 255) / 256), 256, 0, st>>>(a);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t delta_of_type(const ffn_ray_delta& a, bool back, hipStream_t st) {
+  if (a.key_dim <= 32) return delta_by_columns<T, 32>(a, back, st);
+  if (a.key_dim <= 64) return delta_by_columns<T, 64>(a, back, st);
+  return delta_by_columns<T, 128>(a, back, st);
+}
+
+hipError_t delta_f32(const ffn_ray_delta& a, bool back, hipStream_t st);
+hipError_t delta_f16(const ffn_ray_delta& a, bool back, hipStream_t st);
+hipError_t delta_bf16(const ffn_ray_delta& a, bool back, hipStream_t st);
+
+}  // namespace ffn
