@@ -162,31 +162,49 @@ template <typename T> __device__ __forceinline__ void store4(T* p, const f32x4& 
   typedef T tvec __attribute__((ext_vector_type(4)));
   *reinterpret_cast<tvec*>(p) = __builtin_convertvector(x, tvec);
 }
-// four values of an LDS row as a product's operand
-template <typename T> __device__ __forceinline__ typename Delta<T>::Row row_of(const T* p) {
+// A tile of 16 rows and 16 columns in LDS, LD values a row: an operand by rows (this lane's row c, columns 4 g + s) or, the
+// transposed one, by columns (column c, rows 4 g + s).  Neither meets a bank twice.
+template <typename T> struct Tile {
+  static constexpr int LD = sizeof(T) == 4 ? 20 : Delta<T>::EXACT ? 16 : 24, SIZE = DL_C * LD;
+};
+template <typename T> __device__ __forceinline__ typename Delta<T>::Row row_of(const T* tile, int c, int g) {
+  const T* p = tile + c * Tile<T>::LD + 4 * g;
   if constexpr (Delta<T>::EXACT) return *reinterpret_cast<const b16x4*>(p);
   else return load4(p);
 }
-// column c of the rows 4 g .. 4 g + 3 from `tile` on, LD apart: the transposed operand
-template <typename T, int LD> __device__ __forceinline__ typename Delta<T>::Row col_of(const T* tile, int c, int g) {
+template <typename T> __device__ __forceinline__ typename Delta<T>::Row col_of(const T* tile, int c, int g) {
   if constexpr (Delta<T>::EXACT) {
     typedef __attribute__((address_space(3))) s16x4* lds_quad;
-    return __builtin_bit_cast(b16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad)(tile + (4 * g + (c >> 2)) * LD + 4 * (c & 3))));
+    return __builtin_bit_cast(b16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad)(tile + (4 * g + (c >> 2)) * Tile<T>::LD + 4 * (c & 3))));
   } else {
     f32x4 x;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) x[s] = (float)tile[(4 * g + s) * LD + c];
+    for (int s = 0; s < 4; ++s) x[s] = (float)tile[(4 * g + s) * Tile<T>::LD + c];
     return x;
   }
 }
 
-// sum over the 16 lanes of a group
+// x of another lane of this lane's 16, by one of the moves within them (0 where there is none)
+template <int MOVE> __device__ __forceinline__ float moved(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), MOVE, 0xF, 0xF, true));
+}
+// sum over the 16 lanes of a group: within pairs, fours, halves, and of both
 __device__ __forceinline__ f32x4 sum16(f32x4 x) {
 #pragma unroll
-  for (int d = 1; d < 16; d *= 2) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] += __shfl_xor(x[r], d);
+  for (int r = 0; r < 4; ++r) {
+    x[r] += moved<0xB1>(x[r]);
+    x[r] += moved<0x4E>(x[r]);
+    x[r] += moved<0x141>(x[r]);
+    x[r] += moved<0x140>(x[r]);
   }
+  return x;
+}
+// sum over this lane and those after it in its 16
+__device__ __forceinline__ float sum_after(float x) {
+  x += moved<0x101>(x);
+  x += moved<0x102>(x);
+  x += moved<0x104>(x);
+  x += moved<0x108>(x);
   return x;
 }
 
@@ -460,11 +478,11 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int b) {
 
 template <typename T, int DK, int W>
 __global__ __launch_bounds__(64 * W) void k_delta_fwd(const ffn_ray_delta a) {
-  constexpr int NT = DK / 16, LDK = DK + 16 / (int)sizeof(T), CH = W < 4 ? W : 4;
+  constexpr int NT = DK / 16, TILE = Tile<T>::SIZE, CH = W < 4 ? W : 4;
   typedef Delta<T> Ops;
   typedef typename Ops::Row Row;
   __shared__ float Tm[CH][DL_C * DL_LD], Pm[CH][DL_C * DL_LD], vec[CH][DL_VEC];
-  __shared__ __align__(16) T Kl[CH * DL_C * LDK], Ql[CH * DL_C * LDK];
+  __shared__ __align__(16) T Kl[CH * NT * TILE], Ql[CH * NT * TILE];
   const int64_t block = block_number(), teams = (int64_t)a.rays.num_rays * a.v_heads;
   if (block >= teams) {
     clear_rows(a, block - teams, (T*)a.o, (int64_t)a.v_heads * a.val_dim);
@@ -511,8 +529,8 @@ __global__ __launch_bounds__(64 * W) void k_delta_fwd(const ffn_ray_delta a) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         typedef typename RawRow<T, NT>::tvec tvec;
-        *reinterpret_cast<tvec*>(&Kl[(DL_C * w + c) * LDK + 16 * t + 4 * g]) = kr.v[t];
-        *reinterpret_cast<tvec*>(&Ql[(DL_C * w + c) * LDK + 16 * t + 4 * g]) = qr.v[t];
+        *reinterpret_cast<tvec*>(Kl + (w * NT + t) * TILE + c * Tile<T>::LD + 4 * g) = kr.v[t];
+        *reinterpret_cast<tvec*>(Ql + (w * NT + t) * TILE + c * Tile<T>::LD + 4 * g) = qr.v[t];
       }
       prepare_chunk<T>(kf, qf, gates.decay(ck, g), gates.beta(ck, c), a.scale, c, g, Tm[w], Pm[w], (float*)nullptr, vec[w]);
       fetch(p0 + DL_C * (CH + w));
@@ -525,12 +543,12 @@ __global__ __launch_bounds__(64 * W) void k_delta_fwd(const ffn_ray_delta a) {
       if (p < ch.count) {
         const Chunk ck(ch, p);
         if (a.marks && p && p % DL_MARK == 0) store_state(a.marks + (mark_slot(ch, p) * a.v_heads + h) * size, S, a, c, g, w16);
-        const T *Kc = Kl + DL_C * i * LDK, *Qc = Ql + DL_C * i * LDK;
+        const T *Kc = Kl + i * NT * TILE, *Qc = Ql + i * NT * TILE;
         Row kf[NT], qf[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          kf[t] = row_of(Kc + c * LDK + 16 * t + 4 * g);
-          qf[t] = row_of(Qc + c * LDK + 16 * t + 4 * g);
+          kf[t] = row_of(Kc + t * TILE, c, g);
+          qf[t] = row_of(Qc + t * TILE, c, g);
         }
         const f32x4 beta = *reinterpret_cast<const f32x4*>(&vec[i][4 * g]);
         const f32x4 e = *reinterpret_cast<const f32x4*>(&vec[i][16 + 4 * g]);
@@ -559,7 +577,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_fwd(const ffn_ray_delta a) {
         }
         const typename Ops::Full nl = Ops::full(left * n);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) S[t] = Ops::mul(col_of<T, LDK>(Kc + 16 * t, c, g), nl, all * S[t]);
+        for (int t = 0; t < NT; ++t) S[t] = Ops::mul(col_of(Kc + t * TILE, c, g), nl, all * S[t]);
       }
     }
     if constexpr (W > 1) __syncthreads();
@@ -656,45 +674,65 @@ __global__ __launch_bounds__(256) void k_delta_step(const ffn_ray_delta a) {
 // dn, dR, dv and dS go by columns, as S does; dq and dk are sums over the columns: S, dS, n and dR pass through LDS, and a
 // wavefront takes 16 columns of dq and dk.
 
-// An LDS array of float rows as operands of products whose result is rounded to the type: floats, or two parts each.
-template <typename T, int LD> struct Plane {
-  static constexpr int WORDS = 1;  // a value's four bytes
+// Tiles of 16 x 16 floats in LDS, put down by columns as products leave them (column c, rows 4 g + r) and taken up by rows,
+// as operands of products whose result is rounded to the type: floats, or two parts each.
+template <typename T> struct Tiles {
+  static constexpr int WORDS = 256;  // of a tile
   float* p;
-  __device__ __forceinline__ void set(int row, int col, float x) {
+  __device__ __forceinline__ void set(int tile, int c, int g, const f32x4& x) const {
     if constexpr (Delta<T>::EXACT) {
-      __bf16* q = (__bf16*)p;
-      const uint32_t w = __builtin_bit_cast(uint32_t, x);
-      q[row * 2 * LD + col] = __builtin_bit_cast(__bf16, (uint16_t)(w >> 16));
-      const float rest = x - __builtin_bit_cast(float, w & 0xFFFF0000u);
-      q[row * 2 * LD + LD + col] = __builtin_bit_cast(__bf16, (uint16_t)(__builtin_bit_cast(uint32_t, rest) >> 16));
+      set(tile, c, g, parts_of<2>(x));
     } else {
-      p[row * LD + col] = x;
+      // row 4 g + r is the (4 r + g)th, its fours of columns in an order that goes by r: neither side meets a bank twice
+#pragma unroll
+      for (int r = 0; r < 4; ++r) p[tile * WORDS + (4 * r + g) * 16 + 4 * ((c >> 2) ^ r) + (c & 3)] = x[r];
     }
   }
-  __device__ __forceinline__ typename Delta<T>::Two get(int row, int col) const {
+  template <int N> __device__ __forceinline__ void set(int tile, int c, int g, const Parts<N>& x) const {
+    __bf16* q = (__bf16*)(p + tile * WORDS) + c * 16 + 4 * g;  // transposed, so that four rows lie side by side
+    *reinterpret_cast<b16x4*>(q) = x.p[0];
+    *reinterpret_cast<b16x4*>(q + 256) = x.p[1];
+  }
+  __device__ __forceinline__ typename Delta<T>::Two get(int tile, int c, int g) const {
     if constexpr (Delta<T>::EXACT) {
-      const __bf16* q = (const __bf16*)p + row * 2 * LD + col;
-      return {{*reinterpret_cast<const b16x4*>(q), *reinterpret_cast<const b16x4*>(q + LD)}};
+      const __bf16* q = (const __bf16*)(p + tile * WORDS);
+      return {{col_of(q, c, g), col_of(q + 256, c, g)}};
     } else {
-      return *reinterpret_cast<const f32x4*>(p + row * LD + col);
+      return *reinterpret_cast<const f32x4*>(p + tile * WORDS + (4 * (c & 3) + (c >> 2)) * 16 + 4 * (g ^ (c & 3)));
     }
   }
 };
+// the same for values of the type
+template <typename T> struct RowTiles {
+  T* p;
+  __device__ __forceinline__ void set(int tile, int c, int g, const f32x4& x) const {
+    if constexpr (Delta<T>::EXACT) {
+      *reinterpret_cast<b16x4*>(p + tile * Tile<T>::SIZE + c * 16 + 4 * g) = __builtin_convertvector(x, b16x4);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) p[tile * Tile<T>::SIZE + (4 * g + r) * Tile<T>::LD + c] = (T)x[r];
+    }
+  }
+  __device__ __forceinline__ typename Delta<T>::Row get(int tile, int c, int g) const {
+    if constexpr (Delta<T>::EXACT) return col_of(p + tile * Tile<T>::SIZE, c, g);
+    else return row_of(p + tile * Tile<T>::SIZE, c, g);
+  }
+};
 
-// sum over the W tiles of 16 columns of the operands that a and b give for a column
+// sum over the W tiles of the operands that a and b give for a tile
 template <typename T, int W, typename A, typename B>
 __device__ __forceinline__ f32x4 mul_cols(A a, B b, f32x4 c) {
 #pragma unroll
-  for (int u = 0; u + 1 < W; u += 2) c = Delta<T>::mul(a(16 * u), a(16 * u + 16), b(16 * u), b(16 * u + 16), c);
+  for (int u = 0; u + 1 < W; u += 2) c = Delta<T>::mul(a(u), a(u + 1), b(u), b(u + 1), c);
   // the last odd one in sums of its own: a product of K = 16 right behind one of K = 32 on the same sums gave wrong results
-  if constexpr (W % 2) c = c + Delta<T>::mul(a(16 * W - 16), b(16 * W - 16), f32x4{0.f, 0.f, 0.f, 0.f});
+  if constexpr (W % 2) c = c + Delta<T>::mul(a(W - 1), b(W - 1), f32x4{0.f, 0.f, 0.f, 0.f});
   return c;
 }
 
 template <typename T, int DK, int W> struct DeltaLds {
-  static constexpr int LDV = 16 * W + (Delta<T>::EXACT ? 8 : 4), LDK = DK + 16 / (int)sizeof(T), SQ = DL_C * DL_LD;
-  static constexpr int WORDS = DL_SEG * (3 * SQ + DL_VEC) + 2 * SQ + (2 * DL_C + DK) * LDV + W * 32;
-  static constexpr int BYTES = WORDS * 4 + (2 * DL_MARK * LDK + DL_C * (16 * W + 8)) * (int)sizeof(T);
+  static constexpr int SQ = DL_C * DL_LD, NT = DK / 16;
+  static constexpr int WORDS = DL_SEG * (3 * SQ + DL_VEC) + 2 * SQ + (2 + NT) * W * Tiles<T>::WORDS + W * 32;
+  static constexpr int BYTES = WORDS * 4 + (2 * DL_SEG * NT + W) * Tile<T>::SIZE * (int)sizeof(T);
 };
 
 template <typename T, int DK, int W>
@@ -702,7 +740,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
   typedef Delta<T> Ops;
   typedef typename Ops::Row Row;
   typedef DeltaLds<T, DK, W> L;
-  constexpr int NT = DK / 16, TP = (NT + W - 1) / W, LDK = L::LDK, LDV = L::LDV, LDG = 16 * W + 8, SQ = L::SQ;
+  constexpr int NT = DK / 16, TP = (NT + W - 1) / W, SQ = L::SQ, TILE = Tile<T>::SIZE;
   extern __shared__ __align__(16) float lds[];
   const int64_t block = block_number(), teams = (int64_t)a.rays.num_rays * a.v_heads;
   const bool shared = a.heads != a.v_heads;
@@ -725,11 +763,12 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
   float* vecs = Dm + DL_SEG * SQ;
   float* Xm = vecs + DL_SEG * DL_VEC;
   float* Ym = Xm + SQ;
-  Plane<T, LDV> Nl{Ym + SQ}, Rl{Ym + SQ + DL_C * LDV}, Sl{Ym + SQ + 2 * DL_C * LDV};
-  float* sums = Sl.p + DK * LDV;
+  // n, dR; S and dS, tile t W + u: rows of tile t, columns of wavefront u
+  const Tiles<T> Nl{Ym + SQ}, Rl{Nl.p + W * Tiles<T>::WORDS}, Sl{Rl.p + W * Tiles<T>::WORDS};
+  float* sums = Sl.p + NT * W * Tiles<T>::WORDS;
   T* Kl = (T*)(sums + W * 32);
-  T* Ql = Kl + DL_MARK * LDK;
-  T* Gl = Ql + DL_MARK * LDK;  // do
+  T* Ql = Kl + DL_SEG * NT * TILE;
+  const RowTiles<T> Gl{Ql + DL_SEG * NT * TILE};  // do
   const T* q = (const T*)a.q + hk * a.q_head;
   const T* k = (const T*)a.k + hk * a.k_head;
   const T* v = (const T*)a.v + h * a.v_head;
@@ -754,7 +793,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
         gr[i].load(dout, a.do_row, ck, g, w16 + c, a.val_dim);
       }
     }
-    f32x4 S[DL_SEG + 1][NT], n[DL_SEG];
+    f32x4 S[DL_SEG][NT], n[DL_SEG];
     const float* from = p0 ? a.marks + (mark_slot(ch, p0) * a.v_heads + h) * size : a.h0 ? a.h0 + block * size : nullptr;
     load_state(S[0], from, a, c, g, w16);
     for (int i = w; i < DL_SEG; i += W) {
@@ -774,33 +813,34 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         typedef typename RawRow<T, NT>::tvec tvec;
-        *reinterpret_cast<tvec*>(&Kl[(DL_C * i + c) * LDK + 16 * t + 4 * g]) = kr.v[t];
-        *reinterpret_cast<tvec*>(&Ql[(DL_C * i + c) * LDK + 16 * t + 4 * g]) = qr.v[t];
+        *reinterpret_cast<tvec*>(Kl + (i * NT + t) * TILE + c * Tile<T>::LD + 4 * g) = kr.v[t];
+        *reinterpret_cast<tvec*>(Ql + (i * NT + t) * TILE + c * Tile<T>::LD + 4 * g) = qr.v[t];
       }
       prepare_chunk<T>(kf, qf, gates.decay(ck, g), gates.beta(ck, c), a.scale, c, g, Tm + i * SQ, Pm + i * SQ, Dm + i * SQ,
                        vecs + i * DL_VEC);
     }
     sync();
-    // the segment's states S[0] .. S[DL_SEG] and writes n
+    // the states before the segment's chunks, and their writes n
 #pragma unroll
     for (int i = 0; i < DL_SEG; ++i) {
       if (p0 + DL_C * i < ch.count) {
         const Chunk ck(ch, p0 + DL_C * i);
-        const T* Kc = Kl + DL_C * i * LDK;
+        const T* Kc = Kl + i * NT * TILE;
         const float* vec = vecs + i * DL_VEC;
         Row kf[NT];
         typename Ops::Full full[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          kf[t] = row_of(Kc + c * LDK + 16 * t + 4 * g);
+          kf[t] = row_of(Kc + t * TILE, c, g);
           full[t] = Ops::full(S[i][t]);
         }
         const f32x4 beta = *reinterpret_cast<const f32x4*>(vec + 4 * g), e = *reinterpret_cast<const f32x4*>(vec + 16 + 4 * g);
         const f32x4 R = beta * (vr[i].value(ck, g, w16 + c, a.val_dim) - e * mul_tiles<T>(kf, full, zero));
         n[i] = mul16(*reinterpret_cast<const f32x4*>(Tm + i * SQ + c * DL_LD + 4 * g), R, zero);
+        if (i + 1 == DL_SEG || p0 + DL_C * (i + 1) >= ch.count) continue;
         const typename Ops::Full nl = Ops::full(*reinterpret_cast<const f32x4*>(vec + 32 + 4 * g) * n[i]);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) S[i + 1][t] = Ops::mul(col_of<T, LDK>(Kc + 16 * t, c, g), nl, vec[48] * S[i][t]);
+        for (int t = 0; t < NT; ++t) S[i + 1 < DL_SEG ? i + 1 : i][t] = Ops::mul(col_of(Kc + t * TILE, c, g), nl, vec[48] * S[i][t]);
       }
     }
 #pragma unroll
@@ -809,7 +849,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
       if (p < ch.count) {
         asm volatile("" : "+v"(c), "+v"(g));
         const Chunk ck(ch, p);
-        const T *Kc = Kl + DL_C * i * LDK, *Qc = Ql + DL_C * i * LDK;
+        const T *Kc = Kl + i * NT * TILE, *Qc = Ql + i * NT * TILE;
         const float *vec = vecs + i * DL_VEC, *Tc = Tm + i * SQ, *Pc = Pm + i * SQ, *Dc = Dm + i * SQ;
         const int vcol = w16 + c;
         const f32x4 beta = *reinterpret_cast<const f32x4*>(vec + 4 * g), e = *reinterpret_cast<const f32x4*>(vec + 16 + 4 * g);
@@ -817,12 +857,12 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
         // by columns: dn, dR, dv
         const f32x4 go = gr[i].value(ck, g, vcol, a.val_dim), vv = vr[i].value(ck, g, vcol, a.val_dim);
         f32x4 dn, dR, col;
+        typename Ops::Full full[NT];  // of dS
         {
           Row kf[NT];
-          typename Ops::Full full[NT];
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            kf[t] = row_of(Kc + c * LDK + 16 * t + 4 * g);
+            kf[t] = row_of(Kc + t * TILE, c, g);
             full[t] = Ops::full(dS[t]);
           }
           dn = left * mul_tiles<T>(kf, full, zero);
@@ -844,27 +884,23 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
           for (int r = 0; r < 4; ++r) {
             if (4 * g + r < ck.many && vcol < a.val_dim)
               *const_cast<T*>(row_ptr(dv + vcol, ck.at(4 * g + r), stride)) = (T)(beta[r] * dR[r]);
-            Nl.set(4 * g + r, vcol, n[i][r]);
-            Rl.set(4 * g + r, vcol, dR[r]);
-            Gl[(4 * g + r) * LDG + vcol] = (T)go[r];
           }
         }
-        float inner = 0.f;
+        Nl.set(w, c, g, n[i]);
+        Rl.set(w, c, g, dR);
+        Gl.set(w, c, g, go);
+        float inner = 0.f;  // dS . S at the chunk's end: what was there at its start ..
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            inner = __builtin_fmaf(dS[t][r], S[i + 1][t][r], inner);
-            Sl.set(16 * t + 4 * g + r, vcol, S[i][t][r]);
-          }
+          for (int r = 0; r < 4; ++r) inner = __builtin_fmaf(dS[t][r], S[i][t][r], inner);
+          Sl.set(t * W + w, c, g, S[i][t]);
         }
-        inner += __shfl_xor(inner, 16);
-        inner += __shfl_xor(inner, 32);
-        if (g == 3) to_decay[3] = inner;  // the chunk's last row
+        inner *= vec[48];
         sync();
-        const auto g_row = [&](int col) { return row_of(Gl + c * LDG + col + 4 * g); };
-        const auto n_row = [&](int col) { return Nl.get(c, col + 4 * g); };
-        const auto r_row = [&](int col) { return Rl.get(c, col + 4 * g); };
+        const auto g_row = [&](int u) { return Gl.get(u, c, g); };
+        const auto n_row = [&](int u) { return Nl.get(u, c, g); };
+        const auto r_row = [&](int u) { return Rl.get(u, c, g); };
         // X and Y (the first and the second wavefront, where there are two); products with S
         if (w == 0 || w == 1) {
           const f32x4 D = *reinterpret_cast<const f32x4*>(Dc + c * DL_LD + 4 * g);
@@ -886,7 +922,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
         for (int j = 0; j < TP; ++j) {
           const int t = w + j * W;
           if (t < NT) {
-            const auto s_row = [&](int col) { return Sl.get(16 * t + c, col + 4 * g); };
+            const auto s_row = [&](int u) { return Sl.get(t * W + u, c, g); };
             dq[j] = mul_cols<T, W>(g_row, s_row, zero);
             lf[j] = mul_cols<T, W>(r_row, s_row, zero);
           }
@@ -896,9 +932,8 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
         const typename Ops::Full fo = Ops::full(a.scale * e * go), fr = Ops::full(-(beta * e) * dR);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) Sl.set(16 * t + 4 * g + r, vcol, dS[t][r]);
-          dS[t] = Ops::mul(col_of<T, LDK>(Kc + 16 * t, c, g), fr, Ops::mul(col_of<T, LDK>(Qc + 16 * t, c, g), fo, vec[48] * dS[t]));
+          Sl.set(t * W + w, c, g, full[t]);
+          dS[t] = Ops::mul(col_of(Kc + t * TILE, c, g), fr, Ops::mul(col_of(Qc + t * TILE, c, g), fo, vec[48] * dS[t]));
         }
         sync();
         f32x4 xc, yc;
@@ -913,12 +948,14 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
         for (int j = 0; j < TP; ++j) {
           const int t = w + j * W, kcol = 16 * t + c;
           if (t < NT) {
-            const auto s_row = [&](int col) { return Sl.get(kcol, col + 4 * g); };
-            const Row kt = col_of<T, LDK>(Kc + 16 * t, c, g), qt = col_of<T, LDK>(Qc + 16 * t, c, g);
+            const auto s_row = [&](int u) { return Sl.get(t * W + u, c, g); };
+            const Row kt = col_of(Kc + t * TILE, c, g), qt = col_of(Qc + t * TILE, c, g);
             const f32x4 kv = Ops::value(kt), qv = Ops::value(qt);
             const f32x4 gq = a.scale * Ops::mul(xr, kt, e * dq[j]);
             const f32x4 gl = Ops::mul(yr, kt, -(e * lf[j]));
-            const f32x4 right = Ops::mul(yt, kt, Ops::mul(xt, qt, left * mul_cols<T, W>(n_row, s_row, zero)));
+            const f32x4 end = left * mul_cols<T, W>(n_row, s_row, zero), right = Ops::mul(yt, kt, Ops::mul(xt, qt, end));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) inner = __builtin_fmaf(kv[r], end[r], inner);  // .. and what the chunk wrote
             const f32x4 gk = beta * gl + right;
             to_beta += kv * gl;
             to_decay += qv * gq + beta * (kv * gl) - kv * right;
@@ -940,6 +977,9 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
             }
           }
         }
+        inner += __shfl_xor(inner, 16);
+        inner += __shfl_xor(inner, 32);
+        if (g == 3) to_decay[3] += inner;  // the chunk's last row
         to_beta = sum16(to_beta);
         to_decay = sum16(to_decay);
         if (c == 0) {
@@ -954,11 +994,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
             db += sums[u * 32 + c];
             dd += sums[u * 32 + 16 + c];
           }
-#pragma unroll
-          for (int d = 1; d < DL_C; d *= 2) {
-            const float x = __shfl_down(dd, d);
-            dd += c + d < DL_C ? x : 0.f;
-          }
+          dd = sum_after(dd);
           if (c < ck.many) {
             const int64_t to = (ck.low + ck.at(c)) * a.v_heads + h;
             ((T*)a.ddecay)[to] = (T)dd;
