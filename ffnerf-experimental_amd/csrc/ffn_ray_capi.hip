@@ -26,6 +26,7 @@ constexpr uint32_t MAX_ROWS = 0x7FFFFF00u;
 constexpr int MAX_SCAN_STRIDE = 1 << 27;
 
 constexpr uint64_t MAX_SCAN_STATES = 1ull << 46;  // channels of all rays: what one launch can count
+constexpr int MAX_DELTA_STRIDE = 1 << 24;
 constexpr uint64_t MAX_DELTA_STATES = 1ull << 36; // heads of all rays: a block each
 
 int elem(int32_t dtype) { return dtype == FFN_F32 ? 4 : dtype == FFN_F16 || dtype == FFN_BF16 ? 2 : 0; }
@@ -162,8 +163,8 @@ int check_delta(const ffn_ray_delta* a, bool backward) {
                            step(rows, a->v_row),     step(vh, a->v_head),      step(rows, a->decay_row), step(vh, a->decay_head),
                            step(rows, a->beta_row),  step(vh, a->beta_head),   backward ? step(rows, a->do_row) : 0,
                            backward ? step(vh, a->do_head) : 0};
-  for (int64_t s : steps)  // the kernels step through a chunk's rows with 32-bit offsets
-    if (s < 0 || s > MAX_SCAN_STRIDE / b) return fail(-1, "strides must be 0 or more, at most %d bytes", MAX_SCAN_STRIDE);
+  for (int64_t s : steps)  // the kernels step through a chunk's rows with products of 24 bits
+    if (s < 0 || s >= MAX_DELTA_STRIDE / b) return fail(-1, "strides must be 0 or more, below %d bytes", MAX_DELTA_STRIDE);
   if (!aligned(a->q, step(rows, a->q_row), b) || !aligned(a->q, step(h, a->q_head), b) || !aligned(a->k, step(rows, a->k_row), b) ||
       !aligned(a->k, step(h, a->k_head), b) || !aligned(a->v, step(rows, a->v_row), b) || !aligned(a->v, step(vh, a->v_head), b))
     return fail(-1, "rows and heads of q, k and v must be 16-byte aligned");

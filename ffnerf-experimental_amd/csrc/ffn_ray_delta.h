@@ -21,6 +21,7 @@
 // at 16 times the rate (K = 32; 8 times at K = 16), to the same accuracy.
 #pragma once
 #include <algorithm>
+#include <type_traits>
 
 #include "ffn_ray_common.h"
 #include "ffn_ray_kernels.h"
@@ -238,23 +239,35 @@ struct Chunk {
   }
 };
 
-// element `at` rows on from the row at p, rows `stride` < 2^27 bytes apart
-template <typename T> __device__ __forceinline__ const T* row_ptr(const T* p, uint32_t at, int64_t stride) {
-  return reinterpret_cast<const T*>(reinterpret_cast<const char*>(p) + at * (uint32_t)(stride * (int64_t)sizeof(T)));
+// `at` < 16 rows and `col` elements on from p, rows `stride` < 2^24 bytes apart: a base of the wavefront and 32 bits of the lane
+template <typename T> __device__ __forceinline__ T* row_ptr(T* p, uint32_t at, int64_t stride, uint32_t col) {
+  typedef typename std::conditional<std::is_const<T>::value, const char, char>::type byte;
+  const uint32_t off = __umul24(at, (uint32_t)(stride * (int64_t)sizeof(T))) + col * (uint32_t)sizeof(T);
+  return reinterpret_cast<T*>(reinterpret_cast<byte*>(p) + off);
 }
+// the rows of places 4 g + r of a chunk
+struct Rows4 {
+  uint32_t at[4];
+  __device__ __forceinline__ Rows4(const Chunk& ck, int g) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) at[r] = ck.at(4 * g + r);
+  }
+};
 
 // this lane's part of a chunk's row c: four values of every 16 columns, as they lie in memory
 template <typename T, int N> struct RawRow {
   typedef T tvec __attribute__((ext_vector_type(4)));
   tvec v[N];
   __device__ __forceinline__ void load(const T* base, int64_t stride, const Chunk& ck, int c, int g, int cols) {
-    const T* p = row_ptr(base + ck.low * stride, ck.at(c), stride);
+    const uint32_t at = ck.at(c);
     if (cols == 16 * N) {
+      const T* p = row_ptr(base + ck.low * stride, at, stride, 4 * g);
 #pragma unroll
-      for (int t = 0; t < N; ++t) v[t] = *reinterpret_cast<const tvec*>(p + 16 * t + 4 * g);
+      for (int t = 0; t < N; ++t) v[t] = *reinterpret_cast<const tvec*>(p + 16 * t);
     } else {
 #pragma unroll
-      for (int t = 0; t < N; ++t) v[t] = *reinterpret_cast<const tvec*>(p + (16 * t + 4 * g < cols ? 16 * t + 4 * g : 0));
+      for (int t = 0; t < N; ++t)
+        v[t] = *reinterpret_cast<const tvec*>(row_ptr(base + ck.low * stride, at, stride, 16 * t + 4 * g < cols ? 16 * t + 4 * g : 0));
     }
   }
   // 0 past the ray's end or the columns
@@ -274,10 +287,9 @@ template <typename T, int N> struct RawRow {
 // column `col` of the chunk's rows 4 g + r
 template <typename T> struct RawCol {
   T v[4];
-  __device__ __forceinline__ void load(const T* base, int64_t stride, const Chunk& ck, int g, int col, int cols) {
-    const T* p = base + ck.low * stride + (col < cols ? col : 0);
+  __device__ __forceinline__ void load(const T* base, int64_t stride, const Chunk& ck, const Rows4& rows, int col, int cols) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = *row_ptr(p, ck.at(4 * g + r), stride);
+    for (int r = 0; r < 4; ++r) v[r] = *row_ptr(base + ck.low * stride, rows.at[r], stride, col < cols ? col : 0);
   }
   __device__ __forceinline__ f32x4 value(const Chunk& ck, int g, int col, int cols) const {
     f32x4 x;
@@ -293,11 +305,11 @@ template <typename T> struct RawCol {
 // the decays of the chunk's rows 4 g + r and the strength of its row c
 template <typename T> struct RawGates {
   T d[4], b;
-  __device__ __forceinline__ void load(const ffn_ray_delta& a, int h, const Chunk& ck, int c, int g) {
+  __device__ __forceinline__ void load(const ffn_ray_delta& a, int h, const Chunk& ck, const Rows4& rows, int c) {
     const T *dp = (const T*)a.decay + ck.low * a.decay_row + h * a.decay_head, *bp = (const T*)a.beta + ck.low * a.beta_row + h * a.beta_head;
-    b = *row_ptr(bp, ck.at(c), a.beta_row);
+    b = *row_ptr(bp, ck.at(c), a.beta_row, 0);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) d[r] = *row_ptr(dp, ck.at(4 * g + r), a.decay_row);
+    for (int r = 0; r < 4; ++r) d[r] = *row_ptr(dp, rows.at[r], a.decay_row, 0);
   }
   __device__ __forceinline__ f32x4 decay(const Chunk& ck, int g) const {
     f32x4 y;
@@ -506,7 +518,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_fwd(const ffn_ray_delta a) {
       const Chunk ck(ch, p);
       kr.load(k, a.k_row, ck, c, g, a.key_dim);
       qr.load(q, a.q_row, ck, c, g, a.key_dim);
-      gates.load(a, h, ck, c, g);
+      gates.load(a, h, ck, Rows4(ck, g), c);
     }
   };
   fetch(DL_C * w);
@@ -518,7 +530,10 @@ __global__ __launch_bounds__(64 * W) void k_delta_fwd(const ffn_ray_delta a) {
     RawCol<T> vr[CH];
 #pragma unroll
     for (int i = 0; i < CH; ++i)
-      if (p0 + DL_C * i < ch.count) vr[i].load(v, a.v_row, Chunk(ch, p0 + DL_C * i), g, w16 + c, a.val_dim);
+      if (p0 + DL_C * i < ch.count) {
+        const Chunk ck(ch, p0 + DL_C * i);
+        vr[i].load(v, a.v_row, ck, Rows4(ck, g), w16 + c, a.val_dim);
+      }
     if (w < CH && p0 + DL_C * w < ch.count) {
       const Chunk ck(ch, p0 + DL_C * w);
       kr.trim(ck, c, g, a.key_dim);
@@ -569,11 +584,11 @@ __global__ __launch_bounds__(64 * W) void k_delta_fwd(const ffn_ray_delta a) {
           y = mul16(Pr, n, qs);
         }
         T* o = (T*)a.o + (ck.low * a.v_heads + h) * a.val_dim;
-        const int64_t stride = (int64_t)a.v_heads * a.val_dim;
         if (w16 + c < a.val_dim) {
+          const Rows4 rows(ck, g);
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (4 * g + r < ck.many) *const_cast<T*>(row_ptr(o + w16 + c, ck.at(4 * g + r), stride)) = (T)y[r];
+            if (4 * g + r < ck.many) *row_ptr(o, rows.at[r], (int64_t)a.v_heads * a.val_dim, w16 + c) = (T)y[r];
         }
         const typename Ops::Full nl = Ops::full(left * n);
 #pragma unroll
@@ -665,9 +680,9 @@ __global__ __launch_bounds__(256) void k_delta_step(const ffn_ray_delta a) {
 
 // The backward pass.  Segments of two chunks from the ray's end, each from the state that the forward kept: its chunks'
 // states and writes again, then the chunks back to front.  With dS the gradient of the state after a chunk:
-//   dn = P^T do + D_15 K dS,  dR = T^T dn,  dv = b dR,  X = D (do n^T) (j <= i),  Y = -D (dR n^T) (j < i)
-//   dq_i = scale (e_i S do_i + sum_j X_ij k_j),  left_i = -e_i S dR_i + sum_j Y_ij k_j
-//   right_j = D_15,j dS n_j + sum_i (scale X_ij q_i + b_i Y_ij k_i),  dk = b left + right,  db_i = k_i.left_i + v_i.dR_i
+//   dn = P^T do + D_15 K dS,  dR = T^T dn,  dv = b dR,  X = scale D (do n^T) (j <= i),  Y = -D (dR n^T) (j < i)
+//   dq_i = scale e_i S do_i + sum_j X_ij k_j,  left_i = -e_i S dR_i + sum_j Y_ij k_j
+//   right_j = D_15,j dS n_j + sum_i (X_ij q_i + b_i Y_ij k_i),  dk = b left + right,  db_i = k_i.left_i + v_i.dR_i
 //   dS' = e_15 dS + sum_i (scale e_i q_i do_i^T - b_i e_i k_i dR_i^T)
 // Every factor e or D a row i was multiplied with gives its sum of products to the decays up to i:
 //   ddecay = sums, from each row to the chunk's end, of q.dq + b k.left - k.right, and at the end dS.S
@@ -702,7 +717,39 @@ template <typename T> struct Tiles {
     }
   }
 };
-// the same for values of the type
+// A 16 x 16 matrix of floats, put down as this lane's row c, columns 4 g + s, and taken up by rows or by columns.
+template <typename T> struct Square {
+  float* p;  // 256
+  __device__ __forceinline__ void set(int c, int g, const f32x4& x) const {
+    if constexpr (Delta<T>::EXACT) {
+      const Parts<2> y = parts_of<2>(x);
+      __bf16* q = (__bf16*)p + c * 16 + 4 * g;
+      *reinterpret_cast<b16x4*>(q) = y.p[0];
+      *reinterpret_cast<b16x4*>(q + 256) = y.p[1];
+    } else {
+      *reinterpret_cast<f32x4*>(p + c * 16 + 4 * (g ^ (c >> 2))) = x;
+    }
+  }
+  __device__ __forceinline__ typename Delta<T>::Two row(int c, int g) const {
+    if constexpr (Delta<T>::EXACT) {
+      const __bf16* q = (const __bf16*)p + c * 16 + 4 * g;
+      return {{*reinterpret_cast<const b16x4*>(q), *reinterpret_cast<const b16x4*>(q + 256)}};
+    } else {
+      return *reinterpret_cast<const f32x4*>(p + c * 16 + 4 * (g ^ (c >> 2)));
+    }
+  }
+  __device__ __forceinline__ typename Delta<T>::Two col(int c, int g) const {
+    if constexpr (Delta<T>::EXACT) {
+      return {{col_of((const __bf16*)p, c, g), col_of((const __bf16*)p + 256, c, g)}};
+    } else {
+      f32x4 x;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) x[s] = p[(4 * g + s) * 16 + 4 * ((c >> 2) ^ g) + (c & 3)];
+      return x;
+    }
+  }
+};
+// values of the type, as Tiles
 template <typename T> struct RowTiles {
   T* p;
   __device__ __forceinline__ void set(int tile, int c, int g, const f32x4& x) const {
@@ -731,7 +778,7 @@ __device__ __forceinline__ f32x4 mul_cols(A a, B b, f32x4 c) {
 
 template <typename T, int DK, int W> struct DeltaLds {
   static constexpr int SQ = DL_C * DL_LD, NT = DK / 16;
-  static constexpr int WORDS = DL_SEG * (3 * SQ + DL_VEC) + 2 * SQ + (2 + NT) * W * Tiles<T>::WORDS + W * 32;
+  static constexpr int WORDS = DL_SEG * (3 * SQ + DL_VEC) + 3 * 256 + (2 + NT) * W * Tiles<T>::WORDS + W * 32;
   static constexpr int BYTES = WORDS * 4 + (2 * DL_SEG * NT + W) * Tile<T>::SIZE * (int)sizeof(T);
 };
 
@@ -761,10 +808,9 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
   float* Pm = Tm + DL_SEG * SQ;
   float* Dm = Pm + DL_SEG * SQ;
   float* vecs = Dm + DL_SEG * SQ;
-  float* Xm = vecs + DL_SEG * DL_VEC;
-  float* Ym = Xm + SQ;
+  const Square<T> Xm{vecs + DL_SEG * DL_VEC}, Ym{Xm.p + 256}, Zm{Ym.p + 256};
   // n, dR; S and dS, tile t W + u: rows of tile t, columns of wavefront u
-  const Tiles<T> Nl{Ym + SQ}, Rl{Nl.p + W * Tiles<T>::WORDS}, Sl{Rl.p + W * Tiles<T>::WORDS};
+  const Tiles<T> Nl{Zm.p + 256}, Rl{Nl.p + W * Tiles<T>::WORDS}, Sl{Rl.p + W * Tiles<T>::WORDS};
   float* sums = Sl.p + NT * W * Tiles<T>::WORDS;
   T* Kl = (T*)(sums + W * 32);
   T* Ql = Kl + DL_SEG * NT * TILE;
@@ -789,8 +835,9 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
     for (int i = 0; i < DL_SEG; ++i) {
       if (p0 + DL_C * i < ch.count) {
         const Chunk ck(ch, p0 + DL_C * i);
-        vr[i].load(v, a.v_row, ck, g, w16 + c, a.val_dim);
-        gr[i].load(dout, a.do_row, ck, g, w16 + c, a.val_dim);
+        const Rows4 rows(ck, g);
+        vr[i].load(v, a.v_row, ck, rows, w16 + c, a.val_dim);
+        gr[i].load(dout, a.do_row, ck, rows, w16 + c, a.val_dim);
       }
     }
     f32x4 S[DL_SEG][NT], n[DL_SEG];
@@ -804,7 +851,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
       RawGates<T> gates;
       kr.load(k, a.k_row, ck, c, g, a.key_dim);
       qr.load(q, a.q_row, ck, c, g, a.key_dim);
-      gates.load(a, h, ck, c, g);
+      gates.load(a, h, ck, Rows4(ck, g), c);
       kr.trim(ck, c, g, a.key_dim);
       qr.trim(ck, c, g, a.key_dim);
       Row kf[NT], qf[NT];
@@ -877,14 +924,12 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
         for (int s = 0; s < 4; ++s) col[s] = Tc[(4 * g + s) * DL_LD + c];
         dR = mul16(col, dn, zero);
         f32x4 to_beta = vv * dR, to_decay = zero;
-        {
+        const Rows4 rows(ck, g);
+        if (vcol < a.val_dim) {
           T* dv = (T*)a.dv + (ck.low * a.v_heads + h) * a.val_dim;
-          const int64_t stride = (int64_t)a.v_heads * a.val_dim;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            if (4 * g + r < ck.many && vcol < a.val_dim)
-              *const_cast<T*>(row_ptr(dv + vcol, ck.at(4 * g + r), stride)) = (T)(beta[r] * dR[r]);
-          }
+          for (int r = 0; r < 4; ++r)
+            if (4 * g + r < ck.many) *row_ptr(dv, rows.at[r], (int64_t)a.v_heads * a.val_dim, vcol) = (T)(beta[r] * dR[r]);
         }
         Nl.set(w, c, g, n[i]);
         Rl.set(w, c, g, dR);
@@ -907,14 +952,15 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
           if (w == 0) {
             f32x4 x = mul_cols<T, W>(n_row, g_row, zero);  // rows j, column i
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = 4 * g + r <= c ? D[r] * x[r] : 0.f;
-            *reinterpret_cast<f32x4*>(Xm + c * DL_LD + 4 * g) = x;
+            for (int r = 0; r < 4; ++r) x[r] = 4 * g + r <= c ? a.scale * D[r] * x[r] : 0.f;
+            Xm.set(c, g, x);
           }
           if (w == 1 || W == 1) {
             f32x4 y = mul_cols<T, W>(n_row, r_row, zero);
 #pragma unroll
             for (int r = 0; r < 4; ++r) y[r] = 4 * g + r < c ? -D[r] * y[r] : 0.f;
-            *reinterpret_cast<f32x4*>(Ym + c * DL_LD + 4 * g) = y;
+            Ym.set(c, g, y);
+            Zm.set(c, g, vec[c] * y);
           }
         }
         f32x4 dq[TP], lf[TP];
@@ -936,14 +982,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
           dS[t] = Ops::mul(col_of(Kc + t * TILE, c, g), fr, Ops::mul(col_of(Qc + t * TILE, c, g), fo, vec[48] * dS[t]));
         }
         sync();
-        f32x4 xc, yc;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          xc[s] = a.scale * Xm[(4 * g + s) * DL_LD + c];
-          yc[s] = beta[s] * Ym[(4 * g + s) * DL_LD + c];
-        }
-        const typename Ops::Two xr = Ops::two(*reinterpret_cast<const f32x4*>(Xm + c * DL_LD + 4 * g)),
-                                yr = Ops::two(*reinterpret_cast<const f32x4*>(Ym + c * DL_LD + 4 * g)), xt = Ops::two(xc), yt = Ops::two(yc);
+        const typename Ops::Two xr = Xm.row(c, g), yr = Ym.row(c, g), xt = Xm.col(c, g), zt = Zm.col(c, g);
 #pragma unroll
         for (int j = 0; j < TP; ++j) {
           const int t = w + j * W, kcol = 16 * t + c;
@@ -951,26 +990,32 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
             const auto s_row = [&](int u) { return Sl.get(t * W + u, c, g); };
             const Row kt = col_of(Kc + t * TILE, c, g), qt = col_of(Qc + t * TILE, c, g);
             const f32x4 kv = Ops::value(kt), qv = Ops::value(qt);
-            const f32x4 gq = a.scale * Ops::mul(xr, kt, e * dq[j]);
+            const f32x4 gq = Ops::mul(xr, kt, a.scale * e * dq[j]);
             const f32x4 gl = Ops::mul(yr, kt, -(e * lf[j]));
-            const f32x4 end = left * mul_cols<T, W>(n_row, s_row, zero), right = Ops::mul(yt, kt, Ops::mul(xt, qt, end));
+            const f32x4 end = left * mul_cols<T, W>(n_row, s_row, zero), right = Ops::mul(zt, kt, Ops::mul(xt, qt, end));
 #pragma unroll
             for (int r = 0; r < 4; ++r) inner = __builtin_fmaf(kv[r], end[r], inner);  // .. and what the chunk wrote
             const f32x4 gk = beta * gl + right;
             to_beta += kv * gl;
             to_decay += qv * gq + beta * (kv * gl) - kv * right;
             if (kcol < a.key_dim) {
+              if (shared) {
+                float* part = (float*)a.workspace + (ck.low * a.v_heads + h) * a.key_dim;
+                const int64_t other = (int64_t)a.rays.n * a.v_heads * a.key_dim, stride = (int64_t)a.v_heads * a.key_dim;
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                if (4 * g + r < ck.many) {
-                  if (shared) {
-                    const int64_t to = ((ck.low + ck.at(4 * g + r)) * a.v_heads + h) * a.key_dim + kcol;
-                    ((float*)a.workspace)[to] = gq[r];
-                    ((float*)a.workspace)[to + (int64_t)a.rays.n * a.v_heads * a.key_dim] = gk[r];
-                  } else {
-                    const int64_t low = (ck.low * a.heads + h) * a.key_dim + kcol, stride = (int64_t)a.heads * a.key_dim;
-                    *const_cast<T*>(row_ptr((T*)a.dq + low, ck.at(4 * g + r), stride)) = (T)gq[r];
-                    *const_cast<T*>(row_ptr((T*)a.dk + low, ck.at(4 * g + r), stride)) = (T)gk[r];
+                for (int r = 0; r < 4; ++r) {
+                  if (4 * g + r < ck.many) {
+                    *row_ptr(part, rows.at[r], stride, kcol) = gq[r];
+                    *row_ptr(part + other, rows.at[r], stride, kcol) = gk[r];
+                  }
+                }
+              } else {
+                const int64_t low = (ck.low * a.heads + h) * a.key_dim, stride = (int64_t)a.heads * a.key_dim;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  if (4 * g + r < ck.many) {
+                    *row_ptr((T*)a.dq + low, rows.at[r], stride, kcol) = (T)gq[r];
+                    *row_ptr((T*)a.dk + low, rows.at[r], stride, kcol) = (T)gk[r];
                   }
                 }
               }

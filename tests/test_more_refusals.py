@@ -109,7 +109,7 @@ def _delta(**kw):
     (dict(scale=float("inf")), "scale="), (dict(rays=dict(n=1 << 31)), "exceed"), (dict(rays=dict(counts=None)), "NULL counts"),
     (dict(rays=dict(ray_ids=None)), "NULL ray_ids"), (dict(rays=dict(num_rays=(1 << 32) - 1), v_heads=32), "2^36"),
     (dict(q=None), "NULL buffer"), (dict(beta=None), "NULL buffer"), (dict(q=P + 2), "aligned"), (dict(k_row=65), "aligned"),
-    (dict(v_head=4), "aligned"), (dict(q_row=-64), "strides"), (dict(decay_head=-1), "strides"), (dict(k_row=(1 << 26) + 8), "strides"), (dict(decay=P + 1), "misaligned"),
+    (dict(v_head=4), "aligned"), (dict(q_row=-64), "strides"), (dict(decay_head=-1), "strides"), (dict(k_row=1 << 23), "strides"), (dict(decay=P + 1), "misaligned"),
     (dict(h0=P + 4), "h0 must"), (dict(marks=P + 4), "16-byte aligned"),
 ])
 def test_delta_refuses(kw, match):
