@@ -34,6 +34,7 @@ constexpr int DL_MARK = DL_C * DL_SEG;
 constexpr int DL_LD = 20;             // LDS row of a 16 x 16 matrix
 constexpr int DL_VEC = 64;            // a chunk's b, e, D_15 and (first of the last 16) e_15
 constexpr float DL_RESET = -1e30f;    // stands for a decay of -infinity, which must not meet a zero in a product
+constexpr int DL_FEW = 2048;          // wavefronts: two a SIMD
 constexpr int DL_CLEAR = 1024;        // rows that one block looks through for those of no ray
 
 // ---------------------------------------------------------------------------
@@ -221,17 +222,22 @@ __device__ __forceinline__ Chain chain_of(const ffn_ray_delta& a, int64_t ray) {
 }
 // where the state before place p (a multiple of DL_MARK above 0) is kept: places of one ray, and of rays that do not
 // overlap, never share a slot
-__device__ __forceinline__ int64_t mark_slot(const Chain& ch, int p) { return (ch.first + p) / DL_MARK; }
+__device__ __forceinline__ int64_t mark_slot(const Chain& ch, int p) { return (uint32_t)(ch.first + p) / DL_MARK; }
 
 // The rows of the chunk at place p0: `many` of them from row `low` on.  Place i's row is low + at(i); past the ray's end it
 // is that of the last place, whose values are then dropped: under a branch each load would wait for the one before it.
 struct Chunk {
-  int64_t low;
+  uint32_t low;
   int many;
   bool back;
   __device__ __forceinline__ Chunk(const Chain& ch, int p0)
       : low(0), many(min(DL_C, ch.count - p0)), back(ch.back) {
-    low = back ? ch.first + ch.count - p0 - many : ch.first + p0;
+    low = (uint32_t)ch.first + (uint32_t)(back ? ch.count - p0 - many : p0);
+  }
+  // its first row in an array of rows `stride` < 2^24 bytes apart
+  template <typename T> __device__ __forceinline__ T* in(T* p, int64_t stride) const {
+    typedef typename std::conditional<std::is_const<T>::value, const char, char>::type byte;
+    return reinterpret_cast<T*>(reinterpret_cast<byte*>(p) + (uint64_t)low * ((uint32_t)stride * (uint32_t)sizeof(T)));
   }
   __device__ __forceinline__ uint32_t at(int i) const {
     const int j = min(i, many - 1);
@@ -261,13 +267,13 @@ template <typename T, int N> struct RawRow {
   __device__ __forceinline__ void load(const T* base, int64_t stride, const Chunk& ck, int c, int g, int cols) {
     const uint32_t at = ck.at(c);
     if (cols == 16 * N) {
-      const T* p = row_ptr(base + ck.low * stride, at, stride, 4 * g);
+      const T* p = row_ptr(ck.in(base, stride), at, stride, 4 * g);
 #pragma unroll
       for (int t = 0; t < N; ++t) v[t] = *reinterpret_cast<const tvec*>(p + 16 * t);
     } else {
 #pragma unroll
       for (int t = 0; t < N; ++t)
-        v[t] = *reinterpret_cast<const tvec*>(row_ptr(base + ck.low * stride, at, stride, 16 * t + 4 * g < cols ? 16 * t + 4 * g : 0));
+        v[t] = *reinterpret_cast<const tvec*>(row_ptr(ck.in(base, stride), at, stride, 16 * t + 4 * g < cols ? 16 * t + 4 * g : 0));
     }
   }
   // 0 past the ray's end or the columns
@@ -289,7 +295,7 @@ template <typename T> struct RawCol {
   T v[4];
   __device__ __forceinline__ void load(const T* base, int64_t stride, const Chunk& ck, const Rows4& rows, int col, int cols) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = *row_ptr(base + ck.low * stride, rows.at[r], stride, col < cols ? col : 0);
+    for (int r = 0; r < 4; ++r) v[r] = *row_ptr(ck.in(base, stride), rows.at[r], stride, col < cols ? col : 0);
   }
   __device__ __forceinline__ f32x4 value(const Chunk& ck, int g, int col, int cols) const {
     f32x4 x;
@@ -306,7 +312,7 @@ template <typename T> struct RawCol {
 template <typename T> struct RawGates {
   T d[4], b;
   __device__ __forceinline__ void load(const ffn_ray_delta& a, int h, const Chunk& ck, const Rows4& rows, int c) {
-    const T *dp = (const T*)a.decay + ck.low * a.decay_row + h * a.decay_head, *bp = (const T*)a.beta + ck.low * a.beta_row + h * a.beta_head;
+    const T *dp = ck.in((const T*)a.decay + h * a.decay_head, a.decay_row), *bp = ck.in((const T*)a.beta + h * a.beta_head, a.beta_row);
     b = *row_ptr(bp, ck.at(c), a.beta_row, 0);
 #pragma unroll
     for (int r = 0; r < 4; ++r) d[r] = *row_ptr(dp, rows.at[r], a.decay_row, 0);
@@ -583,12 +589,12 @@ __global__ __launch_bounds__(64 * W) void k_delta_fwd(const ffn_ray_delta a) {
         } else {
           y = mul16(Pr, n, qs);
         }
-        T* o = (T*)a.o + (ck.low * a.v_heads + h) * a.val_dim;
+        T* o = ck.in((T*)a.o + h * a.val_dim, a.v_heads * a.val_dim);
         if (w16 + c < a.val_dim) {
           const Rows4 rows(ck, g);
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (4 * g + r < ck.many) *row_ptr(o, rows.at[r], (int64_t)a.v_heads * a.val_dim, w16 + c) = (T)y[r];
+            if (4 * g + r < ck.many) *row_ptr(o, rows.at[r], a.v_heads * a.val_dim, w16 + c) = (T)y[r];
         }
         const typename Ops::Full nl = Ops::full(left * n);
 #pragma unroll
@@ -782,7 +788,9 @@ template <typename T, int DK, int W> struct DeltaLds {
   static constexpr int BYTES = WORDS * 4 + (2 * DL_SEG * NT + W) * Tile<T>::SIZE * (int)sizeof(T);
 };
 
-template <typename T, int DK, int W>
+// AHEAD: a segment's rows and state are asked for while the one after it is worked on.  That takes some 60 registers: it is
+// for few blocks, where nothing else hides the loads.
+template <typename T, int DK, int W, bool AHEAD>
 __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
   typedef Delta<T> Ops;
   typedef typename Ops::Row Row;
@@ -792,8 +800,14 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
   const int64_t block = block_number(), teams = (int64_t)a.rays.num_rays * a.v_heads;
   const bool shared = a.heads != a.v_heads;
   if (block >= teams) {
-    clear_rows(a, block - teams, (T*)a.dq, (int64_t)a.heads * a.key_dim);
-    clear_rows(a, block - teams, (T*)a.dk, (int64_t)a.heads * a.key_dim);
+    const int64_t width = (int64_t)a.v_heads * a.key_dim;
+    if (shared) {
+      clear_rows(a, block - teams, (float*)a.workspace, width);
+      clear_rows(a, block - teams, (float*)a.workspace + a.rays.n * width, width);
+    } else {
+      clear_rows(a, block - teams, (T*)a.dq, width);
+      clear_rows(a, block - teams, (T*)a.dk, width);
+    }
     clear_rows(a, block - teams, (T*)a.dv, (int64_t)a.v_heads * a.val_dim);
     clear_rows(a, block - teams, (T*)a.ddecay, (int64_t)a.v_heads);
     clear_rows(a, block - teams, (T*)a.dbeta, (int64_t)a.v_heads);
@@ -827,45 +841,66 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
   };
   f32x4 dS[NT];
   load_state(dS, a.dlast ? a.dlast + block * size : nullptr, a, c, g, w16);
-#pragma unroll 1
-  for (int p0 = ch.count ? (ch.count - 1) / DL_MARK * DL_MARK : -1; p0 >= 0; p0 -= DL_MARK) {
-    asm volatile("" : "+v"(c), "+v"(g));
-    RawCol<T> vr[DL_SEG], gr[DL_SEG];
+  constexpr int MINE = (DL_SEG + W - 1) / W;  // chunks that a wavefront prepares
+  RawRow<T, NT> kr[MINE], qr[MINE];
+  RawGates<T> gates[MINE];
+  RawCol<T> vn[DL_SEG], gn[DL_SEG];
+  f32x4 Sn[NT];
+  const auto fetch = [&](int p0) {
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+      const int p = p0 + DL_C * (w + j * W);
+      if (w + j * W < DL_SEG && p < ch.count) {
+        const Chunk ck(ch, p);
+        kr[j].load(k, a.k_row, ck, c, g, a.key_dim);
+        qr[j].load(q, a.q_row, ck, c, g, a.key_dim);
+        gates[j].load(a, h, ck, Rows4(ck, g), c);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < DL_SEG; ++i) {
       if (p0 + DL_C * i < ch.count) {
         const Chunk ck(ch, p0 + DL_C * i);
         const Rows4 rows(ck, g);
-        vr[i].load(v, a.v_row, ck, rows, w16 + c, a.val_dim);
-        gr[i].load(dout, a.do_row, ck, rows, w16 + c, a.val_dim);
+        vn[i].load(v, a.v_row, ck, rows, w16 + c, a.val_dim);
+        gn[i].load(dout, a.do_row, ck, rows, w16 + c, a.val_dim);
       }
     }
+    load_state(Sn, p0 ? a.marks + (mark_slot(ch, p0) * a.v_heads + h) * size : a.h0 ? a.h0 + block * size : nullptr, a, c, g, w16);
+  };
+  const int last = ch.count ? (ch.count - 1) / DL_MARK * DL_MARK : -1;
+  if (AHEAD && last >= 0) fetch(last);
+#pragma unroll 1
+  for (int p0 = last; p0 >= 0; p0 -= DL_MARK) {
+    asm volatile("" : "+v"(c), "+v"(g));
+    if (!AHEAD) fetch(p0);
+    RawCol<T> vr[DL_SEG], gr[DL_SEG];
     f32x4 S[DL_SEG][NT], n[DL_SEG];
-    const float* from = p0 ? a.marks + (mark_slot(ch, p0) * a.v_heads + h) * size : a.h0 ? a.h0 + block * size : nullptr;
-    load_state(S[0], from, a, c, g, w16);
-    for (int i = w; i < DL_SEG; i += W) {
-      const int p = p0 + DL_C * i;
-      if (p >= ch.count) break;
-      const Chunk ck(ch, p);
-      RawRow<T, NT> kr, qr;
-      RawGates<T> gates;
-      kr.load(k, a.k_row, ck, c, g, a.key_dim);
-      qr.load(q, a.q_row, ck, c, g, a.key_dim);
-      gates.load(a, h, ck, Rows4(ck, g), c);
-      kr.trim(ck, c, g, a.key_dim);
-      qr.trim(ck, c, g, a.key_dim);
-      Row kf[NT], qf[NT];
-      kr.operands(kf);
-      qr.operands(qf);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        typedef typename RawRow<T, NT>::tvec tvec;
-        *reinterpret_cast<tvec*>(Kl + (i * NT + t) * TILE + c * Tile<T>::LD + 4 * g) = kr.v[t];
-        *reinterpret_cast<tvec*>(Ql + (i * NT + t) * TILE + c * Tile<T>::LD + 4 * g) = qr.v[t];
+    for (int i = 0; i < DL_SEG; ++i) vr[i] = vn[i], gr[i] = gn[i];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) S[0][t] = Sn[t];
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+      const int i = w + j * W, p = p0 + DL_C * i;
+      if (i < DL_SEG && p < ch.count) {
+        const Chunk ck(ch, p);
+        kr[j].trim(ck, c, g, a.key_dim);
+        qr[j].trim(ck, c, g, a.key_dim);
+        Row kf[NT], qf[NT];
+        kr[j].operands(kf);
+        qr[j].operands(qf);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          typedef typename RawRow<T, NT>::tvec tvec;
+          *reinterpret_cast<tvec*>(Kl + (i * NT + t) * TILE + c * Tile<T>::LD + 4 * g) = kr[j].v[t];
+          *reinterpret_cast<tvec*>(Ql + (i * NT + t) * TILE + c * Tile<T>::LD + 4 * g) = qr[j].v[t];
+        }
+        prepare_chunk<T>(kf, qf, gates[j].decay(ck, g), gates[j].beta(ck, c), a.scale, c, g, Tm + i * SQ, Pm + i * SQ, Dm + i * SQ,
+                         vecs + i * DL_VEC);
       }
-      prepare_chunk<T>(kf, qf, gates.decay(ck, g), gates.beta(ck, c), a.scale, c, g, Tm + i * SQ, Pm + i * SQ, Dm + i * SQ,
-                       vecs + i * DL_VEC);
     }
+    if (AHEAD && p0) fetch(p0 - DL_MARK);
     sync();
     // the states before the segment's chunks, and their writes n
 #pragma unroll
@@ -926,10 +961,10 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
         f32x4 to_beta = vv * dR, to_decay = zero;
         const Rows4 rows(ck, g);
         if (vcol < a.val_dim) {
-          T* dv = (T*)a.dv + (ck.low * a.v_heads + h) * a.val_dim;
+          T* dv = ck.in((T*)a.dv + h * a.val_dim, a.v_heads * a.val_dim);
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (4 * g + r < ck.many) *row_ptr(dv, rows.at[r], (int64_t)a.v_heads * a.val_dim, vcol) = (T)(beta[r] * dR[r]);
+            if (4 * g + r < ck.many) *row_ptr(dv, rows.at[r], a.v_heads * a.val_dim, vcol) = (T)(beta[r] * dR[r]);
         }
         Nl.set(w, c, g, n[i]);
         Rl.set(w, c, g, dR);
@@ -963,13 +998,13 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
             Zm.set(c, g, vec[c] * y);
           }
         }
-        f32x4 dq[TP], lf[TP];
+        f32x4 sq[TP], lf[TP];
 #pragma unroll
         for (int j = 0; j < TP; ++j) {
           const int t = w + j * W;
           if (t < NT) {
             const auto s_row = [&](int u) { return Sl.get(t * W + u, c, g); };
-            dq[j] = mul_cols<T, W>(g_row, s_row, zero);
+            sq[j] = mul_cols<T, W>(g_row, s_row, zero);
             lf[j] = mul_cols<T, W>(r_row, s_row, zero);
           }
         }
@@ -990,7 +1025,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
             const auto s_row = [&](int u) { return Sl.get(t * W + u, c, g); };
             const Row kt = col_of(Kc + t * TILE, c, g), qt = col_of(Qc + t * TILE, c, g);
             const f32x4 kv = Ops::value(kt), qv = Ops::value(qt);
-            const f32x4 gq = Ops::mul(xr, kt, a.scale * e * dq[j]);
+            const f32x4 gq = Ops::mul(xr, kt, a.scale * e * sq[j]);
             const f32x4 gl = Ops::mul(yr, kt, -(e * lf[j]));
             const f32x4 end = left * mul_cols<T, W>(n_row, s_row, zero), right = Ops::mul(zt, kt, Ops::mul(xt, qt, end));
 #pragma unroll
@@ -1000,8 +1035,9 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
             to_decay += qv * gq + beta * (kv * gl) - kv * right;
             if (kcol < a.key_dim) {
               if (shared) {
-                float* part = (float*)a.workspace + (ck.low * a.v_heads + h) * a.key_dim;
-                const int64_t other = (int64_t)a.rays.n * a.v_heads * a.key_dim, stride = (int64_t)a.v_heads * a.key_dim;
+                const int stride = a.v_heads * a.key_dim;
+                const int64_t other = (int64_t)a.rays.n * stride;
+                float* part = ck.in((float*)a.workspace + h * a.key_dim, stride);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                   if (4 * g + r < ck.many) {
@@ -1010,12 +1046,13 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
                   }
                 }
               } else {
-                const int64_t low = (ck.low * a.heads + h) * a.key_dim, stride = (int64_t)a.heads * a.key_dim;
+                const int stride = a.heads * a.key_dim;
+                T *dq = ck.in((T*)a.dq + h * a.key_dim, stride), *dk = ck.in((T*)a.dk + h * a.key_dim, stride);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                   if (4 * g + r < ck.many) {
-                    *row_ptr((T*)a.dq + low, rows.at[r], stride, kcol) = (T)gq[r];
-                    *row_ptr((T*)a.dk + low, rows.at[r], stride, kcol) = (T)gk[r];
+                    *row_ptr(dq, rows.at[r], stride, kcol) = (T)gq[r];
+                    *row_ptr(dk, rows.at[r], stride, kcol) = (T)gk[r];
                   }
                 }
               }
@@ -1041,7 +1078,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
           }
           dd = sum_after(dd);
           if (c < ck.many) {
-            const int64_t to = (ck.low + ck.at(c)) * a.v_heads + h;
+            const int64_t to = (int64_t)(ck.low + ck.at(c)) * a.v_heads + h;
             ((T*)a.ddecay)[to] = (T)dd;
             ((T*)a.dbeta)[to] = (T)db;
           }
@@ -1052,22 +1089,22 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
   if (a.dh0) store_state(a.dh0 + block * size, dS, a, c, g, w16);
 }
 
-// dq and dk of key heads that value heads share, in a fixed order
+// dq and dk of key heads that value heads share, in a fixed order; four neighbouring columns a thread
 template <typename T>
 __global__ __launch_bounds__(256) void k_delta_join(const ffn_ray_delta a) {
-  const int64_t all = (int64_t)a.rays.n * a.heads * a.key_dim, i = block_number() * 256 + threadIdx.x;
-  if (i >= 2 * all) return;
-  const int64_t j = i < all ? i : i - all, row = j / ((int64_t)a.heads * a.key_dim);
-  const uint32_t r = a.rays.ray_ids[row];
-  if (r >= a.rays.num_rays) return;  // written as 0
-  const int64_t o = a.rays.offsets[r];
-  if (row < o || row - o >= (int64_t)a.rays.counts[r]) return;
-  const int x = (int)(j - row * a.heads * a.key_dim), hk = x / a.key_dim, col = x - hk * a.key_dim, per = a.v_heads / a.heads;
-  const float* from = (const float*)a.workspace + (i < all ? 0 : (int64_t)a.rays.n * a.v_heads * a.key_dim) +
-                      (row * a.v_heads + hk * per) * a.key_dim + col;
-  float s = 0.f;
-  for (int u = 0; u < per; ++u) s += from[(int64_t)u * a.key_dim];
-  ((T*)(i < all ? a.dq : a.dk))[j] = (T)s;
+  const uint32_t quads = (uint32_t)a.key_dim / 4, per = (uint32_t)(a.v_heads / a.heads);
+  const int64_t all = (int64_t)a.rays.n * a.heads * quads, i = block_number() * 256 + threadIdx.x;
+  if (i >= all) return;
+  const int64_t head = quotient(i, (int)quads);  // of row and key head
+  const int64_t at = (head * per * quads + (i - head * quads)) * 4, other = (int64_t)a.rays.n * a.v_heads * a.key_dim;
+  f32x4 q = {0.f, 0.f, 0.f, 0.f}, k = q;
+  for (uint32_t u = 0; u < per; ++u) {
+    const float* from = (const float*)a.workspace + at + (int64_t)u * a.key_dim;
+    q += load4(from);
+    k += load4(from + other);
+  }
+  store4((T*)a.dq + 4 * i, q);
+  store4((T*)a.dk + 4 * i, k);
 }
 
 // ---------------------------------------------------------------------------
@@ -1084,12 +1121,19 @@ hipError_t start_delta(const ffn_ray_delta& a, bool back, hipStream_t st) {
   }
   constexpr int bytes = DeltaLds<T, DK, W>::BYTES;
   static_assert(bytes <= 160 * 1024, "LDS");
-  if (bytes > 64 * 1024) {  // has to be allowed, on the device that is current
-    const hipError_t e = hipFuncSetAttribute((const void*)k_delta_bwd<T, DK, W>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != hipSuccess) return e;
-  }
-  k_delta_bwd<T, DK, W><<<grid, 64 * W, bytes, st>>>(a);
-  return hipGetLastError();
+  const auto start = [&](auto ahead) {
+    constexpr auto kernel = k_delta_bwd<T, DK, W, decltype(ahead)::value>;
+    if (bytes > 64 * 1024) {  // has to be allowed, on the device that is current
+      const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+      if (e != hipSuccess) return e;
+    }
+    kernel<<<grid, 64 * W, bytes, st>>>(a);
+    return hipGetLastError();
+  };
+  // 128 columns leave no registers for it, and a wavefront alone prepares both chunks of a segment
+  if constexpr (DK <= 64 && W > 1)
+    if ((int64_t)a.rays.num_rays * a.v_heads * W <= DL_FEW) return start(std::true_type{});
+  return start(std::false_type{});
 }
 
 template <typename T, int DK>
@@ -1106,7 +1150,7 @@ hipError_t delta_by_columns(const ffn_ray_delta& a, bool back, hipStream_t st) {
   else if (a.val_dim <= 64) e = start_delta<T, DK, 4>(a, back, st);
   else e = start_delta<T, DK, 8>(a, back, st);
   if (!back || e != hipSuccess || a.heads == a.v_heads || !a.rays.n) return e;
-  k_delta_join<T><<<grid_of((2 * (int64_t)a.rays.n * a.heads * a.key_dim + 255) / 256), 256, 0, st>>>(a);
+  k_delta_join<T><<<grid_of(((int64_t)a.rays.n * a.heads * a.key_dim / 4 + 255) / 256), 256, 0, st>>>(a);
   return hipGetLastError();
 }
 
