@@ -360,6 +360,16 @@ __device__ __forceinline__ void store_state(float* to, const f32x4 (&S)[NT], con
   }
 }
 
+// A state that is kept for the backward pass, as the wavefronts hold it: lane after lane, tile after tile.
+template <int NT> __device__ __forceinline__ void load_mark(f32x4 (&S)[NT], const float* from, int w, int lane) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t) S[t] = *reinterpret_cast<const f32x4*>(from + (w * NT + t) * 256 + 4 * lane);
+}
+template <int NT> __device__ __forceinline__ void store_mark(float* to, const f32x4 (&S)[NT], int w, int lane) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(to + (w * NT + t) * 256 + 4 * lane) = S[t];
+}
+
 // exp(x): the product with log2(e) in two parts, so that the result is as accurate as the hardware's 2^x
 __device__ __forceinline__ float exp_of(float x) {
   const float hi = x * 1.442695041f, lo = __builtin_fmaf(x, 1.442695041f, -hi);
@@ -563,7 +573,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_fwd(const ffn_ray_delta a) {
       const int p = p0 + DL_C * i;
       if (p < ch.count) {
         const Chunk ck(ch, p);
-        if (a.marks && p && p % DL_MARK == 0) store_state(a.marks + (mark_slot(ch, p) * a.v_heads + h) * size, S, a, c, g, w16);
+        if (a.marks && p && p % DL_MARK == 0) store_mark(a.marks + (mark_slot(ch, p) * a.v_heads + h) * (NT * W * 256), S, w, lane);
         const T *Kc = Kl + i * NT * TILE, *Qc = Ql + i * NT * TILE;
         Row kf[NT], qf[NT];
 #pragma unroll
@@ -582,13 +592,13 @@ __global__ __launch_bounds__(64 * W) void k_delta_fwd(const ffn_ray_delta a) {
         for (int t = 0; t < NT; ++t) full[t] = Ops::full(S[t]);
         const f32x4 R = beta * (vr[i].value(ck, g, w16 + c, a.val_dim) - e * mul_tiles<T>(kf, full, zero));
         const f32x4 qs = a.scale * e * mul_tiles<T>(qf, full, zero);
-        f32x4 n = mul16(Tr, R, zero), y;
-        if (__any(!finite4(n))) {
-          n = mul16_sick(Tr, R, zero, g);
-          y = mul16_sick(Pr, n, qs, g);
-        } else {
-          y = mul16(Pr, n, qs);
-        }
+        const f32x4 n = mul16(Tr, R, zero);
+        f32x4 y = mul16(Pr, n, qs);
+        const typename Ops::Full nl = Ops::full(left * n);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) S[t] = Ops::mul(col_of(Kc + t * TILE, c, g), nl, all * S[t]);
+        // a sick row leaves its columns of the state sick whatever the rows before it wrote, but not those rows' o
+        if (__any(!finite4(n))) y = mul16_sick(Pr, mul16_sick(Tr, R, zero, g), qs, g);
         T* o = ck.in((T*)a.o + h * a.val_dim, a.v_heads * a.val_dim);
         if (w16 + c < a.val_dim) {
           const Rows4 rows(ck, g);
@@ -596,9 +606,6 @@ __global__ __launch_bounds__(64 * W) void k_delta_fwd(const ffn_ray_delta a) {
           for (int r = 0; r < 4; ++r)
             if (4 * g + r < ck.many) *row_ptr(o, rows.at[r], a.v_heads * a.val_dim, w16 + c) = (T)y[r];
         }
-        const typename Ops::Full nl = Ops::full(left * n);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) S[t] = Ops::mul(col_of(Kc + t * TILE, c, g), nl, all * S[t]);
       }
     }
     if constexpr (W > 1) __syncthreads();
@@ -866,7 +873,8 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
         gn[i].load(dout, a.do_row, ck, rows, w16 + c, a.val_dim);
       }
     }
-    load_state(Sn, p0 ? a.marks + (mark_slot(ch, p0) * a.v_heads + h) * size : a.h0 ? a.h0 + block * size : nullptr, a, c, g, w16);
+    if (p0) load_mark(Sn, a.marks + (mark_slot(ch, p0) * a.v_heads + h) * (NT * W * 256), w, lane);
+    else load_state(Sn, a.h0 ? a.h0 + block * size : nullptr, a, c, g, w16);
   };
   const int last = ch.count ? (ch.count - 1) / DL_MARK * DL_MARK : -1;
   if (AHEAD && last >= 0) fetch(last);
@@ -1110,6 +1118,10 @@ __global__ __launch_bounds__(256) void k_delta_join(const ffn_ray_delta a) {
 // ---------------------------------------------------------------------------
 // launches
 
+// columns of a state's rows and rows, as the kernels hold it
+inline int delta_rows(int key_dim) { return key_dim <= 32 ? 32 : key_dim <= 64 ? 64 : 128; }
+inline int delta_waves(int val_dim) { return val_dim <= 64 ? (val_dim + 15) / 16 : 8; }
+
 inline int64_t delta_clear_blocks(const ffn_ray_delta& a) { return ((int64_t)a.rays.n + DL_CLEAR - 1) / DL_CLEAR; }
 
 template <typename T, int DK, int W>
@@ -1143,12 +1155,12 @@ hipError_t delta_by_columns(const ffn_ray_delta& a, bool back, hipStream_t st) {
     k_delta_step<T, DK><<<grid_of((teams + 3) / 4 + delta_clear_blocks(a)), 256, 0, st>>>(a);
     return hipGetLastError();
   }
-  hipError_t e;
-  if (a.val_dim <= 16) e = start_delta<T, DK, 1>(a, back, st);
-  else if (a.val_dim <= 32) e = start_delta<T, DK, 2>(a, back, st);
-  else if (a.val_dim <= 48) e = start_delta<T, DK, 3>(a, back, st);
-  else if (a.val_dim <= 64) e = start_delta<T, DK, 4>(a, back, st);
-  else e = start_delta<T, DK, 8>(a, back, st);
+  const int W = delta_waves(a.val_dim);
+  const hipError_t e = W == 1   ? start_delta<T, DK, 1>(a, back, st)
+                       : W == 2 ? start_delta<T, DK, 2>(a, back, st)
+                       : W == 3 ? start_delta<T, DK, 3>(a, back, st)
+                       : W == 4 ? start_delta<T, DK, 4>(a, back, st)
+                                : start_delta<T, DK, 8>(a, back, st);
   if (!back || e != hipSuccess || a.heads == a.v_heads || !a.rays.n) return e;
   k_delta_join<T><<<grid_of(((int64_t)a.rays.n * a.heads * a.key_dim / 4 + 255) / 256), 256, 0, st>>>(a);
   return hipGetLastError();
@@ -1156,8 +1168,9 @@ hipError_t delta_by_columns(const ffn_ray_delta& a, bool back, hipStream_t st) {
 
 template <typename T>
 hipError_t delta_of_type(const ffn_ray_delta& a, bool back, hipStream_t st) {
-  if (a.key_dim <= 32) return delta_by_columns<T, 32>(a, back, st);
-  if (a.key_dim <= 64) return delta_by_columns<T, 64>(a, back, st);
+  const int rows = delta_rows(a.key_dim);
+  if (rows == 32) return delta_by_columns<T, 32>(a, back, st);
+  if (rows == 64) return delta_by_columns<T, 64>(a, back, st);
   return delta_by_columns<T, 128>(a, back, st);
 }
 

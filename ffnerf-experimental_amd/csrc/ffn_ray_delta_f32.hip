@@ -6,7 +6,7 @@ namespace ffn {
 hipError_t delta_f32(const ffn_ray_delta& a, bool back, hipStream_t st) { return delta_of_type<float>(a, back, st); }
 
 uint64_t delta_marks(const ffn_ray_delta& a) {
-  return ((uint64_t)a.rays.n + DL_MARK - 1) / DL_MARK * a.v_heads * a.key_dim * a.val_dim * sizeof(float);
+  return ((uint64_t)a.rays.n + DL_MARK - 1) / DL_MARK * a.v_heads * delta_rows(a.key_dim) * delta_waves(a.val_dim) * 16 * sizeof(float);
 }
 uint64_t delta_workspace(const ffn_ray_delta& a) {
   return a.heads == a.v_heads ? 0 : 2ull * a.rays.n * a.v_heads * a.key_dim * sizeof(float);
