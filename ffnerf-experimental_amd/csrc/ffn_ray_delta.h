@@ -504,8 +504,11 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int b) {
   return a >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
 
+// wavefronts a SIMD that the forward's registers are held to, where no spill comes of it
+template <typename T, int DK, int W> constexpr int DL_FWD_WAVES = Delta<T>::EXACT && DK == 32 && W <= 2 ? 5 : 1;
+
 template <typename T, int DK, int W>
-__global__ __launch_bounds__(64 * W) void k_delta_fwd(const ffn_ray_delta a) {
+__global__ __launch_bounds__(64 * W, (DL_FWD_WAVES<T, DK, W>)) void k_delta_fwd(const ffn_ray_delta a) {
   constexpr int NT = DK / 16, TILE = Tile<T>::SIZE, CH = W < 4 ? W : 4;
   typedef Delta<T> Ops;
   typedef typename Ops::Row Row;
@@ -617,7 +620,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_fwd(const ffn_ray_delta a) {
 // Few rows a ray (one more sample of each): the state goes through once, row by row on the vector ALU, and memory bounds
 // it.  A wavefront takes 32 columns of a state: 8 lanes of four columns, 8 groups of rows dk = 8 i + group.
 template <typename T, int DK>
-__global__ __launch_bounds__(256) void k_delta_step(const ffn_ray_delta a) {
+__global__ __launch_bounds__(256, DK <= 32 ? 6 : DK <= 64 ? 5 : 3) void k_delta_step(const ffn_ray_delta a) {
   constexpr int N = DK / 8;
   const int parts = (a.val_dim + 31) / 32;
   const int64_t teams = (int64_t)a.rays.num_rays * a.v_heads * parts, blocks = (teams + 3) / 4;
@@ -957,12 +960,9 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
           }
           dn = left * mul_tiles<T>(kf, full, zero);
         }
-        Row gow;
-        if constexpr (Ops::EXACT) gow = __builtin_convertvector(go, b16x4);
-        else gow = go;
 #pragma unroll
         for (int s = 0; s < 4; ++s) col[s] = Pc[(4 * g + s) * DL_LD + c];
-        dn = Ops::mul(Ops::full(col), gow, dn);
+        dn = mul16(col, go, dn);  // in float: the vector ALU, which would make the parts, is the busier one
 #pragma unroll
         for (int s = 0; s < 4; ++s) col[s] = Tc[(4 * g + s) * DL_LD + c];
         dR = mul16(col, dn, zero);
