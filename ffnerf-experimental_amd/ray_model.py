@@ -1,11 +1,14 @@
-"""A model that looks along its rays, on the operators of ray_ops: an example that trains, and a module to start from.
+"""Models that look along their rays, on the operators of ray_ops: examples that train, and modules to start from.
 
 `march_samples` takes a batch's samples from the occupancy bitfield, `HashEncode` encodes them.  `RayModel` then lets the samples of
 a ray attend to those in front of them (ray_attention: causal in the ray's order, scores that fall with the distance in
 depth), carries features along the ray (ray_scan), sends every sample through the layers of its region of the box
-(expert_plan, expert_linear) and composites opacity and colour back to front (ray_scan again).
+(expert_plan, expert_linear) and composites opacity and colour back to front (ray_scan again).  `RayMixer` is a block of the
+other kind: normalised features (layer_norm), a matrix of what the ray has shown so far (ray_delta), and the layers of a
+sample's own region and of the nearest other one, blended (expert_route, expert_dispatch, expert_combine); it can be asked
+sample by sample, with the rays' states in hand.
 
-    python ffnerf-experimental_amd/ray_model.py --steps 200      # the synthetic ball scene
+    python ffnerf-experimental_amd/ray_model.py --steps 200 [--model mixer]     # the synthetic ball scene
 """
 from __future__ import annotations
 
@@ -18,7 +21,8 @@ import numpy as np
 import torch
 
 import ffn_lib as fl
-from ray_ops import ExpertLinear, RayAttention, RayScan, RaySet, expert_plan, once
+from ray_ops import (ExpertCombine, ExpertDispatch, ExpertLinear, LayerNorm, RayAttention, RayDelta, RayScan, RaySet,
+                     expert_plan, expert_route, once, ray_delta)
 
 
 class HashEncode(torch.autograd.Function):
@@ -107,8 +111,87 @@ class RayModel(torch.nn.Module):
         return RayScan.apply(opacity, torch.sigmoid(y[:, 1:4]), rays, None, True)[1]
 
 
-def train(steps: int = 200, num_rays: int = 1024, lr: float = 3e-3, seed: int = 0, report=None) -> list:
-    """Trains a RayModel on rays of the synthetic ball scene; the loss of each step."""
+class RayMixer(torch.nn.Module):
+    """features: width of the samples' features; cells: regions of the box an axis, each with expert layers of its own;
+    dtype: of the operators (the parameters stay float32)."""
+
+    def __init__(self, features: int, width: int = 64, heads: int = 4, cells: int = 2, box=((0.0,) * 3, (1.0,) * 3),
+                 dtype=torch.bfloat16):
+        super().__init__()
+        if width % (8 * heads):
+            raise ValueError(f"width={width} must be a multiple of 8 heads={heads}")
+        self.width, self.heads, self.cells, self.dtype, experts = width, heads, cells, dtype, cells ** 3
+
+        def weight(*shape):
+            return torch.nn.Parameter(torch.randn(shape) * shape[-1] ** -0.5)
+
+        def norm():
+            return torch.nn.Parameter(torch.ones(width)), torch.nn.Parameter(torch.zeros(width))
+
+        self.W_in, self.W_qkv, self.W_o = weight(width, features), weight(3 * width, width), weight(width, width)
+        self.W_gates, self.b_gates = weight(2 * heads, width), torch.nn.Parameter(torch.tensor([-3.0] * heads + [0.0] * heads))
+        self.W_1, self.b_1 = weight(experts, width, width), torch.nn.Parameter(torch.zeros(experts, width))
+        self.W_2, self.b_2 = weight(experts, width, width), torch.nn.Parameter(torch.zeros(experts, width))
+        self.W_out, self.b_out = weight(4, width), torch.nn.Parameter(torch.zeros(4))
+        (self.n_1, self.m_1), (self.n_2, self.m_2), (self.n_3, self.m_3) = norm(), norm(), norm()
+        self.register_buffer("lo", torch.tensor(box[0]))
+        self.register_buffer("hi", torch.tensor(box[1]))
+
+    def blend(self, samples):
+        """(ids [n, 2], weights [n, 2]): the region of each sample and the one across the nearest face, which has half the
+        weight at that face and none at the centre; -1 where the face is the box's own."""
+        u = ((samples[:, :3] - self.lo) / (self.hi - self.lo) * self.cells).clamp(0, self.cells)
+        c = u.floor().clamp(max=self.cells - 1)
+        off = u - c - 0.5
+        far, axis = off.abs().max(1)
+        to = torch.gather(c, 1, axis[:, None])[:, 0] + torch.sign(torch.gather(off, 1, axis[:, None])[:, 0])
+        other = c.scatter(1, axis[:, None], to[:, None])
+        inside = (to >= 0) & (to < self.cells) & (far > 0)
+        ids = torch.stack([(x[:, 2] * self.cells + x[:, 1]) * self.cells + x[:, 0] for x in (c, other)], 1).to(torch.int32)
+        ids[:, 1] = torch.where(inside, ids[:, 1], -1)
+        w = torch.where(inside, far.clamp(max=0.5), 0.0)
+        return ids, torch.stack((1 - w, w), 1)
+
+    def states(self, num_rays: int) -> torch.Tensor:
+        """States of rays of which nothing has been seen."""
+        d = self.width // self.heads
+        return torch.zeros(num_rays, self.heads, d, d, device=self.lo.device)
+
+    def look(self, samples, features, rays: RaySet, state=None):
+        """Opacity and colour, before their sigmoids, of each sample [n, 4] from it and those in front of it.  state
+        (without gradients): what the rays have shown before these samples; it is moved on in place."""
+        n, ty, d = samples.shape[0], self.dtype, self.width // self.heads
+        x = (features @ self.W_in.t()).to(ty)
+        h = LayerNorm.apply(x, self.n_1, self.m_1)
+        q, k, v = (h @ self.W_qkv.to(ty).t()).view(n, 3, self.heads, d).unbind(1)
+        q, k = (torch.nn.functional.normalize(t.float(), dim=-1).to(ty) for t in (q, k))
+        decay, beta = (h.float() @ self.W_gates.t() + self.b_gates).chunk(2, 1)
+        decay, beta = -torch.nn.functional.softplus(decay).to(ty), torch.sigmoid(beta).to(ty)
+        if state is None:
+            o = RayDelta.apply(q, k, v, decay, beta, rays, None, dict(last=False))[0]
+        else:
+            o = ray_delta(q, k, v, decay, beta, rays, h0=state, last=state)[0]
+        x = x + o.reshape(n, self.width) @ self.W_o.to(ty).t()
+        ids, weights = self.blend(samples)
+        route = expert_route(ids, self.cells ** 3)
+        y = ExpertDispatch.apply(LayerNorm.apply(x, self.n_2, self.m_2), route)
+        y = ExpertLinear.apply(y, self.W_1.to(ty), self.b_1.to(ty), route.plan, True, True, True)
+        y = ExpertLinear.apply(y, self.W_2.to(ty), self.b_2.to(ty), route.plan, False, True, True)
+        x = x + ExpertCombine.apply(y, route, weights)
+        return LayerNorm.apply(x, self.n_3, self.m_3).float() @ self.W_out.t() + self.b_out
+
+    def forward(self, samples, features, rays: RaySet) -> torch.Tensor:
+        """Colour [num_rays, 3] of each ray on a black background."""
+        y = self.look(samples, features, rays)
+        opacity = y[:, :1].expand(-1, 3).contiguous()
+        return RayScan.apply(opacity, torch.sigmoid(y[:, 1:4]), rays, None, True)[1]
+
+
+MODELS = {"attend": RayModel, "mixer": RayMixer}
+
+
+def train(steps: int = 200, num_rays: int = 1024, lr: float = 3e-3, seed: int = 0, report=None, model: str = "attend") -> list:
+    """Trains a model of MODELS on rays of the synthetic ball scene; the loss of each step."""
     import ffnerf_tools as ft
     import synthetic_scene as scene
     torch.manual_seed(seed)
@@ -124,16 +207,16 @@ def train(steps: int = 200, num_rays: int = 1024, lr: float = 3e-3, seed: int = 
     losses = []
     with tempfile.TemporaryDirectory() as d:
         nerf = ft.Nerf(d, "rays", spec=spec, occ=occ)
-        model = RayModel(spec.lf + 3).cuda()
+        net = MODELS[model](spec.lf + 3).cuda()
         table = torch.nn.Parameter(nerf.t["table"])  # the same memory: what the handle reads
-        adam = torch.optim.Adam([dict(params=model.parameters(), lr=lr), dict(params=[table], lr=10 * lr, eps=1e-15)])
+        adam = torch.optim.Adam([dict(params=net.parameters(), lr=lr), dict(params=[table], lr=10 * lr, eps=1e-15)])
         for step in range(steps):
             rays, targets = scene.uniform_batch(cams, num_rays, rng)
             rays = torch.from_numpy(ft.rays_as_array(rays)).cuda()
             want = torch.from_numpy(np.asarray(targets, np.float32)[:, :3].copy()).cuda()
             samples, ray_set = march_samples(nerf, rays, bits, R, dt, max_steps)
             xyz = samples[:, :3].contiguous()
-            colour = model(samples, torch.cat((HashEncode.apply(table, xyz, nerf), xyz), 1), ray_set)
+            colour = net(samples, torch.cat((HashEncode.apply(table, xyz, nerf), xyz), 1), ray_set)
             loss = ((colour - want) ** 2).mean()
             adam.zero_grad()
             loss.backward()
@@ -148,8 +231,9 @@ def main(argv=None) -> int:
     p = argparse.ArgumentParser(description="Train a model that looks along its rays on the synthetic ball scene.")
     p.add_argument("--steps", type=int, default=200)
     p.add_argument("--rays", type=int, default=1024)
+    p.add_argument("--model", choices=sorted(MODELS), default="attend")
     args = p.parse_args(argv)
-    train(args.steps, args.rays, report=lambda s: print(s, flush=True))
+    train(args.steps, args.rays, model=args.model, report=lambda s: print(s, flush=True))
     return 0
 
 
