@@ -166,7 +166,7 @@ __device__ __forceinline__ void rank_rows(const int32_t* __restrict__ ids, const
 // 12.1 / 13.3; 8192 rows 11.4 / 11.4 and 15.8 / 14.0, where three still cost the host more.
 constexpr int PS_NT = 1024, PS_ITEMS = 8, PS_ROWS = PS_NT * PS_ITEMS;
 __global__ __launch_bounds__(PS_NT) void k_plan_small(const int32_t* __restrict__ ids, PlanView v, int bits,
-                                                      uint32_t* __restrict__ plan) {
+                                                      uint32_t* __restrict__ plan, uint32_t* __restrict__ slots) {
   constexpr int NW = PS_NT / 64;
   __shared__ uint32_t first[PL_BINS + 1], total[PL_BINS], part[NW], cnt[NW][PL_BINS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -192,7 +192,11 @@ __global__ __launch_bounds__(PS_NT) void k_plan_small(const int32_t* __restrict_
 #pragma unroll
   for (int q = 0; q < PS_ITEMS; ++q) {
     const int64_t i = w0 + q * 64 + lane;
-    if (i < v.n) plan[v.rows + first[bin[q]] + cnt[wave][bin[q]] + rank[q]] = (uint32_t)i;
+    if (i < v.n) {
+      const uint32_t to = first[bin[q]] + cnt[wave][bin[q]] + rank[q];
+      plan[v.rows + to] = (uint32_t)i;
+      if (slots) slots[i] = to;
+    }
   }
   __syncthreads();
   bin_scan<PS_NT>(total, v.bins, first, part, [](uint32_t c) { return (c + EX_ROWS - 1) / EX_ROWS; });
@@ -201,7 +205,7 @@ __global__ __launch_bounds__(PS_NT) void k_plan_small(const int32_t* __restrict_
 
 __global__ __launch_bounds__(PL_NT) void k_plan_move(const int32_t* __restrict__ ids, PlanView v, int bits, int blocks,
                                                      const uint32_t* __restrict__ block_counts,
-                                                     uint32_t* __restrict__ plan) {
+                                                     uint32_t* __restrict__ plan, uint32_t* __restrict__ slots) {
   constexpr int NW = PL_NT / 64;
   __shared__ uint32_t first[PL_BINS + 1], part[NW], cnt[NW][PL_BINS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -234,7 +238,11 @@ __global__ __launch_bounds__(PL_NT) void k_plan_move(const int32_t* __restrict__
 #pragma unroll
   for (int q = 0; q < PL_ITEMS; ++q) {
     const int64_t i = w0 + q * 64 + lane;
-    if (i < v.n) plan[v.rows + cnt[wave][bin[q]] + rank[q]] = (uint32_t)i;
+    if (i < v.n) {
+      const uint32_t to = cnt[wave][bin[q]] + rank[q];
+      plan[v.rows + to] = (uint32_t)i;
+      if (slots) slots[i] = to;
+    }
   }
 }
 
@@ -245,20 +253,20 @@ uint64_t expert_plan_workspace(uint32_t n, int experts) {
   return n <= PS_ROWS ? 0 : (uint64_t)plan_blocks(n) * (experts + 1) * sizeof(uint32_t);
 }
 
-hipError_t launch_expert_plan(const int32_t* ids, uint32_t n, int experts, uint32_t* plan, uint32_t* workspace,
+hipError_t launch_expert_plan(const int32_t* ids, uint32_t n, int experts, uint32_t* plan, uint32_t* slots, uint32_t* workspace,
                               hipStream_t st) {
   const PlanView v = plan_view(n, experts);
   const int blocks = plan_blocks(n);
   int bits = 1;
   while ((1 << bits) < v.bins) ++bits;
   if (n <= PS_ROWS) {
-    k_plan_small<<<1, PS_NT, 0, st>>>(ids, v, bits, plan);
+    k_plan_small<<<1, PS_NT, 0, st>>>(ids, v, bits, plan, slots);
     return hipGetLastError();
   }
   k_plan_count<<<blocks, PL_NT, 0, st>>>(ids, v, workspace);
   k_plan_scan<<<v.bins, 64, 0, st>>>(workspace, blocks, plan, v);
   const int tile_blocks = (int)((v.n_tiles + PL_BLOCK - 1) / PL_BLOCK);
-  k_plan_move<<<blocks + tile_blocks, PL_NT, 0, st>>>(ids, v, bits, blocks, workspace, plan);
+  k_plan_move<<<blocks + tile_blocks, PL_NT, 0, st>>>(ids, v, bits, blocks, workspace, plan, slots);
   return hipGetLastError();
 }
 

@@ -123,6 +123,19 @@ int check_plan_sizes(uint32_t n, int32_t n_experts) {
   return 0;
 }
 
+int check_plan(const int32_t* ids, uint32_t n, int32_t n_experts, const uint32_t* plan, uint64_t plan_words,
+               const void* workspace, uint64_t workspace_bytes) {
+  if (int rc = check_plan_sizes(n, n_experts)) return rc;
+  if (n && !ids) return fail(-1, "NULL ids");
+  const uint64_t words = ffn::expert_plan_words(n, n_experts), need = ffn::expert_plan_workspace(n, n_experts);
+  if (!plan || !aligned(plan) || plan_words < words)
+    return fail(-1, "plan of %llu words, %llu wanted", (unsigned long long)(plan ? plan_words : 0), (unsigned long long)words);
+  if (need && (!workspace || !aligned(workspace) || workspace_bytes < need))
+    return fail(-1, "workspace of %llu bytes, %llu wanted", (unsigned long long)(workspace ? workspace_bytes : 0),
+                (unsigned long long)need);
+  return 0;
+}
+
 int check_experts(const ffn_experts* a) {
   if (!a) return fail(-1, "NULL arguments");
   if (!elem(a->dtype)) return fail(-1, "dtype=%d is not FFN_F32, FFN_F16 or FFN_BF16", a->dtype);
@@ -299,16 +312,17 @@ int ffn_expert_plan_size(uint32_t n, int32_t n_experts, uint64_t* plan_words, ui
 
 int ffn_expert_plan(const int32_t* ids, uint32_t n, int32_t n_experts, uint32_t* plan, uint64_t plan_words,
                     void* workspace, uint64_t workspace_bytes, void* stream) {
-  if (int rc = check_plan_sizes(n, n_experts)) return rc;
-  if (n && !ids) return fail(-1, "NULL ids");
-  const uint64_t words = ffn::expert_plan_words(n, n_experts), need = ffn::expert_plan_workspace(n, n_experts);
-  if (!plan || !aligned(plan) || plan_words < words)
-    return fail(-1, "plan of %llu words, %llu wanted", (unsigned long long)(plan ? plan_words : 0), (unsigned long long)words);
-  if (need && (!workspace || !aligned(workspace) || workspace_bytes < need))
-    return fail(-1, "workspace of %llu bytes, %llu wanted", (unsigned long long)(workspace ? workspace_bytes : 0),
-                (unsigned long long)need);
-  return launched(ffn::launch_expert_plan(ids, n, n_experts, plan, (uint32_t*)workspace, (hipStream_t)stream),
+  if (int rc = check_plan(ids, n, n_experts, plan, plan_words, workspace, workspace_bytes)) return rc;
+  return launched(ffn::launch_expert_plan(ids, n, n_experts, plan, nullptr, (uint32_t*)workspace, (hipStream_t)stream),
                   "ffn_expert_plan");
+}
+
+int ffn_expert_route(const int32_t* ids, uint32_t places, int32_t n_experts, uint32_t* plan, uint64_t plan_words, uint32_t* slots,
+                     void* workspace, uint64_t workspace_bytes, void* stream) {
+  if (int rc = check_plan(ids, places, n_experts, plan, plan_words, workspace, workspace_bytes)) return rc;
+  if (places && !slots) return fail(-1, "NULL slots");
+  return launched(ffn::launch_expert_plan(ids, places, n_experts, plan, slots, (uint32_t*)workspace, (hipStream_t)stream),
+                  "ffn_expert_route");
 }
 
 int ffn_expert_linear_fwd(const ffn_experts* a, void* stream) {
@@ -365,12 +379,6 @@ int ffn_layer_norm_bwd(const ffn_norm* a, void* stream) {
     return fail(-1, "workspace of %llu bytes, %llu wanted", (unsigned long long)(a->workspace ? a->workspace_bytes : 0),
                 (unsigned long long)need);
   return launched(ffn::launch_norm(*a, true, (hipStream_t)stream), "ffn_layer_norm_bwd");
-}
-
-int ffn_expert_slots(const uint32_t* plan, uint32_t places, int32_t n_experts, uint32_t* slots, void* stream) {
-  if (int rc = check_plan_sizes(places, n_experts)) return rc;
-  if (places && (!plan || !slots)) return fail(-1, "NULL plan or slots");
-  return launched(ffn::launch_route_slots(plan, places, n_experts, slots, (hipStream_t)stream), "ffn_expert_slots");
 }
 
 int ffn_expert_dispatch(const ffn_route* a, void* stream) {

@@ -20,7 +20,8 @@ hipError_t launch_delta(const ffn_ray_delta& a, bool backward, hipStream_t st);
 
 uint64_t expert_plan_words(uint32_t n, int experts);
 uint64_t expert_plan_workspace(uint32_t n, int experts);
-hipError_t launch_expert_plan(const int32_t* ids, uint32_t n, int experts, uint32_t* plan, uint32_t* workspace,
+// slots: the inverse of the plan's rows, or NULL
+hipError_t launch_expert_plan(const int32_t* ids, uint32_t n, int experts, uint32_t* plan, uint32_t* slots, uint32_t* workspace,
                               hipStream_t st);
 uint64_t expert_workspace(const ffn_experts& a);
 hipError_t launch_experts(const ffn_experts& a, bool backward, hipStream_t st);
@@ -28,7 +29,6 @@ hipError_t launch_experts(const ffn_experts& a, bool backward, hipStream_t st);
 uint64_t norm_workspace(const ffn_norm& a);
 hipError_t launch_norm(const ffn_norm& a, bool backward, hipStream_t st);
 
-hipError_t launch_route_slots(const uint32_t* plan, uint32_t places, int n_experts, uint32_t* slots, hipStream_t st);
 hipError_t launch_dispatch(const ffn_route& a, hipStream_t st);
 hipError_t launch_combine(const ffn_route& a, hipStream_t st);
 hipError_t launch_combine_bwd(const ffn_route& a, hipStream_t st);

@@ -1,7 +1,7 @@
 // ffn_route.hip -- rows to several experts and back: copies in the experts' order, weighted sums, their gradients.
 //
-// A plan (ffn_expert_plan) over the n k places (place i k + j: row i's j-th expert) says which place each slot holds; here
-// its inverse, the slot of each place, is kept beside it.  Everything then goes by rows: a team of lanes takes a row, its k
+// The plan over the n k places (place i k + j: row i's j-th expert) says which place each slot holds, and its move writes
+// the inverse, the slot of each place, in the places' order as it goes.  Everything then goes by rows: a team of lanes takes a row, its k
 // slots, and for each of them reads or writes one row of the slots' array.  So the rows' own array is passed over once,
 // and no sum is split: no atomics, one order.  A place of no expert has a slot behind all groups; it is written as 0 and
 // never read.  Memory bounds all of it.
@@ -11,11 +11,6 @@
 namespace ffn {
 
 constexpr int RT_NT = 256;
-
-__global__ __launch_bounds__(RT_NT) void k_route_slots(const uint32_t* __restrict__ places, uint32_t n, uint32_t* __restrict__ slots) {
-  const int64_t s = block_number() * RT_NT + threadIdx.x;
-  if (s < n) slots[places[s]] = (uint32_t)s;
-}
 
 // EL neighbouring columns: 16 bytes, or one column where rows are not aligned
 template <typename T, int EL> struct Part {
@@ -33,13 +28,12 @@ template <typename T, int EL> __device__ __forceinline__ void part_set(typename 
   else v[e] = (T)f;
 }
 
-constexpr int RT_AT_ONCE = 4;  // rows of slots a lane has on their way
-
 enum { ROUTE_OUT, ROUTE_BACK, ROUTE_GRAD };
 
 // OUT: slots_out[slot] = rows_in[i];  BACK: rows_out[i] = sum_j w_ij slots_in[slot_ij];
 // GRAD: slots_out[slot_ij] = w_ij rows_in[i], dweights_ij = rows_in[i] . slots_in[slot_ij]
-template <typename T, int EL, int WHAT>
+// U: rows of slots that a lane has on their way
+template <typename T, int EL, int WHAT, int U>
 __global__ __launch_bounds__(RT_NT) void k_route(const ffn_route a, int team) {
   typedef typename Part<T, EL>::type vec;
   const int lane = threadIdx.x & (team - 1), k = a.k;
@@ -50,83 +44,77 @@ __global__ __launch_bounds__(RT_NT) void k_route(const ffn_route a, int team) {
   const float* weights = a.weights ? a.weights + (there ? i : 0) * k : nullptr;
   const T* in = (const T*)a.rows_in + (there ? i : 0) * a.rows_stride;
   const T* from = (const T*)a.slots_in;
+  T* to = (T*)a.slots_out;
   const int width = there ? a.width : 0;
-  for (int j0 = 0; j0 < k; j0 += WHAT == ROUTE_GRAD ? RT_AT_ONCE : k) {
-    uint32_t slot[RT_AT_ONCE];
-    float w[RT_AT_ONCE], dot[RT_AT_ONCE];
-    if constexpr (WHAT == ROUTE_GRAD) {
+  // U places at a time, every load of them on its way before the first is waited for: places past k are the last one
+  // again, slots of no expert the first one; what is loaded there is dropped
+  for (int c0 = 0; c0 < (WHAT == ROUTE_BACK ? width : 1); c0 += team * EL) {
+    const int cb = c0 + lane * EL;  // of BACK
+    const bool in_row = cb < width;
+    float sum[EL];
 #pragma unroll
-      for (int u = 0; u < RT_AT_ONCE; ++u) {
-        slot[u] = j0 + u < k ? slots[j0 + u] : 0xFFFFFFFFu;
-        w[u] = weights && j0 + u < k ? weights[j0 + u] : 1.f;
+    for (int e = 0; e < EL; ++e) sum[e] = 0.f;
+    for (int j = 0; j < k; j += U) {
+      uint32_t slot[U];
+      float w[U], dot[U];
+      bool kept_u[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        slot[u] = slots[min(j + u, k - 1)];
+        w[u] = WHAT != ROUTE_OUT && weights ? weights[min(j + u, k - 1)] : 1.f;
         dot[u] = 0.f;
       }
-    }
-    for (int c = lane * EL; c < width; c += team * EL) {
-      if constexpr (WHAT == ROUTE_OUT) {
-        const vec x = *reinterpret_cast<const vec*>(in + c);
-        for (int j = 0; j < k; ++j) {
-          const uint32_t s = slots[j];
-          *reinterpret_cast<vec*>((T*)a.slots_out + (int64_t)s * a.width + c) = s < kept ? x : vec{};
+#pragma unroll
+      for (int u = 0; u < U; ++u) kept_u[u] = slot[u] < kept && j + u < k;
+      if constexpr (WHAT == ROUTE_BACK) {
+        vec y[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          y[u] = *reinterpret_cast<const vec*>(from + (int64_t)(kept_u[u] ? slot[u] : 0) * a.slots_stride + (in_row ? cb : 0));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+          for (int e = 0; e < EL; ++e) sum[e] = kept_u[u] ? __builtin_fmaf(w[u], part_at<T, EL>(y[u], e), sum[e]) : sum[e];
         }
-      } else if constexpr (WHAT == ROUTE_BACK) {
-        float sum[EL];
-#pragma unroll
-        for (int e = 0; e < EL; ++e) sum[e] = 0.f;
-        for (int j = 0; j < k; j += RT_AT_ONCE) {
-          vec y[RT_AT_ONCE];
-          float f[RT_AT_ONCE];
-#pragma unroll
-          for (int u = 0; u < RT_AT_ONCE; ++u) {
-            const uint32_t s = j + u < k ? slots[j + u] : 0xFFFFFFFFu;
-            y[u] = vec{};
-            f[u] = 0.f;
-            if (s < kept) {
-              y[u] = *reinterpret_cast<const vec*>(from + (int64_t)s * a.slots_stride + c);
-              f[u] = weights ? weights[j + u] : 1.f;
-            }
-          }
-#pragma unroll
-          for (int u = 0; u < RT_AT_ONCE; ++u) {
-#pragma unroll
-            for (int e = 0; e < EL; ++e) sum[e] = __builtin_fmaf(f[u], part_at<T, EL>(y[u], e), sum[e]);
-          }
-        }
-        vec out;
-#pragma unroll
-        for (int e = 0; e < EL; ++e) part_set<T, EL>(out, e, sum[e]);
-        *reinterpret_cast<vec*>((T*)a.rows_out + i * a.width + c) = out;
       } else {
-        const vec x = *reinterpret_cast<const vec*>(in + c);
-        vec y[RT_AT_ONCE];
+        for (int c = lane * EL; c < width; c += team * EL) {
+          const vec x = *reinterpret_cast<const vec*>(in + c);
+          vec y[U];
+          if (WHAT == ROUTE_GRAD && a.dweights) {
 #pragma unroll
-        for (int u = 0; u < RT_AT_ONCE; ++u) {
-          y[u] = vec{};
-          if (a.dweights && slot[u] < kept) y[u] = *reinterpret_cast<const vec*>(from + (int64_t)slot[u] * a.slots_stride + c);
-        }
-#pragma unroll
-        for (int u = 0; u < RT_AT_ONCE; ++u) {
-          vec d{};
-          if (slot[u] < kept) {
-#pragma unroll
-            for (int e = 0; e < EL; ++e) {
-              const float g = part_at<T, EL>(x, e);
-              dot[u] = __builtin_fmaf(g, part_at<T, EL>(y[u], e), dot[u]);
-              part_set<T, EL>(d, e, w[u] * g);
-            }
+            for (int u = 0; u < U; ++u)
+              y[u] = *reinterpret_cast<const vec*>(from + (int64_t)(kept_u[u] ? slot[u] : 0) * a.slots_stride + c);
           }
-          if (j0 + u < k) *reinterpret_cast<vec*>((T*)a.slots_out + (int64_t)slot[u] * a.width + c) = d;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            vec d{};
+            if constexpr (WHAT == ROUTE_OUT) {
+              if (kept_u[u]) d = x;
+            } else {
+#pragma unroll
+              for (int e = 0; e < EL; ++e) {
+                const float g = part_at<T, EL>(x, e);
+                if (a.dweights) dot[u] = __builtin_fmaf(g, part_at<T, EL>(y[u], e), dot[u]);
+                part_set<T, EL>(d, e, kept_u[u] ? w[u] * g : 0.f);
+              }
+            }
+            if (j + u < k) *reinterpret_cast<vec*>(to + (int64_t)slot[u] * a.width + c) = d;
+          }
+        }
+        if (WHAT == ROUTE_GRAD && a.dweights) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            for (int d = 1; d < team; d *= 2) dot[u] += __shfl_xor(dot[u], d);
+            if (lane == 0 && there && j + u < k) a.dweights[i * k + j + u] = kept_u[u] ? dot[u] : 0.f;
+          }
         }
       }
     }
-    if constexpr (WHAT == ROUTE_GRAD) {
-      if (a.dweights) {
+    if (WHAT == ROUTE_BACK && in_row) {
+      vec out;
 #pragma unroll
-        for (int u = 0; u < RT_AT_ONCE; ++u) {
-          for (int d = 1; d < team; d *= 2) dot[u] += __shfl_xor(dot[u], d);
-          if (lane == 0 && there && j0 + u < k) a.dweights[i * k + j0 + u] = slot[u] < kept ? dot[u] : 0.f;
-        }
-      }
+      for (int e = 0; e < EL; ++e) part_set<T, EL>(out, e, sum[e]);
+      *reinterpret_cast<vec*>((T*)a.rows_out + i * a.width + cb) = out;
     }
   }
 }
@@ -140,7 +128,12 @@ void start(const ffn_route& a, hipStream_t st) {
   int team = 1;  // a power of two, so that it divides a wavefront
   while (team < 64 && team * EL < a.width) team *= 2;
   const int64_t rows = RT_NT / team;
-  k_route<T, EL, WHAT><<<grid_of((a.n + rows - 1) / rows), RT_NT, 0, st>>>(a, team);
+  const dim3 grid = grid_of((a.n + rows - 1) / rows);
+  // 300,007 rows of 64 bytes to 8 experts, us: out 44 with eight places at once, 53 with four; back 60 and 53
+  constexpr int MOST = WHAT == ROUTE_OUT ? 8 : 4;
+  if (a.k <= 2) k_route<T, EL, WHAT, 2><<<grid, RT_NT, 0, st>>>(a, team);
+  else if (a.k <= 4) k_route<T, EL, WHAT, 4><<<grid, RT_NT, 0, st>>>(a, team);
+  else k_route<T, EL, WHAT, MOST><<<grid, RT_NT, 0, st>>>(a, team);
 }
 
 template <typename T, int WHAT>
@@ -164,13 +157,6 @@ hipError_t by_type(const ffn_route& a, hipStream_t st) {
 }
 
 }  // namespace
-
-hipError_t launch_route_slots(const uint32_t* plan, uint32_t places, int n_experts, uint32_t* slots, hipStream_t st) {
-  if (places)
-    k_route_slots<<<grid_of(((int64_t)places + RT_NT - 1) / RT_NT), RT_NT, 0, st>>>(
-        plan + expert_plan_words(places, n_experts) - places, places, slots);
-  return hipGetLastError();
-}
 
 hipError_t launch_dispatch(const ffn_route& a, hipStream_t st) { return by_type<ROUTE_OUT>(a, st); }
 hipError_t launch_combine(const ffn_route& a, hipStream_t st) { return by_type<ROUTE_BACK>(a, st); }

@@ -30,7 +30,7 @@ EXPORTS = [
     "ffn_ray_attention_workspace", "ffn_ray_attention_fwd", "ffn_ray_attention_bwd", "ffn_ray_scan_marks",
     "ffn_ray_scan_workspace", "ffn_ray_scan_fwd", "ffn_ray_scan_bwd", "ffn_expert_plan_size", "ffn_expert_plan",
     "ffn_expert_linear_fwd", "ffn_expert_linear_workspace", "ffn_expert_linear_bwd",
-    "ffn_layer_norm_fwd", "ffn_layer_norm_workspace", "ffn_layer_norm_bwd", "ffn_expert_slots",
+    "ffn_layer_norm_fwd", "ffn_layer_norm_workspace", "ffn_layer_norm_bwd", "ffn_expert_route",
     "ffn_expert_dispatch", "ffn_expert_combine", "ffn_expert_combine_bwd", "ffn_ray_delta_marks",
     "ffn_ray_delta_workspace", "ffn_ray_delta_fwd", "ffn_ray_delta_bwd",
 ]
@@ -244,7 +244,7 @@ def load(path: Path | str | None = None) -> C.CDLL:
     lib.ffn_layer_norm_workspace.argtypes = [C.POINTER(FfnNorm), u64p]
     lib.ffn_layer_norm_fwd.argtypes = [C.POINTER(FfnNorm), _vp]
     lib.ffn_layer_norm_bwd.argtypes = [C.POINTER(FfnNorm), _vp]
-    lib.ffn_expert_slots.argtypes = [_vp, C.c_uint32, C.c_int32, _vp, _vp]
+    lib.ffn_expert_route.argtypes = [_vp, C.c_uint32, C.c_int32, _vp, C.c_uint64, _vp, _vp, C.c_uint64, _vp]
     for name in ("ffn_expert_dispatch", "ffn_expert_combine", "ffn_expert_combine_bwd"):
         getattr(lib, name).argtypes = [C.POINTER(FfnRoute), _vp]
     for name in EXPORTS:

@@ -429,24 +429,32 @@ class ExpertPlan:
         return self.words[self.words.shape[0] - self.n:]
 
 
-def expert_plan(ids: torch.Tensor, n_experts: int) -> ExpertPlan:
-    """Groups rows by the expert ids [n] (int32) of the rows; an id outside [0, n_experts) gives a row to none."""
+def _plan(ids, n_experts, slots):
+    """The plan of ids, a flat tensor of int32 on the GPU, and (given) the slot of each place."""
     lib = fl.load()
-    if not isinstance(ids, torch.Tensor) or not ids.is_cuda or ids.dim() != 1 or ids.dtype != torch.int32:
-        _refuse("ids must be a vector of int32 on the GPU")
     if not hasattr(n_experts, "__index__") or not 1 <= n_experts <= fl.MAX_EXPERTS:
         _refuse(f"n_experts={n_experts!r} must be a whole number of 1 to {fl.MAX_EXPERTS}")
-    dev, n = ids.get_device(), ids.shape[0]
-    _index(ids, "ids", dev)
+    dev, n = ids.get_device(), ids.numel()
     if n >= 1 << 31:
         _refuse(f"{n} rows are too many")
     words, ws = C.c_uint64(), C.c_uint64()
     fl.check(lib.ffn_expert_plan_size(n, n_experts, C.byref(words), C.byref(ws)), "ffn_expert_plan_size")
     plan = torch.empty(words.value, dtype=torch.int32, device=dev)
     w = torch.empty(ws.value, dtype=torch.uint8, device=dev) if ws.value else None
-    _call(lib.ffn_expert_plan, dev, ids.data_ptr(), n, n_experts, plan.data_ptr(), words.value,
-          None if w is None else w.data_ptr(), ws.value)
+    scratch = (None if w is None else w.data_ptr(), ws.value)
+    if slots is None:
+        _call(lib.ffn_expert_plan, dev, ids.data_ptr(), n, n_experts, plan.data_ptr(), words.value, *scratch)
+    else:
+        _call(lib.ffn_expert_route, dev, ids.data_ptr(), n, n_experts, plan.data_ptr(), words.value, slots.data_ptr(), *scratch)
     return ExpertPlan(plan, n, n_experts)
+
+
+def expert_plan(ids: torch.Tensor, n_experts: int) -> ExpertPlan:
+    """Groups rows by the expert ids [n] (int32) of the rows; an id outside [0, n_experts) gives a row to none."""
+    if not isinstance(ids, torch.Tensor) or not ids.is_cuda or ids.dim() != 1 or ids.dtype != torch.int32:
+        _refuse("ids must be a vector of int32 on the GPU")
+    _index(ids, "ids", ids.get_device())
+    return _plan(ids, n_experts, None)
 
 
 def _expert_args(x, W, plan, relu, x_slots, y_slots):
@@ -537,11 +545,8 @@ def expert_route(ids: torch.Tensor, n_experts: int) -> ExpertRoute:
         _refuse("ids must be contiguous")
     if not 1 <= ids.shape[1] <= fl.MAX_EXPERTS:
         _refuse(f"k={ids.shape[1]} must be 1 to {fl.MAX_EXPERTS}")
-    lib = fl.load()
-    plan = expert_plan(ids.view(-1), n_experts)
-    slots = torch.empty(ids.shape, dtype=torch.int32, device=plan.device)
-    _call(lib.ffn_expert_slots, plan.device, plan.words.data_ptr(), plan.n, plan.n_experts, slots.data_ptr())
-    return ExpertRoute(plan, slots)
+    slots = torch.empty(ids.shape, dtype=torch.int32, device=ids.device)
+    return ExpertRoute(_plan(ids, n_experts, slots), slots)
 
 
 def _route_args(x, name, route, slots: bool, weights=None):

@@ -576,10 +576,10 @@ int ffn_layer_norm_workspace(const ffn_norm* a, uint64_t* bytes);  /* of the bac
 /* No atomics: two calls give the same bits. */
 int ffn_layer_norm_bwd(const ffn_norm* a, void* stream);
 
-/* Rows to several experts and back.  With a plan (ffn_expert_plan) over the
- * n k ids of n rows' k experts, place i k + j being row i's j-th:
- * ffn_expert_slots gives the inverse of the plan's rows, slots[place] = the
- * slot that holds it (places = n k).  An array "of slots" is [n k][width] in the
+/* Rows to several experts and back.  ffn_expert_route makes the plan (as
+ * ffn_expert_plan does, of ffn_expert_plan_size) of the n k ids of n rows' k
+ * experts, place i k + j being row i's j-th, and the inverse of its rows,
+ * slots[place] = the slot that holds it (places = n k).  An array "of slots" is [n k][width] in the
  * plan's slot order, what the expert layers take and give under
  * FFN_EXPERTS_X_SLOTS and FFN_EXPERTS_Y_SLOTS.
  *   dispatch     slots_out[slot] = rows_in[i] for each of row i's slots
@@ -606,7 +606,8 @@ typedef struct ffn_route {
   float* dweights;
 } ffn_route;
 
-int ffn_expert_slots(const uint32_t* plan, uint32_t places, int32_t n_experts, uint32_t* slots, void* stream);
+int ffn_expert_route(const int32_t* ids, uint32_t places, int32_t n_experts, uint32_t* plan, uint64_t plan_words,
+                     uint32_t* slots, void* workspace, uint64_t workspace_bytes, void* stream);
 int ffn_expert_dispatch(const ffn_route* a, void* stream);
 int ffn_expert_combine(const ffn_route* a, void* stream);
 int ffn_expert_combine_bwd(const ffn_route* a, void* stream);

@@ -74,9 +74,12 @@ def test_route_refuses_what_only_one_call_needs():
     _refused(lib.ffn_expert_combine, C.byref(_route(rows_out=None)), None, match="NULL buffer")
     _refused(lib.ffn_expert_combine_bwd, C.byref(_route(slots_in=None)), None, match="NULL buffer")
     _refused(lib.ffn_expert_combine_bwd, None, None, match="NULL arguments")
-    _refused(lib.ffn_expert_slots, None, 100, 8, P, None, match="NULL plan")
-    _refused(lib.ffn_expert_slots, P, 1 << 31, 8, P, None, match="exceed")
-    _refused(lib.ffn_expert_slots, P, 100, 0, P, None, match="n_experts=0")
+    _refused(lib.ffn_expert_route, None, 100, 8, P, 1 << 20, P, P, 1 << 20, None, match="NULL ids")
+    _refused(lib.ffn_expert_route, P, 100, 8, P, 1 << 20, None, P, 1 << 20, None, match="NULL slots")
+    _refused(lib.ffn_expert_route, P, 100, 8, P, 10, P, P, 1 << 20, None, match="plan of 10 words")
+    _refused(lib.ffn_expert_route, P, 100000, 8, P, 1 << 20, P, P, 4, None, match="workspace of 4")
+    _refused(lib.ffn_expert_route, P, 1 << 31, 8, P, 1 << 20, P, P, 1 << 20, None, match="exceed")
+    _refused(lib.ffn_expert_route, P, 100, 0, P, 1 << 20, P, P, 1 << 20, None, match="n_experts=0")
 
 
 def test_python_entry_points_refuse():
