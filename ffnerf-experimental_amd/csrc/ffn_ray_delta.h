@@ -55,23 +55,26 @@ __device__ __forceinline__ f32x4 mul16(const f32x4& a, const f32x4& b, f32x4 to)
   return to;
 }
 
-// Four floats as N bfloat16 parts by cutting: 8 bits of the 24 each, so that three are the float itself and two are off by
-// 2^-16 of it.
+// Four floats as three bfloat16 parts, by cutting 8 bits of the 24 each time, which together are the float itself; or as two,
+// the second one rounded, which are off by 2^-17 of it at most and by nothing on average.
 template <int N> struct Parts {
   b16x4 p[N];
 };
-template <int N> __device__ __forceinline__ Parts<N> parts_of(f32x4 x) {
-  Parts<N> y;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-    const u32x4 w = __builtin_bit_cast(u32x4, x);
-    const u32x2 up = {__builtin_amdgcn_perm(w[1], w[0], 0x07060302u), __builtin_amdgcn_perm(w[3], w[2], 0x07060302u)};
-    y.p[i] = __builtin_bit_cast(b16x4, up);
-    if (i + 1 < N) x = x - __builtin_bit_cast(f32x4, w & 0xFFFF0000u);
-  }
-  return y;
+__device__ __forceinline__ b16x4 upper_of(const f32x4& x) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  const u32x4 w = __builtin_bit_cast(u32x4, x);
+  const u32x2 up = {__builtin_amdgcn_perm(w[1], w[0], 0x07060302u), __builtin_amdgcn_perm(w[3], w[2], 0x07060302u)};
+  return __builtin_bit_cast(b16x4, up);
+}
+__device__ __forceinline__ f32x4 rest_of(const f32x4& x) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  return x - __builtin_bit_cast(f32x4, __builtin_bit_cast(u32x4, x) & 0xFFFF0000u);
+}
+template <int N> __device__ __forceinline__ Parts<N> parts_of(const f32x4& x) {
+  const f32x4 r = rest_of(x);
+  if constexpr (N == 2) return {{upper_of(x), __builtin_convertvector(r, b16x4)}};
+  else return {{upper_of(x), upper_of(r), upper_of(rest_of(r))}};
 }
 
 // How a type's rows enter products.  Row: four neighbouring values of a row.  Two: a float operand where the result is
@@ -83,6 +86,7 @@ template <typename T> struct Delta {
   typedef f32x4 Two;
   static __device__ __forceinline__ Full full(const f32x4& x) { return x; }
   static __device__ __forceinline__ Two two(const f32x4& x) { return x; }
+  static __device__ __forceinline__ Two first_two(const Full& x) { return x; }
   static __device__ __forceinline__ Row row(const f32x4& x) { return x; }
   static __device__ __forceinline__ f32x4 value(const Row& x) { return x; }
   // on a product: 16 values of K from each operand's lane parts, then 32
@@ -99,6 +103,7 @@ template <> struct Delta<__bf16> {
   typedef Parts<2> Two;
   static __device__ __forceinline__ Full full(const f32x4& x) { return parts_of<3>(x); }
   static __device__ __forceinline__ Two two(const f32x4& x) { return parts_of<2>(x); }
+  static __device__ __forceinline__ Two first_two(const Full& x) { return {{x.p[0], x.p[1]}}; }
   static __device__ __forceinline__ f32x4 value(const Row& x) { return __builtin_convertvector(x, f32x4); }
   static __device__ __forceinline__ f32x4 mul(const Row& a, const Row& b, const f32x4& c) { return mma16(a, b, c); }
   template <int N> static __device__ __forceinline__ f32x4 mul(const Row& a, const Parts<N>& b, f32x4 c) {
@@ -259,6 +264,19 @@ struct Rows4 {
     for (int r = 0; r < 4; ++r) at[r] = ck.at(4 * g + r);
   }
 };
+
+// column `col` of a chunk's rows 4 g + r, those that are there; p: the chunk's first row
+template <typename T>
+__device__ __forceinline__ void put_rows(T* p, const Chunk& ck, const Rows4& rows, int g, int stride, int col, const f32x4& x) {
+  if (ck.many == DL_C) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) *row_ptr(p, rows.at[r], stride, col) = (T)x[r];
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (4 * g + r < ck.many) *row_ptr(p, rows.at[r], stride, col) = (T)x[r];
+  }
+}
 
 // this lane's part of a chunk's row c: four values of every 16 columns, as they lie in memory
 template <typename T, int N> struct RawRow {
@@ -591,10 +609,14 @@ __global__ __launch_bounds__(64 * W, (DL_FWD_WAVES<T, DK, W>)) void k_delta_fwd(
         const f32x4 Tr = *reinterpret_cast<const f32x4*>(&Tm[i][c * DL_LD + 4 * g]);
         const f32x4 Pr = *reinterpret_cast<const f32x4*>(&Pm[i][c * DL_LD + 4 * g]);
         typename Ops::Full full[NT];
+        typename Ops::Two some[NT];  // enough for o, which is rounded
 #pragma unroll
-        for (int t = 0; t < NT; ++t) full[t] = Ops::full(S[t]);
+        for (int t = 0; t < NT; ++t) {
+          full[t] = Ops::full(S[t]);
+          some[t] = Ops::first_two(full[t]);
+        }
         const f32x4 R = beta * (vr[i].value(ck, g, w16 + c, a.val_dim) - e * mul_tiles<T>(kf, full, zero));
-        const f32x4 qs = a.scale * e * mul_tiles<T>(qf, full, zero);
+        const f32x4 qs = a.scale * e * mul_tiles<T>(qf, some, zero);
         const f32x4 n = mul16(Tr, R, zero);
         f32x4 y = mul16(Pr, n, qs);
         const typename Ops::Full nl = Ops::full(left * n);
@@ -604,10 +626,7 @@ __global__ __launch_bounds__(64 * W, (DL_FWD_WAVES<T, DK, W>)) void k_delta_fwd(
         if (__any(!finite4(n))) y = mul16_sick(Pr, mul16_sick(Tr, R, zero, g), qs, g);
         T* o = ck.in((T*)a.o + h * a.val_dim, a.v_heads * a.val_dim);
         if (w16 + c < a.val_dim) {
-          const Rows4 rows(ck, g);
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (4 * g + r < ck.many) *row_ptr(o, rows.at[r], a.v_heads * a.val_dim, w16 + c) = (T)y[r];
+          put_rows(o, ck, Rows4(ck, g), g, a.v_heads * a.val_dim, w16 + c, y);
         }
       }
     }
@@ -913,7 +932,8 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
     }
     if (AHEAD && p0) fetch(p0 - DL_MARK);
     sync();
-    // the states before the segment's chunks, and their writes n
+    // the states before the segment's chunks, and their writes n: they reach gradients that are rounded to the type, and
+    // not dS, so that two parts are enough
 #pragma unroll
     for (int i = 0; i < DL_SEG; ++i) {
       if (p0 + DL_C * i < ch.count) {
@@ -921,17 +941,17 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
         const T* Kc = Kl + i * NT * TILE;
         const float* vec = vecs + i * DL_VEC;
         Row kf[NT];
-        typename Ops::Full full[NT];
+        typename Ops::Two some[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           kf[t] = row_of(Kc + t * TILE, c, g);
-          full[t] = Ops::full(S[i][t]);
+          some[t] = Ops::two(S[i][t]);
         }
         const f32x4 beta = *reinterpret_cast<const f32x4*>(vec + 4 * g), e = *reinterpret_cast<const f32x4*>(vec + 16 + 4 * g);
-        const f32x4 R = beta * (vr[i].value(ck, g, w16 + c, a.val_dim) - e * mul_tiles<T>(kf, full, zero));
+        const f32x4 R = beta * (vr[i].value(ck, g, w16 + c, a.val_dim) - e * mul_tiles<T>(kf, some, zero));
         n[i] = mul16(*reinterpret_cast<const f32x4*>(Tm + i * SQ + c * DL_LD + 4 * g), R, zero);
         if (i + 1 == DL_SEG || p0 + DL_C * (i + 1) >= ch.count) continue;
-        const typename Ops::Full nl = Ops::full(*reinterpret_cast<const f32x4*>(vec + 32 + 4 * g) * n[i]);
+        const typename Ops::Two nl = Ops::two(*reinterpret_cast<const f32x4*>(vec + 32 + 4 * g) * n[i]);
 #pragma unroll
         for (int t = 0; t < NT; ++t) S[i + 1 < DL_SEG ? i + 1 : i][t] = Ops::mul(col_of(Kc + t * TILE, c, g), nl, vec[48] * S[i][t]);
       }
@@ -970,9 +990,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
         const Rows4 rows(ck, g);
         if (vcol < a.val_dim) {
           T* dv = ck.in((T*)a.dv + h * a.val_dim, a.v_heads * a.val_dim);
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (4 * g + r < ck.many) *row_ptr(dv, rows.at[r], a.v_heads * a.val_dim, vcol) = (T)(beta[r] * dR[r]);
+          put_rows(dv, ck, rows, g, a.v_heads * a.val_dim, vcol, beta * dR);
         }
         Nl.set(w, c, g, n[i]);
         Rl.set(w, c, g, dR);
@@ -1046,23 +1064,13 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
                 const int stride = a.v_heads * a.key_dim;
                 const int64_t other = (int64_t)a.rays.n * stride;
                 float* part = ck.in((float*)a.workspace + h * a.key_dim, stride);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                  if (4 * g + r < ck.many) {
-                    *row_ptr(part, rows.at[r], stride, kcol) = gq[r];
-                    *row_ptr(part + other, rows.at[r], stride, kcol) = gk[r];
-                  }
-                }
+                put_rows(part, ck, rows, g, stride, kcol, gq);
+                put_rows(part + other, ck, rows, g, stride, kcol, gk);
               } else {
                 const int stride = a.heads * a.key_dim;
                 T *dq = ck.in((T*)a.dq + h * a.key_dim, stride), *dk = ck.in((T*)a.dk + h * a.key_dim, stride);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                  if (4 * g + r < ck.many) {
-                    *row_ptr(dq, rows.at[r], stride, kcol) = (T)gq[r];
-                    *row_ptr(dk, rows.at[r], stride, kcol) = (T)gk[r];
-                  }
-                }
+                put_rows(dq, ck, rows, g, stride, kcol, gq);
+                put_rows(dk, ck, rows, g, stride, kcol, gk);
               }
             }
           }
