@@ -35,6 +35,7 @@ constexpr int DL_LD = 20;             // LDS row of a 16 x 16 matrix
 constexpr int DL_VEC = 64;            // a chunk's b, e, D_15 and (first of the last 16) e_15
 constexpr float DL_RESET = -1e30f;    // stands for a decay of -infinity, which must not meet a zero in a product
 constexpr int DL_FEW = 2048;          // wavefronts: two a SIMD
+constexpr int DL_BLOCKS = 4096;       // 16 a CU: more than run at once
 constexpr int DL_CLEAR = 1024;        // rows that one block looks through for those of no ray
 
 // ---------------------------------------------------------------------------
@@ -526,13 +527,16 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int b) {
 template <typename T, int DK, int W> constexpr int DL_FWD_WAVES = Delta<T>::EXACT && DK == 32 && W <= 2 ? 5 : 1;
 
 template <typename T, int DK, int W>
-__global__ __launch_bounds__(64 * W, (DL_FWD_WAVES<T, DK, W>)) void k_delta_fwd(const ffn_ray_delta a) {
+__global__ __launch_bounds__(64 * W, (DL_FWD_WAVES<T, DK, W>)) void k_delta_fwd(const ffn_ray_delta a, int longer) {
   constexpr int NT = DK / 16, TILE = Tile<T>::SIZE, CH = W < 4 ? W : 4;
   typedef Delta<T> Ops;
   typedef typename Ops::Row Row;
   __shared__ float Tm[CH][DL_C * DL_LD], Pm[CH][DL_C * DL_LD], vec[CH][DL_VEC];
   __shared__ __align__(16) T Kl[CH * NT * TILE], Ql[CH * NT * TILE];
-  const int64_t block = block_number(), teams = (int64_t)a.rays.num_rays * a.v_heads;
+  const int64_t teams = (int64_t)a.rays.num_rays * a.v_heads;
+  int64_t block = block_number();
+  const bool first = longer && block < teams;  // of two turns: the rays with more rows than `longer`
+  if (longer && !first) block -= teams;
   if (block >= teams) {
     clear_rows(a, block - teams, (T*)a.o, (int64_t)a.v_heads * a.val_dim);
     return;
@@ -540,6 +544,7 @@ __global__ __launch_bounds__(64 * W, (DL_FWD_WAVES<T, DK, W>)) void k_delta_fwd(
   const int64_t ray = quotient(block, a.v_heads);
   const int h = (int)(block - ray * a.v_heads), hk = h / (a.v_heads / a.heads);
   const Chain ch = chain_of(a, ray);
+  if (longer && (ch.count > longer) != first) return;
   const int lane = threadIdx.x & 63, w = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w16 = 16 * w;
   int c = lane & 15, g = lane >> 4;
   const T* q = (const T*)a.q + hk * a.q_head;
@@ -820,13 +825,16 @@ template <typename T, int DK, int W> struct DeltaLds {
 // AHEAD: a segment's rows and state are asked for while the one after it is worked on.  That takes some 60 registers: it is
 // for few blocks, where nothing else hides the loads.
 template <typename T, int DK, int W, bool AHEAD>
-__global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
+__global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a, int longer) {
   typedef Delta<T> Ops;
   typedef typename Ops::Row Row;
   typedef DeltaLds<T, DK, W> L;
   constexpr int NT = DK / 16, TP = (NT + W - 1) / W, SQ = L::SQ, TILE = Tile<T>::SIZE;
   extern __shared__ __align__(16) float lds[];
-  const int64_t block = block_number(), teams = (int64_t)a.rays.num_rays * a.v_heads;
+  const int64_t teams = (int64_t)a.rays.num_rays * a.v_heads;
+  int64_t block = block_number();
+  const bool first = longer && block < teams;  // of two turns: the rays with more rows than `longer`
+  if (longer && !first) block -= teams;
   const bool shared = a.heads != a.v_heads;
   if (block >= teams) {
     const int64_t width = (int64_t)a.v_heads * a.key_dim;
@@ -845,6 +853,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a) {
   const int64_t ray = quotient(block, a.v_heads);
   const int h = (int)(block - ray * a.v_heads), hk = h / (a.v_heads / a.heads);
   const Chain ch = chain_of(a, ray);
+  if (longer && (ch.count > longer) != first) return;
   const int lane = threadIdx.x & 63, w = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w16 = 16 * w;
   int c = lane & 15, g = lane >> 4;
   float* Tm = lds;
@@ -1132,11 +1141,19 @@ inline int delta_waves(int val_dim) { return val_dim <= 64 ? (val_dim + 15) / 16
 
 inline int64_t delta_clear_blocks(const ffn_ray_delta& a) { return ((int64_t)a.rays.n + DL_CLEAR - 1) / DL_CLEAR; }
 
+// Where rays are many, those of more than twice the mean and four chunks take their turn before the others: one that is
+// begun last would be all that still runs.
+inline int delta_longer(const ffn_ray_delta& a) {
+  if ((int64_t)a.rays.num_rays * a.v_heads < DL_BLOCKS) return 0;
+  return (int)std::max<int64_t>(4 * DL_C, 2 * (int64_t)a.rays.n / a.rays.num_rays);
+}
+
 template <typename T, int DK, int W>
 hipError_t start_delta(const ffn_ray_delta& a, bool back, hipStream_t st) {
-  const dim3 grid = grid_of((int64_t)a.rays.num_rays * a.v_heads + delta_clear_blocks(a));
+  const int longer = delta_longer(a);
+  const dim3 grid = grid_of((int64_t)a.rays.num_rays * a.v_heads * (longer ? 2 : 1) + delta_clear_blocks(a));
   if (!back) {
-    k_delta_fwd<T, DK, W><<<grid, 64 * W, 0, st>>>(a);
+    k_delta_fwd<T, DK, W><<<grid, 64 * W, 0, st>>>(a, longer);
     return hipGetLastError();
   }
   constexpr int bytes = DeltaLds<T, DK, W>::BYTES;
@@ -1147,7 +1164,7 @@ hipError_t start_delta(const ffn_ray_delta& a, bool back, hipStream_t st) {
       const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
       if (e != hipSuccess) return e;
     }
-    kernel<<<grid, 64 * W, bytes, st>>>(a);
+    kernel<<<grid, 64 * W, bytes, st>>>(a, longer);
     return hipGetLastError();
   };
   // 128 columns leave no registers for it, and a wavefront alone prepares both chunks of a segment
