@@ -58,6 +58,27 @@ struct RowPart {
 template <typename T, int EL, int P>
 __device__ __forceinline__ void load_params(const void* p, bool f32, float none, int lane, int team, int width,
                                             float (&to)[P * EL]) {
+  if constexpr (EL > 1) {
+    if (p && !((uintptr_t)p & 15)) {  // whole pieces; rows of pieces end with one
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const int c = (lane + i * team) * EL < width ? (lane + i * team) * EL : 0;
+        if (f32) {
+#pragma unroll
+          for (int e = 0; e < EL; e += 4) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>((const float*)p + c + e);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) to[i * EL + e + q] = v[q];
+          }
+        } else {
+          const typename Piece<T, EL>::type v = *reinterpret_cast<const typename Piece<T, EL>::type*>((const T*)p + c);
+#pragma unroll
+          for (int e = 0; e < EL; ++e) to[i * EL + e] = (float)v[e];
+        }
+      }
+      return;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < P; ++i) {
 #pragma unroll
@@ -337,7 +358,7 @@ void start(const ffn_norm& a, bool backward, const Shape& s, hipStream_t st) {
     if constexpr (P * EL == NM_BLOCK_COLS) {
       if (backward && s.threads <= 512) k_norm_bwd<T, EL, P, 512><<<grid, s.threads, 0, st>>>(a, s.team);
       else if (backward) k_norm_bwd<T, EL, P, 1024><<<grid, s.threads, 0, st>>>(a, s.team);
-      else k_norm_fwd<T, EL, P, 1, true><<<grid, s.threads, 0, st>>>(a, s.team);
+      else k_norm_fwd<T, EL, P, 2, true><<<grid, s.threads, 0, st>>>(a, s.team);
     }
   } else if (backward) {
     k_norm_bwd<T, EL, P, 0><<<grid, s.threads, 0, st>>>(a, s.team);

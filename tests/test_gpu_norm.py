@@ -239,3 +239,20 @@ def test_rows_past_32_bit_offsets():
     assert torch.equal(y, ray_ops.layer_norm(x, w, b)[0])
     assert torch.equal(ray_ops.layer_norm_backward(dy, far, w, mean, rstd)[0],
                        ray_ops.layer_norm_backward(dy, x, w, mean, rstd)[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("typed", [False, True])
+def test_parameters_anywhere(typed, dtype):
+    """Parameters that do not start on 16 bytes: the bits of those that do."""
+    import ray_ops
+    x, w, b, dy = make(30, 256, dtype)
+    if typed:
+        w, b = w.to(dtype), b.to(dtype)
+    wide = torch.zeros(2, 260, dtype=w.dtype, device="cuda")
+    wide[0, 1:257], wide[1, 3:259] = w, b
+    p, q = wide[0, 1:257], wide[1, 3:259]
+    y, mean, rstd = ray_ops.layer_norm(x, w, b)
+    assert torch.equal(y, ray_ops.layer_norm(x, p, q)[0])
+    for s, t in zip(ray_ops.layer_norm_backward(dy, x, w, mean, rstd), ray_ops.layer_norm_backward(dy, x, p, mean, rstd)):
+        assert torch.equal(s, t)
