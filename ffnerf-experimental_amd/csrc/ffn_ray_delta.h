@@ -34,8 +34,7 @@ constexpr int DL_MARK = DL_C * DL_SEG;
 constexpr int DL_LD = 20;             // LDS row of a 16 x 16 matrix
 constexpr int DL_VEC = 64;            // a chunk's b, e, D_15 and (first of the last 16) e_15
 constexpr float DL_RESET = -1e30f;    // stands for a decay of -infinity, which must not meet a zero in a product
-constexpr int DL_FEW = 2048;          // wavefronts: two a SIMD
-constexpr int DL_BLOCKS = 4096;       // 16 a CU: more than run at once
+constexpr int DL_BLOCKS = 4096;       // heads of rays, 16 a CU: more than run at once
 constexpr int DL_CLEAR = 1024;        // rows that one block looks through for those of no ray
 
 // ---------------------------------------------------------------------------
@@ -822,13 +821,16 @@ template <typename T, int DK, int W> struct DeltaLds {
   static constexpr int BYTES = WORDS * 4 + (2 * DL_SEG * NT + W) * Tile<T>::SIZE * (int)sizeof(T);
 };
 
-// AHEAD: a segment's rows and state are asked for while the one after it is worked on.  That takes some 60 registers: it is
-// for few blocks, where nothing else hides the loads.
-template <typename T, int DK, int W, bool AHEAD>
+// AHEAD: a segment's rows and state are asked for while the one after it is worked on (24 rays of up to 4096 rows, 8 heads of
+// 64 x 64, bf16: 1309 us, 1361 without; 8192 marched rays 312 and 319).  Rows that are held as floats cost a wavefront a SIMD
+// for it (3001 rays of fp32, 24 x 40: 426 us, 287 without), 128 columns leave no registers, and a wavefront alone prepares
+// both chunks of a segment.
+template <typename T, int DK, int W>
 __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a, int longer) {
   typedef Delta<T> Ops;
   typedef typename Ops::Row Row;
   typedef DeltaLds<T, DK, W> L;
+  constexpr bool AHEAD = Ops::EXACT && DK <= 64 && W > 1;
   constexpr int NT = DK / 16, TP = (NT + W - 1) / W, SQ = L::SQ, TILE = Tile<T>::SIZE;
   extern __shared__ __align__(16) float lds[];
   const int64_t teams = (int64_t)a.rays.num_rays * a.v_heads;
@@ -1142,7 +1144,8 @@ inline int delta_waves(int val_dim) { return val_dim <= 64 ? (val_dim + 15) / 16
 inline int64_t delta_clear_blocks(const ffn_ray_delta& a) { return ((int64_t)a.rays.n + DL_CLEAR - 1) / DL_CLEAR; }
 
 // Where rays are many, those of more than twice the mean and four chunks take their turn before the others: one that is
-// begun last would be all that still runs.
+// begun last would be all that still runs (8192 marched rays, 4 heads of 32 x 32, bf16: forward 120 us, 127 in one turn,
+// backward 320 and 340).
 inline int delta_longer(const ffn_ray_delta& a) {
   if ((int64_t)a.rays.num_rays * a.v_heads < DL_BLOCKS) return 0;
   return (int)std::max<int64_t>(4 * DL_C, 2 * (int64_t)a.rays.n / a.rays.num_rays);
@@ -1158,23 +1161,18 @@ hipError_t start_delta(const ffn_ray_delta& a, bool back, hipStream_t st) {
   }
   constexpr int bytes = DeltaLds<T, DK, W>::BYTES;
   static_assert(bytes <= 160 * 1024, "LDS");
-  const auto start = [&](auto ahead) {
-    constexpr auto kernel = k_delta_bwd<T, DK, W, decltype(ahead)::value>;
-    if (bytes > 64 * 1024) {  // has to be allowed, on the device that is current
-      const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-      if (e != hipSuccess) return e;
-    }
-    kernel<<<grid, 64 * W, bytes, st>>>(a, longer);
-    return hipGetLastError();
-  };
-  // 128 columns leave no registers for it, and a wavefront alone prepares both chunks of a segment
-  if constexpr (DK <= 64 && W > 1)
-    if ((int64_t)a.rays.num_rays * a.v_heads * W <= DL_FEW) return start(std::true_type{});
-  return start(std::false_type{});
+  if (bytes > 64 * 1024) {  // has to be allowed, on the device that is current
+    const hipError_t e = hipFuncSetAttribute((const void*)k_delta_bwd<T, DK, W>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) return e;
+  }
+  k_delta_bwd<T, DK, W><<<grid, 64 * W, bytes, st>>>(a, longer);
+  return hipGetLastError();
 }
 
 template <typename T, int DK>
 hipError_t delta_by_columns(const ffn_ray_delta& a, bool back, hipStream_t st) {
+  // by the mean of rows a ray: 2048 rays, 4 heads of 64 x 64, bf16, row by row and in chunks, us: one row 52 and 83, three
+  // 71 and 85, six 111 and 90
   if (!back && !a.marks && a.rays.n <= 4ull * a.rays.num_rays) {
     const int64_t teams = (int64_t)a.rays.num_rays * a.v_heads * ((a.val_dim + 31) / 32);
     k_delta_step<T, DK><<<grid_of((teams + 3) / 4 + delta_clear_blocks(a)), 256, 0, st>>>(a);
