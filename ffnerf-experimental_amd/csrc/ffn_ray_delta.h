@@ -174,15 +174,21 @@ template <typename T> __device__ __forceinline__ void store4(T* p, const f32x4& 
 template <typename T> struct Tile {
   static constexpr int LD = sizeof(T) == 4 ? 20 : Delta<T>::EXACT ? 16 : 24, SIZE = DL_C * LD;
 };
+// where a tile has the four values from column 4 u of row r: in 16 bits rows lie side by side, and the lower eight have their
+// halves changed over, so that 32 lanes that take a row each and a four of it meet every bank once
+template <typename T> __device__ __forceinline__ int four_at(int r, int u) {
+  if constexpr (Delta<T>::EXACT) return r * 16 + 4 * (u ^ ((r >> 3) << 1));
+  else return r * Tile<T>::LD + 4 * u;
+}
 template <typename T> __device__ __forceinline__ typename Delta<T>::Row row_of(const T* tile, int c, int g) {
-  const T* p = tile + c * Tile<T>::LD + 4 * g;
+  const T* p = tile + four_at<T>(c, g);
   if constexpr (Delta<T>::EXACT) return *reinterpret_cast<const b16x4*>(p);
   else return load4(p);
 }
 template <typename T> __device__ __forceinline__ typename Delta<T>::Row col_of(const T* tile, int c, int g) {
   if constexpr (Delta<T>::EXACT) {
     typedef __attribute__((address_space(3))) s16x4* lds_quad;
-    return __builtin_bit_cast(b16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad)(tile + (4 * g + (c >> 2)) * Tile<T>::LD + 4 * (c & 3))));
+    return __builtin_bit_cast(b16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad)(tile + four_at<T>(4 * g + (c >> 2), c & 3))));
   } else {
     f32x4 x;
 #pragma unroll
@@ -585,8 +591,8 @@ __global__ __launch_bounds__(64 * W, (DL_FWD_WAVES<T, DK, W>)) void k_delta_fwd(
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         typedef typename RawRow<T, NT>::tvec tvec;
-        *reinterpret_cast<tvec*>(Kl + (w * NT + t) * TILE + c * Tile<T>::LD + 4 * g) = kr.v[t];
-        *reinterpret_cast<tvec*>(Ql + (w * NT + t) * TILE + c * Tile<T>::LD + 4 * g) = qr.v[t];
+        *reinterpret_cast<tvec*>(Kl + (w * NT + t) * TILE + four_at<T>(c, g)) = kr.v[t];
+        *reinterpret_cast<tvec*>(Ql + (w * NT + t) * TILE + four_at<T>(c, g)) = qr.v[t];
       }
       prepare_chunk<T>(kf, qf, gates.decay(ck, g), gates.beta(ck, c), a.scale, c, g, Tm[w], Pm[w], (float*)nullptr, vec[w]);
       fetch(p0 + DL_C * (CH + w));
@@ -743,7 +749,7 @@ template <typename T> struct Tiles {
     }
   }
   template <int N> __device__ __forceinline__ void set(int tile, int c, int g, const Parts<N>& x) const {
-    __bf16* q = (__bf16*)(p + tile * WORDS) + c * 16 + 4 * g;  // transposed, so that four rows lie side by side
+    __bf16* q = (__bf16*)(p + tile * WORDS) + four_at<__bf16>(c, g);  // transposed, so that four rows lie side by side
     *reinterpret_cast<b16x4*>(q) = x.p[0];
     *reinterpret_cast<b16x4*>(q + 256) = x.p[1];
   }
@@ -762,7 +768,7 @@ template <typename T> struct Square {
   __device__ __forceinline__ void set(int c, int g, const f32x4& x) const {
     if constexpr (Delta<T>::EXACT) {
       const Parts<2> y = parts_of<2>(x);
-      __bf16* q = (__bf16*)p + c * 16 + 4 * g;
+      __bf16* q = (__bf16*)p + four_at<__bf16>(c, g);
       *reinterpret_cast<b16x4*>(q) = y.p[0];
       *reinterpret_cast<b16x4*>(q + 256) = y.p[1];
     } else {
@@ -771,7 +777,7 @@ template <typename T> struct Square {
   }
   __device__ __forceinline__ typename Delta<T>::Two row(int c, int g) const {
     if constexpr (Delta<T>::EXACT) {
-      const __bf16* q = (const __bf16*)p + c * 16 + 4 * g;
+      const __bf16* q = (const __bf16*)p + four_at<__bf16>(c, g);
       return {{*reinterpret_cast<const b16x4*>(q), *reinterpret_cast<const b16x4*>(q + 256)}};
     } else {
       return *reinterpret_cast<const f32x4*>(p + c * 16 + 4 * (g ^ (c >> 2)));
@@ -793,7 +799,7 @@ template <typename T> struct RowTiles {
   T* p;
   __device__ __forceinline__ void set(int tile, int c, int g, const f32x4& x) const {
     if constexpr (Delta<T>::EXACT) {
-      *reinterpret_cast<b16x4*>(p + tile * Tile<T>::SIZE + c * 16 + 4 * g) = __builtin_convertvector(x, b16x4);
+      *reinterpret_cast<b16x4*>(p + tile * Tile<T>::SIZE + four_at<T>(c, g)) = __builtin_convertvector(x, b16x4);
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r) p[tile * Tile<T>::SIZE + (4 * g + r) * Tile<T>::LD + c] = (T)x[r];
@@ -934,8 +940,8 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a, int
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           typedef typename RawRow<T, NT>::tvec tvec;
-          *reinterpret_cast<tvec*>(Kl + (i * NT + t) * TILE + c * Tile<T>::LD + 4 * g) = kr[j].v[t];
-          *reinterpret_cast<tvec*>(Ql + (i * NT + t) * TILE + c * Tile<T>::LD + 4 * g) = qr[j].v[t];
+          *reinterpret_cast<tvec*>(Kl + (i * NT + t) * TILE + four_at<T>(c, g)) = kr[j].v[t];
+          *reinterpret_cast<tvec*>(Ql + (i * NT + t) * TILE + four_at<T>(c, g)) = qr[j].v[t];
         }
         prepare_chunk<T>(kf, qf, gates[j].decay(ck, g), gates[j].beta(ck, c), a.scale, c, g, Tm + i * SQ, Pm + i * SQ, Dm + i * SQ,
                          vecs + i * DL_VEC);
