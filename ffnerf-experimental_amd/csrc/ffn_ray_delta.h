@@ -18,7 +18,16 @@
 //
 // Products: in float, by the K = 4 instruction.  Of bfloat16 inputs the rows are exact operands of the 16-bit instruction,
 // and what they meet (S, n, dS: float) goes as three bfloat16 parts, which together are the float itself: three products
-// at 16 times the rate (K = 32; 8 times at K = 16), to the same accuracy.
+// at 16 times the rate (K = 32; 8 times at K = 16), to the same accuracy.  (A product whose second operand has K = 16 too
+// stays in float where making its parts would cost the vector ALU more than the matrix cores save.)
+//
+// What bounds it, us with what memory alone would take of q, k, v, o and their gradients (4.63 TB/s): 8192 marched rays, 4
+// heads of 32 x 32, bf16, forward 136 (43), backward 334 (43): the vector ALU, 61 to 64 % busy, beside the waits of short
+// rays' few chunks; 24 rays of up to 4096 rows, 8 heads of 64 x 64 on 4, bf16, 468 and 1207 + 60 (98 in all): the chain of a
+// ray's 256 chunks, 1.8 and 4.7 us each, at less than a wavefront a SIMD; 3001 rays, 3 heads of 24 x 40, fp32, with states,
+// 109 and 281 (92): vector ALU and fp32 matrix cores a third each.  Tried, us: the next segment's v ahead in the forward 163
+// (149 without), the heads of a ray one after the other in a block 204 and 602 (139 and 352: the longest ray's chain is
+// four times as long), states kept every chunk (twice the marks) not built.
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -87,7 +96,6 @@ template <typename T> struct Delta {
   static __device__ __forceinline__ Full full(const f32x4& x) { return x; }
   static __device__ __forceinline__ Two two(const f32x4& x) { return x; }
   static __device__ __forceinline__ Two first_two(const Full& x) { return x; }
-  static __device__ __forceinline__ Row row(const f32x4& x) { return x; }
   static __device__ __forceinline__ f32x4 value(const Row& x) { return x; }
   // on a product: 16 values of K from each operand's lane parts, then 32
   template <typename A, typename B> static __device__ __forceinline__ f32x4 mul(const A& a, const B& b, const f32x4& c) { return mul16(a, b, c); }
