@@ -333,7 +333,7 @@ template <typename T> struct RawCol {
     f32x4 x;
 #pragma unroll
     for (int r = 0; r < 4; ++r) x[r] = (float)v[r];
-    if (ck.many < DL_C || cols % 16) {
+    if (ck.many < DL_C || cols % 16 || col >= cols) {  // (a wavefront may lie past the columns as a whole)
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[r] = 4 * g + r < ck.many && col < cols ? x[r] : 0.f;
     }

@@ -87,3 +87,24 @@ def test_rows_of_no_ray_and_no_rays():
         o, last, m = ray_ops.ray_delta(*x, s, last=True, marks=True)
         grads = ray_ops.ray_delta_backward(torch.randn_like(o), *x, m, s)
         assert not o.any() and last.shape[0] == 0 and all(not t.any() for t in grads[:5])
+
+
+def test_rows_past_32_bit_offsets():
+    """More than 2^32 bytes between the first row and the last: the bits of rows that lie together."""
+    import ray_ops
+    n, apart = 600, 1 << 22
+    rays = ray_set([300, 17, 283])
+    x = [t.cuda() for t in inputs(n, 1, 1, 32, 32, torch.bfloat16, seed=2)]
+    do = torch.randn(n, 1, 32, device="cuda").to(torch.bfloat16)
+    big = torch.empty(n, apart, dtype=torch.bfloat16, device="cuda")
+    far = []
+    for i, t in enumerate((*x[:3], do)):
+        v = big.as_strided((n, 1, 32), (apart, 32, 1), 64 * i)
+        v.copy_(t)
+        far.append(v)
+    set_ = ray_ops.RaySet(*(t.cuda() for t in rays[:3]))
+    a, b = ray_ops.ray_delta(*x, set_, marks=True), ray_ops.ray_delta(*far[:3], *x[3:], set_, marks=True)
+    assert torch.equal(a[0], b[0])
+    ga = ray_ops.ray_delta_backward(do, *x, a[2], set_)
+    gb = ray_ops.ray_delta_backward(far[3], *far[:3], *x[3:], b[2], set_)
+    assert all(torch.equal(p, q) for p, q in zip(ga[:5], gb[:5]))
