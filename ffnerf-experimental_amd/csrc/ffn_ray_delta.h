@@ -21,13 +21,13 @@
 // at 16 times the rate (K = 32; 8 times at K = 16), to the same accuracy.  (A product whose second operand has K = 16 too
 // stays in float where making its parts would cost the vector ALU more than the matrix cores save.)
 //
-// What bounds it, us with what memory alone would take of q, k, v, o and their gradients (4.63 TB/s): 8192 marched rays, 4
-// heads of 32 x 32, bf16, forward 136 (43), backward 334 (43): the vector ALU, 61 to 64 % busy, beside the waits of short
-// rays' few chunks; 24 rays of up to 4096 rows, 8 heads of 64 x 64 on 4, bf16, 468 and 1207 + 60 (98 in all): the chain of a
-// ray's 256 chunks, 1.8 and 4.7 us each, at less than a wavefront a SIMD; 3001 rays, 3 heads of 24 x 40, fp32, with states,
-// 109 and 281 (92): vector ALU and fp32 matrix cores a third each.  Tried, us: the next segment's v ahead in the forward 163
-// (149 without), the heads of a ray one after the other in a block 204 and 602 (139 and 352: the longest ray's chain is
-// four times as long), states kept every chunk (twice the marks) not built.
+// What bounds it, us a kernel with what memory alone would take of q, k, v, o and their gradients (4.63 TB/s): 8192 marched
+// rays, 4 heads of 32 x 32, bf16, forward 140 (43), backward 370 (43): the vector ALU, beside the waits of short rays' few
+// chunks; 24 rays of up to 4096 rows, 8 heads of 64 x 64 on 4, bf16, 476 and 1361 + 62 (98 in all): what a block does for a
+// chunk, one after the other, 1.8 and 5.3 us for each of a ray's 256, at less than a wavefront a SIMD; 3001 rays, 3 heads of
+// 24 x 40, fp32, with states, 111 and 286 (92): vector ALU and fp32 matrix cores a third each.  Not kept, us when each was
+// tried: the next segment's v ahead in the forward 163 (149 without); the heads of a ray one after the other in a block 204
+// and 602 (139 and 352: the longest ray's chain is four times as long).  Not built: states kept every chunk (twice the marks).
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -64,10 +64,9 @@ __device__ __forceinline__ f32x4 mul16(const f32x4& a, const f32x4& b, f32x4 to)
   return to;
 }
 
-// Four floats as three bfloat16 parts, by cutting 8 bits of the 24 each time, which together are the float itself; or as two,
-// the second one rounded, which are off by 2^-17 of it at most and by nothing on average.
-template <int N> struct Parts {
-  b16x4 p[N];
+// Four floats as three bfloat16 parts, by cutting 8 bits of the 24 each time, which together are the float itself.
+struct Parts {
+  b16x4 p[3];
 };
 __device__ __forceinline__ b16x4 upper_of(const f32x4& x) {
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -80,22 +79,17 @@ __device__ __forceinline__ f32x4 rest_of(const f32x4& x) {
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   return x - __builtin_bit_cast(f32x4, __builtin_bit_cast(u32x4, x) & 0xFFFF0000u);
 }
-template <int N> __device__ __forceinline__ Parts<N> parts_of(const f32x4& x) {
+__device__ __forceinline__ Parts parts_of(const f32x4& x) {
   const f32x4 r = rest_of(x);
-  if constexpr (N == 2) return {{upper_of(x), __builtin_convertvector(r, b16x4)}};
-  else return {{upper_of(x), upper_of(r), upper_of(rest_of(r))}};
+  return {{upper_of(x), upper_of(r), upper_of(rest_of(r))}};
 }
 
-// How a type's rows enter products.  Row: four neighbouring values of a row.  Two: a float operand where the result is
-// rounded to the type (bfloat16: two parts).
+// How a type's rows enter products.  Row: four neighbouring values of a row.  Full: a float operand.
 template <typename T> struct Delta {
   static constexpr bool EXACT = false;
   typedef f32x4 Row;
   typedef f32x4 Full;
-  typedef f32x4 Two;
   static __device__ __forceinline__ Full full(const f32x4& x) { return x; }
-  static __device__ __forceinline__ Two two(const f32x4& x) { return x; }
-  static __device__ __forceinline__ Two first_two(const Full& x) { return x; }
   static __device__ __forceinline__ f32x4 value(const Row& x) { return x; }
   // on a product: 16 values of K from each operand's lane parts, then 32
   template <typename A, typename B> static __device__ __forceinline__ f32x4 mul(const A& a, const B& b, const f32x4& c) { return mul16(a, b, c); }
@@ -107,44 +101,49 @@ template <typename T> struct Delta {
 template <> struct Delta<__bf16> {
   static constexpr bool EXACT = true;
   typedef b16x4 Row;
-  typedef Parts<3> Full;
-  typedef Parts<2> Two;
-  static __device__ __forceinline__ Full full(const f32x4& x) { return parts_of<3>(x); }
-  static __device__ __forceinline__ Two two(const f32x4& x) { return parts_of<2>(x); }
-  static __device__ __forceinline__ Two first_two(const Full& x) { return {{x.p[0], x.p[1]}}; }
+  typedef Parts Full;
+  static __device__ __forceinline__ Full full(const f32x4& x) { return parts_of(x); }
   static __device__ __forceinline__ f32x4 value(const Row& x) { return __builtin_convertvector(x, f32x4); }
   static __device__ __forceinline__ f32x4 mul(const Row& a, const Row& b, const f32x4& c) { return mma16(a, b, c); }
-  template <int N> static __device__ __forceinline__ f32x4 mul(const Row& a, const Parts<N>& b, f32x4 c) {
+  static __device__ __forceinline__ f32x4 mul(const Row& a, const Full& b, f32x4 c) {
 #pragma unroll
-    for (int i = N - 1; i >= 0; --i) c = mma16(a, b.p[i], c);
+    for (int i = 2; i >= 0; --i) c = mma16(a, b.p[i], c);
     return c;
   }
-  template <int N> static __device__ __forceinline__ f32x4 mul(const Parts<N>& a, const Row& b, f32x4 c) {
+  static __device__ __forceinline__ f32x4 mul(const Full& a, const Row& b, f32x4 c) {
 #pragma unroll
-    for (int i = N - 1; i >= 0; --i) c = mma16(a.p[i], b, c);
+    for (int i = 2; i >= 0; --i) c = mma16(a.p[i], b, c);
     return c;
   }
-  static __device__ __forceinline__ f32x4 mul(const Two& a, const Two& b, const f32x4& c) {
-    return mma16(a.p[0], b.p[0], mma16(a.p[0], b.p[1], mma16(a.p[1], b.p[0], c)));
+  // of two floats: six products; those left out are 2^-23 of a b at most, as a rounding of it in float would be
+  static __device__ __forceinline__ f32x4 mul(const Full& a, const Full& b, f32x4 c) {
+#pragma unroll
+    for (int s = 2; s >= 0; --s) {
+#pragma unroll
+      for (int i = 0; i <= s; ++i) c = mma16(a.p[i], b.p[s - i], c);
+    }
+    return c;
   }
   static __device__ __forceinline__ f32x4 mul(const Row& a0, const Row& a1, const Row& b0, const Row& b1, const f32x4& c) {
     return mma32(a0, a1, b0, b1, c);
   }
-  template <int N>
-  static __device__ __forceinline__ f32x4 mul(const Row& a0, const Row& a1, const Parts<N>& b0, const Parts<N>& b1, f32x4 c) {
+  static __device__ __forceinline__ f32x4 mul(const Row& a0, const Row& a1, const Full& b0, const Full& b1, f32x4 c) {
 #pragma unroll
-    for (int i = N - 1; i >= 0; --i) c = mma32(a0, a1, b0.p[i], b1.p[i], c);
+    for (int i = 2; i >= 0; --i) c = mma32(a0, a1, b0.p[i], b1.p[i], c);
     return c;
   }
-  template <int N>
-  static __device__ __forceinline__ f32x4 mul(const Parts<N>& a0, const Parts<N>& a1, const Row& b0, const Row& b1, f32x4 c) {
+  static __device__ __forceinline__ f32x4 mul(const Full& a0, const Full& a1, const Row& b0, const Row& b1, f32x4 c) {
 #pragma unroll
-    for (int i = N - 1; i >= 0; --i) c = mma32(a0.p[i], a1.p[i], b0, b1, c);
+    for (int i = 2; i >= 0; --i) c = mma32(a0.p[i], a1.p[i], b0, b1, c);
     return c;
   }
-  static __device__ __forceinline__ f32x4 mul(const Two& a0, const Two& a1, const Two& b0, const Two& b1, const f32x4& c) {
-    return mma32(a0.p[0], a1.p[0], b0.p[0], b1.p[0],
-                 mma32(a0.p[0], a1.p[0], b0.p[1], b1.p[1], mma32(a0.p[1], a1.p[1], b0.p[0], b1.p[0], c)));
+  static __device__ __forceinline__ f32x4 mul(const Full& a0, const Full& a1, const Full& b0, const Full& b1, f32x4 c) {
+#pragma unroll
+    for (int s = 2; s >= 0; --s) {
+#pragma unroll
+      for (int i = 0; i <= s; ++i) c = mma32(a0.p[i], a1.p[i], b0.p[s - i], b1.p[s - i], c);
+    }
+    return c;
   }
 };
 
@@ -188,6 +187,8 @@ template <typename T> __device__ __forceinline__ int four_at(int r, int u) {
   if constexpr (Delta<T>::EXACT) return r * 16 + 4 * (u ^ ((r >> 3) << 1));
   else return r * Tile<T>::LD + 4 * u;
 }
+// the same of a matrix of floats whose rows lie side by side
+__device__ __forceinline__ int float4_at(int r, int u) { return r * 16 + 4 * (u ^ (r >> 2)); }
 template <typename T> __device__ __forceinline__ typename Delta<T>::Row row_of(const T* tile, int c, int g) {
   const T* p = tile + four_at<T>(c, g);
   if constexpr (Delta<T>::EXACT) return *reinterpret_cast<const b16x4*>(p);
@@ -473,7 +474,7 @@ __device__ __forceinline__ void prepare_chunk(const typename Delta<T>::Row (&kf)
   }
   *reinterpret_cast<f32x4*>(Tm + c * DL_LD + 4 * g) = A;
   *reinterpret_cast<f32x4*>(Pm + c * DL_LD + 4 * g) = P;
-  if (Dm) *reinterpret_cast<f32x4*>(Dm + c * DL_LD + 4 * g) = D;
+  if (Dm) *reinterpret_cast<f32x4*>(Dm + float4_at(c, g)) = D;
   const float e = exp_of(decay[0] + sum[0]);  // in the first group, from the chunk's start to row c
   if (g == 0) {
     vec[c] = beta;
@@ -627,14 +628,10 @@ __global__ __launch_bounds__(64 * W, (DL_FWD_WAVES<T, DK, W>)) void k_delta_fwd(
         const f32x4 Tr = *reinterpret_cast<const f32x4*>(&Tm[i][c * DL_LD + 4 * g]);
         const f32x4 Pr = *reinterpret_cast<const f32x4*>(&Pm[i][c * DL_LD + 4 * g]);
         typename Ops::Full full[NT];
-        typename Ops::Two some[NT];  // enough for o, which is rounded
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          full[t] = Ops::full(S[t]);
-          some[t] = Ops::first_two(full[t]);
-        }
+        for (int t = 0; t < NT; ++t) full[t] = Ops::full(S[t]);
         const f32x4 R = beta * (vr[i].value(ck, g, w16 + c, a.val_dim) - e * mul_tiles<T>(kf, full, zero));
-        const f32x4 qs = a.scale * e * mul_tiles<T>(qf, some, zero);
+        const f32x4 qs = a.scale * e * mul_tiles<T>(qf, full, zero);
         const f32x4 n = mul16(Tr, R, zero);
         f32x4 y = mul16(Pr, n, qs);
         const typename Ops::Full nl = Ops::full(left * n);
@@ -743,28 +740,28 @@ __global__ __launch_bounds__(256, DK <= 32 ? 6 : DK <= 64 ? 5 : 3) void k_delta_
 // wavefront takes 16 columns of dq and dk.
 
 // Tiles of 16 x 16 floats in LDS, put down by columns as products leave them (column c, rows 4 g + r) and taken up by rows,
-// as operands of products whose result is rounded to the type: floats, or two parts each.
+// as operands: floats, or three parts each.
 template <typename T> struct Tiles {
-  static constexpr int WORDS = 256;  // of a tile
+  static constexpr int WORDS = Delta<T>::EXACT ? 3 * 128 : 256;  // of a tile
   float* p;
   __device__ __forceinline__ void set(int tile, int c, int g, const f32x4& x) const {
     if constexpr (Delta<T>::EXACT) {
-      set(tile, c, g, parts_of<2>(x));
+      set(tile, c, g, parts_of(x));
     } else {
       // row 4 g + r is the (4 r + g)th, its fours of columns in an order that goes by r: neither side meets a bank twice
 #pragma unroll
       for (int r = 0; r < 4; ++r) p[tile * WORDS + (4 * r + g) * 16 + 4 * ((c >> 2) ^ r) + (c & 3)] = x[r];
     }
   }
-  template <int N> __device__ __forceinline__ void set(int tile, int c, int g, const Parts<N>& x) const {
+  __device__ __forceinline__ void set(int tile, int c, int g, const Parts& x) const {
     __bf16* q = (__bf16*)(p + tile * WORDS) + four_at<__bf16>(c, g);  // transposed, so that four rows lie side by side
-    *reinterpret_cast<b16x4*>(q) = x.p[0];
-    *reinterpret_cast<b16x4*>(q + 256) = x.p[1];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) *reinterpret_cast<b16x4*>(q + 256 * i) = x.p[i];
   }
-  __device__ __forceinline__ typename Delta<T>::Two get(int tile, int c, int g) const {
+  __device__ __forceinline__ typename Delta<T>::Full get(int tile, int c, int g) const {
     if constexpr (Delta<T>::EXACT) {
       const __bf16* q = (const __bf16*)(p + tile * WORDS);
-      return {{col_of(q, c, g), col_of(q + 256, c, g)}};
+      return {{col_of(q, c, g), col_of(q + 256, c, g), col_of(q + 512, c, g)}};
     } else {
       return *reinterpret_cast<const f32x4*>(p + tile * WORDS + (4 * (c & 3) + (c >> 2)) * 16 + 4 * (g ^ (c & 3)));
     }
@@ -772,28 +769,30 @@ template <typename T> struct Tiles {
 };
 // A 16 x 16 matrix of floats, put down as this lane's row c, columns 4 g + s, and taken up by rows or by columns.
 template <typename T> struct Square {
-  float* p;  // 256
+  static constexpr int WORDS = Tiles<T>::WORDS;
+  float* p;
   __device__ __forceinline__ void set(int c, int g, const f32x4& x) const {
     if constexpr (Delta<T>::EXACT) {
-      const Parts<2> y = parts_of<2>(x);
+      const Parts y = parts_of(x);
       __bf16* q = (__bf16*)p + four_at<__bf16>(c, g);
-      *reinterpret_cast<b16x4*>(q) = y.p[0];
-      *reinterpret_cast<b16x4*>(q + 256) = y.p[1];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) *reinterpret_cast<b16x4*>(q + 256 * i) = y.p[i];
     } else {
-      *reinterpret_cast<f32x4*>(p + c * 16 + 4 * (g ^ (c >> 2))) = x;
+      *reinterpret_cast<f32x4*>(p + float4_at(c, g)) = x;
     }
   }
-  __device__ __forceinline__ typename Delta<T>::Two row(int c, int g) const {
+  __device__ __forceinline__ typename Delta<T>::Full row(int c, int g) const {
     if constexpr (Delta<T>::EXACT) {
       const __bf16* q = (const __bf16*)p + four_at<__bf16>(c, g);
-      return {{*reinterpret_cast<const b16x4*>(q), *reinterpret_cast<const b16x4*>(q + 256)}};
+      return {{*reinterpret_cast<const b16x4*>(q), *reinterpret_cast<const b16x4*>(q + 256), *reinterpret_cast<const b16x4*>(q + 512)}};
     } else {
-      return *reinterpret_cast<const f32x4*>(p + c * 16 + 4 * (g ^ (c >> 2)));
+      return *reinterpret_cast<const f32x4*>(p + float4_at(c, g));
     }
   }
-  __device__ __forceinline__ typename Delta<T>::Two col(int c, int g) const {
+  __device__ __forceinline__ typename Delta<T>::Full col(int c, int g) const {
     if constexpr (Delta<T>::EXACT) {
-      return {{col_of((const __bf16*)p, c, g), col_of((const __bf16*)p + 256, c, g)}};
+      const __bf16* q = (const __bf16*)p;
+      return {{col_of(q, c, g), col_of(q + 256, c, g), col_of(q + 512, c, g)}};
     } else {
       f32x4 x;
 #pragma unroll
@@ -831,20 +830,24 @@ __device__ __forceinline__ f32x4 mul_cols(A a, B b, f32x4 c) {
 
 template <typename T, int DK, int W> struct DeltaLds {
   static constexpr int SQ = DL_C * DL_LD, NT = DK / 16;
-  static constexpr int WORDS = DL_SEG * (3 * SQ + DL_VEC) + 3 * 256 + (2 + NT) * W * Tiles<T>::WORDS + W * 32;
+  static constexpr int RL = W * Tiles<T>::WORDS, XYZ = 3 * Square<T>::WORDS;  // of dR, and of X, Y and Z after it
+  static constexpr int WORDS = DL_SEG * (2 * SQ + 256 + DL_VEC) + (RL > XYZ ? RL : XYZ) + (1 + NT) * W * Tiles<T>::WORDS + W * 32;
   static constexpr int BYTES = WORDS * 4 + (2 * DL_SEG * NT + W) * Tile<T>::SIZE * (int)sizeof(T);
 };
 
-// AHEAD: a segment's rows and state are asked for while the one after it is worked on (24 rays of up to 4096 rows, 8 heads of
-// 64 x 64, bf16: 1309 us, 1361 without; 8192 marched rays 312 and 319).  Rows that are held as floats cost a wavefront a SIMD
-// for it (3001 rays of fp32, 24 x 40: 426 us, 287 without), 128 columns leave no registers, and a wavefront alone prepares
-// both chunks of a segment.
+// Wavefronts a SIMD that the backward's registers are held to, where no spill comes of it.
+template <typename T, int DK, int W> constexpr int DL_BWD_WAVES = Delta<T>::EXACT && DK == 32 && W == 2 ? 3 : 1;
+
+// AHEAD: a segment's rows and state are asked for while the one after it is worked on, where its registers cost no wavefront a
+// SIMD (24 rays of up to 4096 rows, 8 heads of 64 x 64, bf16: 1416 us, 1482 without; 8192 marched rays, 4 heads of 32 x 32,
+// 426 with two wavefronts and 342 without with three; 2048 of 64 x 32 255 with one and 148 without with two), and there is
+// more than one wavefront to prepare a segment's chunks.  Rows that are held as floats cost one, 128 columns leave none.
 template <typename T, int DK, int W>
-__global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a, int longer) {
+__global__ __launch_bounds__(64 * W, (DL_BWD_WAVES<T, DK, W>)) void k_delta_bwd(const ffn_ray_delta a, int longer) {
   typedef Delta<T> Ops;
   typedef typename Ops::Row Row;
   typedef DeltaLds<T, DK, W> L;
-  constexpr bool AHEAD = Ops::EXACT && DK <= 64 && W > 1;
+  constexpr bool AHEAD = Ops::EXACT && (DK == 32 ? W > 2 : DK == 64 && W == 4);
   constexpr int NT = DK / 16, TP = (NT + W - 1) / W, SQ = L::SQ, TILE = Tile<T>::SIZE;
   extern __shared__ __align__(16) float lds[];
   const int64_t teams = (int64_t)a.rays.num_rays * a.v_heads;
@@ -875,11 +878,11 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a, int
   float* Tm = lds;
   float* Pm = Tm + DL_SEG * SQ;
   float* Dm = Pm + DL_SEG * SQ;
-  float* vecs = Dm + DL_SEG * SQ;
-  const Square<T> Xm{vecs + DL_SEG * DL_VEC}, Ym{Xm.p + 256}, Zm{Ym.p + 256};
+  float* vecs = Dm + DL_SEG * 256;
   // n, dR; S and dS, tile t W + u: rows of tile t, columns of wavefront u
-  const Tiles<T> Nl{Zm.p + 256}, Rl{Nl.p + W * Tiles<T>::WORDS}, Sl{Rl.p + W * Tiles<T>::WORDS};
-  float* sums = Sl.p + NT * W * Tiles<T>::WORDS;
+  const Tiles<T> Nl{vecs + DL_SEG * DL_VEC}, Sl{Nl.p + W * Tiles<T>::WORDS}, Rl{Sl.p + NT * W * Tiles<T>::WORDS};
+  const Square<T> Xm{Rl.p}, Ym{Xm.p + Square<T>::WORDS}, Zm{Ym.p + Square<T>::WORDS};  // where dR was
+  float* sums = Rl.p + (L::RL > L::XYZ ? L::RL : L::XYZ);
   T* Kl = (T*)(sums + W * 32);
   T* Ql = Kl + DL_SEG * NT * TILE;
   const RowTiles<T> Gl{Ql + DL_SEG * NT * TILE};  // do
@@ -951,14 +954,13 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a, int
           *reinterpret_cast<tvec*>(Kl + (i * NT + t) * TILE + four_at<T>(c, g)) = kr[j].v[t];
           *reinterpret_cast<tvec*>(Ql + (i * NT + t) * TILE + four_at<T>(c, g)) = qr[j].v[t];
         }
-        prepare_chunk<T>(kf, qf, gates[j].decay(ck, g), gates[j].beta(ck, c), a.scale, c, g, Tm + i * SQ, Pm + i * SQ, Dm + i * SQ,
+        prepare_chunk<T>(kf, qf, gates[j].decay(ck, g), gates[j].beta(ck, c), a.scale, c, g, Tm + i * SQ, Pm + i * SQ, Dm + i * 256,
                          vecs + i * DL_VEC);
       }
     }
     if (AHEAD && p0) fetch(p0 - DL_MARK);
     sync();
-    // the states before the segment's chunks, and their writes n: they reach gradients that are rounded to the type, and
-    // not dS, so that two parts are enough
+    // the states before the segment's chunks, and their writes n
 #pragma unroll
     for (int i = 0; i < DL_SEG; ++i) {
       if (p0 + DL_C * i < ch.count) {
@@ -966,17 +968,17 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a, int
         const T* Kc = Kl + i * NT * TILE;
         const float* vec = vecs + i * DL_VEC;
         Row kf[NT];
-        typename Ops::Two some[NT];
+        typename Ops::Full full[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           kf[t] = row_of(Kc + t * TILE, c, g);
-          some[t] = Ops::two(S[i][t]);
+          full[t] = Ops::full(S[i][t]);
         }
         const f32x4 beta = *reinterpret_cast<const f32x4*>(vec + 4 * g), e = *reinterpret_cast<const f32x4*>(vec + 16 + 4 * g);
-        const f32x4 R = beta * (vr[i].value(ck, g, w16 + c, a.val_dim) - e * mul_tiles<T>(kf, some, zero));
+        const f32x4 R = beta * (vr[i].value(ck, g, w16 + c, a.val_dim) - e * mul_tiles<T>(kf, full, zero));
         n[i] = mul16(*reinterpret_cast<const f32x4*>(Tm + i * SQ + c * DL_LD + 4 * g), R, zero);
         if (i + 1 == DL_SEG || p0 + DL_C * (i + 1) >= ch.count) continue;
-        const typename Ops::Two nl = Ops::two(*reinterpret_cast<const f32x4*>(vec + 32 + 4 * g) * n[i]);
+        const typename Ops::Full nl = Ops::full(*reinterpret_cast<const f32x4*>(vec + 32 + 4 * g) * n[i]);
 #pragma unroll
         for (int t = 0; t < NT; ++t) S[i + 1 < DL_SEG ? i + 1 : i][t] = Ops::mul(col_of(Kc + t * TILE, c, g), nl, vec[48] * S[i][t]);
       }
@@ -988,7 +990,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a, int
         asm volatile("" : "+v"(c), "+v"(g));
         const Chunk ck(ch, p);
         const T *Kc = Kl + i * NT * TILE, *Qc = Ql + i * NT * TILE;
-        const float *vec = vecs + i * DL_VEC, *Tc = Tm + i * SQ, *Pc = Pm + i * SQ, *Dc = Dm + i * SQ;
+        const float *vec = vecs + i * DL_VEC, *Tc = Tm + i * SQ, *Pc = Pm + i * SQ, *Dc = Dm + i * 256;
         const int vcol = w16 + c;
         const f32x4 beta = *reinterpret_cast<const f32x4*>(vec + 4 * g), e = *reinterpret_cast<const f32x4*>(vec + 16 + 4 * g);
         const f32x4 left = *reinterpret_cast<const f32x4*>(vec + 32 + 4 * g);
@@ -1033,20 +1035,18 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a, int
         const auto n_row = [&](int u) { return Nl.get(u, c, g); };
         const auto r_row = [&](int u) { return Rl.get(u, c, g); };
         // X and Y (the first and the second wavefront, where there are two); products with S
+        f32x4 x = zero, y = zero;
         if (w == 0 || w == 1) {
-          const f32x4 D = *reinterpret_cast<const f32x4*>(Dc + c * DL_LD + 4 * g);
+          const f32x4 D = *reinterpret_cast<const f32x4*>(Dc + float4_at(c, g));
           if (w == 0) {
-            f32x4 x = mul_cols<T, W>(n_row, g_row, zero);  // rows j, column i
+            x = mul_cols<T, W>(n_row, g_row, zero);  // rows j, column i
 #pragma unroll
             for (int r = 0; r < 4; ++r) x[r] = 4 * g + r <= c ? a.scale * D[r] * x[r] : 0.f;
-            Xm.set(c, g, x);
           }
           if (w == 1 || W == 1) {
-            f32x4 y = mul_cols<T, W>(n_row, r_row, zero);
+            y = mul_cols<T, W>(n_row, r_row, zero);
 #pragma unroll
             for (int r = 0; r < 4; ++r) y[r] = 4 * g + r < c ? -D[r] * y[r] : 0.f;
-            Ym.set(c, g, y);
-            Zm.set(c, g, vec[c] * y);
           }
         }
         f32x4 sq[TP], lf[TP];
@@ -1060,6 +1060,11 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a, int
           }
         }
         sync();
+        if (w == 0) Xm.set(c, g, x);
+        if (w == 1 || W == 1) {
+          Ym.set(c, g, y);
+          Zm.set(c, g, vec[c] * y);
+        }
         // dS out, and back to the chunk's start
         const typename Ops::Full fo = Ops::full(a.scale * e * go), fr = Ops::full(-(beta * e) * dR);
 #pragma unroll
@@ -1068,7 +1073,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_bwd(const ffn_ray_delta a, int
           dS[t] = Ops::mul(col_of(Kc + t * TILE, c, g), fr, Ops::mul(col_of(Qc + t * TILE, c, g), fo, vec[48] * dS[t]));
         }
         sync();
-        const typename Ops::Two xr = Xm.row(c, g), yr = Ym.row(c, g), xt = Xm.col(c, g), zt = Zm.col(c, g);
+        const typename Ops::Full xr = Xm.row(c, g), yr = Ym.row(c, g), xt = Xm.col(c, g), zt = Zm.col(c, g);
 #pragma unroll
         for (int j = 0; j < TP; ++j) {
           const int t = w + j * W, kcol = 16 * t + c;
