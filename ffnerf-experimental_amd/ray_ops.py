@@ -135,6 +135,11 @@ def once(fn, *inputs):
     return _Once.apply(fn, *inputs) if torch.is_grad_enabled() else fn()
 
 
+def _needed(ctx, i: int) -> bool:
+    """Whether the gradient of argument i is wanted; one that was left out of the call has none."""
+    return i < len(ctx.needs_input_grad) and ctx.needs_input_grad[i]
+
+
 # ---------------------------------------------------------------------------
 # attention
 
@@ -634,7 +639,7 @@ class ExpertCombine(torch.autograd.Function):
     def backward(ctx, dout):
         y, weights = ctx.saved_tensors
         dout = dout if dout.stride(-1) == 1 else dout.contiguous()
-        need = ctx.needs_input_grad[2]
+        need = _needed(ctx, 2)
         dy, dw = once(lambda: expert_combine_backward(dout, y, ctx.route, weights, need_dweights=need), dout, y, weights)
         return dy, None, dw
 
@@ -702,7 +707,7 @@ class LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, mean, rstd = ctx.saved_tensors
         dy = dy if dy.stride(-1) == 1 else dy.contiguous()
-        need_w, need_b = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
+        need_w, need_b = _needed(ctx, 1), _needed(ctx, 2)
         dx, dw, db = once(lambda: layer_norm_backward(dy, x, weight, mean, rstd, need_dx=ctx.needs_input_grad[0],
                                                       need_dw=need_w or need_b), dy, x, weight)
         return dx, dw.to(weight.dtype) if need_w else None, db.to(ctx.bias_dtype) if need_b else None, None
