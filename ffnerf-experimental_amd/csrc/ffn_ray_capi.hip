@@ -26,7 +26,7 @@ constexpr uint32_t MAX_ROWS = 0x7FFFFF00u;
 constexpr int MAX_SCAN_STRIDE = 1 << 27;
 
 constexpr uint64_t MAX_SCAN_STATES = 1ull << 46;  // channels of all rays: what one launch can count
-constexpr int MAX_DELTA_STRIDE = 1 << 24;
+constexpr int MAX_DELTA_STRIDE = 1 << 24;  // of rows
 constexpr uint64_t MAX_DELTA_STATES = 1ull << 36; // heads of all rays: a block each
 
 int elem(int32_t dtype) { return dtype == FFN_F32 ? 4 : dtype == FFN_F16 || dtype == FFN_BF16 ? 2 : 0; }
@@ -172,12 +172,14 @@ int check_delta(const ffn_ray_delta* a, bool backward) {
   const int b = elem(a->dtype);
   const int64_t rows = a->rays.n, h = n ? a->heads : 0, vh = n ? a->v_heads : 0;
   if (n && (!a->q || !a->k || !a->v || !a->decay || !a->beta)) return fail(-1, "NULL buffer");
-  const int64_t steps[] = {step(rows, a->q_row),     step(h, a->q_head),       step(rows, a->k_row),    step(h, a->k_head),
-                           step(rows, a->v_row),     step(vh, a->v_head),      step(rows, a->decay_row), step(vh, a->decay_head),
-                           step(rows, a->beta_row),  step(vh, a->beta_head),   backward ? step(rows, a->do_row) : 0,
-                           backward ? step(vh, a->do_head) : 0};
-  for (int64_t s : steps)  // the kernels step through a chunk's rows with products of 24 bits
-    if (s < 0 || s >= MAX_DELTA_STRIDE / b) return fail(-1, "strides must be 0 or more, below %d bytes", MAX_DELTA_STRIDE);
+  const int64_t row_steps[] = {step(rows, a->q_row),    step(rows, a->k_row),    step(rows, a->v_row), step(rows, a->decay_row),
+                               step(rows, a->beta_row), backward ? step(rows, a->do_row) : 0};
+  for (int64_t s : row_steps)  // the kernels step through a chunk's rows with products of 24 bits
+    if (s < 0 || s >= MAX_DELTA_STRIDE / b) return fail(-1, "row strides must be 0 or more, below %d bytes", MAX_DELTA_STRIDE);
+  const int64_t head_steps[] = {step(h, a->q_head),      step(h, a->k_head),     step(vh, a->v_head), step(vh, a->decay_head),
+                                step(vh, a->beta_head), backward ? step(vh, a->do_head) : 0};
+  for (int64_t s : head_steps)
+    if (s < 0) return fail(-1, "head strides must be 0 or more");
   if (!aligned(a->q, step(rows, a->q_row), b) || !aligned(a->q, step(h, a->q_head), b) || !aligned(a->k, step(rows, a->k_row), b) ||
       !aligned(a->k, step(h, a->k_head), b) || !aligned(a->v, step(rows, a->v_row), b) || !aligned(a->v, step(vh, a->v_head), b))
     return fail(-1, "rows and heads of q, k and v must be 16-byte aligned");

@@ -148,6 +148,7 @@ class FfnExperts(C.Structure):
 
 
 NORM_MAX_WIDTH = 16384  # FFN_NORM_MAX_WIDTH
+DELTA_ROW_BYTES = 1 << 24  # rows of the delta rule lie nearer together
 
 
 class FfnNorm(C.Structure):

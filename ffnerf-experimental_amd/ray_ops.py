@@ -341,9 +341,10 @@ def ray_delta(q, k, v, decay, beta, rays: RaySet, *, h0=None, scale: float | Non
     n_t = beta_t (v_t - a_t S_{t-1}^T k_t), read as o_t = scale S_t^T q_t (scale: 1/sqrt(key dim)).
 
     q and k [n, heads, key_dim], v [n, v_heads, val_dim] (float32, float16 or bfloat16, unit stride along the dims, rows
-    and heads on 16 bytes; v_heads a multiple of heads, which are shared; dims multiples of 8 up to 128), decay (at most 0;
-    -inf forgets what was before) and beta [n, v_heads] of the same type; stable where beta |k|^2 <= 2.  From h0 [num_rays,
-    v_heads, key_dim, val_dim] float32 (None: 0); reverse: from each ray's last row to its first.  o [n, v_heads, val_dim];
+    and heads on 16 bytes, rows less than 16 MiB apart; v_heads a multiple of heads, which are shared; dims multiples of 8
+    up to 128), decay (at most 0; -inf forgets what was before) and beta [n, v_heads] of the same type; stable where
+    beta |k|^2 <= 2.  From h0 [num_rays, v_heads, key_dim, val_dim] float32 (None: 0); reverse: from each ray's last row to
+    its first.  o [n, v_heads, val_dim];
     last: True for the state after each ray, or a tensor that takes it (h0 itself: in place), as h0; marks: what
     ray_delta_backward needs.  Both None unless asked."""
     lib = fl.load()
@@ -401,7 +402,9 @@ class RayDelta(torch.autograd.Function):
     @staticmethod
     def backward(ctx, do, dlast):
         q, k, v, decay, beta, marks, h0 = ctx.saved_tensors
-        if do.stride(-1) != 1 or any(s < 0 or s * do.element_size() % 16 for s in do.stride()[:2]) or do.data_ptr() % 16:
+        b = do.element_size()
+        if (do.stride(-1) != 1 or any(s * b % 16 for s in do.stride()[:2]) or do.data_ptr() % 16
+                or do.stride(0) * b >= fl.DELTA_ROW_BYTES):
             do = do.contiguous()
         dlast = None if dlast is None else dlast.contiguous()
         dq, dk, dv, dg, db, dh0 = once(

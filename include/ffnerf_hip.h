@@ -458,8 +458,9 @@ int ffn_ray_scan_bwd(const ffn_ray_scan* a, void* stream);
  * NaN too, does not reach the o of rows before it.
  * q and k [n][heads][key_dim], v [n][v_heads][val_dim] of dtype with unit stride
  * along the dims; value head h uses key head h / (v_heads / heads).  decay and
- * beta [n][v_heads] of dtype.  Strides in elements, 0 or more and below 2^24 bytes.  key_dim and
- * val_dim multiples of 8, at most 128; rows and heads of q, k, v 16-byte aligned.
+ * beta [n][v_heads] of dtype.  Strides in elements, 0 or more, those of rows
+ * below 2^24 bytes.  key_dim and val_dim multiples of 8, at most 128; rows and
+ * heads of q, k, v 16-byte aligned.
  * o [n][v_heads][val_dim] of dtype; h0, last, dlast, dh0
  * [num_rays][v_heads][key_dim][val_dim] float; all contiguous and 16-byte aligned.  last (NULL: not
  * wanted) is the state after a ray's last row, h0 for a ray without rows, and
