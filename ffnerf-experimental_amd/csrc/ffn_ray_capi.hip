@@ -34,6 +34,12 @@ int elem(int32_t dtype) { return dtype == FFN_F32 ? 4 : dtype == FFN_F16 || dtyp
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 bool aligned(const void* p, int64_t stride, int size) { return aligned(p) && stride * size % 16 == 0; }
 
+// of two buffers of this many bytes
+bool overlap(const void* p, const void* q, uint64_t bytes) {
+  const uintptr_t x = (uintptr_t)p, y = (uintptr_t)q;
+  return (x < y ? y - x : x - y) < bytes;
+}
+
 // the stride of an axis of `count`: that of one place, or none, is any number and leads nowhere
 int64_t step(int64_t count, int64_t stride) { return count > 1 ? stride : 0; }
 
@@ -188,6 +194,14 @@ int check_delta(const ffn_ray_delta* a, bool backward) {
   if (!backward) {
     if (n && !a->o) return fail(-1, "NULL output");
     if (!aligned(a->o) || !aligned(a->last) || !aligned(a->marks)) return fail(-1, "o, last and marks must be 16-byte aligned");
+    const uint64_t states = (uint64_t)a->rays.num_rays * a->v_heads * a->key_dim * a->val_dim * sizeof(float);
+    if (a->h0 && a->last && states) {
+      if (a->last == a->h0) {
+        if (a->marks) return fail(-1, "last is h0, and marks are asked for: the backward reads h0");
+      } else if (overlap(a->last, a->h0, states)) {
+        return fail(-1, "last overlaps h0 without being it");
+      }
+    }
     return 0;
   }
   if (n && (!a->dout || !a->dq || !a->dk || !a->dv || !a->ddecay || !a->dbeta || !a->marks))

@@ -346,7 +346,7 @@ def ray_delta(q, k, v, decay, beta, rays: RaySet, *, h0=None, scale: float | Non
     beta |k|^2 <= 2.  From h0 [num_rays, v_heads, key_dim, val_dim] float32 (None: 0); reverse: from each ray's last row to
     its first.  o [n, v_heads, val_dim];
     last: True for the state after each ray, or a tensor that takes it (h0 itself: in place), as h0; marks: what
-    ray_delta_backward needs.  Both None unless asked."""
+    ray_delta_backward needs (refused with h0 in place, which the backward reads too).  Both None unless asked."""
     lib = fl.load()
     a, dev, state = _delta_args(q, k, v, decay, beta, rays, h0, scale, reverse)
     o = torch.empty(v.shape, dtype=v.dtype, device=dev)

@@ -464,8 +464,9 @@ int ffn_ray_scan_bwd(const ffn_ray_scan* a, void* stream);
  * o [n][v_heads][val_dim] of dtype; h0, last, dlast, dh0
  * [num_rays][v_heads][key_dim][val_dim] float; all contiguous and 16-byte aligned.  last (NULL: not
  * wanted) is the state after a ray's last row, h0 for a ray without rows, and
- * may be h0 itself.  marks (NULL without a backward pass): states the forward
- * keeps for the backward, of ffn_ray_delta_marks bytes. */
+ * may be h0 itself where there are no marks (the backward reads h0); a buffer
+ * that overlaps it otherwise is refused.  marks (NULL without a backward pass):
+ * states the forward keeps for the backward, of ffn_ray_delta_marks bytes. */
 typedef struct ffn_ray_delta {
   int32_t dtype, heads, v_heads, key_dim, val_dim, reverse;
   float scale;
