@@ -158,8 +158,9 @@ class RayMixer(torch.nn.Module):
         return torch.zeros(num_rays, self.heads, d, d, device=self.lo.device)
 
     def look(self, samples, features, rays: RaySet, state=None):
-        """Opacity and colour, before their sigmoids, of each sample [n, 4] from it and those in front of it.  state
-        (without gradients): what the rays have shown before these samples; it is moved on in place."""
+        """Opacity and colour, before their sigmoids, of each sample [n, 4] from it and those in front of it.  state: what
+        the rays have shown before these samples; it is moved on in place.  Gradients are those of these samples: none
+        passes through the state to the ones before them."""
         n, ty, d = samples.shape[0], self.dtype, self.width // self.heads
         x = (features @ self.W_in.t()).to(ty)
         h = LayerNorm.apply(x, self.n_1, self.m_1)
@@ -169,6 +170,10 @@ class RayMixer(torch.nn.Module):
         decay, beta = -torch.nn.functional.softplus(decay).to(ty), torch.sigmoid(beta).to(ty)
         if state is None:
             o = RayDelta.apply(q, k, v, decay, beta, rays, None, dict(last=False))[0]
+        elif torch.is_grad_enabled():
+            o, last = RayDelta.apply(q, k, v, decay, beta, rays, state.detach().clone())  # kept for the backward
+            with torch.no_grad():
+                state.copy_(last)
         else:
             o = ray_delta(q, k, v, decay, beta, rays, h0=state, last=state)[0]
         x = x + o.reshape(n, self.width) @ self.W_o.to(ty).t()
