@@ -388,13 +388,18 @@ def ray_delta_backward(do, q, k, v, decay, beta, marks, rays: RaySet, *, dlast=N
 
 class RayDelta(torch.autograd.Function):
     """(o, last) of ray_delta; differentiable in q, k, v, decay, beta and h0.  options: a dict of scale and reverse, and
-    last=False where the state after the rays is not wanted (None)."""
+    last=False where the state after the rays is not wanted (None).  Marks are made where a gradient is wanted only."""
+
+    @classmethod
+    def apply(cls, q, k, v, decay, beta, rays, h0=None, options=None):
+        return super().apply(q, k, v, decay, beta, rays, h0, options, torch.is_grad_enabled())
 
     @staticmethod
-    def forward(ctx, q, k, v, decay, beta, rays, h0=None, options=None):
+    def forward(ctx, q, k, v, decay, beta, rays, h0, options, grads):
         ctx.options = dict(options or {})
         wanted = ctx.options.pop("last", True)
-        o, last, marks = ray_delta(q, k, v, decay, beta, rays, h0=h0, last=bool(wanted), marks=True, **ctx.options)
+        o, last, marks = ray_delta(q, k, v, decay, beta, rays, h0=h0, last=bool(wanted),
+                                   marks=grads and any(ctx.needs_input_grad), **ctx.options)
         ctx.save_for_backward(q, k, v, decay, beta, marks, h0)
         ctx.rays = rays
         return o, last
@@ -410,7 +415,7 @@ class RayDelta(torch.autograd.Function):
         dq, dk, dv, dg, db, dh0 = once(
             lambda: ray_delta_backward(do, q, k, v, decay, beta, marks, ctx.rays, dlast=dlast, h0=h0, **ctx.options),
             do, dlast, q, k, v, decay, beta, h0)
-        return dq, dk, dv, dg, db, None, dh0, None
+        return dq, dk, dv, dg, db, None, dh0, None, None
 
 
 # ---------------------------------------------------------------------------
