@@ -32,6 +32,7 @@ constexpr uint64_t MAX_DELTA_STATES = 1ull << 36; // heads of all rays: a block 
 int elem(int32_t dtype) { return dtype == FFN_F32 ? 4 : dtype == FFN_F16 || dtype == FFN_BF16 ? 2 : 0; }
 
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
+bool words(const void* p) { return ((uintptr_t)p & 3) == 0; }  // of 4 bytes
 bool aligned(const void* p, int64_t stride, int size) { return aligned(p) && stride * size % 16 == 0; }
 
 // of two buffers of this many bytes
@@ -229,6 +230,8 @@ int check_norm(const ffn_norm* a) {
   const uintptr_t odd = elem(a->dtype) - 1, podd = elem(a->param_dtype) - 1;
   if (((uintptr_t)a->x | (uintptr_t)a->y | (uintptr_t)a->dy | (uintptr_t)a->dx) & odd) return fail(-1, "misaligned buffer");
   if (((uintptr_t)a->weight | (uintptr_t)a->bias) & podd) return fail(-1, "misaligned parameters");
+  if (!words(a->mean) || !words(a->rstd) || !words(a->dweight) || !words(a->dbias))
+    return fail(-1, "misaligned mean, rstd, dweight or dbias");
   return 0;
 }
 
@@ -245,6 +248,8 @@ int check_route(const ffn_route* a) {
   const uintptr_t odd = elem(a->dtype) - 1;
   if (((uintptr_t)a->rows_in | (uintptr_t)a->slots_in | (uintptr_t)a->rows_out | (uintptr_t)a->slots_out) & odd)
     return fail(-1, "misaligned buffer");
+  if (!words(a->plan) || !words(a->slots) || !words(a->weights) || !words(a->dweights))
+    return fail(-1, "misaligned plan, slots, weights or dweights");
   return 0;
 }
 
@@ -337,6 +342,7 @@ int ffn_expert_route(const int32_t* ids, uint32_t places, int32_t n_experts, uin
                      void* workspace, uint64_t workspace_bytes, void* stream) {
   if (int rc = check_plan(ids, places, n_experts, plan, plan_words, workspace, workspace_bytes)) return rc;
   if (places && !slots) return fail(-1, "NULL slots");
+  if (!words(ids) || !words(slots)) return fail(-1, "misaligned ids or slots");
   return launched(ffn::launch_expert_plan(ids, places, n_experts, plan, slots, (uint32_t*)workspace, (hipStream_t)stream),
                   "ffn_expert_route");
 }
