@@ -350,7 +350,8 @@ def ray_delta(q, k, v, decay, beta, rays: RaySet, *, h0=None, scale: float | Non
     lib = fl.load()
     a, dev, state = _delta_args(q, k, v, decay, beta, rays, h0, scale, reverse)
     o = torch.empty(v.shape, dtype=v.dtype, device=dev)
-    if isinstance(last, torch.Tensor):
+    given = isinstance(last, torch.Tensor)
+    if given:
         a.last = _want(last, "last", state, torch.float32, dev)
     else:
         last = torch.empty(state, dtype=torch.float32, device=dev) if last else None
@@ -362,6 +363,8 @@ def ray_delta(q, k, v, decay, beta, rays: RaySet, *, h0=None, scale: float | Non
         m = torch.empty(n.value // 4, dtype=torch.float32, device=dev)
         a.marks = m.data_ptr()
     _call(lib.ffn_ray_delta_fwd, dev, C.byref(a))
+    if given and not last.is_inference():
+        torch.autograd.graph.increment_version(last)  # a backward pass that has saved it must not use what is there now
     return o, last, m
 
 
