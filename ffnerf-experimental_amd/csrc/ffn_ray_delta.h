@@ -754,6 +754,7 @@ __global__ __launch_bounds__(256, DK <= 32 ? 6 : DK <= 64 ? 5 : 3) void k_delta_
 //   dS' = e_15 dS + sum_i (scale e_i q_i do_i^T - b_i e_i k_i dR_i^T)
 // Every factor e or D a row i was multiplied with gives its sum of products to the decays up to i:
 //   ddecay = sums, from each row to the chunk's end, of q.dq + b k.left - k.right, and at the end dS.S
+// to the accuracy of those terms: where a decay is so strong that they cancel, not to its own.
 // dn, dR, dv and dS go by columns, as S does; dq and dk are sums over the columns: S, dS, n and dR pass through LDS, and a
 // wavefront takes 16 columns of dq and dk.
 
@@ -1141,6 +1142,10 @@ __global__ __launch_bounds__(64 * W, (DL_BWD_WAVES<T, DK, W>)) void k_delta_bwd(
             dd += sums[u * 32 + 16 + c];
           }
           dd = sum_after(dd);
+          // a row that nothing passes through, a reset or the first one of a ray, has a gradient of 0, and not what is left of
+          // sums that cancel
+          const float passed = c ? Dc[float4_at(c, (c - 1) >> 2) + ((c - 1) & 3)] : p || a.h0 ? vec[16] : 0.f;
+          if (passed == 0.f && fabsf(dd) <= 3.4e38f) dd = 0.f;
           if (c < ck.many) {
             const int64_t to = (int64_t)(ck.low + ck.at(c)) * a.v_heads + h;
             ((T*)a.ddecay)[to] = (T)dd;

@@ -371,7 +371,8 @@ def ray_delta(q, k, v, decay, beta, rays: RaySet, *, h0=None, scale: float | Non
 def ray_delta_backward(do, q, k, v, decay, beta, marks, rays: RaySet, *, dlast=None, h0=None, scale: float | None = None,
                        reverse: bool = False):
     """(dq, dk, dv, ddecay, dbeta, dh0) of ray_delta's o (do) and last (dlast, None: 0), with its marks and options.  Of the
-    inputs' type; dh0 float32, None without h0."""
+    inputs' type; dh0 float32, None without h0.  ddecay is a sum of products and exact to their size: relative to itself that
+    is less where a decay is strong (some 1e-3 at -8, nothing from -16 on); it is 0 at -inf."""
     lib = fl.load()
     a, dev, state = _delta_args(q, k, v, decay, beta, rays, h0, scale, reverse)
     a.dout = _want(do, "do", v.shape, v.dtype, dev, 1)

@@ -496,7 +496,10 @@ int ffn_ray_delta_workspace(const ffn_ray_delta* a, int32_t backward, uint64_t* 
 int ffn_ray_delta_fwd(const ffn_ray_delta* a, void* stream);
 /* Gradients of sum(o dout) + sum(last dlast), from q, k, v, decay, beta, h0 and
  * the forward's marks of the same sizes; dq and dk summed over the value heads
- * of a key head.  scale gets none.  No atomics: two calls give the same bits. */
+ * of a key head.  scale gets none.  ddecay is a sum of products and exact to their
+ * size (2^-20 of it): where a decay is so strong that next to nothing of the state
+ * passes, it is smaller than that; where nothing does, it is 0.  No atomics: two
+ * calls give the same bits. */
 int ffn_ray_delta_bwd(const ffn_ray_delta* a, void* stream);
 
 #define FFN_MAX_EXPERTS 1024
