@@ -117,7 +117,8 @@ template <> struct Delta<__bf16> {
     for (int i = 2; i >= 0; --i) c = mma16(a.p[i], b, c);
     return c;
   }
-  // of two floats: six products; those left out are 2^-23 of a b at most, as a rounding of it in float would be
+  // of two floats: the six largest of nine products, the smallest first.  Those left out are some 2^-24 of a b, and 2^-20 at
+  // most; with two of them more no result was nearer to 64 bits, and the backward's registers cost a wavefront a SIMD.
   static __device__ __forceinline__ f32x4 mul(const Full& a, const Full& b, f32x4 c) {
 #pragma unroll
     for (int s = 2; s >= 0; --s) {
@@ -1133,6 +1134,9 @@ __global__ __launch_bounds__(64 * W, (DL_BWD_WAVES<T, DK, W>)) void k_delta_bwd(
           *reinterpret_cast<f32x4*>(sums + w * 32 + 4 * g) = to_beta;
           *reinterpret_cast<f32x4*>(sums + w * 32 + 16 + 4 * g) = to_decay;
         }
+        // a row that nothing passes through, a reset or the first one of a ray, has a decay's gradient of 0, and not what is
+        // left of sums that cancel
+        const float passed = c ? Dc[float4_at(c, (c - 1) >> 2) + ((c - 1) & 3)] : p || a.h0 ? vec[16] : 0.f;
         sync();
         if (w == 0 && g == 0) {
           float db = 0.f, dd = 0.f;
@@ -1142,9 +1146,6 @@ __global__ __launch_bounds__(64 * W, (DL_BWD_WAVES<T, DK, W>)) void k_delta_bwd(
             dd += sums[u * 32 + 16 + c];
           }
           dd = sum_after(dd);
-          // a row that nothing passes through, a reset or the first one of a ray, has a gradient of 0, and not what is left of
-          // sums that cancel
-          const float passed = c ? Dc[float4_at(c, (c - 1) >> 2) + ((c - 1) & 3)] : p || a.h0 ? vec[16] : 0.f;
           if (passed == 0.f && fabsf(dd) <= 3.4e38f) dd = 0.f;
           if (c < ck.many) {
             const int64_t to = (int64_t)(ck.low + ck.at(c)) * a.v_heads + h;
