@@ -323,8 +323,9 @@ struct Shape {
 bool fits(const void* p, int64_t row, int64_t n, int size) { return !((uintptr_t)p & 15) && (n < 2 || row * size % 16 == 0); }
 
 // A piece is 16 bytes where every row allows it.  The fewest pieces a lane that a wavefront covers the row with, up to
-// four (16 columns a lane where pieces are columns); then blocks of 4 to 16 wavefronts with 16 columns a lane, which leave
-// a wavefront of 16 the registers for the backward's parameters and their sums.
+// four (16 columns a lane where pieces are columns); then blocks of 4 to 16 wavefronts with 16 columns a lane.  Blocks of 16,
+// past 8192 columns, have 128 registers a lane, and the backward's parameters and their sums do not fit into them (6 to 79
+// are spilled); nor do two rows of single columns in the forward, whose blocks of any size are held to that (2 to 6).
 Shape shape_of(const ffn_norm& a, bool backward) {
   const int size = a.dtype == FFN_F32 ? 4 : 2, el = 16 / size;
   Shape s;

@@ -21,13 +21,16 @@
 // at 16 times the rate (K = 32; 8 times at K = 16), to the same accuracy.  (A product whose second operand has K = 16 too
 // stays in float where making its parts would cost the vector ALU more than the matrix cores save.)
 //
-// What bounds it, us a kernel with what memory alone would take of q, k, v, o and their gradients (4.63 TB/s): 8192 marched
-// rays, 4 heads of 32 x 32, bf16, forward 140 (43), backward 370 (43): the vector ALU, beside the waits of short rays' few
-// chunks; 24 rays of up to 4096 rows, 8 heads of 64 x 64 on 4, bf16, 476 and 1361 + 62 (98 in all): what a block does for a
-// chunk, one after the other, 1.8 and 5.3 us for each of a ray's 256, at less than a wavefront a SIMD; 3001 rays, 3 heads of
-// 24 x 40, fp32, with states, 111 and 286 (92): vector ALU and fp32 matrix cores a third each.  Not kept, us when each was
-// tried: the next segment's v ahead in the forward 163 (149 without); the heads of a ray one after the other in a block 204
-// and 602 (139 and 352: the longest ray's chain is four times as long).  Not built: states kept every chunk (twice the marks).
+// What bounds it, us a kernel in a trace (calls in a row, as the variants further down are compared, take up to a tenth less)
+// with what memory alone would take of q, k, v, o and their gradients (4.63 TB/s): 8192 marched rays, 4 heads of 32 x 32, bf16,
+// forward 137 (43), backward 365 (43): the vector ALU, 61 to 65 % busy, beside the waits of short rays' few chunks; 24 rays of
+// up to 4096 rows, 8 heads of 64 x 64 on 4, bf16, 471 and 1350 + 61 (98 in all): what a block does for a chunk, the chain from
+// state to state and all else between its barriers, 1.8 and 5.3 us for each of a ray's 256, at less than a wavefront a SIMD;
+// 3001 rays, 3 heads of 24 x 40, fp32, with states, 111 and 291 (92): vector ALU and fp32 matrix cores a third each.  Not kept,
+// us when each was tried: the next segment's v ahead in the forward 163 (149 without); the heads of a ray one after the other
+// in a block 204 and 602 (139 and 352: the longest ray's chain is four times as long).  Not built: states kept every chunk
+// (twice the marks).  Backward passes of 128 x 128, and of 128 x 16 in fp32, spill 31 to 154 registers (1024 marched rays, 2
+// heads of 128 x 128, bf16, 408 us in a row).
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -45,7 +48,7 @@ constexpr int DL_VEC = 64;            // a chunk's b, e, D_15 and (first of the 
 constexpr float DL_RESET = -1e30f;    // stands for a decay of -infinity, which must not meet a zero in a product
 constexpr int DL_BLOCKS = 4096;       // heads of rays, 16 a CU: more than run at once
 constexpr int DL_FEW = 8;             // rows of a ray that are taken row by row at most
-constexpr int DL_PICK = 509;          // blocks at least that look for rays of more, two a CU (a prime: rays may be long in a pattern)
+constexpr int DL_PICK = 509;          // blocks that look for rays of more, two a CU; a prime, as rays may be long in a pattern
 constexpr int DL_CLEAR = 1024;        // rows that one block looks through for those of no ray
 
 // ---------------------------------------------------------------------------
@@ -670,7 +673,8 @@ __global__ __launch_bounds__(64 * W, (PICK ? 1 : DL_FWD_WAVES<T, DK, W>)) void k
 }
 
 // Few rows a ray (one more sample of each): the state goes through once, row by row on the vector ALU, and memory bounds
-// it.  Rays of more than `most` rows are left to the chunks.  A wavefront takes 32 columns of a state: 8 lanes of four columns, 8 groups of rows dk = 8 i + group.
+// it.  Rays of more than `most` rows are left to the chunks.  A wavefront takes 32 columns of a state: 8 lanes of four
+// columns, 8 groups of rows dk = 8 i + group.
 template <typename T, int DK>
 __global__ __launch_bounds__(256, DK <= 32 ? 6 : DK <= 64 ? 5 : 3) void k_delta_step(const ffn_ray_delta a, int most) {
   constexpr int N = DK / 8;
@@ -1180,15 +1184,16 @@ __global__ __launch_bounds__(256) void k_delta_join(const ffn_ray_delta a) {
 // ---------------------------------------------------------------------------
 // launches
 
-// columns of a state's rows and rows, as the kernels hold it
+// a state's rows and wavefronts of 16 columns, as the kernels hold it: those of 72 to 112 columns take the time of 128 (1024
+// marched rays, 4 heads, bf16, us: 64 x 64 49 and 152, 64 x 80 127 and 343, 64 x 128 129 and 344); five to seven are not built
 inline int delta_rows(int key_dim) { return key_dim <= 32 ? 32 : key_dim <= 64 ? 64 : 128; }
 inline int delta_waves(int val_dim) { return val_dim <= 64 ? (val_dim + 15) / 16 : 8; }
 
 inline int64_t delta_clear_blocks(const ffn_ray_delta& a) { return ((int64_t)a.rays.n + DL_CLEAR - 1) / DL_CLEAR; }
 
 // Where rays are many, those of more than twice the mean and four chunks take their turn before the others: one that is
-// begun last would be all that still runs (8192 marched rays, 4 heads of 32 x 32, bf16: forward 120 us, 127 in one turn,
-// backward 320 and 340).
+// begun last would be all that still runs (8192 marched rays, 4 heads of 32 x 32, bf16: forward 124 us, 130 in one turn,
+// backward 341 and 360).
 inline int delta_longer(const ffn_ray_delta& a) {
   if ((int64_t)a.rays.num_rays * a.v_heads < DL_BLOCKS) return 0;
   return (int)std::max<int64_t>(4 * DL_C, 2 * (int64_t)a.rays.n / a.rays.num_rays);
@@ -1222,9 +1227,9 @@ hipError_t start_delta(const ffn_ray_delta& a, bool back, bool few, hipStream_t 
 
 template <typename T, int DK>
 hipError_t delta_by_columns(const ffn_ray_delta& a, bool back, hipStream_t st) {
-  // Row by row or in chunks: by the mean of rows a ray (2048 rays, 4 heads of 64 x 64, bf16, us: one row 52 and 83, three 71
-  // and 85, six 111 and 90), and where row by row, by each ray's own: only the GPU knows it, and a second launch looks for
-  // those of more than eight (3 us; one ray of 4096 rows and 2047 without any 488, 8900 row by row).
+  // Row by row or in chunks: by the mean of rows a ray (2048 rays, 4 heads of 64 x 64, bf16, us: one row 55 and 83, three 64
+  // and 82, six 94 and 87), and where row by row, by each ray's own: only the GPU knows it, and a second launch looks for
+  // those of more than eight (3 us of these; one ray of 4096 rows and 2047 without any 488, 8900 row by row).
   const bool few = !back && !a.marks && a.rays.n <= 4ull * a.rays.num_rays;
   const int W = delta_waves(a.val_dim);
   const hipError_t e = W == 1   ? start_delta<T, DK, 1>(a, back, few, st)
